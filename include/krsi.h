@@ -229,6 +229,45 @@ int krsi_relpos_bucket_gather(const float* table, const int32_t* bucket, float* 
 int krsi_relpos_bucket_sum(const float* dpd, const int32_t* bucket, float* dtable, int32_t S,
                            int32_t H, int32_t num_buckets, void* stream);
 
+/* ------------------------- query and key norm with rotation (no counterpart)
+ * The step between the fused projection and the attention: every query and key head is RMS-normalised with
+ * its kind's weight, then rotated by its token's position; value heads are copied.
+ * qkv: [tokens, ld_qkv] of T (any alignment and ld_qkv >= (H + 2 KH) D, unit column stride): H query heads, KH
+ *      key heads and KH value heads of D columns each. wq, wk: [D] of T. out: [tokens, (H + 2 KH) D] of T.
+ * rope: [table_rows, R] fp32, row p the cosines then the sines of the R / 2 angles at position p.
+ * positions: [tokens] int32 or int64 (position_bytes 4 or 8), or NULL: token t is at t % S. A position outside
+ *      the table makes the rotated columns of its token NaN.
+ *   z = w x / sqrt(sum x^2 / D + eps);  y_a = z_a cos - z_b sin, y_b = z_b cos + z_a sin for the pairs
+ *   (i, i + R/2), or (2i, 2i + 1) with interleaved = 1, of the first R columns; y = z in the others.
+ * fp32 from the load to the store, one rounding. Backward: dqkv [tokens, ld_dqkv] (its first (H + 2 KH) D
+ * columns are written), dwq and dwk [D], summed in fp32 in a fixed order; dout as out.
+ * Limits: D % 8 == 0, 8 <= D <= 128, R even, 2 <= R <= D; tokens < 2^31, table_rows >= min(S, tokens) without
+ * positions. No tokens: dwq and dwk are zero. workspace: krsi_qk_norm_rope_bwd_workspace_bytes(D), scratch.  */
+int krsi_qk_norm_rope_fwd(const void* qkv, int64_t ld_qkv, const void* wq, const void* wk, const float* rope,
+                          const void* positions, void* out, int64_t tokens, int32_t S, int32_t H, int32_t KH,
+                          int32_t D, int32_t R, int64_t table_rows, int32_t position_bytes, float eps,
+                          int32_t interleaved, int32_t dtype, void* stream);
+size_t krsi_qk_norm_rope_bwd_workspace_bytes(int32_t D);
+int krsi_qk_norm_rope_bwd(const void* dout, const void* qkv, int64_t ld_qkv, const void* wq, const void* wk,
+                          const float* rope, const void* positions, void* dqkv, int64_t ld_dqkv, void* dwq, void* dwk,
+                          void* workspace, size_t workspace_bytes, int64_t tokens, int32_t S, int32_t H, int32_t KH,
+                          int32_t D, int32_t R, int64_t table_rows, int32_t position_bytes, float eps,
+                          int32_t interleaved, int32_t dtype, void* stream);
+
+/* -------------------------------------------- token embedding (no counterpart)
+ * out[t, :] = T(scale * table[tokens[t], :]); table [V, D] and out [n, D] contiguous, of T, any alignment of
+ * the element; tokens [n] int32 or int64 (token_bytes 4 or 8). A token outside [0, V) gives a row of NaN.
+ * Backward: dtable[v, :] = T(scale * sum of dout[t, :] over tokens[t] == v), every row written, fp32 sums in an
+ * order that the tokens alone decide (no float atomics); tokens outside [0, V) or equal to padding (-1: none)
+ * have no part. workspace: krsi_embedding_bwd_workspace_bytes, scratch.
+ * Limits: n <= 2^30, V <= 2^24, D <= 2^20, scale finite. n = 0: dtable is zero.                           */
+int krsi_embedding_fwd(const void* tokens, int32_t token_bytes, const void* table, void* out, int64_t n, int32_t V,
+                       int32_t D, float scale, int32_t dtype, void* stream);
+size_t krsi_embedding_bwd_workspace_bytes(int64_t n, int32_t V, int32_t D);
+int krsi_embedding_bwd(const void* dout, const void* tokens, int32_t token_bytes, void* dtable, void* workspace,
+                       size_t workspace_bytes, int64_t n, int32_t V, int32_t D, int64_t padding, float scale,
+                       int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -53,4 +53,26 @@ __device__ __forceinline__ T* chunk_at(T* row, int c, int n) {
   return reinterpret_cast<T*>(reinterpret_cast<u32x4*>(row) + c);
 }
 
+// C consecutive elements of any alignment, in registers.
+template <int DT, int C>
+struct Piece {
+  using T = typename Elem<DT>::T;
+  T e[C];
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(e, p, sizeof(e)); }
+  __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, e, sizeof(e)); }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int j = 0; j < C; ++j) f[j] = Elem<DT>::load(e[j]);
+  }
+  __device__ __forceinline__ void set(const float* f) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) e[j] = Elem<DT>::store(f[j]);
+  }
+};
+
+// Entry i of an index tensor of int32 or int64 (bytes 4 or 8).
+__device__ __forceinline__ int64_t load_index(const void* p, int bytes, int64_t i) {
+  return bytes == 8 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
 }  // namespace krsi

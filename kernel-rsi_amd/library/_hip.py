@@ -68,6 +68,14 @@ SIGNATURES = {
                                             _I32, _I32, _I32, _I32, _F32, _P]),
     "krsi_relpos_bucket_gather": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _I32, _P]),
     "krsi_relpos_bucket_sum": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _I32, _P]),
+    "krsi_qk_norm_rope_fwd": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I64,
+                                             _I32, _F32, _I32, _I32, _P]),
+    "krsi_qk_norm_rope_bwd_workspace_bytes": (_SZ, [_I32]),
+    "krsi_qk_norm_rope_bwd": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _SZ, _I64, _I32, _I32,
+                                             _I32, _I32, _I32, _I64, _I32, _F32, _I32, _I32, _P]),
+    "krsi_embedding_fwd": (ctypes.c_int, [_P, _I32, _P, _P, _I64, _I32, _I32, _F32, _I32, _P]),
+    "krsi_embedding_bwd_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "krsi_embedding_bwd": (ctypes.c_int, [_P, _P, _I32, _P, _P, _SZ, _I64, _I32, _I32, _I64, _F32, _I32, _P]),
 }
 
 # KRSI_DTYPE_* codes of the activation dtypes.
@@ -199,6 +207,18 @@ def _dtype(name: str, t: torch.Tensor, like: torch.Tensor | None = None,
     if like is not None and t.dtype != like.dtype:
         raise TypeError(f"{name} must have the dtype of the activations ({like.dtype}), got {t.dtype}")
     return DTYPE_CODES[t.dtype]
+
+
+def _on_device(fn):
+    """fn with its first tensor's device as the current one, which the launch, its stream and what it allocates
+    go to."""
+    @functools.wraps(fn)
+    def call(first, *args):
+        if first.is_cuda and first.device.index != torch.cuda.current_device():
+            with torch.cuda.device(first.device):
+                return fn(first, *args)
+        return fn(first, *args)
+    return call
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -457,4 +477,129 @@ def relpos_bucket_sum(dpd: torch.Tensor, bucket: torch.Tensor, S: int, num_bucke
     dtable = torch.empty(num_buckets, H, device=dpd.device, dtype=torch.float32)
     _check(lib().krsi_relpos_bucket_sum(_ptr(dpd), _ptr(bucket), _ptr(dtable), S, H, num_buckets,
                                         _stream(dpd)))
+    return dtable
+
+
+# ------------------------------------------- query and key norm with rotation
+def _index_bytes(name: str, t: torch.Tensor) -> int:
+    if t.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{name} must be torch.int64 or torch.int32, got {t.dtype}")
+    return t.element_size()
+
+
+def _check_qk(qkv, q_weight, k_weight, rope, positions, B, S, H, KH, D) -> tuple:
+    """(dtype code, row stride of qkv) of a call whose tensors fit each other."""
+    _on_gpu(qkv, q_weight, k_weight, rope, *(() if positions is None else (positions,)))
+    dt = _dtype("qkv", qkv)
+    _dtype("q_weight", q_weight, like=qkv)
+    _dtype("k_weight", k_weight, like=qkv)
+    if min(B, S) < 0 or min(H, KH) < 1:
+        raise ValueError(f"B={B}, S={S}, H={H}, kv_heads={KH} do not describe a batch of heads")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"head dim D={D} unsupported: needs D % 8 == 0 and 8 <= D <= 128")
+    cols = (H + 2 * KH) * D
+    if qkv.dim() != 2 or qkv.shape[0] != B * S or qkv.shape[1] < cols:
+        raise ValueError(f"qkv shape {tuple(qkv.shape)} does not hold B*S={B * S} rows of (H + 2*kv_heads)*D={cols}")
+    ld = qkv.stride(0) if qkv.shape[0] > 1 else qkv.shape[1]
+    if qkv.stride(1) != 1 or ld < cols:
+        raise ValueError("qkv must have unit column stride and rows that do not overlap")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.shape != (D,):
+            raise ValueError(f"{name} shape {tuple(w.shape)} != ({D},)")
+    if rope.dtype != torch.float32:
+        raise TypeError(f"rope must be torch.float32, got {rope.dtype}")
+    if rope.dim() != 2 or rope.shape[0] < 1 or rope.shape[1] % 2 or not 2 <= rope.shape[1] <= D:
+        raise ValueError(f"rope shape {tuple(rope.shape)} is not [positions, R] with R even and 2 <= R <= D={D}")
+    if positions is None:
+        if rope.shape[0] < S:
+            raise ValueError(f"rope has {rope.shape[0]} positions for S={S}")
+    else:
+        _index_bytes("positions", positions)
+        if positions.numel() != B * S:
+            raise ValueError(f"positions has {positions.numel()} entries for B*S={B * S} tokens")
+    return dt, ld
+
+
+@_on_device
+def qk_norm_rope_fwd(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, rope: torch.Tensor,
+                     positions: torch.Tensor | None, B: int, S: int, H: int, KH: int, D: int, eps: float,
+                     interleaved: bool) -> torch.Tensor:
+    """[B*S, (H+2*KH)*D]: query and key heads normalised and rotated, value heads copied."""
+    dt, ld = _check_qk(qkv, q_weight, k_weight, rope, positions, B, S, H, KH, D)
+    q_weight, k_weight, rope = q_weight.contiguous(), k_weight.contiguous(), rope.contiguous()
+    positions = None if positions is None else positions.contiguous()
+    out = torch.empty(B * S, (H + 2 * KH) * D, device=qkv.device, dtype=qkv.dtype)
+    if B * S:
+        _check(lib().krsi_qk_norm_rope_fwd(
+            _ptr(qkv), ld, _ptr(q_weight), _ptr(k_weight), _ptr(rope), _ptr(positions), _ptr(out), B * S, S, H, KH, D,
+            rope.shape[1], rope.shape[0], 0 if positions is None else positions.element_size(), float(eps),
+            int(interleaved), dt, _stream(qkv)))
+    return out
+
+
+@_on_device
+def qk_norm_rope_bwd(dout: torch.Tensor, qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                     rope: torch.Tensor, positions: torch.Tensor | None, B: int, S: int, H: int, KH: int, D: int,
+                     eps: float, interleaved: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """dqkv (qkv's shape; zero past the heads' columns), dq_weight and dk_weight."""
+    dt, ld = _check_qk(qkv, q_weight, k_weight, rope, positions, B, S, H, KH, D)
+    _on_gpu(qkv, dout)
+    _dtype("grad", dout, like=qkv)
+    cols = (H + 2 * KH) * D
+    if dout.shape != (B * S, cols):
+        raise ValueError(f"grad shape {tuple(dout.shape)} != {(B * S, cols)}")
+    dout, rope = dout.contiguous(), rope.contiguous()
+    q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+    positions = None if positions is None else positions.contiguous()
+    dqkv = qkv.new_empty(qkv.shape)
+    if qkv.shape[1] > cols:
+        dqkv[:, cols:].zero_()
+    dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    nbytes = lib().krsi_qk_norm_rope_bwd_workspace_bytes(D)
+    ws = torch.empty(nbytes, device=qkv.device, dtype=torch.uint8)
+    _check(lib().krsi_qk_norm_rope_bwd(
+        _ptr(dout), _ptr(qkv), ld, _ptr(q_weight), _ptr(k_weight), _ptr(rope), _ptr(positions), _ptr(dqkv),
+        dqkv.shape[1], _ptr(dwq), _ptr(dwk), _ptr(ws), nbytes, B * S, max(S, 1), H, KH, D, rope.shape[1],
+        rope.shape[0], 0 if positions is None else positions.element_size(), float(eps), int(interleaved), dt,
+        _stream(qkv)))
+    return dqkv, dwq, dwk
+
+
+# ------------------------------------------------------------ token embedding
+def _check_embedding(tokens: torch.Tensor, table_shape: tuple) -> None:
+    _index_bytes("tokens", tokens)
+    if len(table_shape) != 2 or min(table_shape) < 1:
+        raise ValueError(f"table shape {tuple(table_shape)} is not [V, D]")
+
+
+@_on_device
+def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, scale: float) -> torch.Tensor:
+    """[*tokens.shape, D]: the tokens' rows of table [V, D], scaled."""
+    _on_gpu(tokens, table)
+    dt = _dtype("table", table)
+    _check_embedding(tokens, table.shape)
+    tokens, table = tokens.contiguous(), table.contiguous()
+    V, D = table.shape
+    out = torch.empty(*tokens.shape, D, device=table.device, dtype=table.dtype)
+    if tokens.numel():
+        _check(lib().krsi_embedding_fwd(_ptr(tokens), tokens.element_size(), _ptr(table), _ptr(out), tokens.numel(), V, D,
+                                        float(scale), dt, _stream(table)))
+    return out
+
+
+@_on_device
+def embedding_bwd(dout: torch.Tensor, tokens: torch.Tensor, V: int, scale: float, padding_idx: int) -> torch.Tensor:
+    """dtable [V, D]: the scaled sums of each token's rows of dout [*tokens.shape, D]; padding_idx -1: none."""
+    _on_gpu(dout, tokens)
+    dt = _dtype("grad", dout)
+    if dout.shape[:-1] != tokens.shape or dout.dim() < 1:
+        raise ValueError(f"grad shape {tuple(dout.shape)} does not hold a row for each of tokens {tuple(tokens.shape)}")
+    _check_embedding(tokens, (V, dout.shape[-1]))
+    dout, tokens = dout.contiguous(), tokens.contiguous()
+    n, D = tokens.numel(), dout.shape[-1]
+    dtable = torch.empty(V, D, device=dout.device, dtype=dout.dtype)
+    nbytes = lib().krsi_embedding_bwd_workspace_bytes(n, V, D)
+    ws = torch.empty(max(nbytes, 1), device=dout.device, dtype=torch.uint8)
+    _check(lib().krsi_embedding_bwd(_ptr(dout), _ptr(tokens), tokens.element_size(), _ptr(dtable), _ptr(ws), nbytes, n, V,
+                                    D, padding_idx, float(scale), dt, _stream(dout)))
     return dtable

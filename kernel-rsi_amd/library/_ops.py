@@ -7,7 +7,8 @@ replay.py's per-file module names) does not register the ops twice.
 Op names follow the reference (library/rmsnorm.py:86-103, geglu.py:85-101,
 relpos_attention.py:175-195): krsi::rmsnorm_fwd/bwd, krsi::geglu_fwd/bwd,
 krsi::relpos_attn_fwd/bwd; krsi::relpos_bucket_gather/sum (the T5 table step) and
-krsi::geglu_linear_fwd (the merged projection with the GEGLU epilogue) have no counterpart there. Their schemas are internal to this library.
+krsi::geglu_linear_fwd (the merged projection with the GEGLU epilogue), krsi::qk_norm_rope_fwd/bwd and
+krsi::embedding_fwd/bwd have no counterpart there. Their schemas are internal to this library.
 """
 from __future__ import annotations
 
@@ -196,3 +197,77 @@ def _bucket_backward(ctx, dpd):
 
 
 bucket_gather_op.register_autograd(_bucket_backward, setup_context=_bucket_setup)
+
+# ------------------------------------------- query and key norm with rotation
+
+
+@torch.library.custom_op("krsi::qk_norm_rope_fwd", mutates_args=())
+def qk_norm_rope_fwd_op(qkv: Tensor, q_weight: Tensor, k_weight: Tensor, rope: Tensor, positions: Tensor | None, B: int,
+                        S: int, H: int, KH: int, D: int, eps: float, interleaved: bool) -> Tensor:
+    return _hip.qk_norm_rope_fwd(qkv, q_weight, k_weight, rope, positions, B, S, H, KH, D, eps, interleaved)
+
+
+@qk_norm_rope_fwd_op.register_fake
+def _(qkv, q_weight, k_weight, rope, positions, B, S, H, KH, D, eps, interleaved):
+    return qkv.new_empty((B * S, (H + 2 * KH) * D))
+
+
+@torch.library.custom_op("krsi::qk_norm_rope_bwd", mutates_args=())
+def qk_norm_rope_bwd_op(dout: Tensor, qkv: Tensor, q_weight: Tensor, k_weight: Tensor, rope: Tensor,
+                        positions: Tensor | None, B: int, S: int, H: int, KH: int, D: int, eps: float,
+                        interleaved: bool) -> tuple[Tensor, Tensor, Tensor]:
+    return _hip.qk_norm_rope_bwd(dout, qkv, q_weight, k_weight, rope, positions, B, S, H, KH, D, eps, interleaved)
+
+
+@qk_norm_rope_bwd_op.register_fake
+def _(dout, qkv, q_weight, k_weight, rope, positions, B, S, H, KH, D, eps, interleaved):
+    return qkv.new_empty(qkv.shape), q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
+
+
+def _qk_setup(ctx, inputs, output):
+    qkv, q_weight, k_weight, rope, positions, *dims = inputs
+    ctx.save_for_backward(qkv, q_weight, k_weight, rope, positions)
+    ctx.dims = dims
+
+
+def _qk_backward(ctx, dout):
+    return (*qk_norm_rope_bwd_op(dout.contiguous(), *ctx.saved_tensors, *ctx.dims), *[None] * 9)
+
+
+qk_norm_rope_fwd_op.register_autograd(_qk_backward, setup_context=_qk_setup)
+
+# ------------------------------------------------------------ token embedding
+
+
+@torch.library.custom_op("krsi::embedding_fwd", mutates_args=())
+def embedding_fwd_op(tokens: Tensor, table: Tensor, scale: float, padding_idx: int) -> Tensor:
+    return _hip.embedding_fwd(tokens, table, scale)
+
+
+@embedding_fwd_op.register_fake
+def _(tokens, table, scale, padding_idx):
+    return table.new_empty((*tokens.shape, table.shape[1]))
+
+
+@torch.library.custom_op("krsi::embedding_bwd", mutates_args=())
+def embedding_bwd_op(dout: Tensor, tokens: Tensor, V: int, scale: float, padding_idx: int) -> Tensor:
+    return _hip.embedding_bwd(dout, tokens, V, scale, padding_idx)
+
+
+@embedding_bwd_op.register_fake
+def _(dout, tokens, V, scale, padding_idx):
+    return dout.new_empty((V, dout.shape[-1]))
+
+
+def _embedding_setup(ctx, inputs, output):
+    tokens, table, scale, padding_idx = inputs
+    ctx.save_for_backward(tokens)
+    ctx.args = (table.shape[0], scale, padding_idx)
+
+
+def _embedding_backward(ctx, dout):
+    (tokens,) = ctx.saved_tensors
+    return None, embedding_bwd_op(dout.contiguous(), tokens, *ctx.args), None, None
+
+
+embedding_fwd_op.register_autograd(_embedding_backward, setup_context=_embedding_setup)

@@ -362,3 +362,62 @@ def cpu_eager_step(kind: str, inputs: dict):
         out = relpos_sdpa(qkv, pd, B, S, H, D, inputs["scale"])
         return out if fwd_only else torch.autograd.grad(out, [qkv, pd], inputs["dout"])
     raise ValueError(kind)
+
+
+# ------------------------------------------- query and key norm with rotation
+def _qk_parts(qkv, w_q, w_k, rope, pos, H, KH, D, eps, interleaved):
+    """float64 pieces of qk_norm_rope: x [tokens, H+KH, D], its weights, r, cos, sin and the pair columns."""
+    x = qkv[:, :(H + KH) * D].double().reshape(-1, H + KH, D)
+    w = torch.cat([w_q.double().expand(H, D), w_k.double().expand(KH, D)])
+    r = (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+    R = rope.shape[1]
+    half = torch.arange(R // 2)
+    a, b = (2 * half, 2 * half + 1) if interleaved else (half, half + R // 2)
+    row = rope.double()[pos]
+    return x, w, r, row[:, None, :R // 2], row[:, None, R // 2:], a, b
+
+
+def qk_norm_rope_64(qkv, w_q, w_k, rope, pos, H, KH, D, eps, interleaved):
+    """(y, magnitude of its terms) in float64 on the CPU; pos: a position per token."""
+    x, w, r, c, s, a, b = _qk_parts(qkv, w_q, w_k, rope, pos, H, KH, D, eps, interleaved)
+    z = w * x * r
+    y, mag = z.clone(), z.abs()
+    y[..., a] = z[..., a] * c - z[..., b] * s
+    y[..., b] = z[..., b] * c + z[..., a] * s
+    m = mag[..., a] + mag[..., b]
+    mag[..., a] = mag[..., b] = m
+    v = qkv[:, (H + KH) * D:(H + 2 * KH) * D].double()
+    return torch.cat([y.flatten(1), v], 1), torch.cat([mag.flatten(1), torch.zeros_like(v)], 1)
+
+
+def qk_norm_rope_grads_64(dy, qkv, w_q, w_k, rope, pos, H, KH, D, eps, interleaved):
+    """((dqkv, dw_q, dw_k), the magnitudes of their terms): the closed form in float64.
+    dz = R^T dy, dw = sum dz x r, dn = dz w, dx = r dn - x r^3 mean(dn x)."""
+    x, w, r, c, s, a, b = _qk_parts(qkv, w_q, w_k, rope, pos, H, KH, D, eps, interleaved)
+    g = dy[:, :(H + KH) * D].double().reshape(x.shape)
+    dz, mag = g.clone(), g.abs()
+    dz[..., a] = g[..., a] * c + g[..., b] * s
+    dz[..., b] = g[..., b] * c - g[..., a] * s
+    m = mag[..., a] + mag[..., b]
+    mag[..., a] = mag[..., b] = m
+    dn = dz * w
+    dx = r * dn - x * r ** 3 * (dn * x).mean(-1, keepdim=True)
+    dx_mag = r * mag * w.abs() + x.abs() * r ** 3 * (mag * w.abs() * x.abs()).mean(-1, keepdim=True)
+    dw, dw_mag = (dz * x * r).sum(0), (mag * x.abs() * r).sum(0)
+    v = dy[:, (H + KH) * D:].double()
+    return ((torch.cat([dx.flatten(1), v], 1), dw[:H].sum(0), dw[H:].sum(0)),
+            (torch.cat([dx_mag.flatten(1), torch.zeros_like(v)], 1), dw_mag[:H].sum(0), dw_mag[H:].sum(0)))
+
+
+# ------------------------------------------------------------ token embedding
+def embedding_grad_64(dout, tokens, V, scale, padding_idx=None):
+    """(dtable, scale * sum |dout|, rows per token) in float64: each row of dout added to its token's row; tokens
+    outside [0, V) and padding_idx have none."""
+    tok, g = tokens.reshape(-1).long(), dout.reshape(-1, dout.shape[-1]).double()
+    kept = (tok >= 0) & (tok < V)
+    if padding_idx is not None:
+        kept &= tok != padding_idx
+    tok, g = tok[kept], g[kept]
+    zero = torch.zeros(V, g.shape[1], dtype=torch.float64)
+    return (zero.index_add(0, tok, g) * scale, zero.index_add(0, tok, g.abs()) * abs(scale),
+            torch.bincount(tok, minlength=V)[:, None])

@@ -333,3 +333,42 @@ def test_t5_bucket_map_against_closed_form():
                 continue
             want = min(int(x), 15)
         assert bk == base + want, (dist, bk, base + want)
+
+
+# ------------------------------------------- query and key norm with rotation
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("H,KH,D,R", [(2, 1, 8, 8), (1, 1, 16, 6), (3, 2, 8, 2)])
+def test_qk_norm_rope_closed_form(H, KH, D, R, interleaved):
+    """The oracle's gradient against central differences of its forward (step 1e-5: their error is below
+    1e-9 of the third derivatives plus 1e-16 / 1e-5 of the value), and its rotation keeps each pair's length."""
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(3, (H + 2 * KH) * D, generator=g, dtype=torch.float64)
+    wq, wk = (torch.rand(D, generator=g, dtype=torch.float64) + 0.5 for _ in range(2))
+    angle = torch.rand(5, R // 2, generator=g, dtype=torch.float64) * 6
+    rope, pos = torch.cat([angle.cos(), angle.sin()], 1), torch.tensor([4, 0, 2])
+    args = (rope, pos, H, KH, D, 1e-3, interleaved)
+    dy = torch.randn(qkv.shape, generator=g, dtype=torch.float64)
+    grads, _ = O.qk_norm_rope_grads_64(dy, qkv, wq, wk, *args)
+    for i, leaf in enumerate((qkv, wq, wk)):
+        for at in range(0, leaf.numel(), 3):
+            sides = []
+            for step in (1e-5, -1e-5):
+                moved = [t.clone() for t in (qkv, wq, wk)]
+                moved[i].view(-1)[at] += step
+                sides.append((O.qk_norm_rope_64(*moved, *args)[0] * dy).sum())
+            assert abs((sides[0] - sides[1]) / 2e-5 - grads[i].view(-1)[at]) < 1e-7
+    ones = torch.ones(D, dtype=torch.float64)
+    y = O.qk_norm_rope_64(qkv, ones, ones, *args)[0][:, :(H + KH) * D].view(3, -1, D)
+    x = qkv[:, :(H + KH) * D].view(3, -1, D)
+    z = x * (x.square().mean(-1, keepdim=True) + 1e-3).rsqrt()
+    assert torch.allclose(y.square().sum(-1), z.square().sum(-1), rtol=1e-12, atol=0)
+
+
+def test_embedding_gradient_closed_form():
+    tokens = torch.tensor([[3, 0, 3], [-1, 9, 5]])
+    dout = torch.randn(2, 3, 4, generator=torch.Generator().manual_seed(2))
+    got, _, count = O.embedding_grad_64(dout, tokens, 7, 2.0, padding_idx=5)
+    want = torch.zeros(7, 4, dtype=torch.float64)
+    want[3] = 2 * (dout[0, 0].double() + dout[0, 2].double())
+    want[0] = 2 * dout[0, 1].double()
+    assert torch.equal(got, want) and count[:, 0].tolist() == [1, 0, 0, 2, 0, 0, 0]
