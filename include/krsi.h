@@ -268,6 +268,27 @@ int krsi_embedding_bwd(const void* dout, const void* tokens, int32_t token_bytes
                        size_t workspace_bytes, int64_t n, int32_t V, int32_t D, int64_t padding, float scale,
                        int32_t dtype, void* stream);
 
+/* ---------------- cross entropy of an output projection (no counterpart)
+ * l = x w^T; loss_n = log sum_v exp(l_nv) - l_n,target(n). x [rows, k], w [v, k] contiguous, 16-byte aligned, of T
+ * (KRSI_DTYPE_BF16 or KRSI_DTYPE_F16); l is fp32 and is not kept. targets [rows] int32 or int64 (target_bytes 4
+ * or 8): ignore_index has loss 0 and no gradient; one outside [0, v) makes its loss (and gradients) NaN.
+ * reduction 0: loss [rows] fp32; 1: loss [1], the mean over the targets that are not ignored (NaN if there are
+ * none); 2: loss [1], the sum. stats [rows + 1] fp32, for the backward: lse of each row, then (1, 2) their number.
+ * Backward: dout fp32, [rows] or [1]; dx [rows, k] and dw [v, k] of T, either may be NULL (not wanted). The logits
+ * are computed again in pieces of the vocabulary, whose gradient is rounded to T times a power of two that
+ * keeps the largest at the top of fp16's range. Sums are fp32, in a fixed order.
+ * Limits: k % 64 == 0, k <= 2^20, v <= 2^24, rows <= 2^24. No rows: loss 0 or NaN, dw zero. Workspaces: the
+ * *_workspace_bytes (the backward's holds a piece of rows x v of about 512 MB at most, and fp32 parts of dx). */
+size_t krsi_linear_cross_entropy_fwd_workspace_bytes(int64_t rows, int32_t k, int32_t v);
+size_t krsi_linear_cross_entropy_bwd_workspace_bytes(int64_t rows, int32_t k, int32_t v);
+int krsi_linear_cross_entropy_fwd(const void* x, const void* w, const void* targets, int32_t target_bytes, float* loss,
+                                  float* stats, void* workspace, size_t workspace_bytes, int64_t rows, int32_t k,
+                                  int32_t v, int64_t ignore_index, int32_t reduction, int32_t dtype, void* stream);
+int krsi_linear_cross_entropy_bwd(const float* dout, const void* x, const void* w, const void* targets,
+                                  int32_t target_bytes, const float* stats, void* dx, void* dw, void* workspace,
+                                  size_t workspace_bytes, int64_t rows, int32_t k, int32_t v, int64_t ignore_index,
+                                  int32_t reduction, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

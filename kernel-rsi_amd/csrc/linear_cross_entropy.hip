@@ -1,0 +1,532 @@
+// Softmax cross entropy of an output projection's logits, which are never kept, forward and backward, for gfx950.
+//   l = x w^T                      x [rows, K], w [V, K] (nn.Linear layout), T = bf16 or fp16; l stays fp32
+//   lse_n = log sum_v exp(l_nv),   loss_n = lse_n - l_n,target(n)
+//   dl_nv = (exp(l_nv - lse_n) - [v = target(n)]) g_n,   dx = dl w,   dw = dl^T x
+// Forward: the products' epilogue reduces each wave's 64 columns of a row to a maximum and a sum of exponentials in
+// registers, and keeps the target's logit; a second launch joins a row's pairs, a third adds the losses.
+// Backward, in pieces of the vocabulary (kPieceBytes of dl each): the products again, whose epilogue forms dl, rounded
+// to T; then dw of the piece's rows and the piece's part of dx, which is carried in fp32 from piece to piece.
+// dl is held times a power of two that puts the largest |g| at 2^14..2^15: fp16 then keeps probabilities down to
+// 2^-29 in full precision, and the scale comes off exactly where dx and dw are rounded.
+//
+// What bounds it: the matrix cores (2 rows V K flop forward, 6 backward, 2 of them the logits again).
+#include "chunks.h"
+#include "krsi_device.h"
+#include "krsi_internal.h"
+#include "product_stream.h"
+
+namespace krsi {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kOneBlock = 1024;
+constexpr int64_t kPieceBytes = int64_t(512) << 20;
+constexpr int64_t kMaxWidth = 1 << 20;  // columns of a piece: 64 rows of dl stay below 2^31 bytes
+constexpr int kMinStages = 8;  // stages of a part of a split sum, at least
+
+using Large = StreamTile<2, 4, 8, 4>;  // 256 x 256, 8 waves, one workgroup per CU
+using Small = StreamTile<2, 2, 4, 4>;  // 128 x 128, 4 waves, two per CU
+
+struct Targets {
+  const void* p;
+  int bytes, V;
+  int64_t ignore;
+  // In [0, V), or -1: none (ignored, or outside).
+  __device__ __forceinline__ int at(int64_t row) const {
+    const int64_t t = load_index(p, bytes, row);
+    return t >= 0 && t < V && t != ignore ? (int)t : -1;
+  }
+  __device__ __forceinline__ bool ignored(int64_t row) const { return load_index(p, bytes, row) == ignore; }
+};
+
+// ------------------------------------------------------------------ forward
+// part [slices][rows]: (maximum, sum of exp(l - maximum)) of a row over the slice's 16 CB columns.
+template <int DT, int WM, int WN, int RB, int CB>
+__global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu * WM * WN / 4)) void logits_reduce(
+    Operand x, Operand w, int64_t K, Tiles tiles, Targets targets, float2* __restrict__ part,
+    float* __restrict__ target_logit) {
+  using Tl = StreamTile<WM, WN, RB, CB>;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[Tl::kLds];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+  const int wr = wave / WN, wc = wave % WN;
+  const int64_t rows = x.extent;
+  const int V = (int)w.extent;
+  stream_products<DT, false, false, WM, WN, RB, CB>(x, w, K, tiles, lds, [&](const TileAt& t, f32x4(&acc)[RB][CB]) {
+    const int col0 = (int)t.n0 + 16 * CB * wc + 4 * g;
+    const int64_t slice = t.n0 / (16 * CB) + wc;
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      const int64_t row = t.m0 + 16 * (RB * wr + i) + l16;
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < CB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m = fmaxf(m, col0 + 16 * j + r < V ? acc[i][j][r] : -__builtin_inff());
+      m = fmaxf(m, __shfl_xor(m, 16, kWave));
+      m = fmaxf(m, __shfl_xor(m, 32, kWave));
+      const float base = m == -__builtin_inff() ? 0.f : m;
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < CB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f((acc[i][j][r] - base) * kLog2e);
+          s += col0 + 16 * j + r < V ? e : 0.f;
+        }
+      s += __shfl_xor(s, 16, kWave);
+      s += __shfl_xor(s, 32, kWave);
+      if (row >= rows) continue;
+      if (g == 0) part[slice * rows + row] = float2{m, s};
+      const int at = targets.at(row) - col0;
+#pragma unroll
+      for (int j = 0; j < CB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (at == 16 * j + r) target_logit[row] = acc[i][j][r];
+    }
+  });
+}
+
+// lse and loss of each row from its pairs; 16 rows per workgroup, 16 threads a row, joined in a fixed order.
+__global__ __launch_bounds__(kThreads) void join_rows(const float2* __restrict__ part,
+                                                      const float* __restrict__ target_logit, Targets targets,
+                                                      float* __restrict__ lse, float* __restrict__ loss, int64_t rows,
+                                                      int slices) {
+  __shared__ float2 s[16][16];
+  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int64_t row = (int64_t)blockIdx.x * 16 + r;
+  float2 a{-__builtin_inff(), 0.f};
+  auto join = [](float2 a, float2 b) {
+    if (b.x == -__builtin_inff() && b.y == 0.f) return a;
+    if (a.x == -__builtin_inff() && a.y == 0.f) return b;
+    const float m = fmaxf(a.x, b.x);
+    return float2{m, a.y * expf(a.x - m) + b.y * expf(b.x - m)};
+  };
+  if (row < rows) {
+#pragma unroll 8
+    for (int k = q; k < slices; k += 16) a = join(a, part[(int64_t)k * rows + row]);
+  }
+  s[q][r] = a;
+  __syncthreads();
+  if (q != 0 || row >= rows) return;
+  for (int k = 1; k < 16; ++k) a = join(a, s[k][r]);
+  const float log_sum = logf(a.y);
+  lse[row] = a.x + log_sum;
+  loss[row] = targets.ignored(row) ? 0.f : targets.at(row) < 0 ? __builtin_nanf("") : (a.x - target_logit[row]) + log_sum;
+}
+
+__device__ __forceinline__ double block_sum(double v, double* s) {
+  for (int m = kWave / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
+  if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x / kWave] = v;
+  __syncthreads();
+  double t = s[0];
+  for (int w = 1; w < kOneBlock / kWave; ++w) t += s[w];
+  __syncthreads();
+  return t;
+}
+
+// total = the losses' sum (over the rows that count, with mean); counted = how many rows are not ignored.
+__global__ __launch_bounds__(kOneBlock) void add_losses(const float* __restrict__ loss, Targets targets, int64_t rows,
+                                                        bool mean, float* __restrict__ total, float* __restrict__ counted) {
+  __shared__ double s[kOneBlock / kWave];
+  double sum = 0, n = 0;
+  for (int64_t r = threadIdx.x; r < rows; r += kOneBlock) {
+    sum += loss[r];
+    n += targets.ignored(r) ? 0 : 1;
+  }
+  sum = block_sum(sum, s);
+  n = block_sum(n, s);
+  if (threadIdx.x == 0) {
+    *counted = (float)n;
+    if (total) *total = (float)(mean ? sum / n : sum);
+  }
+}
+
+// ----------------------------------------------------------------- backward
+// coef[row] = g_row times 2^k, k such that the largest finite |g| reaches 2^14 .. 2^15; *back = 2^-k. g: the
+// loss's gradient for the row (per row, or one for all, over the rows that count with mean); 0 where
+// ignored, NaN where the target is outside [0, V).
+__global__ __launch_bounds__(kOneBlock) void row_weights(const float* __restrict__ dout, bool per_row, bool mean,
+                                                         const float* __restrict__ counted, Targets targets,
+                                                         int64_t rows, float* __restrict__ coef,
+                                                         float* __restrict__ back) {
+  __shared__ float s[kOneBlock / kWave];
+  const float share = mean ? 1.f / *counted : 1.f;
+  auto weight = [&](int64_t r) {
+    if (targets.ignored(r)) return 0.f;
+    return targets.at(r) < 0 ? __builtin_nanf("") : dout[per_row ? r : 0] * share;
+  };
+  float top = 0.f;
+  for (int64_t r = threadIdx.x; r < rows; r += kOneBlock) {
+    const float a = fabsf(weight(r));
+    top = a <= 3.4028234663852886e38f ? fmaxf(top, a) : top;
+  }
+  for (int m = kWave / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
+  if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x / kWave] = top;
+  __syncthreads();
+  for (int w = 0; w < kOneBlock / kWave; ++w) top = fmaxf(top, s[w]);
+  int k = 0;
+  if (top > 0.f) {
+    frexpf(top, &k);  // top = f 2^k, f in [1/2, 1)
+    k = min(max(15 - k, -126), 126);
+  }
+  const float scale = ldexpf(1.f, k);
+  for (int64_t r = threadIdx.x; r < rows; r += kOneBlock) coef[r] = weight(r) * scale;
+  if (threadIdx.x == 0) *back = ldexpf(1.f, -k);
+}
+
+// dl [rows, ld] of the piece of the vocabulary that starts at v0 (w and its extent are the piece's): zero past it.
+template <int DT, int WM, int WN, int RB, int CB>
+__global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu * WM * WN / 4)) void logits_grad(
+    Operand x, Operand w, int64_t K, Tiles tiles, Targets targets, int v0, const float* __restrict__ lse,
+    const float* __restrict__ coef, uint16_t* __restrict__ dl, int64_t ld) {
+  using Tl = StreamTile<WM, WN, RB, CB>;
+  using El = Elem<DT>;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[Tl::kLds];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+  const int wr = wave / WN, wc = wave % WN;
+  stream_products<DT, false, false, WM, WN, RB, CB>(x, w, K, tiles, lds, [&](const TileAt& t, f32x4(&acc)[RB][CB]) {
+    const int col0 = (int)t.n0 + 16 * CB * wc + 4 * g;
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      const int64_t row = t.m0 + 16 * (RB * wr + i) + l16;
+      if (row >= x.extent) continue;
+      const float b = lse[row], c = coef[row];
+      const int at = targets.at(row) - v0 - col0;
+#pragma unroll
+      for (int j = 0; j < CB; ++j) {
+        float d[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - b) * kLog2e);
+          d[r] = (p - (at == 16 * j + r ? 1.f : 0.f)) * c;
+          d[r] = c == 0.f || col0 + 16 * j + r >= w.extent ? 0.f : d[r];
+        }
+        *reinterpret_cast<u32x2*>(dl + row * ld + col0 + 16 * j) = u32x2{El::pack2(d[0], d[1]), El::pack2(d[2], d[3])};
+      }
+    }
+  });
+}
+
+// out [M, N] = a b, times *back, rounded to T where the sum is whole (part NULL); else the sum's part into part [splits][M][N],
+// added to what it holds where `add`.
+template <int DT, bool TRA, int WM, int WN, int RB, int CB>
+__global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu * WM * WN / 4)) void grad_product(
+    Operand a, Operand b, int64_t sum, Tiles tiles, int64_t M, int N, const float* __restrict__ back,
+    uint16_t* __restrict__ out, float* __restrict__ part, bool add) {
+  using Tl = StreamTile<WM, WN, RB, CB>;
+  using El = Elem<DT>;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[Tl::kLds];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+  const int wr = wave / WN, wc = wave % WN;
+  const float scale = *back;
+  const bool aligned = ((uintptr_t)out & 7) == 0;
+  stream_products<DT, TRA, true, WM, WN, RB, CB>(a, b, sum, tiles, lds, [&](const TileAt& t, f32x4(&acc)[RB][CB]) {
+    const int col0 = (int)t.n0 + 16 * CB * wc + 4 * g;
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      const int64_t row = t.m0 + 16 * (RB * wr + i) + l16;
+      if (row >= M) continue;
+#pragma unroll
+      for (int j = 0; j < CB; ++j) {
+        const int col = col0 + 16 * j;
+        if (col >= N) continue;
+        if (part) {
+          f32x4* p = reinterpret_cast<f32x4*>(part + ((int64_t)t.split * M + row) * N + col);
+          *p = add ? *p + acc[i][j] : acc[i][j];
+        } else {
+          const f32x4 v = acc[i][j] * scale;
+          uint16_t* p = out + row * N + col;
+          if (aligned) {
+            *reinterpret_cast<u32x2*>(p) = u32x2{El::pack2(v[0], v[1]), El::pack2(v[2], v[3])};
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[r] = El::store(v[r]);
+          }
+        }
+      }
+    }
+  });
+}
+
+// out = T(*back times the parts' sum, in order); zero where there is none.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void add_parts(const float* __restrict__ part, int splits, int64_t n,
+                                                      const float* __restrict__ back, uint16_t* __restrict__ out) {
+  const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 s{0.f, 0.f, 0.f, 0.f};
+  if (splits) {
+    for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * n + i);
+    s *= *back;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) out[i + r] = Elem<DT>::store(s[r]);
+}
+
+// -------------------------------------------------------------------- plans
+template <typename Tl>
+Tiles tiles_of(int64_t M, int64_t N, int64_t sum, bool split) {
+  Tiles t{};
+  t.nrb = (int)ceil_div(M, Tl::kRows);
+  t.ncb = (int)ceil_div(N, Tl::kCols);
+  t.stages = (int)ceil_div(sum, kStage);
+  t.splits = 1;
+  const int64_t tiles = (int64_t)t.nrb * t.ncb, slots = 256 * Tl::kPerCu;
+  if (split && tiles < slots) {
+    const int64_t most = t.stages / kMinStages, want = slots / tiles;
+    t.splits = (int)(most < 1 ? 1 : want < most ? want : most);
+  }
+  t.per = (int)ceil_div(t.stages, t.splits);
+  t.splits = (int)ceil_div(t.stages, t.per);
+  t.total = (int)(tiles * t.splits);
+  return t;
+}
+// Time of the launch in stages of the large tile. The small one has a quarter of the work, two workgroups per CU
+// share it, and it takes 1.2 times as long for the same work (geglu_linear's measurement of the two).
+double cost(const Tiles& t, bool large) {
+  const int slots = 256 * (large ? Large::kPerCu : Small::kPerCu);
+  return (double)ceil_div(t.total, slots) * t.per * (large ? 1.0 : 0.6);
+}
+struct Plan {
+  bool large;
+  Tiles tiles;
+};
+Plan plan_product(int64_t M, int64_t N, int64_t sum, bool split) {
+  const Tiles l = tiles_of<Large>(M, N, sum, split), s = tiles_of<Small>(M, N, sum, split);
+  return cost(l, true) <= cost(s, false) ? Plan{true, l} : Plan{false, s};
+}
+
+// f(tile) with the plan's tile.
+template <int WM_, int WN_, int RB_, int CB_>
+struct Shape {
+  static constexpr int WM = WM_, WN = WN_, RB = RB_, CB = CB_;
+  using Tl = StreamTile<WM, WN, RB, CB>;
+};
+template <typename F>
+void with_tile(const Plan& p, F&& f) {
+  if (p.large)
+    f(Shape<2, 4, 8, 4>{});
+  else
+    f(Shape<2, 2, 4, 4>{});
+}
+
+struct Forward {
+  Plan plan;
+  int slices;
+  size_t part, target_logit, loss, bytes;
+};
+Forward plan_forward(int64_t rows, int K, int V) {
+  Forward f{};
+  f.plan = plan_product(rows, V, K, false);
+  f.slices = f.plan.tiles.ncb * (f.plan.large ? Large::kCols : Small::kCols) / 64;
+  size_t at = 0;
+  auto take = [&](size_t b) {
+    const size_t here = at;
+    at += align256(b);
+    return here;
+  };
+  f.part = take((size_t)f.slices * rows * sizeof(float2));
+  f.target_logit = take((size_t)rows * 4);
+  f.loss = take((size_t)rows * 4);
+  f.bytes = at;
+  return f;
+}
+
+struct Backward {
+  int width, pieces;  // columns of dl, a multiple of 256
+  Plan dx, dw;        // of a whole piece
+  size_t coef, back, dl, dx_part, dw_part, bytes;
+};
+Backward plan_backward(int64_t rows, int K, int V) {
+  Backward b{};
+  const int64_t cols = ceil_div(V, 256) * 256, fit = kPieceBytes / (rows * 2) / 256 * 256;
+  b.pieces = (int)ceil_div(cols, fit < 256 ? 256 : fit < kMaxWidth ? fit : kMaxWidth);
+  b.width = (int)(ceil_div(ceil_div(V, b.pieces), 256) * 256);
+  b.pieces = (int)ceil_div(V, b.width);
+  const int whole = V < b.width ? V : b.width;
+  b.dx = plan_product(rows, K, whole, true);
+  b.dw = plan_product(whole, K, rows, true);
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t here = at;
+    at += align256(n);
+    return here;
+  };
+  b.coef = take((size_t)rows * 4);
+  b.back = take(4);
+  b.dl = take((size_t)rows * b.width * 2);
+  b.dx_part = take(b.dx.tiles.splits > 1 || b.pieces > 1 ? (size_t)b.dx.tiles.splits * rows * K * 4 : 0);
+  b.dw_part = take(b.dw.tiles.splits > 1 ? (size_t)b.dw.tiles.splits * whole * K * 4 : 0);
+  b.bytes = at;
+  return b;
+}
+
+int check(int64_t rows, int32_t k, int32_t v, int32_t target_bytes, int32_t reduction, int32_t dtype) {
+  if (dtype != kBf16 && dtype != kF16) return KRSI_ERR_UNSUPPORTED;
+  if (target_bytes != 4 && target_bytes != 8) return KRSI_ERR_UNSUPPORTED;
+  if (reduction < 0 || reduction > 2) return KRSI_ERR_UNSUPPORTED;
+  if (rows < 0 || k <= 0 || v <= 0) return KRSI_ERR_BAD_SHAPE;
+  // Whole stages of K; byte offsets of a staged tile below 2^31, tile counts of int.
+  if (k % kStage != 0 || k > (1 << 20) || v > (1 << 24) || rows > (1 << 24)) return KRSI_ERR_UNSUPPORTED;
+  if (ceil_div(rows, 128) * ceil_div(v, 128) > (1 << 30) || ceil_div(rows, 128) * ceil_div(k, 128) > (1 << 20) ||
+      ceil_div(v, 128) * ceil_div(k, 128) > (1 << 30))
+    return KRSI_ERR_UNSUPPORTED;
+  return KRSI_OK;
+}
+
+template <int DT>
+int forward(const Operand& x, const Operand& w, int K, const Targets& t, float* loss, float* stats, char* ws,
+            int reduction, hipStream_t st) {
+  const int64_t rows = x.extent;
+  const Forward f = plan_forward(rows, K, (int)w.extent);
+  float2* part = (float2*)(ws + f.part);
+  float* target_logit = (float*)(ws + f.target_logit);
+  float* row_loss = reduction == 0 ? loss : (float*)(ws + f.loss);
+  with_tile(f.plan, [&](auto s) {
+    using S = decltype(s);
+    hipLaunchKernelGGL((logits_reduce<DT, S::WM, S::WN, S::RB, S::CB>), dim3(stream_grid<typename S::Tl>(f.plan.tiles)),
+                       dim3(S::Tl::kThreads), 0, st, x, w, (int64_t)K, f.plan.tiles, t, part, target_logit);
+  });
+  hipLaunchKernelGGL(join_rows, dim3((unsigned)ceil_div(rows, 16)), dim3(kThreads), 0, st, (const float2*)part,
+                     (const float*)target_logit, t, stats, row_loss, rows, f.slices);
+  if (reduction != 0)
+    hipLaunchKernelGGL(add_losses, dim3(1), dim3(kOneBlock), 0, st, (const float*)row_loss, t, rows, reduction == 1, loss,
+                       stats + rows);
+  return launch_status();
+}
+
+template <int DT>
+int backward(const float* dout, const Operand& x, const Operand& w, int K, const Targets& t, const float* stats,
+             uint16_t* dx, uint16_t* dw, char* ws, int reduction, hipStream_t st) {
+  const int64_t rows = x.extent;
+  const int V = (int)w.extent;
+  const Backward b = plan_backward(rows, K, V);
+  float *coef = (float*)(ws + b.coef), *back = (float*)(ws + b.back);
+  uint16_t* dl = (uint16_t*)(ws + b.dl);
+  hipLaunchKernelGGL(row_weights, dim3(1), dim3(kOneBlock), 0, st, dout, reduction == 0, reduction == 1, stats + rows, t,
+                     rows, coef, back);
+  const bool dx_parts = b.dx.tiles.splits > 1 || b.pieces > 1;
+  float* dx_part = dx_parts ? (float*)(ws + b.dx_part) : nullptr;
+  for (int p = 0; p < b.pieces; ++p) {
+    const int v0 = p * b.width, valid = V - v0 < b.width ? V - v0 : b.width;
+    const Operand piece{w.p + (int64_t)v0 * K, K, valid};
+    const Plan lg = plan_product(rows, b.width, K, false);
+    with_tile(lg, [&](auto s) {
+      using S = decltype(s);
+      hipLaunchKernelGGL((logits_grad<DT, S::WM, S::WN, S::RB, S::CB>), dim3(stream_grid<typename S::Tl>(lg.tiles)),
+                         dim3(S::Tl::kThreads), 0, st, x, piece, (int64_t)K, lg.tiles, t, v0, stats, (const float*)coef, dl,
+                         (int64_t)b.width);
+    });
+    if (dx) {
+      // The last piece may be shorter: fewer parts, added to those of the pieces before.
+      Plan pl = b.dx;
+      pl.tiles.stages = (int)ceil_div(valid, kStage);
+      pl.tiles.per = pl.tiles.per < pl.tiles.stages ? pl.tiles.per : pl.tiles.stages;
+      pl.tiles.splits = (int)ceil_div(pl.tiles.stages, pl.tiles.per);
+      pl.tiles.total = pl.tiles.nrb * pl.tiles.ncb * pl.tiles.splits;
+      with_tile(pl, [&](auto s) {
+        using S = decltype(s);
+        hipLaunchKernelGGL((grad_product<DT, false, S::WM, S::WN, S::RB, S::CB>),
+                           dim3(stream_grid<typename S::Tl>(pl.tiles)), dim3(S::Tl::kThreads), 0, st,
+                           Operand{dl, b.width, rows}, Operand{piece.p, K, K}, (int64_t)valid, pl.tiles, rows, K,
+                           (const float*)back, dx, dx_part, p > 0);
+      });
+    }
+    if (dw) {
+      Plan pl = b.dw;
+      pl.tiles.nrb = (int)ceil_div(valid, pl.large ? Large::kRows : Small::kRows);
+      pl.tiles.total = pl.tiles.nrb * pl.tiles.ncb * pl.tiles.splits;
+      const bool parts = pl.tiles.splits > 1;
+      float* dw_part = parts ? (float*)(ws + b.dw_part) : nullptr;
+      uint16_t* out = dw + (int64_t)v0 * K;
+      with_tile(pl, [&](auto s) {
+        using S = decltype(s);
+        hipLaunchKernelGGL((grad_product<DT, true, S::WM, S::WN, S::RB, S::CB>),
+                           dim3(stream_grid<typename S::Tl>(pl.tiles)), dim3(S::Tl::kThreads), 0, st,
+                           Operand{dl, b.width, b.width}, Operand{x.p, K, K}, rows, pl.tiles, (int64_t)valid, K,
+                           (const float*)back, out, dw_part, false);
+      });
+      if (parts)
+        hipLaunchKernelGGL((add_parts<DT>), dim3((unsigned)ceil_div((int64_t)valid * K, 4 * kThreads)), dim3(kThreads), 0,
+                           st, (const float*)dw_part, pl.tiles.splits, (int64_t)valid * K, (const float*)back, out);
+    }
+  }
+  if (dx && dx_parts)
+    hipLaunchKernelGGL((add_parts<DT>), dim3((unsigned)ceil_div(rows * K, 4 * kThreads)), dim3(kThreads), 0, st,
+                       (const float*)dx_part, b.dx.tiles.splits, rows * K, (const float*)back, dx);
+  return launch_status();
+}
+
+// No rows: the loss of none is 0, its mean NaN; dw is zero.
+__global__ void loss_of_none(float* loss, float* counted, bool mean) {
+  *loss = mean ? __builtin_nanf("") : 0.f;
+  *counted = 0.f;
+}
+
+}  // namespace
+}  // namespace krsi
+
+extern "C" {
+
+size_t krsi_linear_cross_entropy_fwd_workspace_bytes(int64_t rows, int32_t k, int32_t v) {
+  using namespace krsi;
+  return rows > 0 && check(rows, k, v, 8, 0, kBf16) == KRSI_OK ? plan_forward(rows, k, v).bytes : 0;
+}
+
+size_t krsi_linear_cross_entropy_bwd_workspace_bytes(int64_t rows, int32_t k, int32_t v) {
+  using namespace krsi;
+  return rows > 0 && check(rows, k, v, 8, 0, kBf16) == KRSI_OK ? plan_backward(rows, k, v).bytes : 0;
+}
+
+int krsi_linear_cross_entropy_fwd(const void* x, const void* w, const void* targets, int32_t target_bytes, float* loss,
+                                  float* stats, void* workspace, size_t workspace_bytes, int64_t rows, int32_t k,
+                                  int32_t v, int64_t ignore_index, int32_t reduction, int32_t dtype, void* stream) {
+  using namespace krsi;
+  const int rc = check(rows, k, v, target_bytes, reduction, dtype);
+  if (rc != KRSI_OK) return rc;
+  if (rows == 0) {
+    if (reduction == 0) return KRSI_OK;
+    if (!loss || !stats) return KRSI_ERR_NULL_POINTER;
+    hipLaunchKernelGGL(loss_of_none, dim3(1), dim3(1), 0, as_stream(stream), loss, stats, reduction == 1);
+    return launch_status();
+  }
+  if (!x || !w || !targets || !loss || !stats) return KRSI_ERR_NULL_POINTER;
+  if (!aligned16(x) || !aligned16(w)) return KRSI_ERR_MISALIGNED;
+  if (!workspace || workspace_bytes < krsi_linear_cross_entropy_fwd_workspace_bytes(rows, k, v))
+    return KRSI_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
+  const Operand xo{(const uint16_t*)x, k, rows}, wo{(const uint16_t*)w, k, v};
+  const Targets t{targets, target_bytes, v, ignore_index};
+  return dtype == kF16 ? forward<kF16>(xo, wo, k, t, loss, stats, (char*)workspace, reduction, as_stream(stream))
+                       : forward<kBf16>(xo, wo, k, t, loss, stats, (char*)workspace, reduction, as_stream(stream));
+}
+
+int krsi_linear_cross_entropy_bwd(const float* dout, const void* x, const void* w, const void* targets,
+                                  int32_t target_bytes, const float* stats, void* dx, void* dw, void* workspace,
+                                  size_t workspace_bytes, int64_t rows, int32_t k, int32_t v, int64_t ignore_index,
+                                  int32_t reduction, int32_t dtype, void* stream) {
+  using namespace krsi;
+  const int rc = check(rows, k, v, target_bytes, reduction, dtype);
+  if (rc != KRSI_OK) return rc;
+  hipStream_t st = as_stream(stream);
+  if (rows == 0) {
+    if (!dw) return KRSI_OK;
+    hipLaunchKernelGGL((add_parts<kBf16>), dim3((unsigned)ceil_div((int64_t)v * k, 4 * kThreads)), dim3(kThreads), 0, st,
+                       (const float*)nullptr, 0, (int64_t)v * k, (const float*)nullptr, (uint16_t*)dw);
+    return launch_status();
+  }
+  if (!dout || !x || !w || !targets || !stats || (!dx && !dw)) return KRSI_ERR_NULL_POINTER;
+  if (!aligned16(x) || !aligned16(w)) return KRSI_ERR_MISALIGNED;
+  if (!workspace || workspace_bytes < krsi_linear_cross_entropy_bwd_workspace_bytes(rows, k, v))
+    return KRSI_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
+  const Operand xo{(const uint16_t*)x, k, rows}, wo{(const uint16_t*)w, k, v};
+  const Targets t{targets, target_bytes, v, ignore_index};
+  return dtype == kF16 ? backward<kF16>(dout, xo, wo, k, t, stats, (uint16_t*)dx, (uint16_t*)dw, (char*)workspace,
+                                        reduction, st)
+                       : backward<kBf16>(dout, xo, wo, k, t, stats, (uint16_t*)dx, (uint16_t*)dw, (char*)workspace,
+                                         reduction, st);
+}
+
+}  // extern "C"

@@ -75,6 +75,12 @@ SIGNATURES = {
                                              _I32, _I32, _I32, _I64, _I32, _F32, _I32, _I32, _P]),
     "krsi_embedding_fwd": (ctypes.c_int, [_P, _I32, _P, _P, _I64, _I32, _I32, _F32, _I32, _P]),
     "krsi_embedding_bwd_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "krsi_linear_cross_entropy_fwd_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "krsi_linear_cross_entropy_bwd_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "krsi_linear_cross_entropy_fwd": (ctypes.c_int, [_P, _P, _P, _I32, _P, _P, _P, _SZ, _I64, _I32, _I32, _I64, _I32,
+                                                     _I32, _P]),
+    "krsi_linear_cross_entropy_bwd": (ctypes.c_int, [_P, _P, _P, _P, _I32, _P, _P, _P, _P, _SZ, _I64, _I32, _I32, _I64,
+                                                     _I32, _I32, _P]),
     "krsi_embedding_bwd": (ctypes.c_int, [_P, _P, _I32, _P, _P, _SZ, _I64, _I32, _I32, _I64, _F32, _I32, _P]),
 }
 
@@ -603,3 +609,71 @@ def embedding_bwd(dout: torch.Tensor, tokens: torch.Tensor, V: int, scale: float
     _check(lib().krsi_embedding_bwd(_ptr(dout), _ptr(tokens), tokens.element_size(), _ptr(dtable), _ptr(ws), nbytes, n, V,
                                     D, padding_idx, float(scale), dt, _stream(dout)))
     return dtable
+
+
+# ----------------------------------- cross entropy of an output projection
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _check_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, reduction: str) -> int:
+    _on_gpu(x, w, targets)
+    dt = _dtype("x", x, allowed=(torch.bfloat16, torch.float16))
+    _dtype("weight", w, like=x)
+    _index_bytes("targets", targets)
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    if x.dim() != 2 or w.dim() != 2 or w.shape[1] != x.shape[1] or w.shape[0] < 1:
+        raise ValueError(f"need x [rows, K] and w [V, K], got {tuple(x.shape)} and {tuple(w.shape)}")
+    if x.shape[1] % 64 or not x.shape[1]:
+        raise ValueError(f"linear_cross_entropy needs K a multiple of 64, got K={x.shape[1]}")
+    if targets.shape != x.shape[:1]:
+        raise ValueError(f"targets shape {tuple(targets.shape)} != {tuple(x.shape[:1])}")
+    return dt
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous, on a 16-byte boundary: itself or a copy."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+@_on_device
+def linear_cross_entropy_fwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore_index: int,
+                             reduction: str) -> tuple[torch.Tensor, torch.Tensor]:
+    """The loss (fp32, [rows] or a scalar) and the statistics that the backward reads, [rows + 1]."""
+    dt = _check_cross_entropy(x, w, targets, reduction)
+    x, w, targets = _aligned(x), _aligned(w), targets.contiguous()
+    (rows, k), v = x.shape, w.shape[0]
+    loss = torch.empty((rows,) if reduction == "none" else (), device=x.device, dtype=torch.float32)
+    stats = torch.empty(rows + 1, device=x.device, dtype=torch.float32)
+    nbytes = lib().krsi_linear_cross_entropy_fwd_workspace_bytes(rows, k, v)
+    ws = torch.empty(max(nbytes, 1), device=x.device, dtype=torch.uint8)
+    _check(lib().krsi_linear_cross_entropy_fwd(_ptr(x), _ptr(w), _ptr(targets), targets.element_size(), _ptr(loss),
+                                               _ptr(stats), _ptr(ws), nbytes, rows, k, v, ignore_index,
+                                               REDUCTIONS[reduction], dt, _stream(x)))
+    return loss, stats
+
+
+@_on_device
+def linear_cross_entropy_bwd(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
+                             stats: torch.Tensor, ignore_index: int, reduction: str, dx: bool = True,
+                             dw: bool = True) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """dx [rows, K] and dw [V, K]; None for the one that is not wanted."""
+    dt = _check_cross_entropy(x, w, targets, reduction)
+    _on_gpu(x, dout, stats)
+    (rows, k), v = x.shape, w.shape[0]
+    if dout.dtype != torch.float32 or dout.numel() != (rows if reduction == "none" else 1):
+        raise ValueError(f"grad {dout.dtype} {tuple(dout.shape)} does not fit the loss")
+    if stats.dtype != torch.float32 or stats.shape != (rows + 1,):
+        raise ValueError(f"stats {stats.dtype} {tuple(stats.shape)} are not those of {rows} rows")
+    dout, stats = dout.contiguous(), stats.contiguous()
+    x, w, targets = _aligned(x), _aligned(w), targets.contiguous()
+    gx = torch.empty_like(x) if dx else None
+    gw = torch.empty_like(w) if dw else None
+    if dx or dw:
+        nbytes = lib().krsi_linear_cross_entropy_bwd_workspace_bytes(rows, k, v)
+        ws = torch.empty(max(nbytes, 1), device=x.device, dtype=torch.uint8)
+        _check(lib().krsi_linear_cross_entropy_bwd(_ptr(dout), _ptr(x), _ptr(w), _ptr(targets), targets.element_size(),
+                                                   _ptr(stats), _ptr(gx), _ptr(gw), _ptr(ws), nbytes, rows, k, v,
+                                                   ignore_index, REDUCTIONS[reduction], dt, _stream(x)))
+    return gx, gw

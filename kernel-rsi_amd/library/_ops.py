@@ -7,8 +7,8 @@ replay.py's per-file module names) does not register the ops twice.
 Op names follow the reference (library/rmsnorm.py:86-103, geglu.py:85-101,
 relpos_attention.py:175-195): krsi::rmsnorm_fwd/bwd, krsi::geglu_fwd/bwd,
 krsi::relpos_attn_fwd/bwd; krsi::relpos_bucket_gather/sum (the T5 table step) and
-krsi::geglu_linear_fwd (the merged projection with the GEGLU epilogue), krsi::qk_norm_rope_fwd/bwd and
-krsi::embedding_fwd/bwd have no counterpart there. Their schemas are internal to this library.
+krsi::geglu_linear_fwd (the merged projection with the GEGLU epilogue), krsi::qk_norm_rope_fwd/bwd,
+krsi::embedding_fwd/bwd and krsi::linear_cross_entropy_fwd/bwd have no counterpart there. Their schemas are internal to this library.
 """
 from __future__ import annotations
 
@@ -271,3 +271,41 @@ def _embedding_backward(ctx, dout):
 
 
 embedding_fwd_op.register_autograd(_embedding_backward, setup_context=_embedding_setup)
+
+# ----------------------------------- cross entropy of an output projection
+
+
+@torch.library.custom_op("krsi::linear_cross_entropy_fwd", mutates_args=())
+def linear_cross_entropy_fwd_op(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int,
+                                reduction: str) -> tuple[Tensor, Tensor]:
+    return _hip.linear_cross_entropy_fwd(x, w, targets, ignore_index, reduction)
+
+
+@linear_cross_entropy_fwd_op.register_fake
+def _(x, w, targets, ignore_index, reduction):
+    rows = x.shape[0]
+    return (x.new_empty((rows,) if reduction == "none" else (), dtype=torch.float32),
+            x.new_empty((rows + 1,), dtype=torch.float32))
+
+
+@torch.library.custom_op("krsi::linear_cross_entropy_bwd", mutates_args=())
+def linear_cross_entropy_bwd_op(dout: Tensor, x: Tensor, w: Tensor, targets: Tensor, stats: Tensor, ignore_index: int,
+                                reduction: str) -> tuple[Tensor, Tensor]:
+    return _hip.linear_cross_entropy_bwd(dout, x, w, targets, stats, ignore_index, reduction)
+
+
+@linear_cross_entropy_bwd_op.register_fake
+def _(dout, x, w, targets, stats, ignore_index, reduction):
+    return x.new_empty(x.shape), w.new_empty(w.shape)
+
+
+def _loss_setup(ctx, inputs, output):
+    x, w, targets, *ctx.args = inputs
+    ctx.save_for_backward(x, w, targets, output[1])
+
+
+def _loss_backward(ctx, dout, _dstats):
+    return (*linear_cross_entropy_bwd_op(dout.contiguous(), *ctx.saved_tensors, *ctx.args), None, None, None)
+
+
+linear_cross_entropy_fwd_op.register_autograd(_loss_backward, setup_context=_loss_setup)

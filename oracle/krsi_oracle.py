@@ -421,3 +421,26 @@ def embedding_grad_64(dout, tokens, V, scale, padding_idx=None):
     zero = torch.zeros(V, g.shape[1], dtype=torch.float64)
     return (zero.index_add(0, tok, g) * scale, zero.index_add(0, tok, g.abs()) * abs(scale),
             torch.bincount(tok, minlength=V)[:, None])
+
+
+# ----------------------------------- cross entropy of an output projection
+def linear_cross_entropy_64(x, w, targets, dout, ignore_index=-100, reduction="mean"):
+    """In float64, on the inputs' device: a dict of loss, dx, dw (the closed form dl = (softmax - onehot) g, dx = dl w,
+    dw = dl^T x) and of what bounds on them take: terms = max_v sum |x||w| of each row, lse, g of each row,
+    and |dl||w|, g p |w|, |dl|^T|x|, (g p)^T|x|. Targets are in range or ignore_index."""
+    x, w, targets = x.double(), w.double(), targets.long()
+    logits = x @ w.t()
+    lse = torch.logsumexp(logits, 1)
+    kept = targets != ignore_index
+    at = torch.where(kept, targets, 0)
+    loss = torch.where(kept, lse - logits.gather(1, at[:, None])[:, 0], 0.0)
+    share = 1.0 / kept.sum() if reduction == "mean" else 1.0
+    g = torch.where(kept, dout.double() * share, 0.0)[:, None]
+    gp = (logits - lse[:, None]).exp() * g
+    dl = gp.clone()
+    dl[torch.arange(len(at)), at] -= g[:, 0]
+    del logits
+    return {"loss": loss if reduction == "none" else loss.sum() * share, "dx": dl @ w, "dw": dl.t() @ x,
+            "terms": (x.abs() @ w.abs().t()).max(1).values, "lse": lse, "g": g[:, 0], "share": share,
+            "dx_mag": dl.abs() @ w.abs(), "dw_mag": dl.abs().t() @ x.abs(),
+            "dx_p": gp.abs() @ w.abs(), "dw_p": gp.abs().t() @ x.abs()}

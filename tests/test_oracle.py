@@ -372,3 +372,27 @@ def test_embedding_gradient_closed_form():
     want[3] = 2 * (dout[0, 0].double() + dout[0, 2].double())
     want[0] = 2 * dout[0, 1].double()
     assert torch.equal(got, want) and count[:, 0].tolist() == [1, 0, 0, 2, 0, 0, 0]
+
+
+# ----------------------------------- cross entropy of an output projection
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_linear_cross_entropy_closed_form(reduction):
+    """Against torch's own cross entropy in float64, and the gradient against central differences of it."""
+    g = torch.Generator().manual_seed(3)
+    x, w = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((6, 5), (9, 5)))
+    targets = torch.tensor([0, 8, -100, 3, 3, -100])
+    dout = torch.randn(6, generator=g, dtype=torch.float64) if reduction == "none" else torch.tensor(0.7)
+    got = O.linear_cross_entropy_64(x, w, targets, dout, reduction=reduction)
+
+    def loss(a, b):
+        return torch.nn.functional.cross_entropy(a @ b.t(), targets, reduction=reduction)
+
+    assert torch.allclose(got["loss"], loss(x, w), rtol=1e-12, atol=1e-14)
+    for name, i in (("dx", 0), ("dw", 1)):
+        for at in range(0, (x, w)[i].numel(), 2):
+            sides = []
+            for step in (1e-5, -1e-5):
+                moved = [x.clone(), w.clone()]
+                moved[i].view(-1)[at] += step
+                sides.append((loss(*moved) * dout).sum())
+            assert abs((sides[0] - sides[1]) / 2e-5 - got[name].view(-1)[at]) < 1e-8
