@@ -6,6 +6,8 @@
 // registers, and keeps the target's logit; a second launch joins a row's pairs, a third adds the losses.
 // Backward, in pieces of the vocabulary (kPieceBytes of dl each): the products again, whose epilogue forms dl, rounded
 // to T; then dw of the piece's rows and the piece's part of dx, which is carried in fp32 from piece to piece.
+// What dl's rounding takes from the target's entry, the largest of a row, is kept in fp32 per row (its rest) and
+// comes back into dx: with it dx is off by 1.1 roundings of its own type where it was by 1.5.
 // dl is held times a power of two that puts the largest |g| at 2^14..2^15: fp16 then keeps probabilities down to
 // 2^-29 in full precision, and the scale comes off exactly where dx and dw are rounded.
 //
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(kOneBlock) void add_losses(const float* __restrict_
 __global__ __launch_bounds__(kOneBlock) void row_weights(const float* __restrict__ dout, bool per_row, bool mean,
                                                          const float* __restrict__ counted, Targets targets,
                                                          int64_t rows, float* __restrict__ coef,
-                                                         float* __restrict__ back) {
+                                                         float* __restrict__ rest, float* __restrict__ back) {
   __shared__ float s[kOneBlock / kWave];
   const float share = mean ? 1.f / *counted : 1.f;
   auto weight = [&](int64_t r) {
@@ -171,7 +173,10 @@ __global__ __launch_bounds__(kOneBlock) void row_weights(const float* __restrict
     k = min(max(15 - k, -126), 126);
   }
   const float scale = ldexpf(1.f, k);
-  for (int64_t r = threadIdx.x; r < rows; r += kOneBlock) coef[r] = weight(r) * scale;
+  for (int64_t r = threadIdx.x; r < rows; r += kOneBlock) {
+    coef[r] = weight(r) * scale;
+    rest[r] = 0.f;
+  }
   if (threadIdx.x == 0) *back = ldexpf(1.f, -k);
 }
 
@@ -179,7 +184,7 @@ __global__ __launch_bounds__(kOneBlock) void row_weights(const float* __restrict
 template <int DT, int WM, int WN, int RB, int CB>
 __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu * WM * WN / 4)) void logits_grad(
     Operand x, Operand w, int64_t K, Tiles tiles, Targets targets, int v0, const float* __restrict__ lse,
-    const float* __restrict__ coef, uint16_t* __restrict__ dl, int64_t ld) {
+    const float* __restrict__ coef, float* __restrict__ rest, uint16_t* __restrict__ dl, int64_t ld) {
   using Tl = StreamTile<WM, WN, RB, CB>;
   using El = Elem<DT>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[Tl::kLds];
@@ -201,6 +206,7 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
           const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - b) * kLog2e);
           d[r] = (p - (at == 16 * j + r ? 1.f : 0.f)) * c;
           d[r] = c == 0.f || col0 + 16 * j + r >= w.extent ? 0.f : d[r];
+          if (at == 16 * j + r) rest[row] = d[r] - El::round(d[r]);
         }
         *reinterpret_cast<u32x2*>(dl + row * ld + col0 + 16 * j) = u32x2{El::pack2(d[0], d[1]), El::pack2(d[2], d[3])};
       }
@@ -208,11 +214,29 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
   });
 }
 
+// What comes back into dx: row n's rest times w[target(n)], in the units of dl.
+struct Rest {
+  const float* rest;   // NULL: none (dw)
+  const uint16_t* w;
+  Targets targets;
+  template <int DT>
+  __device__ __forceinline__ f32x4 at(int64_t row, int N, int col) const {
+    const int t = targets.at(row);
+    f32x4 v{0.f, 0.f, 0.f, 0.f};
+    if (t < 0) return v;
+    const u32x2 raw = *reinterpret_cast<const u32x2*>(w + (int64_t)t * N + col);
+    const float e = rest[row];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = e * Elem<DT>::load((uint16_t)(raw[r / 2] >> (16 * (r % 2))));
+    return v;
+  }
+};
+
 // out [M, N] = a b, times *back, rounded to T where the sum is whole (part NULL); else the sum's part into part [splits][M][N],
 // added to what it holds where `add`.
 template <int DT, bool TRA, int WM, int WN, int RB, int CB>
 __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu * WM * WN / 4)) void grad_product(
-    Operand a, Operand b, int64_t sum, Tiles tiles, int64_t M, int N, const float* __restrict__ back,
+    Operand a, Operand b, int64_t sum, Tiles tiles, int64_t M, int N, const float* __restrict__ back, Rest rest,
     uint16_t* __restrict__ out, float* __restrict__ part, bool add) {
   using Tl = StreamTile<WM, WN, RB, CB>;
   using El = Elem<DT>;
@@ -235,7 +259,9 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
           f32x4* p = reinterpret_cast<f32x4*>(part + ((int64_t)t.split * M + row) * N + col);
           *p = add ? *p + acc[i][j] : acc[i][j];
         } else {
-          const f32x4 v = acc[i][j] * scale;
+          f32x4 v = acc[i][j];
+          if (!TRA) v += rest.at<DT>(row, N, col);
+          v *= scale;
           uint16_t* p = out + row * N + col;
           if (aligned) {
             *reinterpret_cast<u32x2*>(p) = u32x2{El::pack2(v[0], v[1]), El::pack2(v[2], v[3])};
@@ -249,17 +275,18 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
   });
 }
 
-// out = T(*back times the parts' sum, in order); zero where there is none.
+// out [M, N] = T(*back times the parts' sum, in order, and the rest); zero where there is none. blockIdx.x: row.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void add_parts(const float* __restrict__ part, int splits, int64_t n,
-                                                      const float* __restrict__ back, uint16_t* __restrict__ out) {
-  const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
-  if (i >= n) return;
+__global__ __launch_bounds__(kThreads) void add_parts(const float* __restrict__ part, int splits, int64_t M, int N,
+                                                      const float* __restrict__ back, Rest rest,
+                                                      uint16_t* __restrict__ out) {
+  const int col = (blockIdx.y * kThreads + threadIdx.x) * 4;
+  if (col >= N) return;
+  const int64_t row = blockIdx.x, i = row * N + col;
   f32x4 s{0.f, 0.f, 0.f, 0.f};
-  if (splits) {
-    for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * n + i);
-    s *= *back;
-  }
+  for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * M * N + i);
+  if (rest.rest) s += rest.at<DT>(row, N, col);
+  if (splits) s *= *back;
 #pragma unroll
   for (int r = 0; r < 4; ++r) out[i + r] = Elem<DT>::store(s[r]);
 }
@@ -336,7 +363,7 @@ Forward plan_forward(int64_t rows, int K, int V) {
 struct Backward {
   int width, pieces;  // columns of dl, a multiple of 256
   Plan dx, dw;        // of a whole piece
-  size_t coef, back, dl, dx_part, dw_part, bytes;
+  size_t coef, rest, back, dl, dx_part, dw_part, bytes;
 };
 Backward plan_backward(int64_t rows, int K, int V) {
   Backward b{};
@@ -354,6 +381,7 @@ Backward plan_backward(int64_t rows, int K, int V) {
     return here;
   };
   b.coef = take((size_t)rows * 4);
+  b.rest = take((size_t)rows * 4);
   b.back = take(4);
   b.dl = take((size_t)rows * b.width * 2);
   b.dx_part = take(b.dx.tiles.splits > 1 || b.pieces > 1 ? (size_t)b.dx.tiles.splits * rows * K * 4 : 0);
@@ -402,10 +430,11 @@ int backward(const float* dout, const Operand& x, const Operand& w, int K, const
   const int64_t rows = x.extent;
   const int V = (int)w.extent;
   const Backward b = plan_backward(rows, K, V);
-  float *coef = (float*)(ws + b.coef), *back = (float*)(ws + b.back);
+  float *coef = (float*)(ws + b.coef), *rest = (float*)(ws + b.rest), *back = (float*)(ws + b.back);
+  const Rest to_dx{rest, w.p, t}, to_dw{nullptr, nullptr, t};
   uint16_t* dl = (uint16_t*)(ws + b.dl);
   hipLaunchKernelGGL(row_weights, dim3(1), dim3(kOneBlock), 0, st, dout, reduction == 0, reduction == 1, stats + rows, t,
-                     rows, coef, back);
+                     rows, coef, rest, back);
   const bool dx_parts = b.dx.tiles.splits > 1 || b.pieces > 1;
   float* dx_part = dx_parts ? (float*)(ws + b.dx_part) : nullptr;
   for (int p = 0; p < b.pieces; ++p) {
@@ -415,7 +444,7 @@ int backward(const float* dout, const Operand& x, const Operand& w, int K, const
     with_tile(lg, [&](auto s) {
       using S = decltype(s);
       hipLaunchKernelGGL((logits_grad<DT, S::WM, S::WN, S::RB, S::CB>), dim3(stream_grid<typename S::Tl>(lg.tiles)),
-                         dim3(S::Tl::kThreads), 0, st, x, piece, (int64_t)K, lg.tiles, t, v0, stats, (const float*)coef, dl,
+                         dim3(S::Tl::kThreads), 0, st, x, piece, (int64_t)K, lg.tiles, t, v0, stats, (const float*)coef, rest, dl,
                          (int64_t)b.width);
     });
     if (dx) {
@@ -430,7 +459,7 @@ int backward(const float* dout, const Operand& x, const Operand& w, int K, const
         hipLaunchKernelGGL((grad_product<DT, false, S::WM, S::WN, S::RB, S::CB>),
                            dim3(stream_grid<typename S::Tl>(pl.tiles)), dim3(S::Tl::kThreads), 0, st,
                            Operand{dl, b.width, rows}, Operand{piece.p, K, K}, (int64_t)valid, pl.tiles, rows, K,
-                           (const float*)back, dx, dx_part, p > 0);
+                           (const float*)back, to_dx, dx, dx_part, p > 0);
       });
     }
     if (dw) {
@@ -445,16 +474,16 @@ int backward(const float* dout, const Operand& x, const Operand& w, int K, const
         hipLaunchKernelGGL((grad_product<DT, true, S::WM, S::WN, S::RB, S::CB>),
                            dim3(stream_grid<typename S::Tl>(pl.tiles)), dim3(S::Tl::kThreads), 0, st,
                            Operand{dl, b.width, b.width}, Operand{x.p, K, K}, rows, pl.tiles, (int64_t)valid, K,
-                           (const float*)back, out, dw_part, false);
+                           (const float*)back, to_dw, out, dw_part, false);
       });
       if (parts)
-        hipLaunchKernelGGL((add_parts<DT>), dim3((unsigned)ceil_div((int64_t)valid * K, 4 * kThreads)), dim3(kThreads), 0,
-                           st, (const float*)dw_part, pl.tiles.splits, (int64_t)valid * K, (const float*)back, out);
+        hipLaunchKernelGGL((add_parts<DT>), dim3((unsigned)valid, (unsigned)ceil_div(K, 4 * kThreads)), dim3(kThreads), 0,
+                           st, (const float*)dw_part, pl.tiles.splits, (int64_t)valid, K, (const float*)back, to_dw, out);
     }
   }
   if (dx && dx_parts)
-    hipLaunchKernelGGL((add_parts<DT>), dim3((unsigned)ceil_div(rows * K, 4 * kThreads)), dim3(kThreads), 0, st,
-                       (const float*)dx_part, b.dx.tiles.splits, rows * K, (const float*)back, dx);
+    hipLaunchKernelGGL((add_parts<DT>), dim3((unsigned)rows, (unsigned)ceil_div(K, 4 * kThreads)), dim3(kThreads), 0, st,
+                       (const float*)dx_part, b.dx.tiles.splits, rows, K, (const float*)back, to_dx, dx);
   return launch_status();
 }
 
@@ -512,8 +541,8 @@ int krsi_linear_cross_entropy_bwd(const float* dout, const void* x, const void* 
   hipStream_t st = as_stream(stream);
   if (rows == 0) {
     if (!dw) return KRSI_OK;
-    hipLaunchKernelGGL((add_parts<kBf16>), dim3((unsigned)ceil_div((int64_t)v * k, 4 * kThreads)), dim3(kThreads), 0, st,
-                       (const float*)nullptr, 0, (int64_t)v * k, (const float*)nullptr, (uint16_t*)dw);
+    hipLaunchKernelGGL((add_parts<kBf16>), dim3((unsigned)v, (unsigned)ceil_div(k, 4 * kThreads)), dim3(kThreads), 0, st,
+                       (const float*)nullptr, 0, (int64_t)v, (int)k, (const float*)nullptr, Rest{}, (uint16_t*)dw);
     return launch_status();
   }
   if (!dout || !x || !w || !targets || !stats || (!dx && !dw)) return KRSI_ERR_NULL_POINTER;

@@ -292,6 +292,156 @@ struct BucketFn : torch::autograd::Function<BucketFn> {
   }
 };
 
+// ------------------------------------------- query and key norm with rotation
+// Each launch below goes to its tensors' device, which need not be the current one.
+struct QkArgs {
+  int64_t tokens;
+  int S, H, KH, D, R;
+  int64_t table_rows, ld;
+  int position_bytes;
+  QkArgs(const std::vector<int64_t>& d, const Tensor& qkv, const Tensor& rope, const Tensor& positions)
+      : tokens(d[0]), S((int)d[1]), H((int)d[2]), KH((int)d[3]), D((int)d[4]), R((int)rope.size(1)),
+        table_rows(rope.size(0)), ld(qkv.size(0) > 1 ? qkv.stride(0) : qkv.size(1)),
+        position_bytes(positions.defined() ? (int)positions.element_size() : 0) {}
+};
+const void* data_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct QkNormRopeFn : torch::autograd::Function<QkNormRopeFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& wq, const Tensor& wk, const Tensor& rope,
+                        const std::optional<Tensor>& given, int64_t tokens, int64_t S, int64_t H, int64_t KH, int64_t D,
+                        double eps, int64_t interleaved) {
+    const c10::DeviceGuard guard(qkv.device());
+    const Tensor positions = given ? *given : Tensor();
+    const std::vector<int64_t> dims{tokens, S, H, KH, D, interleaved};
+    const QkArgs a(dims, qkv, rope, positions);
+    Tensor out = at::empty({tokens, (H + 2 * KH) * D}, qkv.options());
+    forward_status(krsi_qk_norm_rope_fwd(qkv.data_ptr(), a.ld, wq.data_ptr(), wk.data_ptr(), rope.data_ptr<float>(),
+                                         data_or_null(positions), out.data_ptr(), tokens, a.S, a.H, a.KH, a.D, a.R,
+                                         a.table_rows, a.position_bytes, (float)eps, (int)interleaved, dtype_code(qkv),
+                                         stream_of(qkv)));
+    ctx->save_for_backward({qkv, wq, wk, rope, positions});
+    ctx->saved_data["dims"] = dims;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["cols"] = qkv.size(1);
+    ctx->saved_data["table"] = rope.sizes().vec();
+    ctx->saved_data["positions"] = positions.defined() ? (int64_t)positions.scalar_type() : (int64_t)-1;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const c10::DeviceGuard guard(grads[0].device());
+    const auto saved = ctx->get_saved_variables();
+    const auto dims = ctx->saved_data["dims"].toIntVector();
+    const int64_t tokens = dims[0], H = dims[2], KH = dims[3], D = dims[4], heads = (H + 2 * KH) * D;
+    const Tensor dy = grads[0].contiguous();
+    const Tensor &qkv = saved[0], wq = saved[1].contiguous(), wk = saved[2].contiguous(), rope = saved[3].contiguous();
+    const int64_t cols = ctx->saved_data["cols"].toInt(), kind = ctx->saved_data["positions"].toInt();
+    check_saved("qkv", qkv, dy, dy.scalar_type(), {tokens, cols});
+    TORCH_CHECK_VALUE(qkv.stride(1) == 1 && (tokens <= 1 || qkv.stride(0) >= heads), "saved qkv came back with strides ",
+                      qkv.strides());
+    check_saved("q_weight", wq, dy, dy.scalar_type(), {D});
+    check_saved("k_weight", wk, dy, dy.scalar_type(), {D});
+    check_saved("rope", rope, dy, at::kFloat, ctx->saved_data["table"].toIntVector());
+    Tensor positions;
+    if (kind >= 0) {
+      positions = saved[4].contiguous();
+      check_saved("positions", positions, dy, (at::ScalarType)kind, {tokens});
+    }
+    const QkArgs a(dims, qkv, rope, positions);
+    Tensor dqkv = at::empty({tokens, cols}, qkv.options());
+    if (cols > heads) dqkv.narrow(1, heads, cols - heads).zero_();
+    Tensor dwq = at::empty({D}, wq.options()), dwk = at::empty({D}, wk.options());
+    const size_t bytes = krsi_qk_norm_rope_bwd_workspace_bytes(a.D);
+    Tensor ws = at::empty({(int64_t)bytes}, qkv.options().dtype(at::kByte));
+    backward_status(krsi_qk_norm_rope_bwd(
+        dy.data_ptr(), qkv.data_ptr(), a.ld, wq.data_ptr(), wk.data_ptr(), rope.data_ptr<float>(),
+        data_or_null(positions), dqkv.data_ptr(), cols, dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), bytes, tokens, a.S,
+        a.H, a.KH, a.D, a.R, a.table_rows, a.position_bytes, (float)ctx->saved_data["eps"].toDouble(), (int)dims[5],
+        dtype_code(qkv), stream_of(qkv)));
+    variable_list out(12);
+    out[0] = dqkv, out[1] = dwq, out[2] = dwk;
+    return out;
+  }
+};
+
+// ------------------------------------------------------------ token embedding
+struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& table, double scale, int64_t padding) {
+    const c10::DeviceGuard guard(table.device());
+    auto shape = tokens.sizes().vec();
+    const int64_t V = table.size(0), D = table.size(1);
+    shape.push_back(D);
+    Tensor out = at::empty(shape, table.options());
+    forward_status(krsi_embedding_fwd(tokens.data_ptr(), (int)tokens.element_size(), table.data_ptr(), out.data_ptr(),
+                                      tokens.numel(), (int)V, (int)D, (float)scale, dtype_code(table), stream_of(table)));
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["shape"] = shape;
+    ctx->saved_data["args"] = std::vector<int64_t>{V, padding, (int64_t)tokens.scalar_type()};
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const c10::DeviceGuard guard(grads[0].device());
+    const Tensor dy = grads[0].contiguous(), tokens = ctx->get_saved_variables()[0].contiguous();
+    auto shape = ctx->saved_data["shape"].toIntVector();
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const int64_t V = args[0], D = shape.back();
+    shape.pop_back();
+    check_saved("tokens", tokens, dy, (at::ScalarType)args[2], shape);
+    Tensor dtable = at::empty({V, D}, dy.options());
+    const size_t bytes = krsi_embedding_bwd_workspace_bytes(tokens.numel(), (int)V, (int)D);
+    Tensor ws = at::empty({(int64_t)bytes}, dy.options().dtype(at::kByte));
+    backward_status(krsi_embedding_bwd(dy.data_ptr(), tokens.data_ptr(), (int)tokens.element_size(), dtable.data_ptr(),
+                                       ws.data_ptr(), bytes, tokens.numel(), (int)V, (int)D, args[1],
+                                       (float)ctx->saved_data["scale"].toDouble(), dtype_code(dy), stream_of(dy)));
+    return {Tensor(), dtable, Tensor(), Tensor()};
+  }
+};
+
+// ----------------------------------- cross entropy of an output projection
+struct LinearCrossEntropyFn : torch::autograd::Function<LinearCrossEntropyFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& targets,
+                        int64_t ignore_index, int64_t reduction) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t rows = x.size(0), k = x.size(1), v = w.size(0);
+    const auto fp32 = x.options().dtype(at::kFloat);
+    Tensor loss = reduction == 0 ? at::empty({rows}, fp32) : at::empty({}, fp32), stats = at::empty({rows + 1}, fp32);
+    const size_t bytes = krsi_linear_cross_entropy_fwd_workspace_bytes(rows, (int)k, (int)v);
+    Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    forward_status(krsi_linear_cross_entropy_fwd(x.data_ptr(), w.data_ptr(), targets.data_ptr(),
+                                                 (int)targets.element_size(), loss.data_ptr<float>(),
+                                                 stats.data_ptr<float>(), ws.data_ptr(), bytes, rows, (int)k, (int)v,
+                                                 ignore_index, (int)reduction, dtype_code(x), stream_of(x)));
+    ctx->save_for_backward({x, w, targets, stats});
+    ctx->saved_data["args"] =
+        std::vector<int64_t>{rows, k, v, ignore_index, reduction, (int64_t)targets.scalar_type(), (int64_t)x.scalar_type()};
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const c10::DeviceGuard guard(grads[0].device());
+    const auto a = ctx->saved_data["args"].toIntVector();
+    const int64_t rows = a[0], k = a[1], v = a[2];
+    const auto saved = ctx->get_saved_variables();
+    const Tensor dout = grads[0].contiguous(), targets = saved[2].contiguous(), stats = saved[3].contiguous();
+    Tensor x = saved[0].contiguous(), w = saved[1].contiguous();
+    check_saved("x", x, dout, (at::ScalarType)a[6], {rows, k});
+    check_saved("weight", w, dout, (at::ScalarType)a[6], {v, k});
+    check_saved("targets", targets, dout, (at::ScalarType)a[5], {rows});
+    check_saved("stats", stats, dout, at::kFloat, {rows + 1});
+    if (!aligned16(x)) x = x.clone();  // a saved tensor that came back elsewhere
+    if (!aligned16(w)) w = w.clone();
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = at::empty({rows, k}, x.options());
+    if (ctx->needs_input_grad(1)) dw = at::empty({v, k}, w.options());
+    const size_t bytes = krsi_linear_cross_entropy_bwd_workspace_bytes(rows, (int)k, (int)v);
+    Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    backward_status(krsi_linear_cross_entropy_bwd(
+        dout.data_ptr<float>(), x.data_ptr(), w.data_ptr(), targets.data_ptr(), (int)targets.element_size(),
+        stats.data_ptr<float>(), dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr,
+        ws.data_ptr(), bytes, rows, (int)k, (int)v, a[3], (int)a[4], dtype_code(x), stream_of(x)));
+    return {dx, dw, Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // ---------------------------------------------------------------- Python entries
 // An entry as Python calls it: C++ exceptions, of the argument tests too, become Python ones.
 using Args = PyObject* const*;
@@ -411,6 +561,66 @@ PyObject* py_bucket_table(Args a, Py_ssize_t n) {
   return unlocked([&] { return BucketFn::apply(*table, *bucket, S); });
 }
 
+bool index_dtype(const Tensor& t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
+
+PyObject* py_qk_norm_rope(Args a, Py_ssize_t n) {
+  const Tensor *qkv, *wq, *wk, *rope, *pos = nullptr;
+  int64_t B, S, H, KH, D, interleaved;
+  double eps;
+  if (n != 12 || !plain_context() || !tensor_arg(a[0], &qkv) || !tensor_arg(a[1], &wq) || !tensor_arg(a[2], &wk) ||
+      !tensor_arg(a[3], &rope) || (a[4] != Py_None && !tensor_arg(a[4], &pos)) || !int_arg(a[5], 1, kIntMax, &B) ||
+      !int_arg(a[6], 1, kIntMax, &S) || !int_arg(a[7], 1, 65535, &H) || !int_arg(a[8], 1, 65535, &KH) ||
+      !int_arg(a[9], 8, 128, &D) || !float_arg(a[10], &eps) || !int_arg(a[11], 0, 1, &interleaved))
+    Py_RETURN_NONE;
+  const int64_t cols = (H + 2 * KH) * D;
+  if (qkv->dim() != 2 || dtype_code(*qkv) < 0 || D % 8 || qkv->size(0) != B * S || qkv->size(1) < cols ||
+      qkv->stride(1) != 1 || (qkv->size(0) > 1 && qkv->stride(0) < cols))
+    Py_RETURN_NONE;
+  for (const Tensor* w : {wq, wk})
+    if (w->scalar_type() != qkv->scalar_type() || w->dim() != 1 || w->size(0) != D || !w->is_contiguous() ||
+        w->device() != qkv->device())
+      Py_RETURN_NONE;
+  if (rope->scalar_type() != at::kFloat || rope->dim() != 2 || rope->size(0) < 1 || rope->size(1) < 2 ||
+      rope->size(1) > D || rope->size(1) % 2 || !rope->is_contiguous() || rope->requires_grad() ||
+      rope->device() != qkv->device() || (!pos && rope->size(0) < S))
+    Py_RETURN_NONE;
+  if (pos && (!index_dtype(*pos) || pos->dim() != 1 || pos->numel() != B * S || !pos->is_contiguous() ||
+              pos->device() != qkv->device()))
+    Py_RETURN_NONE;
+  const std::optional<Tensor> positions = pos ? std::make_optional(*pos) : std::nullopt;
+  return unlocked([&] { return QkNormRopeFn::apply(*qkv, *wq, *wk, *rope, positions, B * S, S, H, KH, D, eps, interleaved); });
+}
+
+PyObject* py_embedding(Args a, Py_ssize_t n) {
+  const Tensor *tokens, *table;
+  double scale;
+  int64_t padding;
+  if (n != 4 || !plain_context() || !tensor_arg(a[0], &tokens) || !tensor_arg(a[1], &table) || !float_arg(a[2], &scale) ||
+      !int_arg(a[3], -1, kIntMax, &padding))
+    Py_RETURN_NONE;
+  if (!index_dtype(*tokens) || !tokens->is_contiguous() || tokens->numel() == 0 || table->dim() != 2 ||
+      dtype_code(*table) < 0 || table->numel() == 0 || !table->is_contiguous() || table->device() != tokens->device() ||
+      table->size(0) > kIntMax || table->size(1) > kIntMax)
+    Py_RETURN_NONE;
+  return unlocked([&] { return EmbeddingFn::apply(*tokens, *table, scale, padding); });
+}
+
+PyObject* py_linear_cross_entropy(Args a, Py_ssize_t n) {
+  const Tensor *x, *w, *targets;
+  int64_t ignore_index, reduction;
+  if (n != 5 || !plain_context() || !tensor_arg(a[0], &x) || !tensor_arg(a[1], &w) || !tensor_arg(a[2], &targets) ||
+      !int_arg(a[3], INT64_MIN, INT64_MAX, &ignore_index) || !int_arg(a[4], 0, 2, &reduction))
+    Py_RETURN_NONE;
+  if (x->dim() != 2 || w->dim() != 2 || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kHalf) ||
+      w->scalar_type() != x->scalar_type() || w->size(1) != x->size(1) || x->numel() == 0 || w->numel() == 0 ||
+      x->size(1) % 64 || x->size(1) > kIntMax || w->size(0) > kIntMax || !x->is_contiguous() || !w->is_contiguous() ||
+      !aligned16(*x) || !aligned16(*w) || !index_dtype(*targets) || targets->dim() != 1 ||
+      targets->size(0) != x->size(0) || !targets->is_contiguous() || w->device() != x->device() ||
+      targets->device() != x->device())
+    Py_RETURN_NONE;
+  return unlocked([&] { return LinearCrossEntropyFn::apply(*x, *w, *targets, ignore_index, reduction); });
+}
+
 PyObject* py_set_module(PyObject*, PyObject* m) {
   Py_XDECREF(g_hip_module);
   Py_INCREF(m);
@@ -424,6 +634,9 @@ PyMethodDef kMethods[] = {
     {"geglu_linear", (PyCFunction)(void*)entry<py_geglu_linear>, METH_FASTCALL, nullptr},
     {"relpos_attention", (PyCFunction)(void*)entry<py_relpos_attention>, METH_FASTCALL, nullptr},
     {"bucket_table", (PyCFunction)(void*)entry<py_bucket_table>, METH_FASTCALL, nullptr},
+    {"qk_norm_rope", (PyCFunction)(void*)entry<py_qk_norm_rope>, METH_FASTCALL, nullptr},
+    {"embedding", (PyCFunction)(void*)entry<py_embedding>, METH_FASTCALL, nullptr},
+    {"linear_cross_entropy", (PyCFunction)(void*)entry<py_linear_cross_entropy>, METH_FASTCALL, nullptr},
     {"set_module", py_set_module, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_krsi_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -124,6 +124,7 @@ class _NoNative:
         return None
 
     rmsnorm = geglu = geglu_linear = relpos_attention = bucket_table = _none
+    qk_norm_rope = embedding = linear_cross_entropy = _none
 
 
 _native = None

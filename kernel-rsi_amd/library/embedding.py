@@ -51,7 +51,8 @@ def embedding(tokens, table, scale=1.0, *, padding_idx=None):
         pad = padding_idx % V
     if compiling():
         return _ops().embedding_fwd_op(tokens, table, float(scale), pad)
-    return Embedding.apply(tokens, table, float(scale), pad)
+    out = _hip.native().embedding(tokens, table, float(scale), pad)
+    return Embedding.apply(tokens, table, float(scale), pad) if out is None else out
 
 
 def reference(tokens, table, scale=1.0, *, padding_idx=None):

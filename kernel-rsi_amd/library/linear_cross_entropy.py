@@ -55,8 +55,10 @@ def linear_cross_entropy(x, w, targets, *, ignore_index=-100, reduction="mean"):
     if compiling():
         loss = _ops().linear_cross_entropy_fwd_op(x, w, targets, ignore_index, reduction)[0]
     else:
-        loss = LinearCrossEntropy.apply(x, w, targets, ignore_index, reduction)
-    return loss.view(shape) if reduction == "none" else loss
+        loss = _hip.native().linear_cross_entropy(x, w, targets, ignore_index, _hip.REDUCTIONS.get(reduction))
+        if loss is None:
+            loss = LinearCrossEntropy.apply(x, w, targets, ignore_index, reduction)
+    return loss.view(shape) if loss.dim() and loss.shape != shape else loss
 
 
 def reference(x, w, targets, *, ignore_index=-100, reduction="mean"):

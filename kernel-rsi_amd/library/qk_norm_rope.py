@@ -72,6 +72,10 @@ def _in_place_layout(qkv, cols):
 def qk_norm_rope(qkv, q_weight, k_weight, rope, B, S, H, D, eps, *, kv_heads=None, positions=None, interleaved=False):
     """qkv with its query and key heads normalised and rotated (see the module)."""
     kv = H if kv_heads is None else kv_heads
+    if not compiling():
+        out = _hip.native().qk_norm_rope(qkv, q_weight, k_weight, rope, positions, B, S, H, kv, D, eps, int(interleaved))
+        if out is not None:
+            return out
     if rope.requires_grad:
         raise ValueError("rope is a constant of qk_norm_rope: it gets no gradient, but requires one")
     qkv = _in_place_layout(qkv, (H + 2 * kv) * D)
