@@ -9,10 +9,13 @@
 // Backward in three launches:
 //   group_tokens  one launch that sorts the positions by token, stably. Workgroup j owns the rows v = j (mod
 //                 groups), so that neighbouring ids, of which the low ones are often the frequent ones, go to
-//                 different workgroups. Each reads all tokens twice (from L2): it counts its own per row and
+//                 different workgroups. Each reads all tokens (from L2): it counts its own per row and
 //                 wave in LDS and the tokens of lower groups (its offset), then places its positions in order.
-//   sum_rows      rows of at most kPiece tokens: a wave (or a part of one, where rows are short) adds them in order
-//                 and writes the row; and, per piece of kPiece sorted positions, fp32 partial sums of longer rows.
+//                 That is latency; the launch's other workgroups meanwhile write dtable's zeros, most of its bytes,
+//                 as one stream whatever the rows' alignment.
+//   sum_rows      rows of at most kPiece tokens, found from their first sorted place: a wave (or a part of one,
+//                 where rows are short) adds them in order and writes the row; and, per piece of kPiece sorted
+//                 places, fp32 partial sums of longer rows.
 //   sum_pieces    longer rows: their pieces' partial sums, in order.
 #include "chunks.h"
 #include "krsi_device.h"
@@ -27,8 +30,11 @@ constexpr int kGroupThreads = 1024;
 constexpr int kGroupWaves = kGroupThreads / kWave;
 constexpr int kGroupRows = 1024;   // most rows of a group: one per thread in its scan, 64 KB of counters
 constexpr int kGroups = 256;       // groups at least (fewer for fewer rows): a workgroup per CU
+constexpr int kFillBlocks = 1024;  // workgroups that write zeros, at most
 constexpr int kPiece = 32;         // sorted positions per piece
+constexpr int kHeld = 8;           // tokens that a thread of group_tokens keeps from its count to its placing
 constexpr int kSumWaves = 16;
+constexpr int kSumPieces = 8;      // pieces whose rows a workgroup of sum_pieces looks after
 constexpr int kSumCols = 256;      // columns per workgroup of sum_pieces
 
 // A wave holds 64 >> shift rows at a time; chunk k of a lane is chunk lane_in_row + k (1 << shift) of the row.
@@ -76,28 +82,56 @@ struct Groups {
   int32_t *order, *row_of, *start, *count, *total;
 };
 
+// Workgroups from `groups` on: zeros into [zeros, zeros + bytes), 16-byte chunks between its unaligned ends.
+__device__ __forceinline__ void write_zeros(char* zeros, int64_t bytes, int block, int blocks) {
+  const int64_t head = min((int64_t)(-(intptr_t)zeros & 15), bytes), chunks = (bytes - head) / 16;
+  u32x4* p = reinterpret_cast<u32x4*>(zeros + head);
+  const int64_t step = (int64_t)blocks * kGroupThreads;
+  for (int64_t i = (int64_t)block * kGroupThreads + threadIdx.x; i < chunks; i += step)
+    __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u}, p + i);
+  if (block == 0 && threadIdx.x < 16) {
+    const int64_t tail = head + chunks * 16 + threadIdx.x;
+    if (threadIdx.x < head) zeros[threadIdx.x] = 0;
+    if (tail < bytes) zeros[tail] = 0;
+  }
+}
+
 __global__ __launch_bounds__(kGroupThreads) void group_tokens(const void* __restrict__ tokens, int token_bytes, int n,
-                                                              int V, int group_shift, int64_t padding, Groups out) {
+                                                              int V, int group_shift, int64_t padding, Groups out,
+                                                              char* __restrict__ zeros, int64_t bytes) {
   __shared__ int count[kGroupWaves][kGroupRows];
   __shared__ int sums[2][kGroupWaves];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  const int j = blockIdx.x, mask = (1 << group_shift) - 1;
+  const int groups = 1 << group_shift, j = blockIdx.x, mask = groups - 1;
+  if (j >= groups) {
+    write_zeros(zeros, bytes, j - groups, gridDim.x - groups);
+    return;
+  }
   for (int w = 0; w < kGroupWaves; ++w) count[w][tid] = 0;
-  __syncthreads();
   // Each wave goes over a contiguous part of the tokens, so that order by wave, then by place in it, is theirs.
   const int per = (n + kGroupThreads - 1) / kGroupThreads * kWave;
   const int64_t first = (int64_t)wave * per;
   const int begin = (int)(first < n ? first : n), end = (int)(first + per < n ? first + per : n);
-  auto token_at = [&](int i) -> int {  // -1: none, or one that is not counted
-    const int64_t t = i < end ? load_index(tokens, token_bytes, i) : -1;
-    return t >= 0 && t < V && t != padding ? (int)t : -1;
+  int held[kHeld];
+  auto load = [&](int i0) {  // the lane's tokens of kHeld rounds; -1: none, or one that is not counted
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int i = i0 + k * kWave + lane;
+      const int64_t t = i < end ? load_index(tokens, token_bytes, i) : -1;
+      held[k] = t >= 0 && t < V && t != padding ? (int)t : -1;
+    }
   };
+  load(begin);
+  __syncthreads();
   int lower = 0;
-#pragma unroll 4
-  for (int i = begin + lane; i < end; i += kWave) {
-    const int t = token_at(i);
-    lower += t >= 0 && (t & mask) < j;
-    if (t >= 0 && (t & mask) == j) atomicAdd(&count[wave][t >> group_shift], 1);
+  for (int i0 = begin; i0 < end; i0 += kHeld * kWave) {
+    if (i0 != begin) load(i0);
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int t = held[k];
+      lower += t >= 0 && (t & mask) < j;
+      if (t >= 0 && (t & mask) == j) atomicAdd(&count[wave][t >> group_shift], 1);
+    }
   }
   for (int m = kWave / 2; m >= 1; m >>= 1) lower += __shfl_xor(lower, m, kWave);
   if (lane == 0) sums[0][wave] = lower;
@@ -122,30 +156,34 @@ __global__ __launch_bounds__(kGroupThreads) void group_tokens(const void* __rest
   for (int w = 0; w < wave; ++w) at += sums[1][w];
   for (int w = 0; w < kGroupWaves; ++w) count[w][tid] += at;
   const int64_t v = j + ((int64_t)tid << group_shift);
-  if (v < V) {
+  if (v < V && all) {
     out.start[v] = at;
     out.count[v] = all;
   }
-  if (j == (int)gridDim.x - 1 && tid == kGroupThreads - 1) *out.total = at + all;
+  if (j == groups - 1 && tid == kGroupThreads - 1) *out.total = at + all;
   __syncthreads();
   // The lanes of one row take consecutive places, in lane order.
-  for (int i0 = begin; i0 < end; i0 += kWave) {
-    const int i = i0 + lane, t = token_at(i), row = t >> group_shift;
-    const bool mine = t >= 0 && (t & mask) == j;
-    uint64_t left = __ballot(mine);
-    while (left) {
-      const int leader = __builtin_ctzll(left);
-      const int its_row = __builtin_amdgcn_readlane(row, leader);
-      const uint64_t same = __ballot(mine && row == its_row);
-      int place = 0;
-      if (lane == leader) place = atomicAdd(&count[wave][row], __popcll(same));
-      place = __builtin_amdgcn_readlane(place, leader);
-      if (same >> lane & 1) {
-        const int p = place + __popcll(same & ((uint64_t(1) << lane) - 1));
-        out.order[p] = i;
-        out.row_of[p] = t;
+  for (int i0 = begin; i0 < end; i0 += kHeld * kWave) {
+    if (per > kHeld * kWave) load(i0);
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int t = held[k], row = t >> group_shift;
+      const bool mine = t >= 0 && (t & mask) == j;
+      uint64_t left = __ballot(mine);
+      while (left) {
+        const int leader = __builtin_ctzll(left);
+        const int its_row = __builtin_amdgcn_readlane(row, leader);
+        const uint64_t same = __ballot(mine && row == its_row);
+        int place = 0;
+        if (lane == leader) place = atomicAdd(&count[wave][row], __popcll(same));
+        place = __builtin_amdgcn_readlane(place, leader);
+        if (same >> lane & 1) {
+          const int p = place + __popcll(same & ((uint64_t(1) << lane) - 1));
+          out.order[p] = i0 + k * kWave + lane;
+          out.row_of[p] = t;
+        }
+        left &= ~same;
       }
-      left &= ~same;
     }
   }
 }
@@ -176,12 +214,13 @@ __device__ __forceinline__ void add_places(float (&acc)[K][C], const typename El
 }
 
 // Workgroups below piece_blocks: a wave per piece, its parts of longer rows into part [pieces][2][D] (slot 0: of
-// a row that starts at or before the piece's first place, slot 1: after it). The others: rows.
+// a row that starts at or before the piece's first place, slot 1: after it). The others: rows, by the sorted
+// place that is a row's first.
 template <int DT, int C, int K>
 __global__ __launch_bounds__(kThreads) void sum_rows(const typename Elem<DT>::T* __restrict__ g, Groups in,
                                                      typename Elem<DT>::T* __restrict__ dtable,
-                                                     float* __restrict__ part, int piece_blocks, int V, int D,
-                                                     int nch, int shift, float scale) {
+                                                     float* __restrict__ part, int piece_blocks, int D, int nch,
+                                                     int shift, float scale) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave_in_block = threadIdx.x / kWave;
   float acc[K][C];
@@ -211,11 +250,12 @@ __global__ __launch_bounds__(kThreads) void sum_rows(const typename Elem<DT>::T*
     return;
   }
   const int64_t wave = (int64_t)(blockIdx.x - piece_blocks) * kWaves + wave_in_block;
-  const int64_t v = (wave << (6 - shift)) + (lane >> shift);
-  if (v >= V) return;
-  const int count = in.count[v];
-  if (count > kPiece) return;
-  const int start = in.start[v], c0 = blockIdx.y * (K << shift) + (lane & ((1 << shift) - 1));
+  const int64_t place = (wave << (6 - shift)) + (lane >> shift);
+  if (place >= *in.total) return;
+  const int64_t v = in.row_of[place];
+  const int start = in.start[v], count = in.count[v];
+  if (place != start || count > kPiece) return;
+  const int c0 = blockIdx.y * (K << shift) + (lane & ((1 << shift) - 1));
   add_places<DT, C, K>(acc, g, in.order, start, start + count, D, nch, c0, 1 << shift);
   auto* dst = dtable + v * D;
 #pragma unroll
@@ -230,7 +270,7 @@ __global__ __launch_bounds__(kThreads) void sum_rows(const typename Elem<DT>::T*
   }
 }
 
-// Workgroup (x, y): the longer rows whose first piece is one of 64 x .. 64 x + 63, columns 256 y .. + 255. Wave w adds
+// Workgroup (x, y): the longer rows whose first piece is one of 8 x .. 8 x + 7, columns 256 y .. + 255. Wave w adds
 // pieces w, w + 16, ... of the row, then the waves' sums are added in order.
 template <int DT>
 __global__ __launch_bounds__(kSumWaves * kWave) void sum_pieces(const float* __restrict__ part, Groups in,
@@ -239,10 +279,10 @@ __global__ __launch_bounds__(kSumWaves * kWave) void sum_pieces(const float* __r
   __shared__ float s[kSumWaves][kSumCols];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int total = *in.total;
-  const int64_t p_lane = (int64_t)blockIdx.x * kWave + lane, a = p_lane * kPiece;
+  const int64_t p_lane = (int64_t)blockIdx.x * kSumPieces + lane, a = p_lane * kPiece;
   int row = 0;
   bool begins = false;
-  if (a < total) {
+  if (lane < kSumPieces && a < total) {
     row = in.row_of[(a + kPiece < total ? a + kPiece : total) - 1];
     begins = in.count[row] > kPiece && in.start[row] >= a;
   }
@@ -251,7 +291,7 @@ __global__ __launch_bounds__(kSumWaves * kWave) void sum_pieces(const float* __r
     const int l = __builtin_ctzll(left);
     left &= left - 1;
     const int v = __builtin_amdgcn_readlane(row, l), start = in.start[v];
-    const int64_t p = (int64_t)blockIdx.x * kWave + l, last = ((int64_t)start + in.count[v] - 1) / kPiece;
+    const int64_t p = (int64_t)blockIdx.x * kSumPieces + l, last = ((int64_t)start + in.count[v] - 1) / kPiece;
     const int slot = start == p * kPiece ? 0 : 1;
     float acc[kSumCols / kWave] = {};
 #pragma unroll 4
@@ -404,20 +444,24 @@ int krsi_embedding_bwd(const void* dout, const void* tokens, int32_t token_bytes
   float* part = (float*)(base + w.part);
   hipStream_t st = as_stream(stream);
   const int gs = group_shift_of(V);
-  hipLaunchKernelGGL(group_tokens, dim3(1u << gs), dim3(kGroupThreads), 0, st, tokens, (int)token_bytes, (int)n, (int)V,
-                     gs, padding, g);
+  const int64_t bytes = (int64_t)V * D * (dtype == kF32 ? 4 : 2);
+  const int64_t fill = ceil_div(bytes, 16 * kGroupThreads * 4);
+  hipLaunchKernelGGL(group_tokens, dim3((1u << gs) + (unsigned)(fill < kFillBlocks ? fill : kFillBlocks)),
+                     dim3(kGroupThreads), 0, st, tokens, (int)token_bytes, (int)n, (int)V, gs, padding, g, (char*)dtable,
+                     bytes);
+  if (n == 0) return launch_status();
   const Cut r = cut_rows(dtype, D);
   const int piece_blocks = (int)ceil_div(w.pieces, kWaves);
-  const int64_t row_blocks = ceil_div(ceil_div(V, kWave >> r.shift), kWaves);
+  const int64_t row_blocks = ceil_div(ceil_div(n, kWave >> r.shift), kWaves);
   return with_kernel(dtype, r, [&](auto dt, auto c, auto k) {
     constexpr int DT = decltype(dt)::value;
     using T = typename Elem<DT>::T;
     hipLaunchKernelGGL((sum_rows<DT, decltype(c)::value, decltype(k)::value>),
                        dim3((unsigned)(piece_blocks + row_blocks), (unsigned)r.blocks), dim3(kThreads), 0, st,
-                       (const T*)dout, g, (T*)dtable, part, piece_blocks, (int)V, (int)D, r.nch, r.shift, scale);
+                       (const T*)dout, g, (T*)dtable, part, piece_blocks, (int)D, r.nch, r.shift, scale);
     if (w.pieces)
       hipLaunchKernelGGL((sum_pieces<DT>),
-                         dim3((unsigned)ceil_div(w.pieces, kWave), (unsigned)ceil_div(D, kSumCols)),
+                         dim3((unsigned)ceil_div(w.pieces, kSumPieces), (unsigned)ceil_div(D, kSumCols)),
                          dim3(kSumWaves * kWave), 0, st, (const float*)part, g, (T*)dtable, (int)D, scale);
     return launch_status();
   });

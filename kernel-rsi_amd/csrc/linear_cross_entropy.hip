@@ -24,7 +24,8 @@ constexpr int kThreads = 256;
 constexpr int kOneBlock = 1024;
 constexpr int64_t kPieceBytes = int64_t(512) << 20;
 constexpr int64_t kMaxWidth = 1 << 20;  // columns of a piece: 64 rows of dl stay below 2^31 bytes
-constexpr int kMinStages = 8;  // stages of a part of a split sum, at least
+constexpr int kMinStages = 8;   // stages of a part of a split sum, at least
+constexpr int kMaxSplits = 64;  // parts of a sum
 
 using Large = StreamTile<2, 4, 8, 4>;  // 256 x 256, 8 waves, one workgroup per CU
 using Small = StreamTile<2, 2, 4, 4>;  // 128 x 128, 4 waves, two per CU
@@ -56,65 +57,83 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
   stream_products<DT, false, false, WM, WN, RB, CB>(x, w, K, tiles, lds, [&](const TileAt& t, f32x4(&acc)[RB][CB]) {
     const int col0 = (int)t.n0 + 16 * CB * wc + 4 * g;
     const int64_t slice = t.n0 / (16 * CB) + wc;
+    auto reduce = [&](auto whole) {  // a tile within the vocabulary, or one that ends past it
+      constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      const int64_t row = t.m0 + 16 * (RB * wr + i) + l16;
-      float m = -__builtin_inff();
+      for (int i = 0; i < RB; ++i) {
+        const int64_t row = t.m0 + 16 * (RB * wr + i) + l16;
+        float m = -__builtin_inff();
 #pragma unroll
-      for (int j = 0; j < CB; ++j)
+        for (int j = 0; j < CB; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) m = fmaxf(m, col0 + 16 * j + r < V ? acc[i][j][r] : -__builtin_inff());
-      m = fmaxf(m, __shfl_xor(m, 16, kWave));
-      m = fmaxf(m, __shfl_xor(m, 32, kWave));
-      const float base = m == -__builtin_inff() ? 0.f : m;
-      float s = 0.f;
+          for (int r = 0; r < 4; ++r) {
+            if (!WHOLE && col0 + 16 * j + r >= V) acc[i][j][r] = -__builtin_inff();
+            m = fmaxf(m, acc[i][j][r]);
+          }
+        m = fmaxf(m, __shfl_xor(m, 16, kWave));
+        m = fmaxf(m, __shfl_xor(m, 32, kWave));
+        const float base = m == -__builtin_inff() ? 0.f : m;
+        float s = 0.f;
 #pragma unroll
-      for (int j = 0; j < CB; ++j)
+        for (int j = 0; j < CB; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f((acc[i][j][r] - base) * kLog2e);
-          s += col0 + 16 * j + r < V ? e : 0.f;
+          for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * kLog2e);
+        s += __shfl_xor(s, 16, kWave);
+        s += __shfl_xor(s, 32, kWave);
+        if (row >= rows) continue;
+        if (g == 0) part[slice * rows + row] = float2{m, s};
+        const int at = targets.at(row) - col0;
+        if ((unsigned)at < 16 * CB && (at & 15) < 4) {
+#pragma unroll
+          for (int j = 0; j < CB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (at == 16 * j + r) target_logit[row] = acc[i][j][r];
         }
-      s += __shfl_xor(s, 16, kWave);
-      s += __shfl_xor(s, 32, kWave);
-      if (row >= rows) continue;
-      if (g == 0) part[slice * rows + row] = float2{m, s};
-      const int at = targets.at(row) - col0;
-#pragma unroll
-      for (int j = 0; j < CB; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (at == 16 * j + r) target_logit[row] = acc[i][j][r];
-    }
+      }
+    };
+    if (t.n0 + Tl::kCols <= V)
+      reduce(std::true_type{});
+    else
+      reduce(std::false_type{});
   });
 }
 
-// lse and loss of each row from its pairs; 16 rows per workgroup, 16 threads a row, joined in a fixed order.
-__global__ __launch_bounds__(kThreads) void join_rows(const float2* __restrict__ part,
-                                                      const float* __restrict__ target_logit, Targets targets,
-                                                      float* __restrict__ lse, float* __restrict__ loss, int64_t rows,
-                                                      int slices) {
-  __shared__ float2 s[16][16];
-  const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const int64_t row = (int64_t)blockIdx.x * 16 + r;
-  float2 a{-__builtin_inff(), 0.f};
-  auto join = [](float2 a, float2 b) {
-    if (b.x == -__builtin_inff() && b.y == 0.f) return a;
-    if (a.x == -__builtin_inff() && a.y == 0.f) return b;
-    const float m = fmaxf(a.x, b.x);
-    return float2{m, a.y * expf(a.x - m) + b.y * expf(b.x - m)};
-  };
-  if (row < rows) {
+// lse and loss of each row from its pairs, in a fixed order: 16 rows per workgroup, 64 threads a row, the maximum
+// first, then the sums to its base. (With 16 threads a row that joined pair after pair it took 18 us for 2048 rows
+// of 502 pairs, a third of the memory's rate at 2048 pairs of 8192 rows.)
+constexpr int kJoinRows = 16, kJoinParts = kOneBlock / kJoinRows;
+__global__ __launch_bounds__(kOneBlock) void join_rows(const float2* __restrict__ part,
+                                                       const float* __restrict__ target_logit, Targets targets,
+                                                       float* __restrict__ lse, float* __restrict__ loss, int64_t rows,
+                                                       int slices) {
+  __shared__ float top[kJoinParts][kJoinRows], sum[kJoinParts][kJoinRows];
+  const int r = threadIdx.x % kJoinRows, q = threadIdx.x / kJoinRows;
+  const int64_t row = (int64_t)blockIdx.x * kJoinRows + r;
+  const bool live = row < rows;
+  const float2* p = part + (live ? row : 0);
+  float m = -__builtin_inff();
 #pragma unroll 8
-    for (int k = q; k < slices; k += 16) a = join(a, part[(int64_t)k * rows + row]);
-  }
-  s[q][r] = a;
+  for (int k = q; k < slices; k += kJoinParts) m = fmaxf(m, p[(int64_t)k * rows].x);
+  top[q][r] = m;
   __syncthreads();
-  if (q != 0 || row >= rows) return;
-  for (int k = 1; k < 16; ++k) a = join(a, s[k][r]);
-  const float log_sum = logf(a.y);
-  lse[row] = a.x + log_sum;
-  loss[row] = targets.ignored(row) ? 0.f : targets.at(row) < 0 ? __builtin_nanf("") : (a.x - target_logit[row]) + log_sum;
+  m = top[0][r];
+#pragma unroll 8
+  for (int k = 1; k < kJoinParts; ++k) m = fmaxf(m, top[k][r]);
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = q; k < slices; k += kJoinParts) {
+    const float2 a = p[(int64_t)k * rows];
+    s += a.y == 0.f ? 0.f : a.y * __builtin_amdgcn_exp2f((a.x - m) * kLog2e);
+  }
+  sum[q][r] = s;
+  __syncthreads();
+  if (q != 0 || !live) return;
+#pragma unroll 8
+  for (int k = 1; k < kJoinParts; ++k) s += sum[k][r];
+  const float log_sum = logf(s);
+  lse[row] = m + log_sum;
+  loss[row] = targets.ignored(row) ? 0.f : targets.at(row) < 0 ? __builtin_nanf("") : (m - target_logit[row]) + log_sum;
 }
 
 __device__ __forceinline__ double block_sum(double v, double* s) {
@@ -198,18 +217,26 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
       if (row >= x.extent) continue;
       const float b = lse[row], c = coef[row];
       const int at = targets.at(row) - v0 - col0;
+      float d[4 * CB];
 #pragma unroll
-      for (int j = 0; j < CB; ++j) {
-        float d[4];
+      for (int j = 0; j < 4 * CB; ++j) d[j] = __builtin_amdgcn_exp2f((acc[i][j / 4][j % 4] - b) * kLog2e) * c;
+      if ((unsigned)at < 16 * CB && (at & 15) < 4) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - b) * kLog2e);
-          d[r] = (p - (at == 16 * j + r ? 1.f : 0.f)) * c;
-          d[r] = c == 0.f || col0 + 16 * j + r >= w.extent ? 0.f : d[r];
-          if (at == 16 * j + r) rest[row] = d[r] - El::round(d[r]);
-        }
-        *reinterpret_cast<u32x2*>(dl + row * ld + col0 + 16 * j) = u32x2{El::pack2(d[0], d[1]), El::pack2(d[2], d[3])};
+        for (int j = 0; j < 4 * CB; ++j)
+          if (at == 16 * (j / 4) + j % 4) {
+            d[j] = (__builtin_amdgcn_exp2f((acc[i][j / 4][j % 4] - b) * kLog2e) - 1.f) * c;
+            rest[row] = d[j] - El::round(d[j]);
+          }
       }
+      if (t.n0 + Tl::kCols > w.extent) {
+#pragma unroll
+        for (int j = 0; j < 4 * CB; ++j) d[j] = col0 + 16 * (j / 4) + j % 4 < w.extent ? d[j] : 0.f;
+      }
+      const uint32_t keep = c == 0.f ? 0u : 0xffffffffu;  // a row without weight has no gradient, whatever it holds
+#pragma unroll
+      for (int j = 0; j < CB; ++j)
+        *reinterpret_cast<u32x2*>(dl + row * ld + col0 + 16 * j) =
+            u32x2{El::pack2(d[4 * j], d[4 * j + 1]) & keep, El::pack2(d[4 * j + 2], d[4 * j + 3]) & keep};
     }
   });
 }
@@ -293,35 +320,42 @@ __global__ __launch_bounds__(kThreads) void add_parts(const float* __restrict__ 
 
 // -------------------------------------------------------------------- plans
 template <typename Tl>
-Tiles tiles_of(int64_t M, int64_t N, int64_t sum, bool split) {
+Tiles tiles_of(int64_t M, int64_t N, int64_t sum, int splits) {
   Tiles t{};
   t.nrb = (int)ceil_div(M, Tl::kRows);
   t.ncb = (int)ceil_div(N, Tl::kCols);
   t.stages = (int)ceil_div(sum, kStage);
-  t.splits = 1;
-  const int64_t tiles = (int64_t)t.nrb * t.ncb, slots = 256 * Tl::kPerCu;
-  if (split && tiles < slots) {
-    const int64_t most = t.stages / kMinStages, want = slots / tiles;
-    t.splits = (int)(most < 1 ? 1 : want < most ? want : most);
-  }
-  t.per = (int)ceil_div(t.stages, t.splits);
+  t.per = (int)ceil_div(t.stages, splits);
   t.splits = (int)ceil_div(t.stages, t.per);
-  t.total = (int)(tiles * t.splits);
+  t.total = (int)((int64_t)t.nrb * t.ncb * t.splits);
   return t;
-}
-// Time of the launch in stages of the large tile. The small one has a quarter of the work, two workgroups per CU
-// share it, and it takes 1.2 times as long for the same work (geglu_linear's measurement of the two).
-double cost(const Tiles& t, bool large) {
-  const int slots = 256 * (large ? Large::kPerCu : Small::kPerCu);
-  return (double)ceil_div(t.total, slots) * t.per * (large ? 1.0 : 0.6);
 }
 struct Plan {
   bool large;
   Tiles tiles;
 };
+// The tile, and the parts of the sum where it may be cut, by an estimate in stages of the large tile (1.6 us on a
+// CU at full rate): rounds of workgroups times the stages of each and its epilogue (4, or 8 where it writes fp32
+// parts, which all CUs do at once), and the parts' addition (4 M N bytes per part at 5 TB/s). The small tile has a
+// quarter of the work, two workgroups per CU share it, and it takes 1.2 times as long for the same work
+// (geglu_linear's measurement of the two).
 Plan plan_product(int64_t M, int64_t N, int64_t sum, bool split) {
-  const Tiles l = tiles_of<Large>(M, N, sum, split), s = tiles_of<Small>(M, N, sum, split);
-  return cost(l, true) <= cost(s, false) ? Plan{true, l} : Plan{false, s};
+  Plan best{};
+  double least = 0;
+  const int64_t stages = ceil_div(sum, kStage), most = split ? stages / kMinStages : 1;
+  for (int s = 1; s == 1 || (s <= most && s <= kMaxSplits); ++s) {
+    for (bool large : {true, false}) {
+      const Tiles t = large ? tiles_of<Large>(M, N, sum, s) : tiles_of<Small>(M, N, sum, s);
+      const double each = (t.per + (s > 1 ? 8 : 4)) * (large ? 1.0 : 0.6);
+      const double cost = (double)ceil_div(t.total, 256 * (large ? Large::kPerCu : Small::kPerCu)) * each +
+                          (s > 1 ? 5e-7 * (double)M * (double)N * s : 0);
+      if (best.tiles.total == 0 || cost < least) {
+        best = Plan{large, t};
+        least = cost;
+      }
+    }
+  }
+  return best;
 }
 
 // f(tile) with the plan's tile.
@@ -416,7 +450,7 @@ int forward(const Operand& x, const Operand& w, int K, const Targets& t, float* 
     hipLaunchKernelGGL((logits_reduce<DT, S::WM, S::WN, S::RB, S::CB>), dim3(stream_grid<typename S::Tl>(f.plan.tiles)),
                        dim3(S::Tl::kThreads), 0, st, x, w, (int64_t)K, f.plan.tiles, t, part, target_logit);
   });
-  hipLaunchKernelGGL(join_rows, dim3((unsigned)ceil_div(rows, 16)), dim3(kThreads), 0, st, (const float2*)part,
+  hipLaunchKernelGGL(join_rows, dim3((unsigned)ceil_div(rows, kJoinRows)), dim3(kOneBlock), 0, st, (const float2*)part,
                      (const float*)target_logit, t, stats, row_loss, rows, f.slices);
   if (reduction != 0)
     hipLaunchKernelGGL(add_losses, dim3(1), dim3(kOneBlock), 0, st, (const float*)row_loss, t, rows, reduction == 1, loss,
