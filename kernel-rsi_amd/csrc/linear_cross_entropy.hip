@@ -49,7 +49,7 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
     Operand x, Operand w, int64_t K, Tiles tiles, Targets targets, float2* __restrict__ part,
     float* __restrict__ target_logit) {
   using Tl = StreamTile<WM, WN, RB, CB>;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[Tl::kLds];
+  __shared__ __attribute__((aligned(512))) uint16_t lds[Tl::kLds];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
   const int wr = wave / WN, wc = wave % WN;
   const int64_t rows = x.extent;
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
     const float* __restrict__ coef, float* __restrict__ rest, uint16_t* __restrict__ dl, int64_t ld) {
   using Tl = StreamTile<WM, WN, RB, CB>;
   using El = Elem<DT>;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[Tl::kLds];
+  __shared__ __attribute__((aligned(512))) uint16_t lds[Tl::kLds];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
   const int wr = wave / WN, wc = wave % WN;
   stream_products<DT, false, false, WM, WN, RB, CB>(x, w, K, tiles, lds, [&](const TileAt& t, f32x4(&acc)[RB][CB]) {
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
     uint16_t* __restrict__ out, float* __restrict__ part, bool add) {
   using Tl = StreamTile<WM, WN, RB, CB>;
   using El = Elem<DT>;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[Tl::kLds];
+  __shared__ __attribute__((aligned(512))) uint16_t lds[Tl::kLds];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
   const int wr = wave / WN, wc = wave % WN;
   const float scale = *back;

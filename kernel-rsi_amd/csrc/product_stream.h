@@ -79,7 +79,7 @@ __device__ __forceinline__ TileAt tile_at(const Tiles& t, int v) {
 
 // Calls epilogue(tile, acc) for every tile of this workgroup: acc[i][j][r] is row 16 (RB wr + i) + l16, column
 // 16 (CB wc + j) + 4 g + r of the tile, for lane 16 g + l16 of wave (wr, wc). The grid is the tiles, or fewer
-// where every part of the sum has two stages at least.
+// where every part of the sum has two stages at least. lds: Tl::kLds elements on a 512-byte boundary.
 template <int DT, bool TRA, bool TRB, int WM, int WN, int RB, int CB, typename Epilogue>
 __device__ __forceinline__ void stream_products(const Operand a, const Operand b, int64_t sum, const Tiles tiles,
                                                 uint16_t* lds, Epilogue&& epilogue) {
@@ -89,25 +89,23 @@ __device__ __forceinline__ void stream_products(const Operand a, const Operand b
   const int wr = wave / WN, wc = wave % WN;
   const int wv = __builtin_amdgcn_readfirstlane(wave);
 
-  // Chunk q = i * threads + tid of a staged tile: this lane's byte offset into the tile's memory.
-  auto offset = [&](auto tr, const Operand& o, int64_t o0, int width, int q) {
-    constexpr bool TR = decltype(tr)::value;
-    const int chunks = TR ? width / 8 : kStage / 8, r = q / chunks;
-    const int col = 8 * ((q & (chunks - 1)) ^ stage_swizzle<TR>(r));
-    return TR && o0 + col >= o.extent ? kPastEnd : (uint32_t)(r * o.ld + col) * 2u;
-  };
   using TagA = std::bool_constant<TRA>;
   using TagB = std::bool_constant<TRB>;
-  // Of a tile in memory: byte offsets per request (they depend on the tile only where TR meets the extent's end).
-  uint32_t aoff[Tl::kADma], boff[Tl::kBDma];
-  auto offsets_a = [&](const TileAt& t) {
-#pragma unroll
-    for (int i = 0; i < Tl::kADma; ++i) aoff[i] = opaque(offset(TagA{}, a, t.m0, Tl::kRows, i * Tl::kThreads + tid));
+  // Chunk q = i * threads + tid of a staged tile: row q / chunks of it. Request i's rows lie a whole number of
+  // swizzle periods (16 rows) below request 0's, so one byte offset per lane serves all requests of an operand, whose
+  // resource starts i steps further on (a register per request cost spills in the products of two TR operands).
+  constexpr int kAStep = TRA ? Tl::kThreads * 8 / Tl::kRows : Tl::kThreads * 8 / kStage;  // rows from request to request
+  constexpr int kBStep = TRB ? Tl::kThreads * 8 / Tl::kCols : Tl::kThreads * 8 / kStage;
+  static_assert(kAStep % 16 == 0 && kBStep % 16 == 0, "whole swizzle periods");
+  auto offset = [&](auto tr, const Operand& o, int64_t o0, int width) {
+    constexpr bool TR = decltype(tr)::value;
+    const int chunks = TR ? width / 8 : kStage / 8, r = tid / chunks;
+    const int col = 8 * ((tid & (chunks - 1)) ^ stage_swizzle<TR>(r));
+    return opaque(TR && o0 + col >= o.extent ? kPastEnd : (uint32_t)(r * o.ld + col) * 2u);
   };
-  auto offsets_b = [&](const TileAt& t) {
-#pragma unroll
-    for (int i = 0; i < Tl::kBDma; ++i) boff[i] = opaque(offset(TagB{}, b, t.n0, Tl::kCols, i * Tl::kThreads + tid));
-  };
+  uint32_t aoff, boff;  // they depend on the tile only where TR meets the extent's end
+  auto offsets_a = [&](const TileAt& t) { aoff = offset(TagA{}, a, t.m0, Tl::kRows); };
+  auto offsets_b = [&](const TileAt& t) { boff = offset(TagB{}, b, t.n0, Tl::kCols); };
   // A stage's memory: base and bytes up to the operand's end, none where the stage lies past it.
   struct Stage {
     const uint16_t *a, *b;
@@ -134,24 +132,35 @@ __device__ __forceinline__ void stream_products(const Operand a, const Operand b
     return s;
   };
   auto request = [&](const Stage& s, int buf, int i) {
-    if (i < Tl::kADma)
-      dma16(make_rsrc(s.a, s.abytes), aoff[i],
-            (uint32_t)(uintptr_t)(lds_void*)(As + buf * Tl::kA + (i * Tl::kThreads + 64 * wv) * 8));
-    else
-      dma16(make_rsrc(s.b, s.bbytes), boff[i - Tl::kADma],
-            (uint32_t)(uintptr_t)(lds_void*)(Bs + buf * Tl::kB + ((i - Tl::kADma) * Tl::kThreads + 64 * wv) * 8));
+    const bool of_a = i < Tl::kADma;
+    const int k = of_a ? i : i - Tl::kADma;
+    const int64_t ahead = of_a ? (int64_t)k * kAStep * a.ld : (int64_t)k * kBStep * b.ld;
+    const int left = (int)(of_a ? s.abytes : s.bbytes) - (int)(ahead * 2);  // an operand's tile has less than 2^31 bytes
+    uint16_t* const to = of_a ? As + buf * Tl::kA : Bs + buf * Tl::kB;
+    dma16(make_rsrc((of_a ? s.a : s.b) + ahead, (uint32_t)max(left, 0)), of_a ? aoff : boff,
+          (uint32_t)(uintptr_t)(lds_void*)(to + (k * Tl::kThreads + 64 * wv) * 8));
   };
 
-  // Operand reads of k-step s (32 of the stage's 64): outputs 16 o + l16, summed indices 32 s + 8 g .. + 7.
+  // Operand reads of k-step s (32 of the stage's 64): outputs 16 o + l16, summed indices 32 s + 8 g .. + 7. A TR
+  // read's chunk differs from that of o = 0 in bits of the address alone (rows are 256 bytes at least): one address
+  // register per operand and an exclusive or per read, redone in each stage rather than kept.
   const int trow = 8 * g + (l16 >> 2), tsw = stage_swizzle<true>(trow), tb = (l16 & 3) >> 1, te = 4 * (l16 & 1);
-  auto read_operand = [&](auto tr, const uint16_t* t, int width, int s, int o) {
+  auto tr_base = [&](const uint16_t* t, int width) {
+    return (uint32_t)(uintptr_t)(lds_void*)t + 2u * (uint32_t)(trow * width + 8 * (tb ^ tsw) + te);
+  };
+  uint32_t abase = 0, bbase = 0;
+  if (TRA) abase = tr_base(As, Tl::kRows);
+  if (TRB) bbase = tr_base(Bs, Tl::kCols);
+  auto read_operand = [&](auto tr, const uint16_t* t, uint32_t base, int tile, int width, int buf, int s, int o) {
     if constexpr (decltype(tr)::value) {
-      const uint16_t* q = t + (32 * s + trow) * width + 8 * ((2 * o + tb) ^ tsw) + te;
-      const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q));
-      const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 4 * width)));
+      const uint32_t at = (base ^ (uint32_t)(o << 5)) + 2u * (uint32_t)(buf * tile + 32 * s * width);
+      const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at));
+      const u32x2 y =
+          __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(at + 8u * width)));
       return u32x4{x[0], x[1], y[0], y[1]};
     } else {
-      return *reinterpret_cast<const u32x4*>(t + (16 * o + l16) * kStage + 8 * ((4 * s + g) ^ stage_swizzle<false>(l16)));
+      return *reinterpret_cast<const u32x4*>(t + buf * tile + (16 * o + l16) * kStage +
+                                             8 * ((4 * s + g) ^ stage_swizzle<false>(l16)));
     }
   };
   u32x4 ra[2][RB], rb[2][CB];
@@ -159,14 +168,16 @@ __device__ __forceinline__ void stream_products(const Operand a, const Operand b
   static_assert(kReads * 2 <= kProducts && kEvery >= 2, "one k-step's products hold its reads and requests");
   auto read = [&](int s, int buf, int o) {
     if (o < CB)
-      rb[s][o] = read_operand(TagB{}, Bs + buf * Tl::kB, Tl::kCols, s, CB * wc + o);
+      rb[s][o] = read_operand(TagB{}, Bs, bbase, Tl::kB, Tl::kCols, buf, s, CB * wc + o);
     else
-      ra[s][o - CB] = read_operand(TagA{}, As + buf * Tl::kA, Tl::kRows, s, RB * wr + o - CB);
+      ra[s][o - CB] = read_operand(TagA{}, As, abase, Tl::kA, Tl::kRows, buf, s, RB * wr + o - CB);
   };
   f32x4 acc[RB][CB];
   // The products of k-step s, the reads of the next k-step after the even ones, in k-step 1 the requests of the
   // stage after the next spread over them. b first: a lane holds four columns of one row.
   auto products = [&](int s, int rbuf, const Stage& d) {
+    if (TRA) abase = opaque(abase);
+    if (TRB) bbase = opaque(bbase);
 #pragma unroll
     for (int m = 0; m < kProducts; ++m) {
       const int i = m / CB, j = m % CB;
