@@ -60,6 +60,13 @@ struct Piece {
   T e[C];
   __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(e, p, sizeof(e)); }
   __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, e, sizeof(e)); }
+  // Written once, not read back: non-temporal where it is a whole 16-byte chunk.
+  __device__ __forceinline__ void store_stream(T* p) const {
+    if constexpr (sizeof(e) == 16)
+      __builtin_nontemporal_store(__builtin_bit_cast(u32x4, *this), reinterpret_cast<u32x4_any*>(p));
+    else
+      store(p);
+  }
   __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
     for (int j = 0; j < C; ++j) f[j] = Elem<DT>::load(e[j]);

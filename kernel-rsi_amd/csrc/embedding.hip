@@ -13,9 +13,9 @@
 //                 wave in LDS and the tokens of lower groups (its offset), then places its positions in order.
 //                 That is latency; the launch's other workgroups meanwhile write dtable's zeros, most of its bytes,
 //                 as one stream whatever the rows' alignment.
-//   sum_rows      rows of at most kPiece tokens, found from their first sorted place: a wave (or a part of one,
-//                 where rows are short) adds them in order and writes the row; and, per piece of kPiece sorted
-//                 places, fp32 partial sums of longer rows.
+//   sum_rows      rows of at most a piece of tokens, found from their first sorted place: a wave (or a part of one,
+//                 where rows are short) adds them in order and writes the row; and, per piece of 16 or 32
+//                 sorted places, fp32 partial sums of longer rows.
 //   sum_pieces    longer rows: their pieces' partial sums, in order.
 #include "chunks.h"
 #include "krsi_device.h"
@@ -30,8 +30,10 @@ constexpr int kGroupThreads = 1024;
 constexpr int kGroupWaves = kGroupThreads / kWave;
 constexpr int kGroupRows = 1024;   // most rows of a group: one per thread in its scan, 64 KB of counters
 constexpr int kGroups = 256;       // groups at least (fewer for fewer rows): a workgroup per CU
-constexpr int kFillBlocks = 1024;  // workgroups that write zeros, at most
-constexpr int kPiece = 32;         // sorted positions per piece
+constexpr int kFillChunks = 8;     // 16-byte chunks of zeros that a thread of group_tokens writes: 128 KB per workgroup
+// Sorted positions per piece, log2. Short pieces spread the frequent tokens' rows wider, and cost a partial row each:
+// bf16 8191 tokens of 1024 columns 32.7 us with 16, 38.7 with 32, 48.9 with 64; 32768 of 4096: 332, 315, 336.
+int piece_shift_of(int64_t n) { return n <= 8192 ? 4 : 5; }
 constexpr int kHeld = 8;           // tokens that a thread of group_tokens keeps from its count to its placing
 constexpr int kSumWaves = 16;
 constexpr int kSumPieces = 8;      // pieces whose rows a workgroup of sum_pieces looks after
@@ -72,7 +74,7 @@ __global__ __launch_bounds__(kThreads) void embedding_fwd(const void* __restrict
 #pragma unroll
     for (int j = 0; j < C; ++j) f[j] = inside ? f[j] * scale : __builtin_nanf("");
     v[k].set(f);
-    v[k].store(dst + chunk_start<C>(c, D));
+    v[k].store_stream(dst + chunk_start<C>(c, D));  // bf16 [32768, 4096]: 82.5 -> 72 us
   }
 }
 
@@ -80,15 +82,18 @@ __global__ __launch_bounds__(kThreads) void embedding_fwd(const void* __restrict
 // count[v]; *total: places in all.
 struct Groups {
   int32_t *order, *row_of, *start, *count, *total;
+  int piece_shift;
 };
 
-// Workgroups from `groups` on: zeros into [zeros, zeros + bytes), 16-byte chunks between its unaligned ends.
-__device__ __forceinline__ void write_zeros(char* zeros, int64_t bytes, int block, int blocks) {
+// Workgroups from `groups` on: zeros into [zeros, zeros + bytes), kFillChunks 16-byte chunks per thread between its
+// unaligned ends.
+__device__ __forceinline__ void write_zeros(char* zeros, int64_t bytes, int block) {
   const int64_t head = min((int64_t)(-(intptr_t)zeros & 15), bytes), chunks = (bytes - head) / 16;
   u32x4* p = reinterpret_cast<u32x4*>(zeros + head);
-  const int64_t step = (int64_t)blocks * kGroupThreads;
-  for (int64_t i = (int64_t)block * kGroupThreads + threadIdx.x; i < chunks; i += step)
-    __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u}, p + i);
+  const int64_t first = (int64_t)block * (kGroupThreads * kFillChunks) + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < kFillChunks; ++k)
+    if (first + k * kGroupThreads < chunks) __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u}, p + first + k * kGroupThreads);
   if (block == 0 && threadIdx.x < 16) {
     const int64_t tail = head + chunks * 16 + threadIdx.x;
     if (threadIdx.x < head) zeros[threadIdx.x] = 0;
@@ -104,7 +109,7 @@ __global__ __launch_bounds__(kGroupThreads) void group_tokens(const void* __rest
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int groups = 1 << group_shift, j = blockIdx.x, mask = groups - 1;
   if (j >= groups) {
-    write_zeros(zeros, bytes, j - groups, gridDim.x - groups);
+    write_zeros(zeros, bytes, j - groups);
     return;
   }
   for (int w = 0; w < kGroupWaves; ++w) count[w][tid] = 0;
@@ -188,7 +193,30 @@ __global__ __launch_bounds__(kGroupThreads) void group_tokens(const void* __rest
   }
 }
 
-// acc[k][:] = sum over the sorted places [from, to) of the lane's chunks of g.
+// acc[k][:] = sum over the sorted places [from, to) of the lane's chunks of g, in order. Batches of B places, whose
+// positions and then rows are all requested before the first is added: one place after another is two memory
+// latencies each (a piece of 32 rows: 30 us).
+template <int DT, int C, int K, int B>
+__device__ __forceinline__ void add_batch(float (&acc)[K][C], const typename Elem<DT>::T* g, const int32_t* order, int at,
+                                          int D, int nch, int c0, int step) {
+  Piece<DT, C> v[B][K];
+  int pos[B];
+#pragma unroll
+  for (int i = 0; i < B; ++i) pos[i] = order[at + i];
+#pragma unroll
+  for (int i = 0; i < B; ++i)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[i][k].load(g + (int64_t)pos[i] * D + chunk_start<C>(min(c0 + k * step, nch - 1), D));
+#pragma unroll
+  for (int i = 0; i < B; ++i)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float f[C];
+      v[i][k].get(f);
+#pragma unroll
+      for (int j = 0; j < C; ++j) acc[k][j] += f[j];
+    }
+}
 template <int DT, int C, int K>
 __device__ __forceinline__ void add_places(float (&acc)[K][C], const typename Elem<DT>::T* g, const int32_t* order,
                                            int from, int to, int D, int nch, int c0, int step) {
@@ -196,21 +224,10 @@ __device__ __forceinline__ void add_places(float (&acc)[K][C], const typename El
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int j = 0; j < C; ++j) acc[k][j] = 0.f;
-#pragma unroll 4
-  for (int i = from; i < to; ++i) {
-    const auto* src = g + (int64_t)order[i] * D;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = c0 + k * step;
-      if (c >= nch) continue;
-      Piece<DT, C> v;
-      float f[C];
-      v.load(src + chunk_start<C>(c, D));
-      v.get(f);
-#pragma unroll
-      for (int j = 0; j < C; ++j) acc[k][j] += f[j];
-    }
-  }
+  constexpr int B = K >= 4 ? 4 : 8;
+  for (; from + B <= to; from += B) add_batch<DT, C, K, B>(acc, g, order, from, D, nch, c0, step);
+  for (; from + 2 <= to; from += 2) add_batch<DT, C, K, 2>(acc, g, order, from, D, nch, c0, step);
+  if (from < to) add_batch<DT, C, K, 1>(acc, g, order, from, D, nch, c0, step);
 }
 
 // Workgroups below piece_blocks: a wave per piece, its parts of longer rows into part [pieces][2][D] (slot 0: of
@@ -223,12 +240,13 @@ __global__ __launch_bounds__(kThreads) void sum_rows(const typename Elem<DT>::T*
                                                      int shift, float scale) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave_in_block = threadIdx.x / kWave;
+  const int piece = 1 << in.piece_shift;
   float acc[K][C];
   if ((int)blockIdx.x < piece_blocks) {
-    const int64_t p = (int64_t)blockIdx.x * kWaves + wave_in_block, a = p * kPiece;
+    const int64_t p = (int64_t)blockIdx.x * kWaves + wave_in_block, a = p << in.piece_shift;
     const int total = *in.total;
     if (a >= total) return;
-    const int from = (int)a, to = a + kPiece < total ? from + kPiece : total;
+    const int from = (int)a, to = a + piece < total ? from + piece : total;
     const int head = in.row_of[from], tail = in.row_of[to - 1];
     const int c0 = blockIdx.y * (K * kWave) + lane;
     auto write = [&](int slot) {
@@ -239,11 +257,11 @@ __global__ __launch_bounds__(kThreads) void sum_rows(const typename Elem<DT>::T*
         if (c < nch) __builtin_memcpy(dst + chunk_start<C>(c, D), acc[k], sizeof(acc[k]));
       }
     };
-    if (in.count[head] > kPiece) {
+    if (in.count[head] > piece) {
       add_places<DT, C, K>(acc, g, in.order, from, min(to, in.start[head] + in.count[head]), D, nch, c0, kWave);
       write(0);
     }
-    if (in.count[tail] > kPiece && in.start[tail] > from) {
+    if (in.count[tail] > piece && in.start[tail] > from) {
       add_places<DT, C, K>(acc, g, in.order, in.start[tail], to, D, nch, c0, kWave);
       write(1);
     }
@@ -254,7 +272,7 @@ __global__ __launch_bounds__(kThreads) void sum_rows(const typename Elem<DT>::T*
   if (place >= *in.total) return;
   const int64_t v = in.row_of[place];
   const int start = in.start[v], count = in.count[v];
-  if (place != start || count > kPiece) return;
+  if (place != start || count > piece) return;
   const int c0 = blockIdx.y * (K << shift) + (lane & ((1 << shift) - 1));
   add_places<DT, C, K>(acc, g, in.order, start, start + count, D, nch, c0, 1 << shift);
   auto* dst = dtable + v * D;
@@ -279,20 +297,21 @@ __global__ __launch_bounds__(kSumWaves * kWave) void sum_pieces(const float* __r
   __shared__ float s[kSumWaves][kSumCols];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int total = *in.total;
-  const int64_t p_lane = (int64_t)blockIdx.x * kSumPieces + lane, a = p_lane * kPiece;
+  const int piece = 1 << in.piece_shift;
+  const int64_t p_lane = (int64_t)blockIdx.x * kSumPieces + lane, a = p_lane * piece;
   int row = 0;
   bool begins = false;
   if (lane < kSumPieces && a < total) {
-    row = in.row_of[(a + kPiece < total ? a + kPiece : total) - 1];
-    begins = in.count[row] > kPiece && in.start[row] >= a;
+    row = in.row_of[(a + piece < total ? a + piece : total) - 1];
+    begins = in.count[row] > piece && in.start[row] >= a;
   }
   uint64_t left = __ballot(begins);
   while (left) {
     const int l = __builtin_ctzll(left);
     left &= left - 1;
     const int v = __builtin_amdgcn_readlane(row, l), start = in.start[v];
-    const int64_t p = (int64_t)blockIdx.x * kSumPieces + l, last = ((int64_t)start + in.count[v] - 1) / kPiece;
-    const int slot = start == p * kPiece ? 0 : 1;
+    const int64_t p = (int64_t)blockIdx.x * kSumPieces + l, last = ((int64_t)start + in.count[v] - 1) >> in.piece_shift;
+    const int slot = start == p << in.piece_shift ? 0 : 1;
     float acc[kSumCols / kWave] = {};
 #pragma unroll 4
     for (int64_t q = p + wave; q <= last; q += kSumWaves) {
@@ -373,7 +392,8 @@ struct Workspace {
 };
 Workspace lay_out(int64_t n, int V, int D) {
   Workspace w{};
-  w.pieces = n > kPiece ? ceil_div(n, kPiece) : 0;
+  const int64_t piece = (int64_t)1 << piece_shift_of(n);
+  w.pieces = n > piece ? ceil_div(n, piece) : 0;
   size_t at = 0;
   auto take = [&](size_t b) {
     const size_t here = at;
@@ -440,13 +460,13 @@ int krsi_embedding_bwd(const void* dout, const void* tokens, int32_t token_bytes
   if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
   char* base = static_cast<char*>(workspace);
   const Groups g{(int32_t*)(base + w.order), (int32_t*)(base + w.row_of), (int32_t*)(base + w.start),
-                 (int32_t*)(base + w.count), (int32_t*)(base + w.total)};
+                 (int32_t*)(base + w.count), (int32_t*)(base + w.total), piece_shift_of(n)};
   float* part = (float*)(base + w.part);
   hipStream_t st = as_stream(stream);
   const int gs = group_shift_of(V);
   const int64_t bytes = (int64_t)V * D * (dtype == kF32 ? 4 : 2);
-  const int64_t fill = ceil_div(bytes, 16 * kGroupThreads * 4);
-  hipLaunchKernelGGL(group_tokens, dim3((1u << gs) + (unsigned)(fill < kFillBlocks ? fill : kFillBlocks)),
+  const int64_t fill = ceil_div(bytes, 16 * kGroupThreads * kFillChunks);
+  hipLaunchKernelGGL(group_tokens, dim3((1u << gs) + (unsigned)fill),
                      dim3(kGroupThreads), 0, st, tokens, (int)token_bytes, (int)n, (int)V, gs, padding, g, (char*)dtable,
                      bytes);
   if (n == 0) return launch_status();
