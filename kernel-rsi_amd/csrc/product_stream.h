@@ -38,10 +38,11 @@ __device__ __forceinline__ int stage_swizzle(int r) {
   return TR ? ((r & 3) | ((r >> 3) & 1) << 2) << 1 : (r >> 1) & 7;
 }
 
+// All sizes fit 31 bits (in 64 the loop's scalars did not fit their registers); element offsets take 64.
 struct Operand {
   const uint16_t* p;
-  int64_t ld;     // elements between rows
-  int64_t extent; // of the output index
+  int ld;      // elements between rows
+  int extent;  // of the output index
 };
 
 template <int WM, int WN, int RB, int CB>
@@ -65,23 +66,22 @@ struct Tiles {
 constexpr int kTileGroup = 4;
 
 struct TileAt {
-  int64_t m0, n0;
-  int split, s0, s1;  // stages [s0, s1)
+  int m0, n0, split, s0, s1;  // stages [s0, s1)
 };
 template <int ROWS, int COLS>
 __device__ __forceinline__ TileAt tile_at(const Tiles& t, int v) {
   const int vv = xcd_tile(v, t.total), tiles = t.nrb * t.ncb, split = vv / tiles, tile = vv - split * tiles;
   const int per_group = kTileGroup * t.ncb, grp = tile / per_group, in_grp = tile - grp * per_group;
   const int gsz = min(kTileGroup, t.nrb - grp * kTileGroup);
-  return TileAt{(int64_t)(grp * kTileGroup + in_grp % gsz) * ROWS, (int64_t)(in_grp / gsz) * COLS, split,
-                split * t.per, min(t.stages, (split + 1) * t.per)};
+  return TileAt{(grp * kTileGroup + in_grp % gsz) * ROWS, in_grp / gsz * COLS, split, split * t.per,
+                min(t.stages, (split + 1) * t.per)};
 }
 
 // Calls epilogue(tile, acc) for every tile of this workgroup: acc[i][j][r] is row 16 (RB wr + i) + l16, column
 // 16 (CB wc + j) + 4 g + r of the tile, for lane 16 g + l16 of wave (wr, wc). The grid is the tiles, or fewer
 // where every part of the sum has two stages at least. lds: Tl::kLds elements on a 512-byte boundary.
 template <int DT, bool TRA, bool TRB, int WM, int WN, int RB, int CB, typename Epilogue>
-__device__ __forceinline__ void stream_products(const Operand a, const Operand b, int64_t sum, const Tiles tiles,
+__device__ __forceinline__ void stream_products(const Operand a, const Operand b, int sum, const Tiles tiles,
                                                 uint16_t* lds, Epilogue&& epilogue) {
   using Tl = StreamTile<WM, WN, RB, CB>;
   uint16_t *const As = lds, *const Bs = lds + 2 * Tl::kA;
@@ -97,7 +97,7 @@ __device__ __forceinline__ void stream_products(const Operand a, const Operand b
   constexpr int kAStep = TRA ? Tl::kThreads * 8 / Tl::kRows : Tl::kThreads * 8 / kStage;  // rows from request to request
   constexpr int kBStep = TRB ? Tl::kThreads * 8 / Tl::kCols : Tl::kThreads * 8 / kStage;
   static_assert(kAStep % 16 == 0 && kBStep % 16 == 0, "whole swizzle periods");
-  auto offset = [&](auto tr, const Operand& o, int64_t o0, int width) {
+  auto offset = [&](auto tr, const Operand& o, int o0, int width) {
     constexpr bool TR = decltype(tr)::value;
     const int chunks = TR ? width / 8 : kStage / 8, r = tid / chunks;
     const int col = 8 * ((tid & (chunks - 1)) ^ stage_swizzle<TR>(r));
@@ -106,36 +106,35 @@ __device__ __forceinline__ void stream_products(const Operand a, const Operand b
   uint32_t aoff, boff;  // they depend on the tile only where TR meets the extent's end
   auto offsets_a = [&](const TileAt& t) { aoff = offset(TagA{}, a, t.m0, Tl::kRows); };
   auto offsets_b = [&](const TileAt& t) { boff = offset(TagB{}, b, t.n0, Tl::kCols); };
-  // A stage's memory: base and bytes up to the operand's end, none where the stage lies past it.
+  // A stage's memory: base and bytes up to the operand's end (less than 2^31), none where the stage lies past it.
   struct Stage {
     const uint16_t *a, *b;
-    uint32_t abytes, bbytes;
+    int abytes, bbytes;
   };
-  auto bytes_of = [](int64_t n) { return (uint32_t)(n > 0 ? n * 2 : 0); };
   auto stage_of = [&](const TileAt& t, int st) {
-    const int64_t k0 = (int64_t)st * kStage, left = sum - k0 < kStage ? sum - k0 : kStage;
+    const int k0 = st * kStage, left = max(min(sum - k0, kStage), 0);
     Stage s;
     if constexpr (TRA) {
-      s.a = a.p + k0 * a.ld + t.m0;
-      s.abytes = bytes_of(left * a.ld - t.m0);
+      s.a = a.p + (int64_t)k0 * a.ld + t.m0;
+      s.abytes = 2 * (left * a.ld - t.m0);
     } else {
-      s.a = a.p + t.m0 * a.ld + k0;
-      s.abytes = bytes_of((a.extent - t.m0 < Tl::kRows ? a.extent - t.m0 : Tl::kRows) * a.ld - k0);
+      s.a = a.p + (int64_t)t.m0 * a.ld + k0;
+      s.abytes = 2 * (min(a.extent - t.m0, Tl::kRows) * a.ld - k0);
     }
     if constexpr (TRB) {
-      s.b = b.p + k0 * b.ld + t.n0;
-      s.bbytes = bytes_of(left * b.ld - t.n0);
+      s.b = b.p + (int64_t)k0 * b.ld + t.n0;
+      s.bbytes = 2 * (left * b.ld - t.n0);
     } else {
-      s.b = b.p + t.n0 * b.ld + k0;
-      s.bbytes = bytes_of((b.extent - t.n0 < Tl::kCols ? b.extent - t.n0 : Tl::kCols) * b.ld - k0);
+      s.b = b.p + (int64_t)t.n0 * b.ld + k0;
+      s.bbytes = 2 * (min(b.extent - t.n0, Tl::kCols) * b.ld - k0);
     }
     return s;
   };
   auto request = [&](const Stage& s, int buf, int i) {
     const bool of_a = i < Tl::kADma;
     const int k = of_a ? i : i - Tl::kADma;
-    const int64_t ahead = of_a ? (int64_t)k * kAStep * a.ld : (int64_t)k * kBStep * b.ld;
-    const int left = (int)(of_a ? s.abytes : s.bbytes) - (int)(ahead * 2);  // an operand's tile has less than 2^31 bytes
+    const int ahead = of_a ? k * kAStep * a.ld : k * kBStep * b.ld;
+    const int left = (of_a ? s.abytes : s.bbytes) - 2 * ahead;
     uint16_t* const to = of_a ? As + buf * Tl::kA : Bs + buf * Tl::kB;
     dma16(make_rsrc((of_a ? s.a : s.b) + ahead, (uint32_t)max(left, 0)), of_a ? aoff : boff,
           (uint32_t)(uintptr_t)(lds_void*)(to + (k * Tl::kThreads + 64 * wv) * 8));
