@@ -30,6 +30,7 @@ constexpr int kMinStages = 8;   // stages of a part of a split sum, at least
 constexpr int kMaxSplits = 64;  // parts of a sum
 
 using Large = StreamTile<2, 4, 8, 4>;  // 256 x 256, 8 waves, one workgroup per CU
+using Medium = StreamTile<2, 4, 6, 4>;  // 192 x 256, 8 waves: of logits (a TR operand's tile is a power of two wide)
 using Small = StreamTile<2, 2, 4, 4>;  // 128 x 128, 4 waves, two per CU
 
 struct Targets {
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
 // lse and loss of each row from its pairs, in a fixed order: 16 rows per workgroup, 64 threads a row, the maximum
 // first, then the sums to its base. (With 16 threads a row that joined pair after pair it took 18 us for 2048 rows
 // of 502 pairs, a third of the memory's rate at 2048 pairs of 8192 rows.)
-constexpr int kJoinRows = 16, kJoinParts = kOneBlock / kJoinRows;
+constexpr int kJoinRows = 16, kJoinParts = kOneBlock / kJoinRows, kJoinHeld = 8;
 __global__ __launch_bounds__(kOneBlock) void join_rows(const float2* __restrict__ part,
                                                        const float* __restrict__ target_logit, Targets targets,
                                                        float* __restrict__ lse, float* __restrict__ loss, int64_t rows,
@@ -114,19 +115,27 @@ __global__ __launch_bounds__(kOneBlock) void join_rows(const float2* __restrict_
   const bool live = row < rows;
   const float2* p = part + (live ? row : 0);
   float m = -__builtin_inff();
+  float2 held[kJoinHeld];
+#pragma unroll
+  for (int k = 0; k < kJoinHeld; ++k) {
+    const int at = q + k * kJoinParts;
+    held[k] = at < slices ? p[(int64_t)at * rows] : float2{m, 0.f};
+  }
+#pragma unroll
+  for (int k = 0; k < kJoinHeld; ++k) m = fmaxf(m, held[k].x);
 #pragma unroll 8
-  for (int k = q; k < slices; k += kJoinParts) m = fmaxf(m, p[(int64_t)k * rows].x);
+  for (int k = q + kJoinHeld * kJoinParts; k < slices; k += kJoinParts) m = fmaxf(m, p[(int64_t)k * rows].x);
   top[q][r] = m;
   __syncthreads();
   m = top[0][r];
 #pragma unroll 8
   for (int k = 1; k < kJoinParts; ++k) m = fmaxf(m, top[k][r]);
   float s = 0.f;
+  auto add = [&](float2 a) { s += a.y == 0.f ? 0.f : a.y * __builtin_amdgcn_exp2f((a.x - m) * kLog2e); };
+#pragma unroll
+  for (int k = 0; k < kJoinHeld; ++k) add(held[k]);
 #pragma unroll 8
-  for (int k = q; k < slices; k += kJoinParts) {
-    const float2 a = p[(int64_t)k * rows];
-    s += a.y == 0.f ? 0.f : a.y * __builtin_amdgcn_exp2f((a.x - m) * kLog2e);
-  }
+  for (int k = q + kJoinHeld * kJoinParts; k < slices; k += kJoinParts) add(p[(int64_t)k * rows]);
   sum[q][r] = s;
   __syncthreads();
   if (q != 0 || !live) return;
@@ -167,43 +176,43 @@ __global__ __launch_bounds__(kOneBlock) void add_losses(const float* __restrict_
 // ----------------------------------------------------------------- backward
 // coef[row] = g_row times 2^k, k such that the largest finite |g| reaches 2^14 .. 2^15; *back = 2^-k. g: the
 // loss's gradient for the row (per row, or one for all, over the rows that count with mean); 0 where
-// ignored, NaN where the target is outside [0, V). rest and, by the workgroups after the first, last are cleared.
+// ignored, NaN where the target is outside [0, V). rest and last are cleared. Per row, workgroup 0 finds the
+// largest and does all rows; else every workgroup knows it and does its share.
 __global__ __launch_bounds__(kOneBlock) void row_weights(const float* __restrict__ dout, bool per_row, bool mean,
                                                          const float* __restrict__ counted, Targets targets,
-                                                         int64_t rows, float* __restrict__ coef,
+                                                         int rows, float* __restrict__ coef,
                                                          float* __restrict__ rest, int* last,
                                                          float* __restrict__ back) {
   __shared__ float s[kOneBlock / kWave];
-  if (blockIdx.x > 0) {
-    const int v = 4 * ((blockIdx.x - 1) * kOneBlock + threadIdx.x);  // the array is padded to whole chunks
-    if (v < targets.V) *reinterpret_cast<u32x4*>(last + v) = u32x4{~0u, ~0u, ~0u, ~0u};
-    return;
-  }
-  const float share = mean ? 1.f / *counted : 1.f;
-  auto weight = [&](int64_t r) {
+  const int me = blockIdx.x * kOneBlock + threadIdx.x, all = gridDim.x * kOneBlock;
+  for (int v = 4 * me; v < targets.V; v += 4 * all)  // the array is padded to whole chunks
+    *reinterpret_cast<u32x4*>(last + v) = u32x4{~0u, ~0u, ~0u, ~0u};
+  if (per_row && blockIdx.x > 0) return;
+  const float one = per_row ? 0.f : *dout * (mean ? 1.f / *counted : 1.f);
+  auto weight = [&](int r) {
     if (targets.ignored(r)) return 0.f;
-    return targets.at(r) < 0 ? __builtin_nanf("") : dout[per_row ? r : 0] * share;
+    return targets.at(r) < 0 ? __builtin_nanf("") : per_row ? dout[r] : one;
   };
-  float top = 0.f;
-  for (int64_t r = threadIdx.x; r < rows; r += kOneBlock) {
-    const float a = fabsf(weight(r));
-    top = a <= 3.4028234663852886e38f ? fmaxf(top, a) : top;
+  auto finite = [](float a) { return a <= 3.4028234663852886e38f ? a : 0.f; };
+  float top = finite(fabsf(one));
+  if (per_row) {
+    for (int r = threadIdx.x; r < rows; r += kOneBlock) top = fmaxf(top, finite(fabsf(weight(r))));
+    for (int m = kWave / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
+    if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x / kWave] = top;
+    __syncthreads();
+    for (int w = 0; w < kOneBlock / kWave; ++w) top = fmaxf(top, s[w]);
   }
-  for (int m = kWave / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
-  if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x / kWave] = top;
-  __syncthreads();
-  for (int w = 0; w < kOneBlock / kWave; ++w) top = fmaxf(top, s[w]);
   int k = 0;
   if (top > 0.f) {
     frexpf(top, &k);  // top = f 2^k, f in [1/2, 1)
     k = min(max(15 - k, -126), 126);
   }
   const float scale = ldexpf(1.f, k);
-  for (int64_t r = threadIdx.x; r < rows; r += kOneBlock) {
+  for (int r = per_row ? threadIdx.x : me; r < rows; r += per_row ? kOneBlock : all) {
     coef[r] = weight(r) * scale;
     rest[r] = 0.f;
   }
-  if (threadIdx.x == 0) *back = ldexpf(1.f, -k);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *back = ldexpf(1.f, -k);
 }
 
 // dl [rows, ld] of the piece of the vocabulary that starts at v0 (w and its extent are the piece's): zero past it.
@@ -382,26 +391,30 @@ Tiles tiles_of(int64_t M, int64_t N, int64_t sum, int splits) {
   return t;
 }
 struct Plan {
-  bool large;
+  int tile;  // 0: Large, 1: Medium, 2: Small
   Tiles tiles;
 };
-// The tile, and the parts of the sum where it may be cut, by an estimate in stages of the large tile (1.6 us on a
+// The tile, and (not of logits, which are reduced whole) the parts of the sum, by an estimate in stages of the large tile (1.6 us on a
 // CU at full rate): rounds of workgroups times the stages of each and its epilogue (4, or 8 where it writes fp32
-// parts, which all CUs do at once), and the parts' addition (4 M N bytes per part at 5 TB/s). The small tile has a
-// quarter of the work, two workgroups per CU share it, and it takes 1.2 times as long for the same work
-// (geglu_linear's measurement of the two).
-Plan plan_product(int64_t M, int64_t N, int64_t sum, bool split) {
+// parts, which all CUs do at once), and the parts' addition (4 M N bytes per part at 5 TB/s). The medium tile has
+// three quarters of the work and takes 1.15 times as long for the same (bf16 [300, 1152], V 32128: 29 us, the large one
+// 36; [4099, 2048], V 50257: 755, 736); the small one has a quarter, two workgroups per CU share it,
+// and it takes 1.2 times as long for the same work (geglu_linear's measurement of the two).
+Plan plan_product(int64_t M, int64_t N, int64_t sum, bool logits) {
   Plan best{};
   double least = 0;
-  const int64_t stages = ceil_div(sum, kStage), most = split ? stages / kMinStages : 1;
+  const int64_t stages = ceil_div(sum, kStage), most = logits ? 1 : stages / kMinStages;
   for (int s = 1; s == 1 || (s <= most && s <= kMaxSplits); ++s) {
-    for (bool large : {true, false}) {
-      const Tiles t = large ? tiles_of<Large>(M, N, sum, s) : tiles_of<Small>(M, N, sum, s);
-      const double each = (t.per + (s > 1 ? 8 : 4)) * (large ? 1.0 : 0.6);
-      const double cost = (double)ceil_div(t.total, 256 * (large ? Large::kPerCu : Small::kPerCu)) * each +
+    for (int tile = 0; tile < 3; ++tile) {
+      if (tile == 1 && !logits) continue;
+      const Tiles t = tile == 0   ? tiles_of<Large>(M, N, sum, s)
+                      : tile == 1 ? tiles_of<Medium>(M, N, sum, s)
+                                  : tiles_of<Small>(M, N, sum, s);
+      const double each = (t.per + (s > 1 ? 8 : 4)) * (tile == 0 ? 1.0 : tile == 1 ? 0.86 : 0.6);
+      const double cost = (double)ceil_div(t.total, 256 * (tile == 2 ? Small::kPerCu : 1)) * each +
                           (s > 1 ? 5e-7 * (double)M * (double)N * s : 0);
       if (best.tiles.total == 0 || cost < least) {
-        best = Plan{large, t};
+        best = Plan{tile, t};
         least = cost;
       }
     }
@@ -416,12 +429,21 @@ struct Shape {
   using Tl = StreamTile<WM, WN, RB, CB>;
 };
 template <typename F>
-void with_tile(const Plan& p, F&& f) {
-  if (p.large)
+void with_grad_tile(const Plan& p, F&& f) {
+  if (p.tile == 0)
     f(Shape<2, 4, 8, 4>{});
   else
     f(Shape<2, 2, 4, 4>{});
 }
+template <typename F>
+void with_logits_tile(const Plan& p, F&& f) {
+  if (p.tile == 1)
+    f(Shape<2, 4, 6, 4>{});
+  else
+    with_grad_tile(p, f);
+}
+int rows_of(const Plan& p) { return p.tile == 0 ? Large::kRows : p.tile == 1 ? Medium::kRows : Small::kRows; }
+int cols_of(const Plan& p) { return p.tile == 2 ? Small::kCols : Large::kCols; }
 
 struct Forward {
   Plan plan;
@@ -430,8 +452,8 @@ struct Forward {
 };
 Forward plan_forward(int64_t rows, int K, int V) {
   Forward f{};
-  f.plan = plan_product(rows, V, K, false);
-  f.slices = f.plan.tiles.ncb * (f.plan.large ? Large::kCols : Small::kCols) / 64;
+  f.plan = plan_product(rows, V, K, true);
+  f.slices = f.plan.tiles.ncb * cols_of(f.plan) / 64;
   size_t at = 0;
   auto take = [&](size_t b) {
     const size_t here = at;
@@ -457,8 +479,8 @@ Backward plan_backward(int64_t rows, int K, int V) {
   b.width = (int)(ceil_div(ceil_div(V, b.pieces), 256) * 256);
   b.pieces = (int)ceil_div(V, b.width);
   const int whole = V < b.width ? V : b.width;
-  b.dx = plan_product(rows, K, whole, true);
-  b.dw = plan_product(whole, K, rows, true);
+  b.dx = plan_product(rows, K, whole, false);
+  b.dw = plan_product(whole, K, rows, false);
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t here = at;
@@ -497,7 +519,7 @@ int forward(const Operand& x, const Operand& w, int K, const Targets& t, float* 
   float2* part = (float2*)(ws + f.part);
   float* target_logit = (float*)(ws + f.target_logit);
   float* row_loss = reduction == 0 ? loss : (float*)(ws + f.loss);
-  with_tile(f.plan, [&](auto s) {
+  with_logits_tile(f.plan, [&](auto s) {
     using S = decltype(s);
     hipLaunchKernelGGL((logits_reduce<DT, S::WM, S::WN, S::RB, S::CB>), dim3(stream_grid<typename S::Tl>(f.plan.tiles)),
                        dim3(S::Tl::kThreads), 0, st, x, w, K, f.plan.tiles, t, part, target_logit);
@@ -519,7 +541,7 @@ void launch_product(const Plan& pl, const Operand& a, const Operand& b, int sum,
                        dim3(stream_grid<typename S::Tl>(pl.tiles)), dim3(S::Tl::kThreads), 0, st, a, b, sum, pl.tiles, M, N,
                        back, rest, out, part, add);
   };
-  with_tile(pl, [&](auto s) {
+  with_grad_tile(pl, [&](auto s) {
     if (part)
       launch(s, std::true_type{});
     else
@@ -536,15 +558,15 @@ int backward(const float* dout, const Operand& x, const Operand& w, int K, const
   int* last = (int*)(ws + b.last);
   const Rest to_dx{rest, w.p, nullptr, t};
   uint16_t* dl = (uint16_t*)(ws + b.dl);
-  hipLaunchKernelGGL(row_weights, dim3(1 + (unsigned)ceil_div(V, 4 * kOneBlock)), dim3(kOneBlock), 0, st, dout, reduction == 0, reduction == 1, stats + rows, t,
+  hipLaunchKernelGGL(row_weights, dim3((unsigned)ceil_div(rows + V / 4, 4 * kOneBlock)), dim3(kOneBlock), 0, st, dout, reduction == 0, reduction == 1, stats + rows, t,
                      rows, coef, rest, last, back);
   const bool dx_parts = b.dx.tiles.splits > 1 || b.pieces > 1;
   float* dx_part = dx_parts ? (float*)(ws + b.dx_part) : nullptr;
   for (int p = 0; p < b.pieces; ++p) {
     const int v0 = p * b.width, valid = V - v0 < b.width ? V - v0 : b.width;
     const Operand piece{w.p + (int64_t)v0 * K, K, valid};
-    const Plan lg = plan_product(rows, b.width, K, false);
-    with_tile(lg, [&](auto s) {
+    const Plan lg = plan_product(rows, b.width, K, true);
+    with_logits_tile(lg, [&](auto s) {
       using S = decltype(s);
       hipLaunchKernelGGL((logits_grad<DT, S::WM, S::WN, S::RB, S::CB>), dim3(stream_grid<typename S::Tl>(lg.tiles)),
                          dim3(S::Tl::kThreads), 0, st, x, piece, K, lg.tiles, t, v0, stats, (const float*)coef, rest, last, dl,
@@ -562,7 +584,7 @@ int backward(const float* dout, const Operand& x, const Operand& w, int K, const
     }
     if (dw) {
       Plan pl = b.dw;
-      pl.tiles.nrb = (int)ceil_div(valid, pl.large ? Large::kRows : Small::kRows);
+      pl.tiles.nrb = (int)ceil_div(valid, rows_of(pl));
       pl.tiles.total = pl.tiles.nrb * pl.tiles.ncb * pl.tiles.splits;
       const bool parts = pl.tiles.splits > 1;
       float* dw_part = parts ? (float*)(ws + b.dw_part) : nullptr;
