@@ -241,8 +241,8 @@ int krsi_relpos_bucket_sum(const float* dpd, const int32_t* bucket, float* dtabl
  *   (i, i + R/2), or (2i, 2i + 1) with interleaved = 1, of the first R columns; y = z in the others.
  * fp32 from the load to the store, one rounding. Backward: dqkv [tokens, ld_dqkv] (its first (H + 2 KH) D
  * columns are written), dwq and dwk [D], summed in fp32 in a fixed order; dout as out.
- * Limits: D % 8 == 0, 8 <= D <= 128, R even, 2 <= R <= D; tokens < 2^31, table_rows >= min(S, tokens) without
- * positions. No tokens: dwq and dwk are zero. workspace: krsi_qk_norm_rope_bwd_workspace_bytes(D), scratch.  */
+ * Limits: D % 8 == 0, 8 <= D <= 128, R even, 2 <= R <= D; tokens < 2^31 (and waves below 2^26:
+ * tokens * (H + 2 KH) <= 2^26 fits at every D), table_rows >= min(S, tokens) without positions. No tokens: dwq and dwk are zero. workspace: krsi_qk_norm_rope_bwd_workspace_bytes(D), scratch.  */
 int krsi_qk_norm_rope_fwd(const void* qkv, int64_t ld_qkv, const void* wq, const void* wk, const float* rope,
                           const void* positions, void* out, int64_t tokens, int32_t S, int32_t H, int32_t KH,
                           int32_t D, int32_t R, int64_t table_rows, int32_t position_bytes, float eps,
@@ -260,7 +260,7 @@ int krsi_qk_norm_rope_bwd(const void* dout, const void* qkv, int64_t ld_qkv, con
  * Backward: dtable[v, :] = T(scale * sum of dout[t, :] over tokens[t] == v), every row written, fp32 sums in an
  * order that the tokens alone decide (no float atomics); tokens outside [0, V) or equal to padding (-1: none)
  * have no part. workspace: krsi_embedding_bwd_workspace_bytes, scratch.
- * Limits: n <= 2^30, V <= 2^24, D <= 2^20, scale finite. n = 0: dtable is zero.                           */
+ * Limits: n <= 2^25, V <= 2^24, D <= 2^20, scale finite. n = 0: dtable is zero.                           */
 int krsi_embedding_fwd(const void* tokens, int32_t token_bytes, const void* table, void* out, int64_t n, int32_t V,
                        int32_t D, float scale, int32_t dtype, void* stream);
 size_t krsi_embedding_bwd_workspace_bytes(int64_t n, int32_t V, int32_t D);
@@ -277,8 +277,10 @@ int krsi_embedding_bwd(const void* dout, const void* tokens, int32_t token_bytes
  * Backward: dout fp32, [rows] or [1]; dx [rows, k] and dw [v, k] of T, either may be NULL (not wanted). The logits
  * are computed again in pieces of the vocabulary, whose gradient is rounded to T times a power of two that
  * keeps the largest at the top of fp16's range. Sums are fp32, in a fixed order.
- * Limits: k % 64 == 0, k <= 2^20, v <= 2^24, rows <= 2^24. No rows: loss 0 or NaN, dw zero. Workspaces: the
- * *_workspace_bytes (the backward's holds a piece of rows x v of about 512 MB at most, and fp32 parts of dx). */
+ * Limits: k % 64 == 0, k <= 2^20, v and rows <= 2^23 (ceil(rows / 128) ceil(v / 128) <= 2^23, of v and k as
+ * well, of rows and k <= 2^18). No rows: loss 0 or NaN, dw zero. Workspaces: the *_workspace_bytes (the forward's
+ * holds 8 bytes per row and 64 logits, of about 512 MB's worth of rows at a time; the backward's a piece of rows x v,
+ * 512 MB or 4096 columns wide, and fp32 parts of dx). */
 size_t krsi_linear_cross_entropy_fwd_workspace_bytes(int64_t rows, int32_t k, int32_t v);
 size_t krsi_linear_cross_entropy_bwd_workspace_bytes(int64_t rows, int32_t k, int32_t v);
 int krsi_linear_cross_entropy_fwd(const void* x, const void* w, const void* targets, int32_t target_bytes, float* loss,

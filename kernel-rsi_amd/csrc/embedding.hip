@@ -412,7 +412,7 @@ Workspace lay_out(int64_t n, int V, int D) {
 
 int check(int64_t n, int V, int D, int token_bytes, float scale, int dtype) {
   if (dtype != kBf16 && dtype != kF16 && dtype != kF32) return KRSI_ERR_UNSUPPORTED;
-  if (n < 0 || n > (1 << 30) || V <= 0 || V > (1 << 24) || D <= 0 || D > (1 << 20))
+  if (n < 0 || n > (1 << 25) || V <= 0 || V > (1 << 24) || D <= 0 || D > (1 << 20))
     return KRSI_ERR_BAD_SHAPE;
   if (token_bytes != 4 && token_bytes != 8) return KRSI_ERR_UNSUPPORTED;
   if (!(scale == scale) || scale > 3.0e38f || scale < -3.0e38f) return KRSI_ERR_BAD_SCALE;

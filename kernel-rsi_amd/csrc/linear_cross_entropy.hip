@@ -4,7 +4,7 @@
 //   dl_nv = (exp(l_nv - lse_n) - [v = target(n)]) g_n,   dx = dl w,   dw = dl^T x
 // Forward: the products' epilogue reduces each wave's 64 columns of a row to a maximum and a sum of exponentials in
 // registers, and keeps the target's logit; a second launch joins a row's pairs, a third adds the losses.
-// Backward, in pieces of the vocabulary (kPieceBytes of dl each): the products again, whose epilogue forms dl, rounded
+// Backward, in pieces of the vocabulary (512 MB of dl each, or 4096 columns): the products again, whose epilogue forms dl, rounded
 // to T; then dw of the piece's rows and the piece's part of dx, which is carried in fp32 from piece to piece.
 // What dl's rounding takes from the target's entry, the largest of a row, is kept in fp32 per row (its rest) and
 // comes back into dx, and into dw's row of the target from the last of the rows that have it (rows of w that many
@@ -24,7 +24,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kOneBlock = 1024;
-constexpr int64_t kPieceBytes = int64_t(512) << 20;
+constexpr int64_t kPieceBytes = int64_t(512) << 20;  // of dl in the backward, and of a row's pairs in the forward
+constexpr int64_t kMinWidth = 4096;  // columns of a piece at least: dx's fp32 sums are read and written once per piece
 constexpr int64_t kMaxWidth = 1 << 20;  // columns of a piece: 64 rows of dl stay below 2^31 bytes
 constexpr int kMinStages = 8;   // stages of a part of a split sum, at least
 constexpr int kMaxSplits = 64;  // parts of a sum
@@ -394,12 +395,12 @@ struct Plan {
   int tile;  // 0: Large, 1: Medium, 2: Small
   Tiles tiles;
 };
-// The tile, and (not of logits, which are reduced whole) the parts of the sum, by an estimate in stages of the large tile (1.6 us on a
-// CU at full rate): rounds of workgroups times the stages of each and its epilogue (4, or 8 where it writes fp32
-// parts, which all CUs do at once), and the parts' addition (4 M N bytes per part at 5 TB/s). The medium tile has
-// three quarters of the work and takes 1.15 times as long for the same (bf16 [300, 1152], V 32128: 29 us, the large one
-// 36; [4099, 2048], V 50257: 755, 736); the small one has a quarter, two workgroups per CU share it,
-// and it takes 1.2 times as long for the same work (geglu_linear's measurement of the two).
+// The tile, and (not of logits, which are reduced whole) the parts of the sum, by an estimate in stages of the large
+// tile (1.6 us on a CU at full rate): rounds of workgroups times the stages of each and its epilogue (4, or 8 where it
+// writes fp32 parts, which all CUs do at once), and the parts' addition (4 M N bytes per part at 5 TB/s). The medium
+// tile has three quarters of the work and takes 1.15 times as long for the same (bf16 [300, 1152], V 32128: 29 us, the
+// large one 36; [4099, 2048], V 50257: 755, 736); the small one has a quarter, two workgroups per CU share it, and it
+// takes 1.2 times as long for the same work (geglu_linear's measurement of the two).
 Plan plan_product(int64_t M, int64_t N, int64_t sum, bool logits) {
   Plan best{};
   double least = 0;
@@ -446,22 +447,21 @@ int rows_of(const Plan& p) { return p.tile == 0 ? Large::kRows : p.tile == 1 ? M
 int cols_of(const Plan& p) { return p.tile == 2 ? Small::kCols : Large::kCols; }
 
 struct Forward {
-  Plan plan;
-  int slices;
+  int chunk;  // rows whose pairs are kept at a time
   size_t part, target_logit, loss, bytes;
 };
 Forward plan_forward(int64_t rows, int K, int V) {
   Forward f{};
-  f.plan = plan_product(rows, V, K, true);
-  f.slices = f.plan.tiles.ncb * cols_of(f.plan) / 64;
+  const int64_t pairs = ceil_div(V, 256) * 4, fit = kPieceBytes / (pairs * (int64_t)sizeof(float2)) / 256 * 256;
+  f.chunk = (int)(rows < 2048 || rows < fit ? rows : fit < 2048 ? 2048 : fit);
   size_t at = 0;
   auto take = [&](size_t b) {
     const size_t here = at;
     at += align256(b);
     return here;
   };
-  f.part = take((size_t)f.slices * rows * sizeof(float2));
-  f.target_logit = take((size_t)rows * 4);
+  f.part = take((size_t)pairs * f.chunk * sizeof(float2));
+  f.target_logit = take((size_t)f.chunk * 4);
   f.loss = take((size_t)rows * 4);
   f.bytes = at;
   return f;
@@ -475,7 +475,7 @@ struct Backward {
 Backward plan_backward(int64_t rows, int K, int V) {
   Backward b{};
   const int64_t cols = ceil_div(V, 256) * 256, fit = kPieceBytes / (rows * 2) / 256 * 256;
-  b.pieces = (int)ceil_div(cols, fit < 256 ? 256 : fit < kMaxWidth ? fit : kMaxWidth);
+  b.pieces = (int)ceil_div(cols, fit < kMinWidth ? kMinWidth : fit < kMaxWidth ? fit : kMaxWidth);
   b.width = (int)(ceil_div(ceil_div(V, b.pieces), 256) * 256);
   b.pieces = (int)ceil_div(V, b.width);
   const int whole = V < b.width ? V : b.width;
@@ -503,10 +503,10 @@ int check(int64_t rows, int32_t k, int32_t v, int32_t target_bytes, int32_t redu
   if (target_bytes != 4 && target_bytes != 8) return KRSI_ERR_UNSUPPORTED;
   if (reduction < 0 || reduction > 2) return KRSI_ERR_UNSUPPORTED;
   if (rows < 0 || k <= 0 || v <= 0) return KRSI_ERR_BAD_SHAPE;
-  // Whole stages of K; byte offsets of a staged tile below 2^31, tile counts of int.
-  if (k % kStage != 0 || k > (1 << 20) || v > (1 << 24) || rows > (1 << 24)) return KRSI_ERR_UNSUPPORTED;
-  if (ceil_div(rows, 128) * ceil_div(v, 128) > (1 << 30) || ceil_div(rows, 128) * ceil_div(k, 128) > (1 << 20) ||
-      ceil_div(v, 128) * ceil_div(k, 128) > (1 << 30))
+  // Whole stages of K; byte offsets of a staged tile below 2^31; grids of less than 2^32 threads.
+  if (k % kStage != 0 || k > (1 << 20) || v > (1 << 23) || rows > (1 << 23)) return KRSI_ERR_UNSUPPORTED;
+  if (ceil_div(rows, 128) * ceil_div(v, 128) > (1 << 23) || ceil_div(rows, 128) * ceil_div(k, 128) > (1 << 18) ||
+      ceil_div(v, 128) * ceil_div(k, 128) > (1 << 23))
     return KRSI_ERR_UNSUPPORTED;
   return KRSI_OK;
 }
@@ -519,13 +519,19 @@ int forward(const Operand& x, const Operand& w, int K, const Targets& t, float* 
   float2* part = (float2*)(ws + f.part);
   float* target_logit = (float*)(ws + f.target_logit);
   float* row_loss = reduction == 0 ? loss : (float*)(ws + f.loss);
-  with_logits_tile(f.plan, [&](auto s) {
-    using S = decltype(s);
-    hipLaunchKernelGGL((logits_reduce<DT, S::WM, S::WN, S::RB, S::CB>), dim3(stream_grid<typename S::Tl>(f.plan.tiles)),
-                       dim3(S::Tl::kThreads), 0, st, x, w, K, f.plan.tiles, t, part, target_logit);
-  });
-  hipLaunchKernelGGL(join_rows, dim3((unsigned)ceil_div(rows, kJoinRows)), dim3(kOneBlock), 0, st, (const float2*)part,
-                     (const float*)target_logit, t, stats, row_loss, rows, f.slices);
+  for (int r0 = 0; r0 < rows; r0 += f.chunk) {
+    const Operand xr{x.p + (int64_t)r0 * K, K, rows - r0 < f.chunk ? rows - r0 : f.chunk};
+    const Targets tr{(const char*)t.p + (int64_t)r0 * t.bytes, t.bytes, t.V, t.ignore};
+    const Plan pl = plan_product(xr.extent, w.extent, K, true);
+    with_logits_tile(pl, [&](auto s) {
+      using S = decltype(s);
+      hipLaunchKernelGGL((logits_reduce<DT, S::WM, S::WN, S::RB, S::CB>), dim3(stream_grid<typename S::Tl>(pl.tiles)),
+                         dim3(S::Tl::kThreads), 0, st, xr, w, K, pl.tiles, tr, part, target_logit);
+    });
+    hipLaunchKernelGGL(join_rows, dim3((unsigned)ceil_div(xr.extent, kJoinRows)), dim3(kOneBlock), 0, st,
+                       (const float2*)part, (const float*)target_logit, tr, stats + r0, row_loss + r0,
+                       (int64_t)xr.extent, pl.tiles.ncb * cols_of(pl) / 64);
+  }
   if (reduction != 0)
     hipLaunchKernelGGL(add_losses, dim3(1), dim3(kOneBlock), 0, st, (const float*)row_loss, t, rows, reduction == 1, loss,
                        stats + rows);

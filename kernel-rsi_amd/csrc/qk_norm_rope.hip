@@ -313,7 +313,7 @@ template <int DT, int C, bool INTER>
 int launch_fwd(Args a, void* out, hipStream_t st) {
   lay_out(a, C, kU);
   const int64_t waves = a.tokens * a.per;
-  if (waves > 0x7fffffff) return KRSI_ERR_BAD_SHAPE;
+  if (waves >= (1 << 26)) return KRSI_ERR_BAD_SHAPE;  // grids of less than 2^32 threads
   hipLaunchKernelGGL((qk_norm_rope_fwd<DT, C, kU, INTER>), dim3((unsigned)ceil_div(waves, kWaves)), dim3(kThreads), 0,
                      st, a, (typename Elem<DT>::T*)out);
   return launch_status();
@@ -326,7 +326,7 @@ int launch_bwd(Args a, const void* dy, void* dx, int64_t lddx, void* dwq, void* 
   if (a.tokens > 0) {
     lay_out(a, C, kU);
     const int64_t waves = a.tokens * a.per;
-    if (waves > 0x7fffffff) return KRSI_ERR_BAD_SHAPE;
+    if (waves >= (1 << 26)) return KRSI_ERR_BAD_SHAPE;  // grids of less than 2^32 threads
     const int64_t need = ceil_div(waves, kWaves);
     blocks = (int)(need < bwd_blocks(C) ? need : bwd_blocks(C));
     hipLaunchKernelGGL((qk_norm_rope_bwd<DT, C, kU, INTER>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a,

@@ -97,6 +97,21 @@ def test_pieces_of_the_vocabulary(dt):
     _verify(out, *torch.autograd.grad(out, leaves, dout), x, w, targets, dout, device="cuda")
 
 
+def test_rows_in_chunks():
+    """More rows than the forward keeps pairs of at a time: the rows' losses are those of the chunks alone."""
+    rows, K, V = 4300, 64, 1 << 20
+    log(f"linear_cross_entropy in chunks of rows x[{rows},{K}] w[{V},{K}]")
+    x, w, targets = _inputs(rows, K, V, torch.bfloat16)
+    targets[[5, 4200]] = -100
+    with torch.no_grad():
+        out = L.linear_cross_entropy(x, w, targets, reduction="none")
+        parts = [L.linear_cross_entropy(x[a:b], w, targets[a:b], reduction="none") for a, b in ((0, 4096), (4096, rows))]
+        assert torch.equal(out, torch.cat(parts))
+        some = torch.arange(0, rows, 173, device="cuda")
+        ref = torch.nn.functional.cross_entropy(x[some].double() @ w.double().t(), targets[some], reduction="none")
+        assert ((out[some].double() - ref).abs() < 2e-4).all()  # 2 K u 10 + (64 + V / 1024 + 8 * 14) u = 1.5e-4
+
+
 def test_gradient_scales_exactly():
     """dout times a power of two: the gradients times that power, bitwise (dl's own scale is one too)."""
     log("linear_cross_entropy gradient scale")
