@@ -58,40 +58,55 @@ __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu *
   const int wr = wave / WN, wc = wave % WN;
   const int rows = x.extent, V = w.extent;
   stream_products<DT, false, false, WM, WN, RB, CB>(x, w, K, tiles, lds, [&](const TileAt& t, f32x4(&acc)[RB][CB]) {
-    const int col0 = t.n0 + 16 * CB * wc + 4 * g;
+    const int col0 = t.n0 + 16 * CB * wc + 4 * g, row0 = t.m0 + 16 * RB * wr + l16;
     const int slice = t.n0 / (16 * CB) + wc;
+    // Every step for all rows before the next step: loads, then lane exchanges, overlap (row after row the epilogue
+    // took as long as five stages).
+    int at[RB];
+#pragma unroll
+    for (int i = 0; i < RB; ++i) at[i] = targets.at(min(row0 + 16 * i, rows - 1)) - col0;
     auto reduce = [&](auto whole) {  // a tile within the vocabulary, or one that ends past it
       constexpr bool WHOLE = decltype(whole)::value;
+      float m[RB], s[RB];
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
-        const int row = t.m0 + 16 * (RB * wr + i) + l16;
-        float m = -__builtin_inff();
+        m[i] = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < CB; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if (!WHOLE && col0 + 16 * j + r >= V) acc[i][j][r] = -__builtin_inff();
-            m = fmaxf(m, acc[i][j][r]);
+            m[i] = fmaxf(m[i], acc[i][j][r]);
           }
-        m = fmaxf(m, __shfl_xor(m, 16, kWave));
-        m = fmaxf(m, __shfl_xor(m, 32, kWave));
-        const float base = m == -__builtin_inff() ? 0.f : m;
-        float s = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < RB; ++i) m[i] = fmaxf(m[i], __shfl_xor(m[i], 16, kWave));
+#pragma unroll
+      for (int i = 0; i < RB; ++i) m[i] = fmaxf(m[i], __shfl_xor(m[i], 32, kWave));
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const float base = m[i] == -__builtin_inff() ? 0.f : m[i];
+        s[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < CB; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * kLog2e);
-        s += __shfl_xor(s, 16, kWave);
-        s += __shfl_xor(s, 32, kWave);
+          for (int r = 0; r < 4; ++r) s[i] += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * kLog2e);
+      }
+#pragma unroll
+      for (int i = 0; i < RB; ++i) s[i] += __shfl_xor(s[i], 16, kWave);
+#pragma unroll
+      for (int i = 0; i < RB; ++i) s[i] += __shfl_xor(s[i], 32, kWave);
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const int row = row0 + 16 * i;
         if (row >= rows) continue;
-        if (g == 0) part[(int64_t)slice * rows + row] = float2{m, s};
-        const int at = targets.at(row) - col0;
-        if ((unsigned)at < 16 * CB && (at & 15) < 4) {
+        if (g == 0) part[(int64_t)slice * rows + row] = float2{m[i], s[i]};
+        if ((unsigned)at[i] < 16 * CB && (at[i] & 15) < 4) {
 #pragma unroll
           for (int j = 0; j < CB; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (at == 16 * j + r) target_logit[row] = acc[i][j][r];
+              if (at[i] == 16 * j + r) target_logit[row] = acc[i][j][r];
         }
       }
     };
