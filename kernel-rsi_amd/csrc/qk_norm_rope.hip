@@ -12,10 +12,14 @@
 // heads of 128]: forward 69.6 us (5.8 TB/s), backward 112 us (4.8 TB/s); a copy of 2 GB runs at 4.9.
 // Outputs are stored past the caches (73 and 114 us without).
 // Layout: a lane holds C elements of one half of the pairs and the C elements that they rotate with, so the
-// rotation stays in registers; D / (2 C) lanes (rounded up to a power of two, the group) hold a head and reduce its
-// square sum by shuffles. C is the widest of 8, 4, 2, 1 (16 bytes at most) that cuts both R / 2 and the rest
-// evenly. A wave takes one token's cos and sin into registers and runs that token's heads past them, 64 /
-// group at a time, U times with all loads first.
+// rotation stays in registers; the lanes of a head (their number rounded up to a power of two, the group) reduce its
+// square sum by shuffles. C is the widest of 8, 4, 2, 1 (16 bytes at most) that a half of the rotated columns and
+// of the rest holds; where it does not divide them the last lane's columns end at the half's end, and those that
+// it shares with the lane before count once in a sum. (With the widest C that divides them, bf16 [16384, 48 heads of
+// 72]: 64 / 108 us forward / backward, here 46 / 108; where 36 columns rotate, 98 / 171, here 46 / 99.)
+// A wave takes a token's cos and sin into registers and runs that token's heads past them, 64 / group at a time,
+// twice with all loads first. Where a token has fewer heads than that, a wave takes as many tokens as fill it
+// ([16384, 4 heads of 64]: 9.3 / 29.6 us with one, 4.6 / 15.1).
 #include "chunks.h"
 #include "krsi_device.h"
 #include "krsi_internal.h"
@@ -41,18 +45,27 @@ struct Args {
   int S, H, KH, D, R, position_bytes;
   int lanes, rotating;  // lanes that hold a head, and how many of them rotate
   int group_shift;      // log2 of the group
-  int per;              // waves' worth of heads per token
+  int heads_shift;      // log2 of the heads of one token that a wave runs at a time
+  int per;              // waves' worth of heads per token; 0: a wave takes more than one token at a time
   float eps;
 };
 
-// This lane's columns of a head: C from e0 and C from e1. Interleaved pairs lie within the 2 C columns from e0.
+// This lane's columns of a head: C from e0 and C from e1, of which the first dup0 and dup1 are another lane's too.
+// Interleaved pairs lie within the 2 C columns from e0.
 template <int C, bool INTER>
 struct Columns {
-  int e0, e1;
+  int e0, e1, dup0, dup1;
+  bool rotates;
   __device__ __forceinline__ Columns(const Args& a, int p) {
-    e0 = INTER || p >= a.rotating ? 2 * p * C : p * C;
-    e1 = INTER || p >= a.rotating ? e0 + C : a.R / 2 + p * C;
+    rotates = p < a.rotating;
+    const int i = rotates ? p : p - a.rotating, base = rotates ? 0 : a.R, half = (rotates ? a.R : a.D - a.R) / 2;
+    const int at = min(i * C, half - C), dup = i * C - at;  // of a half; of both halves' pairs where interleaved
+    e0 = base + (INTER ? 2 * at : at);
+    e1 = INTER ? e0 + C : e0 + half;
+    dup0 = INTER ? min(2 * dup, C) : dup;
+    dup1 = INTER ? max(2 * dup - C, 0) : dup;
   }
+  __device__ __forceinline__ bool shared(int j) const { return j < C ? j < dup0 : j - C < dup1; }
 };
 // Element j of the lane's 2 C as a[i], b[i] of pair i: identity where halves rotate, even and odd where interleaved.
 template <int C, bool INTER>
@@ -65,27 +78,21 @@ __device__ __forceinline__ int64_t position_of(const Args& a, int64_t t) {
   return load_index(a.positions, a.position_bytes, t);
 }
 
-// cos and sin of the lane's pairs at token t: 1 and 0 for lanes past R, NaN for a position outside the table.
-template <int C>
-__device__ __forceinline__ void load_rotation(const Args& a, int64_t t, int p, float* c, float* s) {
+// cos and sin of the lane's pairs at token t, NaN for a position outside the table. A lane that does not rotate loads
+// others and does not use them.
+template <int C, bool INTER>
+__device__ __forceinline__ void load_rotation(const Args& a, const Columns<C, INTER>& col, int64_t t, float* c,
+                                              float* s) {
   const int64_t pos = position_of(a, t);
   const bool inside = pos >= 0 && pos < a.table_rows;
-  if (p < a.rotating) {
-    const float* row = a.rope + (inside ? pos : 0) * a.R + p * C;
-    Piece<kF32, C> pc, ps;
-    pc.load(row);
-    ps.load(row + a.R / 2);
+  const float* row = a.rope + (inside ? pos : 0) * a.R + (col.rotates ? INTER ? col.e0 / 2 : col.e0 : 0);
+  Piece<kF32, C> pc, ps;
+  pc.load(row);
+  ps.load(row + a.R / 2);
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      c[j] = inside ? pc.e[j] : __builtin_nanf("");
-      s[j] = inside ? ps.e[j] : __builtin_nanf("");
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      c[j] = 1.f;
-      s[j] = 0.f;
-    }
+  for (int j = 0; j < C; ++j) {
+    c[j] = inside ? pc.e[j] : __builtin_nanf("");
+    s[j] = inside ? ps.e[j] : __builtin_nanf("");
   }
 }
 
@@ -94,49 +101,65 @@ __device__ __forceinline__ float group_sum(float v, int shift) {
   return v;
 }
 
-template <int DT, int C, int U, bool INTER>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_fwd(Args a, typename Elem<DT>::T* __restrict__ out) {
+// Token and head of a lane group's u-th turn in a wave's item.
+constexpr int kU = 2;
+struct Turn {
+  int64_t t;
+  int h;
+};
+template <bool FEW>
+__device__ __forceinline__ Turn turn_of(const Args& a, int64_t item, int sub, int u) {
+  if constexpr (FEW) {
+    const int tokens_shift = 6 - a.group_shift - a.heads_shift;
+    return Turn{((item * kU + u) << tokens_shift) + (sub >> a.heads_shift), sub & ((1 << a.heads_shift) - 1)};
+  }
+  const int64_t t = (uint32_t)item / (uint32_t)a.per;
+  return Turn{t, ((int)(item - t * a.per) * kU + u) * (kWave >> a.group_shift) + sub};
+}
+
+// FEW: a wave takes more than one token at a time. (A flag of the call instead costs the others 7 %: their token is a
+// scalar.)
+template <int DT, int C, bool INTER, bool RAGGED, bool FEW>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_fwd(Args a, int64_t items,
+                                                             typename Elem<DT>::T* __restrict__ out) {
   using El = Elem<DT>;
   using T = typename El::T;
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t wave = (int64_t)blockIdx.x * kWaves + threadIdx.x / kWave;
-  const int64_t t = (uint32_t)wave / (uint32_t)a.per;
-  if (t >= a.tokens) return;
-  const int part = (int)(wave - t * a.per);
-  const int p = lane & ((1 << a.group_shift) - 1), sub = lane >> a.group_shift, hp = kWave >> a.group_shift;
+  const int64_t item = (int64_t)blockIdx.x * kWaves + threadIdx.x / kWave;
+  if (item >= items) return;
+  const int p = lane & ((1 << a.group_shift) - 1), sub = lane >> a.group_shift;
   const bool active = p < a.lanes;
-  const Columns<C, INTER> col(a, p);
+  const Columns<C, INTER> col(a, active ? p : 0);
   const int heads = a.H + 2 * a.KH, normed = a.H + a.KH;
-  const T* xr = (const T*)a.x + t * a.ldx;
-  T* yr = out + t * (int64_t)heads * a.D;
 
-  Piece<DT, C> x0[U], x1[U];
+  Turn at[kU];
+  bool live[kU];
+  Piece<DT, C> x0[kU], x1[kU];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int h = (part * U + u) * hp + sub;
-    const bool live = active && h < heads;
-    const T* src = xr + (int64_t)(live ? h : 0) * a.D;
-    x0[u].load(src + (active ? col.e0 : 0));
-    x1[u].load(src + (active ? col.e1 : 0));
+  for (int u = 0; u < kU; ++u) {
+    at[u] = turn_of<FEW>(a, item, sub, u);
+    live[u] = active && at[u].h < heads && (!FEW || at[u].t < a.tokens);
+    const T* src = (const T*)a.x + (FEW && !live[u] ? 0 : at[u].t) * a.ldx + (live[u] ? at[u].h : 0) * a.D;
+    x0[u].load(src + col.e0);
+    x1[u].load(src + col.e1);
   }
   float c[C], s[C];
-  load_rotation<C>(a, t, p, c, s);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int h = (part * U + u) * hp + sub;
-    const bool live = active && h < heads;
+  for (int u = 0; u < kU; ++u) {
+    if (u == 0 || FEW) load_rotation<C, INTER>(a, col, FEW && !live[u] ? 0 : at[u].t, c, s);
+    const int h = at[u].h;
     float v[2 * C], ss = 0.f;
     x0[u].get(v);
     x1[u].get(v + C);
 #pragma unroll
-    for (int j = 0; j < 2 * C; ++j) ss += v[j] * v[j];
+    for (int j = 0; j < 2 * C; ++j) ss += RAGGED && col.shared(j) ? 0.f : v[j] * v[j];
     ss = group_sum(active ? ss : 0.f, a.group_shift);
-    if (!live) continue;
+    if (!live[u]) continue;
     if (h < normed) {
       const float r = 1.0f / __fsqrt_rn(ss / (float)a.D + a.eps);
       const T* w = (const T*)(h < a.H ? a.wq : a.wk);
       Piece<DT, C> w0, w1;
-      float wv[2 * C], y[2 * C];
+      float wv[2 * C];
       w0.load(w + col.e0);
       w1.load(w + col.e1);
       w0.get(wv);
@@ -146,39 +169,40 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_fwd(Args a, typename El
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         const float za = v[first_of<C, INTER>(i)], zb = v[second_of<C, INTER>(i)];
-        y[first_of<C, INTER>(i)] = za * c[i] - zb * s[i];
-        y[second_of<C, INTER>(i)] = zb * c[i] + za * s[i];
+        v[first_of<C, INTER>(i)] = col.rotates ? za * c[i] - zb * s[i] : za;
+        v[second_of<C, INTER>(i)] = col.rotates ? zb * c[i] + za * s[i] : zb;
       }
-      x0[u].set(y);
-      x1[u].set(y + C);
+      x0[u].set(v);
+      x1[u].set(v + C);
     }
-    T* dst = yr + (int64_t)h * a.D;
+    T* dst = out + at[u].t * (int64_t)(heads * a.D) + h * a.D;
     x0[u].store_stream(dst + col.e0);
     x1[u].store_stream(dst + col.e1);
   }
 }
 
-// A fixed grid of waves walks the (token, part) items and keeps its share of both weights' gradients in
-// registers; each workgroup writes one partial row [2, D] of them.
-template <int DT, int C, int U, bool INTER>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd(Args a, const typename Elem<DT>::T* __restrict__ dy,
+// A fixed grid of waves walks the items and keeps its share of both weights' gradients in registers; each workgroup
+// writes one partial row [2, D] of them.
+template <int DT, int C, bool INTER, bool RAGGED, bool FEW>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd(Args a, int64_t items,
+                                                             const typename Elem<DT>::T* __restrict__ dy,
                                                              typename Elem<DT>::T* __restrict__ dx, int64_t lddx,
                                                              float* __restrict__ part_rows) {
   using El = Elem<DT>;
   using T = typename El::T;
   __shared__ float fold[kWaves][2 * 128];
   const int lane = threadIdx.x & (kWave - 1), wv_id = threadIdx.x / kWave;
-  const int p = lane & ((1 << a.group_shift) - 1), sub = lane >> a.group_shift, hp = kWave >> a.group_shift;
+  const int p = lane & ((1 << a.group_shift) - 1), sub = lane >> a.group_shift;
   const bool active = p < a.lanes;
-  const Columns<C, INTER> col(a, p);
+  const Columns<C, INTER> col(a, active ? p : 0);
   const int heads = a.H + 2 * a.KH, normed = a.H + a.KH;
   float wq[2 * C], wk[2 * C], dwq[2 * C], dwk[2 * C];
   {
     Piece<DT, C> q0, q1, k0, k1;
-    q0.load((const T*)a.wq + (active ? col.e0 : 0));
-    q1.load((const T*)a.wq + (active ? col.e1 : 0));
-    k0.load((const T*)a.wk + (active ? col.e0 : 0));
-    k1.load((const T*)a.wk + (active ? col.e1 : 0));
+    q0.load((const T*)a.wq + col.e0);
+    q1.load((const T*)a.wq + col.e1);
+    k0.load((const T*)a.wk + col.e0);
+    k1.load((const T*)a.wk + col.e1);
     q0.get(wq);
     q1.get(wq + C);
     k0.get(wk);
@@ -187,49 +211,47 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd(Args a, const typen
 #pragma unroll
   for (int j = 0; j < 2 * C; ++j) dwq[j] = dwk[j] = 0.f;
 
-  const int64_t items = a.tokens * a.per;
-  for (int64_t it = (int64_t)blockIdx.x * kWaves + wv_id; it < items; it += (int64_t)gridDim.x * kWaves) {
-    const int64_t t = (uint32_t)it / (uint32_t)a.per;
-    const int part = (int)(it - t * a.per);
-    const T* xr = (const T*)a.x + t * a.ldx;
-    const T* gr = dy + t * (int64_t)heads * a.D;
-    T* dr = dx + t * lddx;
-    Piece<DT, C> x0[U], x1[U], g0[U], g1[U];
+  for (int64_t item = (int64_t)blockIdx.x * kWaves + wv_id; item < items; item += (int64_t)gridDim.x * kWaves) {
+    Turn at[kU];
+    bool live[kU];
+    Piece<DT, C> x0[kU], x1[kU], g0[kU], g1[kU];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = (part * U + u) * hp + sub;
-      const int64_t at = (int64_t)(active && h < heads ? h : 0) * a.D;
-      const int64_t xat = (int64_t)(active && h < normed ? h : 0) * a.D;
-      g0[u].load(gr + at + (active ? col.e0 : 0));
-      g1[u].load(gr + at + (active ? col.e1 : 0));
-      x0[u].load(xr + xat + (active ? col.e0 : 0));
-      x1[u].load(xr + xat + (active ? col.e1 : 0));
+    for (int u = 0; u < kU; ++u) {
+      at[u] = turn_of<FEW>(a, item, sub, u);
+      live[u] = active && at[u].h < heads && (!FEW || at[u].t < a.tokens);
+      const int64_t t = FEW && !live[u] ? 0 : at[u].t;
+      const int h = live[u] ? at[u].h : 0, hx = h < normed ? h : 0;
+      const T *xr = (const T*)a.x + t * a.ldx + hx * a.D, *gr = dy + t * (int64_t)(heads * a.D) + h * a.D;
+      g0[u].load(gr + col.e0);
+      g1[u].load(gr + col.e1);
+      x0[u].load(xr + col.e0);
+      x1[u].load(xr + col.e1);
     }
     float c[C], s[C];
-    load_rotation<C>(a, t, p, c, s);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = (part * U + u) * hp + sub;
-      const bool live = active && h < heads;
-      float x[2 * C], g[2 * C], dz[2 * C], ss = 0.f, dot = 0.f;
+    for (int u = 0; u < kU; ++u) {
+      if (u == 0 || FEW) load_rotation<C, INTER>(a, col, FEW && !live[u] ? 0 : at[u].t, c, s);
+      const int h = at[u].h;
+      float x[2 * C], dz[2 * C], ss = 0.f, dot = 0.f;
       x0[u].get(x);
       x1[u].get(x + C);
-      g0[u].get(g);
-      g1[u].get(g + C);
+      g0[u].get(dz);
+      g1[u].get(dz + C);
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        const float ga = g[first_of<C, INTER>(i)], gb = g[second_of<C, INTER>(i)];
-        dz[first_of<C, INTER>(i)] = ga * c[i] + gb * s[i];
-        dz[second_of<C, INTER>(i)] = gb * c[i] - ga * s[i];
+        const float ga = dz[first_of<C, INTER>(i)], gb = dz[second_of<C, INTER>(i)];
+        dz[first_of<C, INTER>(i)] = col.rotates ? ga * c[i] + gb * s[i] : ga;
+        dz[second_of<C, INTER>(i)] = col.rotates ? gb * c[i] - ga * s[i] : gb;
       }
 #pragma unroll
       for (int j = 0; j < 2 * C; ++j) {
-        ss += x[j] * x[j];
-        dot += dz[j] * (h < a.H ? wq[j] : wk[j]) * x[j];
+        const bool skip = RAGGED && col.shared(j);
+        ss += skip ? 0.f : x[j] * x[j];
+        dot += skip ? 0.f : dz[j] * (h < a.H ? wq[j] : wk[j]) * x[j];
       }
       ss = group_sum(active ? ss : 0.f, a.group_shift);
       dot = group_sum(active ? dot : 0.f, a.group_shift);
-      if (!live) continue;
+      if (!live[u]) continue;
       if (h < normed) {
         const float r = 1.0f / __fsqrt_rn(ss / (float)a.D + a.eps);
         const float m = r * r * r * (dot / (float)a.D);
@@ -243,13 +265,13 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd(Args a, const typen
         g0[u].set(x);
         g1[u].set(x + C);
       }
-      T* dst = dr + (int64_t)h * a.D;
+      T* dst = dx + at[u].t * lddx + h * a.D;
       g0[u].store_stream(dst + col.e0);
       g1[u].store_stream(dst + col.e1);
     }
   }
 
-  // The wave's heads, then the workgroup's waves, in a fixed order.
+  // The wave's heads, then the workgroup's waves, in a fixed order. Lanes that share a column have the same sum of it.
 #pragma unroll
   for (int j = 0; j < 2 * C; ++j) {
     for (int m = 1 << a.group_shift; m < kWave; m <<= 1) {
@@ -292,45 +314,60 @@ __global__ __launch_bounds__(kSumThreads) void weight_sum(const float* __restric
   (col < D ? dwq[col] : dwk[col - D]) = Elem<DT>::store(acc);
 }
 
-// Elements of a lane's half: the widest power of two, 16 bytes at most, that divides R / 2 and the rest in pairs.
-int width_of(int dtype, int D, int R) {
-  int c = dtype == kF32 ? 4 : 8;
-  while (R % (2 * c) != 0 || D % (2 * c) != 0) c >>= 1;
+// Elements of a lane's half: the widest power of two, 16 bytes at most, that a half of the rotated columns and of
+// the others (if there are others) holds. Backward up to 64 columns at most 4: with 8 half as many waves fit the
+// registers (bf16 [16384, 48 heads], 40, 48, 56 and 64 columns: 66, 65, 70, 72 us with 8, 55, 58, 59, 65 with 4;
+// 96 and 128 columns: 100, 111, and 109, 123).
+int width_of(int dtype, int D, int R, bool backward) {
+  int c = dtype == kF32 || (backward && D <= 64) ? 4 : 8;
+  while (R / 2 < c || (R < D && (D - R) / 2 < c)) c >>= 1;
   return c;
 }
+bool ragged(int c, int D, int R) { return R / 2 % c != 0 || (D - R) / 2 % c != 0; }
 
-constexpr int kU = 2;
-
-void lay_out(Args& a, int c, int u) {
-  a.lanes = a.D / (2 * c);
-  a.rotating = a.R / (2 * c);
+// The lanes' shares of a call, and its items (waves' turns of kU).
+int64_t lay_out(Args& a, int c) {
+  a.rotating = (int)ceil_div(a.R / 2, c);
+  a.lanes = a.rotating + (int)ceil_div((a.D - a.R) / 2, c);
   a.group_shift = 0;
   while ((1 << a.group_shift) < a.lanes) ++a.group_shift;
-  a.per = (int)ceil_div(a.H + 2 * (int64_t)a.KH, (int64_t)u * (kWave >> a.group_shift));
+  const int heads = a.H + 2 * a.KH, at_a_time = kWave >> a.group_shift;
+  a.heads_shift = 0;
+  while ((1 << a.heads_shift) < heads && (1 << a.heads_shift) < at_a_time) ++a.heads_shift;
+  if (2 << a.heads_shift <= at_a_time) {
+    a.per = 0;
+    return ceil_div(a.tokens, (int64_t)kU * (at_a_time >> a.heads_shift));
+  }
+  a.per = (int)ceil_div(heads, (int64_t)kU * at_a_time);
+  return a.tokens * a.per;
 }
 
-template <int DT, int C, bool INTER>
+template <int DT, int C, bool INTER, bool RAGGED>
 int launch_fwd(Args a, void* out, hipStream_t st) {
-  lay_out(a, C, kU);
-  const int64_t waves = a.tokens * a.per;
-  if (waves >= (1 << 26)) return KRSI_ERR_BAD_SHAPE;  // grids of less than 2^32 threads
-  hipLaunchKernelGGL((qk_norm_rope_fwd<DT, C, kU, INTER>), dim3((unsigned)ceil_div(waves, kWaves)), dim3(kThreads), 0,
-                     st, a, (typename Elem<DT>::T*)out);
+  const int64_t items = lay_out(a, C);
+  if (items >= (1 << 26)) return KRSI_ERR_BAD_SHAPE;  // grids of less than 2^32 threads
+  auto launch = [&](auto few) {
+    hipLaunchKernelGGL((qk_norm_rope_fwd<DT, C, INTER, RAGGED, decltype(few)::value>),
+                       dim3((unsigned)ceil_div(items, kWaves)), dim3(kThreads), 0, st, a, items,
+                       (typename Elem<DT>::T*)out);
+  };
+  a.per ? launch(std::false_type{}) : launch(std::true_type{});
   return launch_status();
 }
 
-template <int DT, int C, bool INTER>
+template <int DT, int C, bool INTER, bool RAGGED>
 int launch_bwd(Args a, const void* dy, void* dx, int64_t lddx, void* dwq, void* dwk, float* part, hipStream_t st) {
   using T = typename Elem<DT>::T;
   int blocks = 0;
   if (a.tokens > 0) {
-    lay_out(a, C, kU);
-    const int64_t waves = a.tokens * a.per;
-    if (waves >= (1 << 26)) return KRSI_ERR_BAD_SHAPE;  // grids of less than 2^32 threads
-    const int64_t need = ceil_div(waves, kWaves);
+    const int64_t items = lay_out(a, C), need = ceil_div(items, kWaves);
+    if (items >= (1 << 26)) return KRSI_ERR_BAD_SHAPE;
     blocks = (int)(need < bwd_blocks(C) ? need : bwd_blocks(C));
-    hipLaunchKernelGGL((qk_norm_rope_bwd<DT, C, kU, INTER>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a,
-                       (const T*)dy, (T*)dx, lddx, part);
+    auto launch = [&](auto few) {
+      hipLaunchKernelGGL((qk_norm_rope_bwd<DT, C, INTER, RAGGED, decltype(few)::value>), dim3((unsigned)blocks),
+                         dim3(kThreads), 0, st, a, items, (const T*)dy, (T*)dx, lddx, part);
+    };
+    a.per ? launch(std::false_type{}) : launch(std::true_type{});
     const int rc = launch_status();
     if (rc != KRSI_OK) return rc;
   }
@@ -339,34 +376,40 @@ int launch_bwd(Args a, const void* dy, void* dx, int64_t lddx, void* dwq, void* 
   return launch_status();
 }
 
-// f(dtype, width, interleaved) as constants.
-template <int DT, typename F>
-int with_width(int c, bool inter, F&& f) {
-  auto two = [&](auto w) {
-    return inter ? f(std::integral_constant<int, DT>{}, w, std::true_type{})
-                 : f(std::integral_constant<int, DT>{}, w, std::false_type{});
-  };
+// f(dtype, width, interleaved, ragged) as constants.
+template <typename DT, typename C, typename F>
+int with_forms(bool inter, bool rag, F&& f) {
+  if constexpr (C::value > 1) {
+    if (rag) return inter ? f(DT{}, C{}, std::true_type{}, std::true_type{}) : f(DT{}, C{}, std::false_type{}, std::true_type{});
+  }
+  return inter ? f(DT{}, C{}, std::true_type{}, std::false_type{}) : f(DT{}, C{}, std::false_type{}, std::false_type{});
+}
+template <int DT_, typename F>
+int with_width(int c, bool inter, bool rag, F&& f) {
+  using DT = std::integral_constant<int, DT_>;
   switch (c) {
     case 8:
-      if constexpr (DT != kF32) return two(std::integral_constant<int, 8>{});
+      if constexpr (DT_ != kF32) return with_forms<DT, std::integral_constant<int, 8>>(inter, rag, f);
       return KRSI_ERR_UNSUPPORTED;
     case 4:
-      return two(std::integral_constant<int, 4>{});
+      return with_forms<DT, std::integral_constant<int, 4>>(inter, rag, f);
     case 2:
-      return two(std::integral_constant<int, 2>{});
+      return with_forms<DT, std::integral_constant<int, 2>>(inter, rag, f);
     default:
-      return two(std::integral_constant<int, 1>{});
+      return with_forms<DT, std::integral_constant<int, 1>>(inter, rag, f);
   }
 }
 template <typename F>
-int with_kernel(int dtype, int c, bool inter, F&& f) {
+int with_kernel(int dtype, int D, int R, bool inter, bool backward, F&& f) {
+  const int c = width_of(dtype, D, R, backward);
+  const bool rag = ragged(c, D, R);
   switch (dtype) {
     case kF16:
-      return with_width<kF16>(c, inter, f);
+      return with_width<kF16>(c, inter, rag, f);
     case kF32:
-      return with_width<kF32>(c, inter, f);
+      return with_width<kF32>(c, inter, rag, f);
     default:
-      return with_width<kBf16>(c, inter, f);
+      return with_width<kBf16>(c, inter, rag, f);
   }
 }
 
@@ -399,9 +442,9 @@ int krsi_qk_norm_rope_fwd(const void* qkv, int64_t ld_qkv, const void* wq, const
   if (rc != KRSI_OK) return rc;
   if (tokens == 0) return KRSI_OK;
   if (!qkv || !wq || !wk || !rope || !out) return KRSI_ERR_NULL_POINTER;
-  Args a{qkv, wq, wk, positions, rope, ld_qkv, tokens, table_rows, S, H, KH, D, R, position_bytes, 0, 0, 0, 0, eps};
-  return with_kernel(dtype, width_of(dtype, D, R), interleaved == 1, [&](auto dt, auto c, auto inter) {
-    return launch_fwd<dt(), c(), inter()>(a, out, as_stream(stream));
+  Args a{qkv, wq, wk, positions, rope, ld_qkv, tokens, table_rows, S, H, KH, D, R, position_bytes, 0, 0, 0, 0, 0, eps};
+  return with_kernel(dtype, D, R, interleaved == 1, false, [&](auto dt, auto c, auto inter, auto rag) {
+    return launch_fwd<dt(), c(), inter(), rag()>(a, out, as_stream(stream));
   });
 }
 
@@ -425,9 +468,9 @@ int krsi_qk_norm_rope_bwd(const void* dout, const void* qkv, int64_t ld_qkv, con
     if (!workspace || workspace_bytes < krsi_qk_norm_rope_bwd_workspace_bytes(D)) return KRSI_ERR_WORKSPACE;
     if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
   }
-  Args a{qkv, wq, wk, positions, rope, ld_qkv, tokens, table_rows, S, H, KH, D, R, position_bytes, 0, 0, 0, 0, eps};
-  return with_kernel(dtype, width_of(dtype, D, R), interleaved == 1, [&](auto dt, auto c, auto inter) {
-    return launch_bwd<dt(), c(), inter()>(a, dout, dqkv, ld_dqkv, dwq, dwk, (float*)workspace, as_stream(stream));
+  Args a{qkv, wq, wk, positions, rope, ld_qkv, tokens, table_rows, S, H, KH, D, R, position_bytes, 0, 0, 0, 0, 0, eps};
+  return with_kernel(dtype, D, R, interleaved == 1, true, [&](auto dt, auto c, auto inter, auto rag) {
+    return launch_bwd<dt(), c(), inter(), rag()>(a, dout, dqkv, ld_dqkv, dwq, dwk, (float*)workspace, as_stream(stream));
   });
 }
 

@@ -58,6 +58,10 @@ CASES = [  # B, S, H, KH, D, R, interleaved, positions
     (2, 33, 5, 5, 24, 10, False, True),      # R / 2 odd
     (1, 65, 33, 11, 96, 96, True, True),     # heads that no wave divides
     (2, 2049, 4, 2, 64, 64, False, False),   # more items than a backward's waves
+    (1, 37, 1, 1, 72, 36, False, True),      # several tokens to a wave; chunks that share columns in both parts
+    (2, 5, 1, 1, 8, 4, True, False),         # as many tokens to a wave as there are
+    (1, 40, 2, 2, 72, 44, True, False),      # shared columns, adjacent pairs
+    (3, 1, 7, 1, 104, 54, False, True),
 ]
 
 
