@@ -5,6 +5,9 @@
 // reproducible. Tokens outside [0, V) and the padding token have no part in them.
 //
 // What bounds both: HBM (forward: the named rows in, out; backward: g in, dtable out, most of whose rows are zeros).
+// bf16 [32768, 4096], V 131072: forward 71 us, backward 315 (of 1.3 GB: 4.3 TB/s); [8191, 1024], V 32128: 5 and 33
+// (of 83 MB), where group_tokens' latency and the last rows' sums are a half each; 500 tokens there: 2.4 and 24. From
+// about 100000 tokens on, group_tokens' two passes over all tokens in each workgroup are the larger part.
 //
 // Backward in three launches:
 //   group_tokens  one launch that sorts the positions by token, stably. Workgroup j owns the rows v = j (mod

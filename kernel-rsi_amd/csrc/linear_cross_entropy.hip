@@ -13,7 +13,10 @@
 // dl is held times a power of two that puts the largest |g| at 2^14..2^15: fp16 then keeps probabilities down to
 // 2^-29 in full precision, and the scale comes off exactly where dx and dw are rounded.
 //
-// What bounds it: the matrix cores (2 rows V K flop forward, 6 backward, 2 of them the logits again).
+// What bounds it: the matrix cores (2 rows V K flop forward, 6 backward, 2 of them the logits again). bf16 [8192,
+// 4096], V 131072: 6.4 ms of logits (1370 TFLOP/s), backward 20.6 ms (1280 over its three products); the vendor's
+// product of such sizes runs at 1390, 1295 and 1125 TFLOP/s in the three orientations. [2048, 1024], V 32128: 121 and
+// 399 us, where 16 stages a tile leave the epilogues a fifth.
 #include "chunks.h"
 #include "krsi_device.h"
 #include "krsi_internal.h"
@@ -24,7 +27,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kOneBlock = 1024;
-constexpr int64_t kPieceBytes = int64_t(512) << 20;  // of dl in the backward, and of a row's pairs in the forward
+// Bytes of dl in the backward, and of the rows' pairs in the forward. Backward at [8192, 1024], V 32128: 1637 us in
+// pieces of 128 MB (5), 1500 in pieces of 256 to 1024 (3 to 1); [4099, 2048], V 50257: 2632, 2620 with 256, 2440.
+constexpr int64_t kPieceBytes = int64_t(512) << 20;
 constexpr int64_t kMinWidth = 4096;  // columns of a piece at least: dx's fp32 sums are read and written once per piece
 constexpr int64_t kMaxWidth = 1 << 20;  // columns of a piece: 64 rows of dl stay below 2^31 bytes
 constexpr int kMinStages = 8;   // stages of a part of a split sum, at least
@@ -190,15 +195,22 @@ __global__ __launch_bounds__(kOneBlock) void add_losses(const float* __restrict_
 }
 
 // ----------------------------------------------------------------- backward
-// coef[row] = g_row times 2^k, k such that the largest finite |g| reaches 2^14 .. 2^15; *back = 2^-k. g: the
+// What the backward needs of a row, in one load.
+struct alignas(16) RowInfo {
+  float lse, coef;  // coef 0: no weight
+  int target;       // -1: none
+  int unused;
+};
+
+// coef = g_row times 2^k, k such that the largest finite |g| reaches 2^14 .. 2^15; *back = 2^-k. g: the
 // loss's gradient for the row (per row, or one for all, over the rows that count with mean); 0 where
 // ignored, NaN where the target is outside [0, V). rest and last are cleared. Per row, workgroup 0 finds the
 // largest and does all rows; else every workgroup knows it and does its share.
 __global__ __launch_bounds__(kOneBlock) void row_weights(const float* __restrict__ dout, bool per_row, bool mean,
                                                          const float* __restrict__ counted, Targets targets,
-                                                         int rows, float* __restrict__ coef,
-                                                         float* __restrict__ rest, int* last,
-                                                         float* __restrict__ back) {
+                                                         int rows, const float* __restrict__ lse,
+                                                         RowInfo* __restrict__ info, float* __restrict__ rest,
+                                                         int* last, float* __restrict__ back) {
   __shared__ float s[kOneBlock / kWave];
   const int me = blockIdx.x * kOneBlock + threadIdx.x, all = gridDim.x * kOneBlock;
   for (int v = 4 * me; v < targets.V; v += 4 * all)  // the array is padded to whole chunks
@@ -225,7 +237,7 @@ __global__ __launch_bounds__(kOneBlock) void row_weights(const float* __restrict
   }
   const float scale = ldexpf(1.f, k);
   for (int r = per_row ? threadIdx.x : me; r < rows; r += per_row ? kOneBlock : all) {
-    coef[r] = weight(r) * scale;
+    info[r] = RowInfo{lse[r], weight(r) * scale, targets.at(r), 0};
     rest[r] = 0.f;
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) *back = ldexpf(1.f, -k);
@@ -235,22 +247,24 @@ __global__ __launch_bounds__(kOneBlock) void row_weights(const float* __restrict
 // rest[row]: see above; last[v]: the last row whose target is v.
 template <int DT, int WM, int WN, int RB, int CB>
 __global__ __launch_bounds__(64 * WM * WN, (StreamTile<WM, WN, RB, CB>::kPerCu * WM * WN / 4)) void logits_grad(
-    Operand x, Operand w, int K, Tiles tiles, Targets targets, int v0, const float* __restrict__ lse,
-    const float* __restrict__ coef, float* __restrict__ rest, int* last,
-    uint16_t* __restrict__ dl, int ld) {
+    Operand x, Operand w, int K, Tiles tiles, int v0, const RowInfo* __restrict__ info, float* __restrict__ rest,
+    int* last, uint16_t* __restrict__ dl, int ld) {
   using Tl = StreamTile<WM, WN, RB, CB>;
   using El = Elem<DT>;
   __shared__ __attribute__((aligned(512))) uint16_t lds[Tl::kLds];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
   const int wr = wave / WN, wc = wave % WN;
   stream_products<DT, false, false, WM, WN, RB, CB>(x, w, K, tiles, lds, [&](const TileAt& t, f32x4(&acc)[RB][CB]) {
-    const int col0 = t.n0 + 16 * CB * wc + 4 * g;
+    const int col0 = t.n0 + 16 * CB * wc + 4 * g, row0 = t.m0 + 16 * RB * wr + l16;
+    RowInfo of[2];  // of this row and the next
+    of[0] = info[min(row0, x.extent - 1)];
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
-      const int row = t.m0 + 16 * (RB * wr + i) + l16;
+      const int row = row0 + 16 * i;
+      if (i + 1 < RB) of[(i + 1) % 2] = info[min(row + 16, x.extent - 1)];
       if (row >= x.extent) continue;
-      const float b = lse[row], c = coef[row];
-      const int at = targets.at(row) - v0 - col0;
+      const float b = of[i % 2].lse, c = of[i % 2].coef;
+      const int at = of[i % 2].target - v0 - col0;
       float d[4 * CB];
 #pragma unroll
       for (int j = 0; j < 4 * CB; ++j) d[j] = __builtin_amdgcn_exp2f((acc[i][j / 4][j % 4] - b) * kLog2e) * c;
@@ -485,7 +499,7 @@ Forward plan_forward(int64_t rows, int K, int V) {
 struct Backward {
   int width, pieces;  // columns of dl, a multiple of 256
   Plan dx, dw;        // of a whole piece
-  size_t coef, rest, last, back, dl, dx_part, dw_part, bytes;
+  size_t info, rest, last, back, dl, dx_part, dw_part, bytes;
 };
 Backward plan_backward(int64_t rows, int K, int V) {
   Backward b{};
@@ -502,7 +516,7 @@ Backward plan_backward(int64_t rows, int K, int V) {
     at += align256(n);
     return here;
   };
-  b.coef = take((size_t)rows * 4);
+  b.info = take((size_t)rows * sizeof(RowInfo));
   b.rest = take((size_t)rows * 4);
   b.last = take((size_t)V * 4);
   b.back = take(4);
@@ -575,12 +589,13 @@ int backward(const float* dout, const Operand& x, const Operand& w, int K, const
              uint16_t* dx, uint16_t* dw, char* ws, int reduction, hipStream_t st) {
   const int rows = x.extent, V = w.extent;
   const Backward b = plan_backward(rows, K, V);
-  float *coef = (float*)(ws + b.coef), *rest = (float*)(ws + b.rest), *back = (float*)(ws + b.back);
+  RowInfo* info = (RowInfo*)(ws + b.info);
+  float *rest = (float*)(ws + b.rest), *back = (float*)(ws + b.back);
   int* last = (int*)(ws + b.last);
   const Rest to_dx{rest, w.p, nullptr, t};
   uint16_t* dl = (uint16_t*)(ws + b.dl);
   hipLaunchKernelGGL(row_weights, dim3((unsigned)ceil_div(rows + V / 4, 4 * kOneBlock)), dim3(kOneBlock), 0, st, dout, reduction == 0, reduction == 1, stats + rows, t,
-                     rows, coef, rest, last, back);
+                     rows, stats, info, rest, last, back);
   const bool dx_parts = b.dx.tiles.splits > 1 || b.pieces > 1;
   float* dx_part = dx_parts ? (float*)(ws + b.dx_part) : nullptr;
   for (int p = 0; p < b.pieces; ++p) {
@@ -590,7 +605,7 @@ int backward(const float* dout, const Operand& x, const Operand& w, int K, const
     with_logits_tile(lg, [&](auto s) {
       using S = decltype(s);
       hipLaunchKernelGGL((logits_grad<DT, S::WM, S::WN, S::RB, S::CB>), dim3(stream_grid<typename S::Tl>(lg.tiles)),
-                         dim3(S::Tl::kThreads), 0, st, x, piece, K, lg.tiles, t, v0, stats, (const float*)coef, rest, last, dl,
+                         dim3(S::Tl::kThreads), 0, st, x, piece, K, lg.tiles, v0, (const RowInfo*)info, rest, last, dl,
                          b.width);
     });
     if (dx) {
