@@ -242,7 +242,9 @@ int krsi_relpos_bucket_sum(const float* dpd, const int32_t* bucket, float* dtabl
  * fp32 from the load to the store, one rounding. Backward: dqkv [tokens, ld_dqkv] (its first (H + 2 KH) D
  * columns are written), dwq and dwk [D], summed in fp32 in a fixed order; dout as out.
  * Limits: D % 8 == 0, 8 <= D <= 128, R even, 2 <= R <= D; tokens < 2^31 (and waves below 2^26:
- * tokens * (H + 2 KH) <= 2^26 fits at every D), table_rows >= min(S, tokens) without positions. No tokens: dwq and dwk are zero. workspace: krsi_qk_norm_rope_bwd_workspace_bytes(D), scratch.  */
+ * tokens * (H + 2 KH) <= 2^26 fits at every D), table_rows >= min(S, tokens) without positions. No tokens: dwq
+ * and dwk are zero. workspace: krsi_qk_norm_rope_bwd_workspace_bytes(D), scratch. No buffer overlaps another that is
+ * written.                                                                                                */
 int krsi_qk_norm_rope_fwd(const void* qkv, int64_t ld_qkv, const void* wq, const void* wk, const float* rope,
                           const void* positions, void* out, int64_t tokens, int32_t S, int32_t H, int32_t KH,
                           int32_t D, int32_t R, int64_t table_rows, int32_t position_bytes, float eps,
@@ -271,7 +273,8 @@ int krsi_embedding_bwd(const void* dout, const void* tokens, int32_t token_bytes
 /* ---------------- cross entropy of an output projection (no counterpart)
  * l = x w^T; loss_n = log sum_v exp(l_nv) - l_n,target(n). x [rows, k], w [v, k] contiguous, 16-byte aligned, of T
  * (KRSI_DTYPE_BF16 or KRSI_DTYPE_F16); l is fp32 and is not kept. targets [rows] int32 or int64 (target_bytes 4
- * or 8): ignore_index has loss 0 and no gradient; one outside [0, v) makes its loss (and gradients) NaN.
+ * or 8): ignore_index has loss 0 and no gradient (its row of x has to be finite where dw is wanted, which adds it
+ * times zero); one outside [0, v) makes its loss (and gradients) NaN.
  * reduction 0: loss [rows] fp32; 1: loss [1], the mean over the targets that are not ignored (NaN if there are
  * none); 2: loss [1], the sum. stats [rows + 1] fp32, for the backward: lse of each row, then (1, 2) their number.
  * Backward: dout fp32, [rows] or [1]; dx [rows, k] and dw [v, k] of T, either may be NULL (not wanted). The logits

@@ -6,7 +6,7 @@
 //                                                          (2 i, 2 i + 1) where interleaved; y = z past R
 // Value heads are copied. Everything between the load and the store is fp32: one rounding, at the store.
 // Backward, from dy: the pair's inverse rotation gives dz; dw = sum over tokens and heads of dz x r;
-//   dn = dz w;  dx = r dn - x r^3 sum(dn x) / D.
+//   dn = dz w;  n = x r;  dx = r (dn - n r sum(dn x) / D).
 //
 // What bounds it: HBM (forward 2 bytes moved per byte of qkv; backward dy, q and k in, dqkv out). bf16 [16384, 48
 // heads of 128]: forward 69.6 us (5.8 TB/s), backward 112 us (4.8 TB/s); a copy of 2 GB runs at 4.9.
@@ -254,13 +254,13 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd(Args a, int64_t ite
       if (!live[u]) continue;
       if (h < normed) {
         const float r = 1.0f / __fsqrt_rn(ss / (float)a.D + a.eps);
-        const float m = r * r * r * (dot / (float)a.D);
+        const float m = dot * r / (float)a.D;
 #pragma unroll
         for (int j = 0; j < 2 * C; ++j) {
-          const float d = dz[j] * x[j] * r;
+          const float n = x[j] * r, d = dz[j] * n;  // (with r^3 formed, heads below 1e-13 or above 1e12 left its range)
           dwq[j] += h < a.H ? d : 0.f;
           dwk[j] += h < a.H ? 0.f : d;
-          x[j] = r * (dz[j] * (h < a.H ? wq[j] : wk[j])) - x[j] * m;
+          x[j] = r * (dz[j] * (h < a.H ? wq[j] : wk[j]) - n * m);
         }
         g0[u].set(x);
         g1[u].set(x + C);
@@ -380,7 +380,8 @@ int launch_bwd(Args a, const void* dy, void* dx, int64_t lddx, void* dwq, void* 
 template <typename DT, typename C, typename F>
 int with_forms(bool inter, bool rag, F&& f) {
   if constexpr (C::value > 1) {
-    if (rag) return inter ? f(DT{}, C{}, std::true_type{}, std::true_type{}) : f(DT{}, C{}, std::false_type{}, std::true_type{});
+    if (rag)
+      return inter ? f(DT{}, C{}, std::true_type{}, std::true_type{}) : f(DT{}, C{}, std::false_type{}, std::true_type{});
   }
   return inter ? f(DT{}, C{}, std::true_type{}, std::false_type{}) : f(DT{}, C{}, std::false_type{}, std::false_type{});
 }

@@ -8,7 +8,8 @@ Op names follow the reference (library/rmsnorm.py:86-103, geglu.py:85-101,
 relpos_attention.py:175-195): krsi::rmsnorm_fwd/bwd, krsi::geglu_fwd/bwd,
 krsi::relpos_attn_fwd/bwd; krsi::relpos_bucket_gather/sum (the T5 table step) and
 krsi::geglu_linear_fwd (the merged projection with the GEGLU epilogue), krsi::qk_norm_rope_fwd/bwd,
-krsi::embedding_fwd/bwd and krsi::linear_cross_entropy_fwd/bwd have no counterpart there. Their schemas are internal to this library.
+krsi::embedding_fwd/bwd and krsi::linear_cross_entropy_fwd/bwd have no counterpart there. Their schemas are internal
+to this library.
 """
 from __future__ import annotations
 

@@ -8,8 +8,8 @@ pieces of the vocabulary; each piece's gradient is rounded to x's dtype (times a
 keeps small probabilities) and multiplied into dx, which is carried in fp32, and dw. It allocates a piece of about
 512 MB at most, where the logits themselves take 4 bytes for each row and vocabulary entry.
 The loss is fp32: its mean over the targets that are not ignore_index (NaN if there are none), their sum,
-or with reduction="none" the loss of each (0 where ignored). A target outside [0, V) that is not ignore_index
-makes the loss, and the gradients, NaN. bf16 or fp16, K a multiple of 64. Usable under
+or with reduction="none" the loss of each (0 where ignored, whatever its row of x holds; dw, which adds that row times
+zero, needs it finite). A target outside [0, V) that is not ignore_index makes the loss, and the gradients, NaN. bf16 or fp16, K a multiple of 64. Usable under
 torch.compile(fullgraph=True).
 """
 import sys

@@ -38,12 +38,12 @@ def _check(name, got, ref, mag, steps, dt):
     assert got.shape == ref.shape and bool(((got - ref).abs() <= bound).all()), (name, worst)
 
 
-def _verify(out, grads, dout, qkv, wq, wk, rope, pos, H, KH, D, inter, dt):
+def _verify(out, grads, dout, qkv, wq, wk, rope, pos, H, KH, D, inter, dt, eps=EPS):
     args = [t.detach().cpu() for t in (qkv, wq, wk, rope)]
     pos = pos.reshape(-1).cpu().long()
     tokens = len(pos)
-    _check("out", out.detach(), *O.qk_norm_rope_64(*args, pos, H, KH, D, EPS, inter), D / 2 + 16, dt)
-    refs, mags = O.qk_norm_rope_grads_64(dout.cpu(), *args, pos, H, KH, D, EPS, inter)
+    _check("out", out.detach(), *O.qk_norm_rope_64(*args, pos, H, KH, D, eps, inter), D / 2 + 16, dt)
+    refs, mags = O.qk_norm_rope_grads_64(dout.cpu(), *args, pos, H, KH, D, eps, inter)
     for name, got, ref, mag, n in zip(("dqkv", "dwq", "dwk"), grads, refs, mags, (0, tokens * H, tokens * KH)):
         _check(name, got, ref, mag, 2.5 * D + 16 + n, dt)
 
@@ -151,6 +151,20 @@ def test_zero_rows_infinities_and_nan():
     assert (o[0, 1] == 0).all() and torch.isfinite(dx.view(S, 3 * H, D)[0, 1]).all()
     assert torch.isnan(o[1, 2]).any() and torch.isnan(o[2, 5]).any()
     assert torch.isfinite(dx.view(S, 3 * H, D)[~touched]).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=lambda d: str(d).split(".")[-1])
+@pytest.mark.parametrize("size", [1e-16, 1e16])
+def test_small_and_large_heads(size, dt):
+    """Heads whose squares still fit fp32, though the cube of their norm does not."""
+    log(f"qk_norm_rope heads of {size} {dt}")
+    B, S, H, D = 1, 5, 3, 64
+    qkv, wq, wk, rope = _inputs(B, S, H, H, D, D, dt)
+    leaves = [t.requires_grad_(True) for t in (qkv * size, wq, wk)]
+    dout = seeded(qkv.shape, 9, dtype=dt)
+    out = Q.qk_norm_rope(*leaves, rope, B, S, H, D, 1e-36)
+    grads = torch.autograd.grad(out, leaves, dout)
+    _verify(out, grads, dout, *leaves, rope, torch.arange(S), H, H, D, False, dt, 1e-36)
 
 
 def test_empty_batch():
