@@ -9,17 +9,17 @@
 //   dn = dz w;  n = x r;  dx = r (dn - n r sum(dn x) / D).
 //
 // What bounds it: HBM (forward 2 bytes moved per byte of qkv; backward dy, q and k in, dqkv out). bf16 [16384, 48
-// heads of 128]: forward 69.6 us (5.8 TB/s), backward 112 us (4.8 TB/s); a copy of 2 GB runs at 4.9.
-// Outputs are stored past the caches (73 and 114 us without).
+// heads of 128]: forward 69.0 us (5.8 TB/s), backward 105 us (5.1 TB/s); a copy of 2 GB runs at 4.9.
+// Outputs are stored past the caches (forward 73 us without).
 // Layout: a lane holds C elements of one half of the pairs and the C elements that they rotate with, so the
 // rotation stays in registers; the lanes of a head (their number rounded up to a power of two, the group) reduce its
 // square sum by shuffles. C is the widest of 8, 4, 2, 1 (16 bytes at most) that a half of the rotated columns and
 // of the rest holds; where it does not divide them the last lane's columns end at the half's end, and those that
 // it shares with the lane before count once in a sum. (With the widest C that divides them, bf16 [16384, 48 heads of
-// 72]: 64 / 108 us forward / backward, here 46 / 108; where 36 columns rotate, 98 / 171, here 46 / 99.)
+// 72]: 64 / 108 us forward / backward, here 46 / 88; where 36 columns rotate, 98 / 171, here 46 / 88.)
 // A wave takes a token's cos and sin into registers and runs that token's heads past them, 64 / group at a time,
 // twice with all loads first. Where a token has fewer heads than that, a wave takes as many tokens as fill it
-// ([16384, 4 heads of 64]: 9.3 / 29.6 us with one, 4.6 / 15.1).
+// ([16384, 4 heads of 64]: 9.3 / 29.6 us with one, 4.6 / 14.9).
 #include "chunks.h"
 #include "krsi_device.h"
 #include "krsi_internal.h"
@@ -32,9 +32,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kBwdBlocks = 1024;  // of a backward, at most: partial rows of dw
-// Workgroups of a backward: what the chip holds at once by its registers (8 columns: 182, two waves per SIMD; 4:
-// 116, four). bf16 [16384, 48 heads of 128]: 114 us with 512 workgroups, 119 with 1024, 129 with 2048; fp32 [4096,
-// 36 heads of 80]: 41, 34, 37.
+// Workgroups of a backward: what the chip holds at once by its registers (8 columns: 212, two waves per SIMD; 4:
+// 112, four). bf16 [16384, 48 heads of 128]: 105 us with 512 workgroups, 109 with 1024; fp32 [4096, 36 heads of
+// 80]: 41, 34.
 constexpr int bwd_blocks(int c) { return c == 8 ? kBwdBlocks / 2 : kBwdBlocks; }
 
 // What both directions need of a call, by value.
@@ -232,39 +232,58 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd(Args a, int64_t ite
     for (int u = 0; u < kU; ++u) {
       if (u == 0 || FEW) load_rotation<C, INTER>(a, col, FEW && !live[u] ? 0 : at[u].t, c, s);
       const int h = at[u].h;
-      float x[2 * C], dz[2 * C], ss = 0.f, dot = 0.f;
-      x0[u].get(x);
-      x1[u].get(x + C);
-      g0[u].get(dz);
-      g1[u].get(dz + C);
+      // A head of weight w, whose gradient's share is dw. All lanes of a head take the same branch: they exchange sums.
+      auto head = [&](const float(&w)[2 * C], float(&dw)[2 * C]) {
+        float x[2 * C], dz[2 * C], ss = 0.f, dot = 0.f;
+        x0[u].get(x);
+        x1[u].get(x + C);
+        g0[u].get(dz);
+        g1[u].get(dz + C);
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const float ga = dz[first_of<C, INTER>(i)], gb = dz[second_of<C, INTER>(i)];
-        dz[first_of<C, INTER>(i)] = col.rotates ? ga * c[i] + gb * s[i] : ga;
-        dz[second_of<C, INTER>(i)] = col.rotates ? gb * c[i] - ga * s[i] : gb;
-      }
+        for (int i = 0; i < C; ++i) {
+          const float ga = dz[first_of<C, INTER>(i)], gb = dz[second_of<C, INTER>(i)];
+          dz[first_of<C, INTER>(i)] = col.rotates ? ga * c[i] + gb * s[i] : ga;
+          dz[second_of<C, INTER>(i)] = col.rotates ? gb * c[i] - ga * s[i] : gb;
+        }
 #pragma unroll
-      for (int j = 0; j < 2 * C; ++j) {
-        const bool skip = RAGGED && col.shared(j);
-        ss += skip ? 0.f : x[j] * x[j];
-        dot += skip ? 0.f : dz[j] * (h < a.H ? wq[j] : wk[j]) * x[j];
-      }
-      ss = group_sum(active ? ss : 0.f, a.group_shift);
-      dot = group_sum(active ? dot : 0.f, a.group_shift);
-      if (!live[u]) continue;
-      if (h < normed) {
+        for (int j = 0; j < 2 * C; ++j) {
+          const bool skip = RAGGED && col.shared(j);
+          ss += skip ? 0.f : x[j] * x[j];
+          dot += skip ? 0.f : dz[j] * w[j] * x[j];
+        }
+        ss = group_sum(active ? ss : 0.f, a.group_shift);
+        dot = group_sum(active ? dot : 0.f, a.group_shift);
+        if (!live[u]) return;
         const float r = 1.0f / __fsqrt_rn(ss / (float)a.D + a.eps);
         const float m = dot * r / (float)a.D;
 #pragma unroll
         for (int j = 0; j < 2 * C; ++j) {
-          const float n = x[j] * r, d = dz[j] * n;  // (with r^3 formed, heads below 1e-13 or above 1e12 left its range)
-          dwq[j] += h < a.H ? d : 0.f;
-          dwk[j] += h < a.H ? 0.f : d;
-          x[j] = r * (dz[j] * (h < a.H ? wq[j] : wk[j]) - n * m);
+          const float n = x[j] * r;  // (with r^3 formed, heads below 1e-13 or above 1e12 left its range)
+          dw[j] += dz[j] * n;
+          x[j] = r * (dz[j] * w[j] - n * m);
         }
         g0[u].set(x);
         g1[u].set(x + C);
+      };
+      // Heads of both weights in the wave, or few registers to spare: each lane selects its own. (With 8 columns the
+      // branches save a twelfth of the time; with 4 they leave three waves per SIMD of four.)
+      const int first = __builtin_amdgcn_readfirstlane(h - sub);
+      if (FEW || C < 8 || (first < a.H && first + (kWave >> a.group_shift) > a.H)) {
+        float w[2 * C], dw[2 * C];
+#pragma unroll
+        for (int j = 0; j < 2 * C; ++j) w[j] = h < a.H ? wq[j] : wk[j], dw[j] = 0.f;
+        if (h < normed) head(w, dw);
+#pragma unroll
+        for (int j = 0; j < 2 * C; ++j) {
+          dwq[j] += h < a.H ? dw[j] : 0.f;
+          dwk[j] += h < a.H ? 0.f : dw[j];
+        }
+      } else if (h < a.H) {
+        head(wq, dwq);
+      } else if (h < normed) {
+        head(wk, dwk);
       }
+      if (!live[u]) continue;
       T* dst = dx + at[u].t * lddx + h * a.D;
       g0[u].store_stream(dst + col.e0);
       g1[u].store_stream(dst + col.e1);
@@ -316,8 +335,8 @@ __global__ __launch_bounds__(kSumThreads) void weight_sum(const float* __restric
 
 // Elements of a lane's half: the widest power of two, 16 bytes at most, that a half of the rotated columns and of
 // the others (if there are others) holds. Backward up to 64 columns at most 4: with 8 half as many waves fit the
-// registers (bf16 [16384, 48 heads], 40, 48, 56 and 64 columns: 66, 65, 70, 72 us with 8, 55, 58, 59, 65 with 4;
-// 96 and 128 columns: 100, 111, and 109, 123).
+// registers (bf16 [16384, 48 heads], 40, 48, 56 and 64 columns: 65, 66, 70, 71 us with 8, 56, 58, 60, 63 with 4;
+// 96 and 128 columns: 93, 105, and 109, 118).
 int width_of(int dtype, int D, int R, bool backward) {
   int c = dtype == kF32 || (backward && D <= 64) ? 4 : 8;
   while (R / 2 < c || (R < D && (D - R) / 2 < c)) c >>= 1;
