@@ -269,12 +269,12 @@ def time_calls(fns: list, warmup: int = 5, reps: int = 20, graph: bool = True) -
     return Timer(fns).measure(warmup=warmup, reps=reps, graph=graph)
 
 
-def time_ab(variants: dict, rounds: int = 5, reps: int = 10) -> dict:
+def time_ab(variants: dict, rounds: int = 5, reps: int = 10, graph: bool = True) -> dict:
     """Time variants (name -> list of callables) in interleaved rounds of alternating order.
-    Every variant is captured up front; if any cannot be, all are timed eagerly."""
+    Every variant is captured up front; if any cannot be, or without graph, all are timed eagerly."""
     timers = {name: Timer(fns) for name, fns in variants.items()}
-    refused = [name for name, t in timers.items() if not t.capture()]
-    use_graph = not refused
+    refused = [name for name, t in timers.items() if graph and not t.capture()]
+    use_graph = graph and not refused
     note = None
     if refused:
         note = (f"all variants timed eagerly: {refused} could not be graph-captured "
@@ -326,10 +326,11 @@ def _trial(fn, inputs, dtype=None, cot=None):
     return [out.detach(), *(g.detach() for g in grads)], cot
 
 
-def selftest_autograd(fn, ref, inputs: list, slack: float = 2.0, time: bool = True) -> dict:
+def selftest_autograd(fn, ref, inputs: list, slack: float = 2.0, time: bool = True, graph: bool = True) -> dict:
     """fn against ref (output and the gradient of every floating input) on one random
     cotangent: fp32 reference, eager original and candidate; then fn under
-    torch.compile(fullgraph=True); then forward + backward timings of all of them."""
+    torch.compile(fullgraph=True); then forward + backward timings of all of them (without graph: of eager
+    calls alone)."""
     with pure_fp32():
         ref32, cot = _trial(ref, inputs, torch.float32)
     orig, _ = _trial(ref, inputs, cot=cot)
@@ -357,7 +358,7 @@ def selftest_autograd(fn, ref, inputs: list, slack: float = 2.0, time: bool = Tr
     if not time:
         return {**result, "compiled": compiled}
 
-    t = time_ab(variants, rounds=3)
+    t = time_ab(variants, rounds=3, graph=graph)
     us = {name: round(v["device_ms"] * 1e3, 1) for name, v in t.items()}
 
     def speed(base, cand):

@@ -64,7 +64,9 @@ def selftest():
 
     tokens = torch.randint(0, 32128, (4096,), device="cuda")
     table = torch.randn(32128, 1024, device="cuda", dtype=torch.bfloat16)
-    return selftest_autograd(lambda t: embedding(tokens, t, 32.0), lambda t: reference(tokens, t, 32.0), [table])
+    # torch's own gradient of an embedding sorts by library calls that must not be captured: a replay of them faulted.
+    return selftest_autograd(lambda t: embedding(tokens, t, 32.0), lambda t: reference(tokens, t, 32.0), [table],
+                             graph=False)
 
 
 if __name__ == "__main__":

@@ -54,7 +54,10 @@ def run_one(name: str) -> dict:
 
 def _selftest_step(name: str):
     """(leaves, fn, cotangent) of the module's selftest shape, for the host-cost probe."""
+    import embedding
     import geglu
+    import linear_cross_entropy
+    import qk_norm_rope
     import relpos_attention
     import rmsnorm
     g = torch.Generator(device="cuda").manual_seed(0)
@@ -70,6 +73,19 @@ def _selftest_step(name: str):
         B, S, H, D = 4, 512, 16, 64
         return ([rnd(B * S, 3 * H * D, scale=0.6), rnd(H, 2 * S - 1, dtype=torch.float32)],
                 lambda q, p: relpos_attention.relpos_attention(q, p, B, S, H, D, 1.0), rnd(B * S, H * D))
+    if name == "qk_norm_rope":
+        B, S, H, D = 4, 512, 16, 128
+        rope = qk_norm_rope.rope_table(S, D)
+        return ([rnd(B * S, 3 * H * D), rnd(D), rnd(D)],
+                lambda q, a, b: qk_norm_rope.qk_norm_rope(q, a, b, rope, B, S, H, D, 1e-6), rnd(B * S, 3 * H * D))
+    if name == "embedding":
+        tokens = torch.randint(0, 32128, (4096,), device="cuda", generator=g)
+        return [rnd(32128, 1024)], lambda t: embedding.embedding(tokens, t, 32.0), rnd(4096, 1024)
+    if name == "linear_cross_entropy":
+        targets = torch.randint(0, 32128, (2048,), device="cuda", generator=g)
+        return ([rnd(2048, 1024), rnd(32128, 1024, scale=1 / 32)],
+                lambda x, w: linear_cross_entropy.linear_cross_entropy(x, w, targets, reduction="none"),
+                rnd(2048, dtype=torch.float32))
     return None
 
 
@@ -110,8 +126,8 @@ def host_cost(name: str, calls: int = 50) -> dict:
 
 def summary(name: str, r: dict) -> str:
     if "error" in r and "kernel_us" not in r:
-        return f"{name:<18} ERROR  {r['error'][:200]}"
-    parts = [f"{name:<18} {'PASS' if r['pass'] else 'FAIL'}",
+        return f"{name:<20} ERROR  {r['error'][:200]}"
+    parts = [f"{name:<20} {'PASS' if r['pass'] else 'FAIL'}",
              f"eager {r['kernel_us']:.1f} us (reference {r['reference_us']:.1f} us, "
              f"{r['speedup']:.2f}x, {r['significance']})"]
     c = r.get("compiled", {})
@@ -141,7 +157,7 @@ def main(argv=None) -> int:
             record["host_costs"][name] = host_cost(name)
         except Exception as e:  # noqa: BLE001 - the cost probe is informative only
             record["host_costs"][name] = {"error": f"{type(e).__name__}: {e}"}
-        print(f"{'':<18} host cost per eager fwd+bwd: {record['host_costs'][name]}", flush=True)
+        print(f"{'':<20} host cost per eager fwd+bwd: {record['host_costs'][name]}", flush=True)
     text = json.dumps(record, indent=2, default=str) + "\n"
     out_dir = args.out_dir
     out_dir.mkdir(parents=True, exist_ok=True)
