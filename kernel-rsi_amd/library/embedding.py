@@ -6,7 +6,7 @@ scale * table[token], rounded once. The gradient of table sums the output gradie
 fp32, over positions that one kernel has sorted by token: no float atomics, so it is bitwise reproducible.
 Every row of it is written, zero where no token names it. A token outside [0, V) gives a row of NaN and
 adds to no gradient. padding_idx: a row whose gradient stays zero (negative: counted from V).
-bf16, fp16 or fp32, V up to 2^24. Usable under torch.compile(fullgraph=True).
+bf16, fp16 or fp32, V up to 2^24, up to 2^25 tokens. Usable under torch.compile(fullgraph=True).
 """
 import sys
 from pathlib import Path
