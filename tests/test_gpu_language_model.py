@@ -113,6 +113,26 @@ def test_captured_step_replays_to_the_eager_one():
         assert torch.equal(loss, want) and all(torch.equal(a, b) for a, b in zip(grads, wants)), i
 
 
+def test_steps_on_two_streams_at_once():
+    """Steps of two batches, each on its own stream, none waiting for the other: bitwise those made one after another."""
+    log("language model steps on two streams")
+    p, (tokens, targets), rope = parameters(), batch(), Q.rope_table(S, D)
+    batches = [(tokens, targets), (tokens.flip(1).contiguous(), targets.flip(0).contiguous())]
+    want = [step(Library, leaves_of(p), t, u, rope) for t, u in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    mine = [leaves_of(p) for _ in batches]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(3):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(step(Library, mine[i], *batches[i], rope))
+    torch.cuda.synchronize()
+    for (loss, grads), runs in zip(want, got):
+        for other, others in runs:
+            assert torch.equal(loss, other) and all(torch.equal(a, b) for a, b in zip(grads, others))
+
+
 def test_single_tokens_at_their_positions():
     """One token of each sequence (S = 1) with its position: the rows that the whole sequences give, bitwise."""
     log("embedding and qk_norm_rope of single tokens")

@@ -130,6 +130,16 @@ def test_native_hands_back_what_is_not_plain():
         assert n.linear_cross_entropy(*args) is None
 
 
+def test_calls_that_nothing_records():
+    """With grad mode on and no input that requires a gradient: the same values, and no node."""
+    log("operators: unrecorded calls")
+    for fn, py, _, inputs, _ in _cases(torch.bfloat16):
+        a = fn(*inputs)
+        assert not a.requires_grad and a.grad_fn is None and torch.equal(a, py(*inputs))
+        with torch.inference_mode():
+            assert torch.equal(fn(*inputs), a)
+
+
 def test_double_backward_is_refused():
     log("operators: double backward")
     for fn, _, _, inputs, _ in _cases(torch.bfloat16):
