@@ -8,7 +8,6 @@ of kernel-rsi_amd/library. `listed()` has the named cases, `draw()` further ones
 """
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -145,7 +144,6 @@ def prepare(case: dict, seed: int) -> dict:
 
 
 # ------------------------------------------------------------------ one pass
-@functools.cache
 def _library():
     path = str(Path(__file__).resolve().parents[1] / "kernel-rsi_amd" / "library")
     if path not in sys.path:
