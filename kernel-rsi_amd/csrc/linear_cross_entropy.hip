@@ -199,7 +199,7 @@ __global__ __launch_bounds__(kOneBlock) void add_losses(const float* __restrict_
 // What the backward needs of a row, in one load.
 struct alignas(16) RowInfo {
   float lse, coef;  // coef 0: no weight
-  int target;       // -1: none
+  int target;       // -1: none, or no weight (such a row has no rest and is not the last to name a target)
   int unused;
 };
 
@@ -238,7 +238,8 @@ __global__ __launch_bounds__(kOneBlock) void row_weights(const float* __restrict
   }
   const float scale = ldexpf(1.f, k);
   for (int r = per_row ? threadIdx.x : me; r < rows; r += per_row ? kOneBlock : all) {
-    info[r] = RowInfo{lse[r], weight(r) * scale, targets.at(r), 0};
+    const float c = weight(r) * scale;
+    info[r] = RowInfo{lse[r], c, c == 0.f ? -1 : targets.at(r), 0};
     rest[r] = 0.f;
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) *back = ldexpf(1.f, -k);

@@ -29,3 +29,29 @@ def _verify(dt, ignored, unweighted):
 def test_rounding_of_the_target_comes_back(dt, ignored):
     log(f"linear_cross_entropy, equal logits, {C.V} targets, {ignored} ignored {dt}")
     _verify(dt, ignored, 0)
+
+
+@DTYPES
+def test_rows_without_weight_take_nothing_from_the_target(dt):
+    """Rows of weight 0 behind the ones that count: the rest of the rows that count comes back all the same."""
+    log(f"linear_cross_entropy, equal logits, rows of weight 0 last {dt}")
+    _verify(dt, 100, C.V // 2)
+
+
+@DTYPES
+def test_rows_without_weight_have_no_gradient(dt):
+    """dx of a row of weight 0 is 0 whatever the row holds, in one part and in parts that are added."""
+    for rows, K, V in ((50, 128, 300), (40, 64, 9000)):
+        log(f"linear_cross_entropy, NaN and infinities in rows of weight 0, x[{rows},{K}] w[{V},{K}] {dt}")
+        g = torch.Generator().manual_seed(4)
+        x = torch.randn(rows, K, generator=g).to(dt).cuda()
+        w = (torch.randn(V, K, generator=g) / K ** 0.5).to(dt).cuda()
+        targets = torch.randint(0, V, (rows,), generator=g).cuda()
+        dout = torch.randn(rows, generator=g).cuda()
+        dout[3:6] = 0.0
+        (ref,) = torch.autograd.grad(L.linear_cross_entropy(x.requires_grad_(True), w, targets, reduction="none"), x, dout)
+        odd = x.detach().clone()
+        odd[3, 5], odd[4, 6], odd[5] = float("nan"), float("inf"), float("-inf")
+        odd.requires_grad_(True)
+        (dx,) = torch.autograd.grad(L.linear_cross_entropy(odd, w, targets, reduction="none"), odd, dout)
+        assert not dx[3:6].any() and torch.equal(dx, ref)
