@@ -291,13 +291,14 @@ def _(x, w, targets, ignore_index, reduction):
 
 @torch.library.custom_op("krsi::linear_cross_entropy_bwd", mutates_args=())
 def linear_cross_entropy_bwd_op(dout: Tensor, x: Tensor, w: Tensor, targets: Tensor, stats: Tensor, ignore_index: int,
-                                reduction: str) -> tuple[Tensor, Tensor]:
-    return _hip.linear_cross_entropy_bwd(dout, x, w, targets, stats, ignore_index, reduction)
+                                reduction: str, dx: bool, dw: bool) -> tuple[Tensor, Tensor]:
+    grads = _hip.linear_cross_entropy_bwd(dout, x, w, targets, stats, ignore_index, reduction, dx, dw)
+    return tuple(x.new_empty(0) if g is None else g for g in grads)  # an op returns tensors: an empty one, not wanted
 
 
 @linear_cross_entropy_bwd_op.register_fake
-def _(dout, x, w, targets, stats, ignore_index, reduction):
-    return x.new_empty(x.shape), w.new_empty(w.shape)
+def _(dout, x, w, targets, stats, ignore_index, reduction, dx, dw):
+    return x.new_empty(x.shape if dx else 0), x.new_empty(w.shape if dw else 0)
 
 
 def _loss_setup(ctx, inputs, output):
@@ -306,7 +307,9 @@ def _loss_setup(ctx, inputs, output):
 
 
 def _loss_backward(ctx, dout, _dstats):
-    return (*linear_cross_entropy_bwd_op(dout.contiguous(), *ctx.saved_tensors, *ctx.args), None, None, None)
+    wanted = ctx.needs_input_grad[:2]
+    grads = linear_cross_entropy_bwd_op(dout.contiguous(), *ctx.saved_tensors, *ctx.args, *wanted)
+    return (*(g if needed else None for g, needed in zip(grads, wanted)), None, None, None)
 
 
 linear_cross_entropy_fwd_op.register_autograd(_loss_backward, setup_context=_loss_setup)
