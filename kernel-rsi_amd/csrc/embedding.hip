@@ -5,8 +5,8 @@
 // reproducible. Tokens outside [0, V) and the padding token have no part in them.
 //
 // What bounds both: HBM (forward: the named rows in, out; backward: g in, dtable out, most of whose rows are zeros).
-// bf16 [32768, 4096], V 131072: forward 71 us, backward 315 (of 1.3 GB: 4.3 TB/s); [8191, 1024], V 32128: 5 and 33
-// (of 83 MB), where group_tokens' latency and the last rows' sums are a half each; 500 tokens there: 2.4 and 24. From
+// bf16 [32768, 4096], V 131072: forward 72 us, backward 302 (of 1.34 GB: 4.4 TB/s); [8191, 1024], V 32128: 5 and 33
+// (of 83 MB), where group_tokens' latency and the last rows' sums are a half each; 500 tokens there: 2.4 and 23. From
 // about 100000 tokens on, group_tokens' two passes over all tokens in each workgroup are the larger part.
 //
 // Backward in three launches:
@@ -34,8 +34,14 @@ constexpr int kGroupWaves = kGroupThreads / kWave;
 constexpr int kGroupRows = 1024;   // most rows of a group: one per thread in its scan, 64 KB of counters
 constexpr int kGroups = 256;       // groups at least (fewer for fewer rows): a workgroup per CU
 constexpr int kFillChunks = 8;     // 16-byte chunks of zeros that a thread of group_tokens writes: 128 KB per workgroup
-// Sorted positions per piece, log2. Short pieces spread the frequent tokens' rows wider, and cost a partial row each:
-// bf16 8191 tokens of 1024 columns 32.7 us with 16, 38.7 with 32, 48.9 with 64; 32768 of 4096: 332, 315, 336.
+// Sorted positions per piece, log2. Short pieces spread the frequent tokens' rows wider, and cost a partial row each.
+// Where they cross depends on the ids, which the host does not know, more than on the columns. The backward with 16
+// and with 32, us, bf16, V 32128, rows of 256 / 1024 / 4096: ids as frequent as 1 / id,
+//   4096 tokens 21 / 25 / 75 and 24 / 29 / 85;  8192: 22 / 31 / 81 and 24 / 36 / 89;  12288: 27 / 38 / 87 and 28 / 43 / 92;
+//   16384: 30 / 41 / 98 and 30 / 45 / 96;  24576: 39 / 53 / 125 and 36 / 49 / 114;
+// half of the tokens one id, 4096: 27 / 31 / 78 and 23 / 29 / 86;  8192: 40 / 48 / 97 and 31 / 43 / 96;
+//   12288: 55 / 64 / 113 and 42 / 55 / 102;  ids of one frequency: the same. Of the first kind 64 is slower than 32 from
+// 2048 to 32768 tokens (1024 columns or more), and 8 slower than 16 from 8192 on.
 int piece_shift_of(int64_t n) { return n <= 8192 ? 4 : 5; }
 constexpr int kHeld = 8;           // tokens that a thread of group_tokens keeps from its count to its placing
 constexpr int kSumWaves = 16;

@@ -11,13 +11,14 @@
 // comes back into dx, and into dw's row of the target from the last of the rows that have it (rows of w that many
 // targets name average it out). bf16 [2048, 1024], V 32128, 2-norm error of dx: 0.0026 without, 0.0019 with (0.0017
 // is the rounding of dx itself).
-// dl is held times a power of two that puts the largest |g| at 2^14..2^15: fp16 then keeps probabilities down to
-// 2^-29 in full precision, and the scale comes off exactly where dx and dw are rounded.
+// dl is held times a power of two that puts the largest |g| at 2^14..2^15: fp16 then keeps its probabilities down to
+// 2^-28 in full precision, and the scale comes off exactly where dx and dw are rounded. One power serves all rows, as dw
+// adds them: in a row whose weight is 2^-k of the largest fp16 keeps them down to 2^(k - 28) (bf16 everywhere).
 //
 // What bounds it: the matrix cores (2 rows V K flop forward, 6 backward, 2 of them the logits again). bf16 [8192,
-// 4096], V 131072: 6.4 ms of logits (1370 TFLOP/s), backward 20.6 ms (1280 over its three products); the vendor's
-// product of such sizes runs at 1390, 1295 and 1125 TFLOP/s in the three orientations. [2048, 1024], V 32128: 121 and
-// 399 us, where 16 stages a tile leave the epilogues a fifth.
+// 4096], V 131072: 6.4 to 6.8 ms of logits by card and run (1370 to 1290 TFLOP/s), backward 20.4 to 20.8 ms (1295 to 1270
+// over its three products); the vendor's product of such sizes runs at 1390, 1295 and 1125 TFLOP/s in the three
+// orientations. [2048, 1024], V 32128: 131 and 411 us, where 16 stages a tile leave the epilogues a fifth.
 #include "chunks.h"
 #include "krsi_device.h"
 #include "krsi_internal.h"

@@ -9,8 +9,8 @@
 //   dn = dz w;  n = x r;  dx = r (dn - n r sum(dn x) / D).
 //
 // What bounds it: HBM (forward 2 bytes moved per byte of qkv; backward dy, q and k in, dqkv out). bf16 [16384, 48
-// heads of 128]: forward 69.0 us (5.8 TB/s), backward 105 us (5.1 TB/s); a copy of 2 GB runs at 4.9.
-// Outputs are stored past the caches (forward 73 us without).
+// heads of 128]: forward 65 to 70 us by card and run (6.2 to 5.8 TB/s), backward 104 us (5.2 TB/s); a copy of 2 GB
+// runs at 4.9. Outputs are stored past the caches (forward 73 us without).
 // Layout: a lane holds C elements of one half of the pairs and the C elements that they rotate with, so the
 // rotation stays in registers; the lanes of a head (their number rounded up to a power of two, the group) reduce its
 // square sum by shuffles. C is the widest of 8, 4, 2, 1 (16 bytes at most) that a half of the rotated columns and
