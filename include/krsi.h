@@ -273,8 +273,8 @@ int krsi_embedding_bwd(const void* dout, const void* tokens, int32_t token_bytes
 /* ---------------- cross entropy of an output projection (no counterpart)
  * l = x w^T; loss_n = log sum_v exp(l_nv) - l_n,target(n). x [rows, k], w [v, k] contiguous, 16-byte aligned, of T
  * (KRSI_DTYPE_BF16 or KRSI_DTYPE_F16); l is fp32 and is not kept. targets [rows] int32 or int64 (target_bytes 4
- * or 8): ignore_index has loss 0 and no gradient (its row of x has to be finite where dw is wanted, which adds it
- * times zero); one outside [0, v) makes its loss (and gradients) NaN.
+ * or 8): ignore_index has loss 0 and no gradient, nor has a row whose dout is 0 (such a row of x has to be finite
+ * where dw is wanted, which adds it times zero); one outside [0, v) makes its loss (and gradients) NaN.
  * reduction 0: loss [rows] fp32; 1: loss [1], the mean over the targets that are not ignored (NaN if there are
  * none); 2: loss [1], the sum. stats [rows + 1] fp32, for the backward: lse of each row, then (1, 2) their number.
  * Backward: dout fp32, [rows] or [1]; dx [rows, k] and dw [v, k] of T, either may be NULL (not wanted). The logits
@@ -282,8 +282,8 @@ int krsi_embedding_bwd(const void* dout, const void* tokens, int32_t token_bytes
  * keeps the largest at the top of fp16's range. Sums are fp32, in a fixed order.
  * Limits: k % 64 == 0, k <= 2^20, v and rows <= 2^23 (ceil(rows / 128) ceil(v / 128) <= 2^23, of v and k as
  * well, of rows and k <= 2^18). No rows: loss 0 or NaN, dw zero. Workspaces: the *_workspace_bytes (the forward's
- * holds 8 bytes per row and 64 logits, of about 512 MB's worth of rows at a time; the backward's a piece of rows x v,
- * 512 MB or 4096 columns wide, and fp32 parts of dx). */
+ * holds 8 bytes per row and 64 logits, of about 512 MB's worth of rows, 2048 at least, at a time; the backward's a piece
+ * of rows x v, 512 MB or 4096 columns wide, and fp32 parts of dx, 4 rows k bytes each, and of the piece's dw). */
 size_t krsi_linear_cross_entropy_fwd_workspace_bytes(int64_t rows, int32_t k, int32_t v);
 size_t krsi_linear_cross_entropy_bwd_workspace_bytes(int64_t rows, int32_t k, int32_t v);
 int krsi_linear_cross_entropy_fwd(const void* x, const void* w, const void* targets, int32_t target_bytes, float* loss,

@@ -5,11 +5,15 @@ x [..., K] hidden states, w [V, K] the projection's weight (nn.Linear or a tied 
 or int64. The loss of a row is log(sum_v exp(l_v)) - l_target for l = x w^T, formed in one pass over the
 vocabulary: the logits are fp32 in registers and are never written. The backward computes them again in
 pieces of the vocabulary; each piece's gradient is rounded to x's dtype (times a power of two, so that fp16
-keeps small probabilities) and multiplied into dx, which is carried in fp32, and dw. It allocates a piece of about
-512 MB at most, where the logits themselves take 4 bytes for each row and vocabulary entry.
+keeps small probabilities; rows of reduction="none" whose weight is 2^-k of the largest keep them down to 2^(k - 28)) and
+multiplied into dx, which is carried in fp32, and dw; they are off by 1.1 to 1.3 times what their own rounding takes. The
+backward allocates a piece, 512 MB or 8192 bytes a row where that is more, and fp32 sums: of dx, 4 rows K bytes for each part
+of its sum, where there are several pieces or parts, and likewise of dw's piece. The logits themselves would take 4 bytes for
+each row and vocabulary entry.
 The loss is fp32: its mean over the targets that are not ignore_index (NaN if there are none), their sum,
-or with reduction="none" the loss of each (0 where ignored, whatever its row of x holds; dw, which adds that row times
-zero, needs it finite). A target outside [0, V) that is not ignore_index makes the loss, and the gradients, NaN. bf16 or fp16, K a multiple of 64. Usable under
+or with reduction="none" the loss of each (0 where ignored, whatever its row of x holds). A row that is ignored, or whose
+loss has gradient 0, gets none, whatever it holds; dw, which adds that row times zero, needs it finite. A target outside
+[0, V) that is not ignore_index makes the loss, and the gradients, NaN. bf16 or fp16, K a multiple of 64. Usable under
 torch.compile(fullgraph=True).
 """
 import sys
