@@ -294,6 +294,27 @@ int krsi_linear_cross_entropy_bwd(const float* dout, const void* x, const void* 
                                   size_t workspace_bytes, int64_t rows, int32_t k, int32_t v, int64_t ignore_index,
                                   int32_t reduction, int32_t dtype, void* stream);
 
+/* ------------------------ residual addition with RMS norm (no counterpart)
+ * The step between a layer's output and the next layer: r = T(x + residual), the stream that goes on, and its norm with
+ * krsi_rmsnorm_fwd's rounding points, y = T(w * T(r * rstd)). x, residual, y, r [rows, n] contiguous and w [n], of T, any
+ * alignment of the element; rstd [rows] fp32 for the backward, or NULL.
+ * 8 bits: z = w * r * rstd in fp32, scale [rows] = max(max|z| / 448, 2^-120), q [rows, n] = e4m3 (OCP, one byte) of
+ * z / scale, round to nearest even: z is about q * scale. residual and r may both be NULL: the norm of x. A row that
+ * holds an infinity or NaN reads back as NaN throughout. krsi_quantize_rows: z is x itself.
+ * Backward: dy, dr the gradients of y and r (dr may be NULL: zero); dx the gradient of x and of residual alike,
+ * T(dr + the norm's), dw [n] summed in fp32 in a fixed order. workspace: *_workspace_bytes, scratch.
+ * Limits: 1 <= n <= 16384 (krsi_quantize_rows: 2^20), rows < 2^26 divided by the waves a row takes (1 up to 1024 columns,
+ * then 4, 8 and 16). No rows: dw zero. No buffer overlaps one that is written.                              */
+int krsi_add_rmsnorm_fwd(const void* x, const void* residual, const void* w, void* y, void* r, float* rstd, int64_t rows,
+                         int32_t n, float eps, int32_t dtype, void* stream);
+int krsi_add_rmsnorm_8bit(const void* x, const void* residual, const void* w, void* q, float* scale, void* r, int64_t rows,
+                          int32_t n, float eps, int32_t dtype, void* stream);
+int krsi_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int32_t n, int32_t dtype, void* stream);
+size_t krsi_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int32_t n);
+int krsi_add_rmsnorm_bwd(const void* dy, const void* dr, const void* r, const void* w, const float* rstd, void* dx,
+                         void* dw, void* workspace, size_t workspace_bytes, int64_t rows, int32_t n, int32_t dtype,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,7 @@
 // shorter than a chunk (in the forward, of up to one element per lane) or wider than 8 chunks
 // per lane take a scalar path with the same math.
 #include "chunks.h"
+#include "column_sum.h"
 #include "krsi_device.h"
 #include "krsi_internal.h"
 
@@ -37,7 +38,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWavesPerBlock = kThreads / kWave;
 constexpr int kBwdMaxBlocks = 512;     // persistent grid of the backward
-constexpr int kColsumWaves = 16;       // waves per column-sum workgroup (64 columns each)
 constexpr int kScalarRowChunk = 64;    // rows per block of the scalar dw kernel
 
 // RAGGED: columns that two chunks share count once in every sum. Before, such rows took the scalar kernels,
@@ -323,32 +323,6 @@ __global__ __launch_bounds__(kThreads) void rms_bwd_dw_scalar(const typename Ele
     acc += Elem<DT>::load(g[i]) * Elem<DT>::round(Elem<DT>::load(x[i]) * rstd[r]);
   }
   part[(int64_t)blockIdx.y * n + col] = acc;
-}
-
-// dw = column sums of the [R, n] fp32 partial rows (R <= 512), in fixed order, in one launch.
-// Block = 64 columns (lane = column) and 16 waves: wave w adds rows w, w + 16, ... in order,
-// then wave 0 adds the 16 wave sums in wave order and writes dtype DT. Each wave has at most
-// 32 rows, all of whose loads it can have in flight.
-template <int DT>
-__global__ __launch_bounds__(kColsumWaves * kWave) void colsum(const float* __restrict__ in, int64_t R,
-                                                               int n, typename Elem<DT>::T* __restrict__ out) {
-  __shared__ float s[kColsumWaves][kWave];
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave = threadIdx.x / kWave;
-  const int col = blockIdx.x * kWave + lane;
-  float acc = 0.f;
-  if (col < n) {
-#pragma unroll 8
-    for (int64_t r = wave; r < R; r += kColsumWaves) acc += in[r * n + col];
-  }
-  s[wave][lane] = acc;
-  __syncthreads();
-  if (wave == 0 && col < n) {
-    float t = s[0][lane];
-#pragma unroll
-    for (int w = 1; w < kColsumWaves; ++w) t += s[w][lane];
-    out[col] = Elem<DT>::store(t);
-  }
 }
 
 bool vec_ok(int n, int e, std::initializer_list<const void*> ptrs) {

@@ -455,6 +455,49 @@ struct LinearCrossEntropyFn : torch::autograd::Function<LinearCrossEntropyFn> {
   }
 };
 
+// ----------------------------------------- residual addition with RMS norm
+struct AddRmsNormFn : torch::autograd::Function<AddRmsNormFn> {
+  // y, r and, where stats is given, the reciprocal roots.
+  static variable_list launch(const Tensor& x, const Tensor& residual, const Tensor& w, double eps, Tensor* stats) {
+    const c10::DeviceGuard guard(x.device());
+    Tensor y = at::empty_like(x), r = at::empty_like(x);
+    if (stats) *stats = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+    forward_status(krsi_add_rmsnorm_fwd(x.data_ptr(), residual.data_ptr(), w.data_ptr(), y.data_ptr(), r.data_ptr(),
+                                        stats ? stats->data_ptr<float>() : nullptr, x.size(0), (int)x.size(1), (float)eps,
+                                        dtype_code(x), stream_of(x)));
+    return {y, r};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& w,
+                               double eps) {
+    Tensor rstd;
+    variable_list out = launch(x, residual, w, eps, &rstd);
+    ctx->save_for_backward({out[1], w, rstd});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["shape"] = std::vector<int64_t>{x.size(0), x.size(1), (int64_t)x.scalar_type()};
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {grads[1], grads[1], Tensor(), Tensor()};  // the stream alone was used
+    const c10::DeviceGuard guard(grads[0].device());
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t rows = shape[0], n = shape[1];
+    const at::ScalarType type = (at::ScalarType)shape[2];
+    const auto saved = ctx->get_saved_variables();
+    const Tensor dy = grads[0].contiguous(), dr = grads[1].defined() ? grads[1].contiguous() : Tensor(),
+                 r = saved[0].contiguous(), w = saved[1].contiguous(), rstd = saved[2].contiguous();
+    check_saved("r", r, dy, type, {rows, n});
+    check_saved("weight", w, dy, type, {n});
+    check_saved("rstd", rstd, dy, at::kFloat, {rows});
+    Tensor dx = at::empty_like(r), dw = at::empty({n}, w.options());
+    const size_t bytes = krsi_add_rmsnorm_bwd_workspace_bytes(rows, (int)n);
+    Tensor ws = at::empty({(int64_t)bytes}, r.options().dtype(at::kByte));
+    backward_status(krsi_add_rmsnorm_bwd(dy.data_ptr(), dr.defined() ? dr.data_ptr() : nullptr, r.data_ptr(), w.data_ptr(),
+                                         rstd.data_ptr<float>(), dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), bytes, rows,
+                                         (int)n, dtype_code(r), stream_of(r)));
+    return {dx, dx, dw, Tensor()};
+  }
+};
+
 // ---------------------------------------------------------------- Python entries
 // An entry as Python calls it: C++ exceptions, of the argument tests too, become Python ones.
 using Args = PyObject* const*;
@@ -479,6 +522,23 @@ PyObject* unlocked(Fn&& fn) {
       out = fn();
     }
     return THPVariable_Wrap(std::move(out));
+  } catch (const NotPlain&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// The same for several tensors, as a tuple; an undefined one is None.
+template <typename Fn>
+PyObject* unlocked_tuple(Fn&& fn) {
+  try {
+    variable_list out;
+    {
+      ReleaseLock released;
+      out = fn();
+    }
+    PyObject* tuple = PyTuple_New((Py_ssize_t)out.size());
+    for (size_t i = 0; tuple && i < out.size(); ++i) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(std::move(out[i])));
+    return tuple;
   } catch (const NotPlain&) {
     Py_RETURN_NONE;
   }
@@ -653,6 +713,46 @@ PyObject* py_linear_cross_entropy(Args a, Py_ssize_t n) {
   });
 }
 
+// x [rows, n], residual (may be null) like it and w [n], contiguous, of one type and device, some rows.
+bool plain_rows(const Tensor& x, const Tensor* residual, const Tensor& w) {
+  if (x.dim() != 2 || !x.is_contiguous() || x.numel() == 0 || dtype_code(x) < 0 || x.size(1) > kIntMax) return false;
+  if (residual && (residual->scalar_type() != x.scalar_type() || residual->sizes() != x.sizes() ||
+                   !residual->is_contiguous() || residual->device() != x.device()))
+    return false;
+  return w.scalar_type() == x.scalar_type() && w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous() &&
+         w.device() == x.device();
+}
+
+PyObject* py_add_rmsnorm(Args a, Py_ssize_t n) {
+  const Tensor *x, *residual, *w;
+  double eps;
+  if (n != 4 || !plain_context() || !tensor_arg(a[0], &x) || !tensor_arg(a[1], &residual) || !tensor_arg(a[2], &w) ||
+      !float_arg(a[3], &eps) || !plain_rows(*x, residual, *w))
+    Py_RETURN_NONE;
+  return unlocked_tuple([&] {
+    return recorded({x, residual, w}) ? AddRmsNormFn::apply(*x, *residual, *w, eps)
+                                      : AddRmsNormFn::launch(*x, *residual, *w, eps, nullptr);
+  });
+}
+
+PyObject* py_add_rmsnorm_8bit(Args a, Py_ssize_t n) {
+  const Tensor *x, *residual = nullptr, *w;
+  double eps;
+  if (n != 4 || !plain_context() || !tensor_arg(a[0], &x) || (a[1] != Py_None && !tensor_arg(a[1], &residual)) ||
+      !tensor_arg(a[2], &w) || !float_arg(a[3], &eps) || !plain_rows(*x, residual, *w))
+    Py_RETURN_NONE;
+  return unlocked_tuple([&]() -> variable_list {
+    const c10::DeviceGuard guard(x->device());
+    Tensor q = at::empty(x->sizes(), x->options().dtype(at::kFloat8_e4m3fn)),
+           scale = at::empty({x->size(0)}, x->options().dtype(at::kFloat)), r;
+    if (residual) r = at::empty(x->sizes(), x->options());
+    forward_status(krsi_add_rmsnorm_8bit(x->data_ptr(), residual ? residual->data_ptr() : nullptr, w->data_ptr(),
+                                         q.data_ptr(), scale.data_ptr<float>(), residual ? r.data_ptr() : nullptr,
+                                         x->size(0), (int)x->size(1), (float)eps, dtype_code(*x), stream_of(*x)));
+    return {q, scale, r};
+  });
+}
+
 PyObject* py_set_module(PyObject*, PyObject* m) {
   Py_XDECREF(g_hip_module);
   Py_INCREF(m);
@@ -669,6 +769,8 @@ PyMethodDef kMethods[] = {
     {"qk_norm_rope", (PyCFunction)(void*)entry<py_qk_norm_rope>, METH_FASTCALL, nullptr},
     {"embedding", (PyCFunction)(void*)entry<py_embedding>, METH_FASTCALL, nullptr},
     {"linear_cross_entropy", (PyCFunction)(void*)entry<py_linear_cross_entropy>, METH_FASTCALL, nullptr},
+    {"add_rmsnorm", (PyCFunction)(void*)entry<py_add_rmsnorm>, METH_FASTCALL, nullptr},
+    {"add_rmsnorm_8bit", (PyCFunction)(void*)entry<py_add_rmsnorm_8bit>, METH_FASTCALL, nullptr},
     {"set_module", py_set_module, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_krsi_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

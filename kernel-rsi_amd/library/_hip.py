@@ -82,6 +82,11 @@ SIGNATURES = {
     "krsi_linear_cross_entropy_bwd": (ctypes.c_int, [_P, _P, _P, _P, _I32, _P, _P, _P, _P, _SZ, _I64, _I32, _I32, _I64,
                                                      _I32, _I32, _P]),
     "krsi_embedding_bwd": (ctypes.c_int, [_P, _P, _I32, _P, _P, _SZ, _I64, _I32, _I32, _I64, _F32, _I32, _P]),
+    "krsi_add_rmsnorm_fwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _F32, _I32, _P]),
+    "krsi_add_rmsnorm_8bit": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _F32, _I32, _P]),
+    "krsi_quantize_rows": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _P]),
+    "krsi_add_rmsnorm_bwd_workspace_bytes": (_SZ, [_I64, _I32]),
+    "krsi_add_rmsnorm_bwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I32, _I32, _P]),
 }
 
 # KRSI_DTYPE_* codes of the activation dtypes.
@@ -125,6 +130,7 @@ class _NoNative:
 
     rmsnorm = geglu = geglu_linear = relpos_attention = bucket_table = _none
     qk_norm_rope = embedding = linear_cross_entropy = _none
+    add_rmsnorm = add_rmsnorm_8bit = _none
 
 
 _native = None
@@ -226,6 +232,12 @@ def _on_device(fn):
                 return fn(first, *args)
         return fn(first, *args)
     return call
+
+
+def refuse_recording(name: str, *ts: torch.Tensor | None) -> None:
+    """Raises where a gradient of an 8-bit result would be recorded: there is none, and it would be lost in silence."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise ValueError(f"{name} has no gradient: call it under torch.no_grad(), or detach its inputs")
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -678,3 +690,91 @@ def linear_cross_entropy_bwd(dout: torch.Tensor, x: torch.Tensor, w: torch.Tenso
                                                    _ptr(stats), _ptr(gx), _ptr(gw), _ptr(ws), nbytes, rows, k, v,
                                                    ignore_index, REDUCTIONS[reduction], dt, _stream(x)))
     return gx, gw
+
+
+# ----------------------------------------- residual addition with RMS norm
+E4M3 = torch.float8_e4m3fn
+
+
+def _check_add_rmsnorm(x2d: torch.Tensor, residual: torch.Tensor | None, w: torch.Tensor) -> int:
+    _on_gpu(x2d, w, *(() if residual is None else (residual,)))
+    dt = _dtype("x2d", x2d)
+    _dtype("weight", w, like=x2d)
+    if x2d.dim() != 2 or not x2d.is_contiguous():
+        raise ValueError("x2d must be a contiguous 2D tensor [rows, N]")
+    if w.shape != x2d.shape[1:]:
+        raise ValueError(f"weight shape {tuple(w.shape)} != ({x2d.shape[1]},)")
+    if residual is not None:
+        _dtype("residual", residual, like=x2d)
+        if residual.shape != x2d.shape or not residual.is_contiguous():
+            raise ValueError(f"residual must be contiguous and of x2d's shape {tuple(x2d.shape)}, got "
+                             f"{tuple(residual.shape)} with strides {residual.stride()}")
+    return dt
+
+
+@_on_device
+def add_rmsnorm_fwd(x2d: torch.Tensor, residual: torch.Tensor, w: torch.Tensor, eps: float,
+                    stats: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """y, r = x2d + residual and (with stats) the reciprocal roots that the backward reads."""
+    dt = _check_add_rmsnorm(x2d, residual, w)
+    w = w.contiguous()
+    rows, n = x2d.shape
+    y, r = torch.empty_like(x2d), torch.empty_like(x2d)
+    rstd = torch.empty(rows, device=x2d.device, dtype=torch.float32) if stats else None
+    if rows:
+        _check(lib().krsi_add_rmsnorm_fwd(_ptr(x2d), _ptr(residual), _ptr(w), _ptr(y), _ptr(r), _ptr(rstd), rows, n,
+                                          float(eps), dt, _stream(x2d)))
+    return y, r, rstd
+
+
+@_on_device
+def add_rmsnorm_bwd(dy: torch.Tensor, dr: torch.Tensor | None, r: torch.Tensor, w: torch.Tensor,
+                    rstd: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gradient of x2d (and of residual alike), and dw."""
+    dt = _check_add_rmsnorm(r, dr, w)
+    _on_gpu(r, dy, rstd)
+    _dtype("grad", dy, like=r)
+    if dy.shape != r.shape:
+        raise ValueError(f"grad shape {tuple(dy.shape)} != {tuple(r.shape)}")
+    rows, n = r.shape
+    if rstd.dtype != torch.float32 or rstd.shape != (rows,):
+        raise ValueError(f"rstd {rstd.dtype} {tuple(rstd.shape)} is not that of {rows} rows")
+    dy, w, rstd = dy.contiguous(), w.contiguous(), rstd.contiguous()
+    dx, dw = torch.empty_like(r), torch.empty_like(w)
+    nbytes = lib().krsi_add_rmsnorm_bwd_workspace_bytes(rows, n)
+    ws = torch.empty(max(nbytes, 1), device=r.device, dtype=torch.uint8)
+    _check(lib().krsi_add_rmsnorm_bwd(_ptr(dy), _ptr(dr), _ptr(r), _ptr(w), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(ws),
+                                      nbytes, rows, n, dt, _stream(r)))
+    return dx, dw
+
+
+@_on_device
+def add_rmsnorm_8bit(x2d: torch.Tensor, residual: torch.Tensor | None, w: torch.Tensor,
+                     eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """Codes and scales of the norm, and r = x2d + residual (None without a residual)."""
+    dt = _check_add_rmsnorm(x2d, residual, w)
+    w = w.contiguous()
+    rows, n = x2d.shape
+    q = torch.empty(rows, n, device=x2d.device, dtype=E4M3)
+    scale = torch.empty(rows, device=x2d.device, dtype=torch.float32)
+    r = None if residual is None else torch.empty_like(x2d)
+    if rows:
+        _check(lib().krsi_add_rmsnorm_8bit(_ptr(x2d), _ptr(residual), _ptr(w), _ptr(q), _ptr(scale), _ptr(r), rows, n,
+                                           float(eps), dt, _stream(x2d)))
+    return q, scale, r
+
+
+@_on_device
+def quantize_rows(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of the rows."""
+    _on_gpu(x2d)
+    dt = _dtype("x2d", x2d)
+    if x2d.dim() != 2:
+        raise ValueError(f"x2d must be [rows, N], got {tuple(x2d.shape)}")
+    x2d = x2d.contiguous()
+    rows, n = x2d.shape
+    q = torch.empty(rows, n, device=x2d.device, dtype=E4M3)
+    scale = torch.empty(rows, device=x2d.device, dtype=torch.float32)
+    if rows:
+        _check(lib().krsi_quantize_rows(_ptr(x2d), _ptr(q), _ptr(scale), rows, n, dt, _stream(x2d)))
+    return q, scale

@@ -8,7 +8,8 @@ Op names follow the reference (library/rmsnorm.py:86-103, geglu.py:85-101,
 relpos_attention.py:175-195): krsi::rmsnorm_fwd/bwd, krsi::geglu_fwd/bwd,
 krsi::relpos_attn_fwd/bwd; krsi::relpos_bucket_gather/sum (the T5 table step) and
 krsi::geglu_linear_fwd (the merged projection with the GEGLU epilogue), krsi::qk_norm_rope_fwd/bwd,
-krsi::embedding_fwd/bwd and krsi::linear_cross_entropy_fwd/bwd have no counterpart there. Their schemas are internal
+krsi::embedding_fwd/bwd, krsi::linear_cross_entropy_fwd/bwd, krsi::add_rmsnorm_fwd/bwd, the 8-bit krsi::add_rmsnorm_8bit,
+krsi::rmsnorm_8bit, krsi::quantize_rows and krsi::linear_8bit have no counterpart there. Their schemas are internal
 to this library.
 """
 from __future__ import annotations
@@ -313,3 +314,68 @@ def _loss_backward(ctx, dout, _dstats):
 
 
 linear_cross_entropy_fwd_op.register_autograd(_loss_backward, setup_context=_loss_setup)
+
+# ----------------------------------------- residual addition with RMS norm
+
+
+@torch.library.custom_op("krsi::add_rmsnorm_fwd", mutates_args=())
+def add_rmsnorm_fwd_op(x2d: Tensor, residual: Tensor, w: Tensor, eps: float) -> tuple[Tensor, Tensor, Tensor]:
+    return _hip.add_rmsnorm_fwd(x2d, residual, w, eps)
+
+
+@add_rmsnorm_fwd_op.register_fake
+def _(x2d, residual, w, eps):
+    return torch.empty_like(x2d), torch.empty_like(x2d), x2d.new_empty((x2d.shape[0],), dtype=torch.float32)
+
+
+@torch.library.custom_op("krsi::add_rmsnorm_bwd", mutates_args=())
+def add_rmsnorm_bwd_op(dy: Tensor, dr: Tensor, r: Tensor, w: Tensor, rstd: Tensor) -> tuple[Tensor, Tensor]:
+    return _hip.add_rmsnorm_bwd(dy, dr, r, w, rstd)
+
+
+@add_rmsnorm_bwd_op.register_fake
+def _(dy, dr, r, w, rstd):
+    return torch.empty_like(r), w.new_empty(w.shape)
+
+
+def _add_rms_setup(ctx, inputs, output):
+    ctx.save_for_backward(output[1], inputs[2], output[2])
+
+
+def _add_rms_backward(ctx, dy, dr, _drstd):
+    dx, dw = add_rmsnorm_bwd_op(dy.contiguous(), dr.contiguous(), *ctx.saved_tensors)
+    return dx, dx, dw, None
+
+
+add_rmsnorm_fwd_op.register_autograd(_add_rms_backward, setup_context=_add_rms_setup)
+
+
+@torch.library.custom_op("krsi::add_rmsnorm_8bit", mutates_args=())
+def add_rmsnorm_8bit_op(x2d: Tensor, residual: Tensor, w: Tensor, eps: float) -> tuple[Tensor, Tensor, Tensor]:
+    return _hip.add_rmsnorm_8bit(x2d, residual, w, eps)
+
+
+@add_rmsnorm_8bit_op.register_fake
+def _(x2d, residual, w, eps):
+    return (torch.empty_like(x2d, dtype=_hip.E4M3), x2d.new_empty((x2d.shape[0],), dtype=torch.float32),
+            torch.empty_like(x2d))
+
+
+@torch.library.custom_op("krsi::rmsnorm_8bit", mutates_args=())
+def rmsnorm_8bit_op(x2d: Tensor, w: Tensor, eps: float) -> tuple[Tensor, Tensor]:
+    return _hip.add_rmsnorm_8bit(x2d, None, w, eps)[:2]
+
+
+@rmsnorm_8bit_op.register_fake
+def _(x2d, w, eps):
+    return torch.empty_like(x2d, dtype=_hip.E4M3), x2d.new_empty((x2d.shape[0],), dtype=torch.float32)
+
+
+@torch.library.custom_op("krsi::quantize_rows", mutates_args=())
+def quantize_rows_op(x2d: Tensor) -> tuple[Tensor, Tensor]:
+    return _hip.quantize_rows(x2d)
+
+
+@quantize_rows_op.register_fake
+def _(x2d):
+    return x2d.new_empty(x2d.shape, dtype=_hip.E4M3), x2d.new_empty((x2d.shape[0],), dtype=torch.float32)
