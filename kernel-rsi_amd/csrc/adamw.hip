@@ -1,0 +1,539 @@
+// One AdamW step over any number of tensors in a few launches, and the norm of all gradients.
+//   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  w = w (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+// g: the gradient times min(1, max_norm / (norm + 1e-6)) where a norm is given; a norm that is not finite leaves everything
+// as it is. w: the fp32 master where there is one, and the parameter its rounding; else the parameter itself. All
+// arithmetic is fp32, 1 - b^t fp64.
+//
+// States of 8 bits: e4m3 codes of m and of s = sqrt(v), with an fp32 scale for each 256 elements of a tensor (the largest
+// magnitude over 448, at least 2^-120). v changes by 1 - b2 in a step, far less than half a step of any 8-bit type: rounded
+// to nearest it would stand still. So codes are rounded up or down at random, m right on average and s right on average in
+// its square, v: between the codes k and k + 1 (in units of their spacing) t goes up with probability (t^2 - k^2) / (2 k + 1).
+// A root above zero stays above zero, which keeps m / s within bounds. The random numbers are a function of the seed, the
+// step, the tensor's number and the element's alone: multiplicative hashing (Knuth) with xor-shifts between.
+//
+// Bound by HBM: 28 bytes a parameter with 16-bit weights and gradients, masters and 32-bit states; 16 with 8-bit ones. What a
+// launch needs to know of each tensor comes as an argument by value, so nothing is copied to the device beforehand and
+// a captured launch holds its own copy.
+#include <algorithm>
+#include <cmath>
+#include <memory>
+#include <new>
+
+#include "chunks.h"
+#include "krsi_device.h"
+#include "krsi_internal.h"
+
+namespace krsi {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 256;        // elements that share a scale
+constexpr int kStepChunk = 8192;   // elements per workgroup of the step
+constexpr int kNormChunk = 65536;  // and of the norm
+
+struct Item {
+  void* param;
+  const void* grad;
+  void *m, *v;
+  float *master, *scales;
+  int64_t n;
+  int32_t first, number;  // its first workgroup of this launch, its number in the list
+};
+constexpr int kItems = 60;  // as many as the 4 KB of a launch's arguments hold
+struct Items {
+  Item item[kItems];
+  int32_t count;
+};
+
+// What a step needs of a tensor, from the first launch.
+struct Factor {
+  float rate;   // lr / (1 - b1^t)
+  float root;   // 1 / sqrt(1 - b2^t)
+  float share;  // of the gradient
+  float decay;  // 1 - lr wd
+  uint32_t key, go;
+  uint32_t pad[2];
+};
+
+__device__ __forceinline__ uint32_t mixed(uint32_t h) {
+  h = (h ^ (h >> 16)) * 0x6A09E667u;  // the fractions of the roots of 2 and 3
+  h = (h ^ (h >> 15)) * 0xBB67AE85u;
+  return h ^ (h >> 16);
+}
+constexpr uint32_t kGolden = 0x9E3779B1u;
+__device__ __forceinline__ uint32_t with_word(uint32_t key, uint32_t word) { return mixed(key * 3u + word * kGolden + 1u); }
+
+// The launch's tensor that workgroup b works on.
+__device__ __forceinline__ int find(const Items& t, int b) {
+  int lo = 0, hi = t.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (t.item[mid].first <= b)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// Eight consecutive elements of any alignment.
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float* f) {
+  using El = Elem<DT>;
+#pragma unroll
+  for (int q = 0; q < 8 / El::E; ++q)
+    El::unpack(load_chunk<true>((const typename El::T*)p + i + q * El::E), f + q * El::E);
+}
+template <int DT>
+__device__ __forceinline__ void store8(void* p, int64_t i, const float* f) {
+  using El = Elem<DT>;
+#pragma unroll
+  for (int q = 0; q < 8 / El::E; ++q)
+    __builtin_nontemporal_store(El::pack(f + q * El::E), reinterpret_cast<u32x4_any*>((typename El::T*)p + i + q * El::E));
+}
+// The first `some` of them.
+template <int DT>
+__device__ __forceinline__ void load_some(const void* p, int64_t i, int some, float* f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = j < some ? Elem<DT>::load(((const typename Elem<DT>::T*)p)[i + j]) : 0.f;
+}
+template <int DT>
+__device__ __forceinline__ void store_some(void* p, int64_t i, int some, const float* f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < some) ((typename Elem<DT>::T*)p)[i + j] = Elem<DT>::store(f[j]);
+}
+template <int DT>
+__device__ __forceinline__ void load_part(const void* p, int64_t i, int some, float* f) {
+  if (some == 8)
+    load8<DT>(p, i, f);
+  else
+    load_some<DT>(p, i, some, f);
+}
+template <int DT>
+__device__ __forceinline__ void store_part(void* p, int64_t i, int some, const float* f) {
+  if (some == 8)
+    store8<DT>(p, i, f);
+  else
+    store_some<DT>(p, i, some, f);
+}
+
+// ------------------------------------------------------------------- norm
+template <int DT>
+__global__ __launch_bounds__(kThreads) void norm_parts(const Items items, float* __restrict__ part) {
+  __shared__ float red[kThreads / kWave];
+  const Item& t = items.item[find(items, blockIdx.x)];
+  const int64_t at = (int64_t)((int)blockIdx.x - t.first) * kNormChunk, end = min(at + kNormChunk, t.n);
+  float sum[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum[j] = 0.f;
+  const int64_t whole = at + (end - at) / 8 * 8;
+#pragma unroll 4
+  for (int64_t i = at + 8 * threadIdx.x; i < whole; i += 8 * kThreads) {
+    float f[8];
+    load8<DT>(t.grad, i, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] += f[j] * f[j];
+  }
+  if (threadIdx.x < end - whole) {
+    const float f = Elem<DT>::load(((const typename Elem<DT>::T*)t.grad)[whole + threadIdx.x]);
+    sum[0] += f * f;
+  }
+  float s = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+  s = wave_sum(s);
+  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+constexpr int kJoin = 1024;
+__global__ __launch_bounds__(kJoin) void norm_join(const float* __restrict__ part, int64_t n, float* __restrict__ norm) {
+  __shared__ double red[kJoin];
+  double s = 0;
+  for (int64_t i = threadIdx.x; i < n; i += kJoin) s += part[i];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  for (int w = kJoin / 2; w > 0; w /= 2) {
+    if (threadIdx.x < (unsigned)w) red[threadIdx.x] += red[threadIdx.x + w];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *norm = (float)sqrt(red[0]);
+}
+
+// ------------------------------------------------------------------- step
+constexpr int kMaskWords = 896;
+struct Mask {
+  uint32_t word[kMaskWords];  // bit i: tensor i of this launch's range has a gradient
+};
+
+__global__ __launch_bounds__(kThreads) void step_factors(const Mask mask, int base, int count, int32_t* __restrict__ steps,
+                                                         Factor* __restrict__ out, const float* __restrict__ lr_at, float lr,
+                                                         double log1, double log2, float wd, const float* __restrict__ norm,
+                                                         float max_norm, uint32_t seed) {
+  const int i = blockIdx.x * kThreads + threadIdx.x;
+  if (i >= count) return;
+  Factor f{};
+  const float total = norm ? *norm : 0.f;
+  if ((mask.word[i / 32] >> (i % 32) & 1u) && fabsf(total) <= 3.402823466e38f) {
+    const int32_t t = steps[base + i] + 1;
+    steps[base + i] = t;
+    if (lr_at) lr = *lr_at;
+    f.rate = (float)((double)lr / -expm1(t * log1));
+    f.root = (float)(1.0 / sqrt(-expm1(t * log2)));
+    f.share = norm ? fminf(max_norm / (total + 1e-6f), 1.f) : 1.f;
+    f.decay = 1.f - lr * wd;
+    f.key = with_word(with_word(mixed(seed), (uint32_t)t), (uint32_t)(base + i));
+    f.go = 1;
+  }
+  out[base + i] = f;
+}
+
+struct Rule {
+  float b1, c1, b2, c2, eps;  // c: 1 - b, formed in fp64
+};
+
+template <int PT, int GT, bool MASTER>
+__global__ __launch_bounds__(kThreads) void step32(const Items items, const Factor* __restrict__ factors, const Rule k) {
+  const Item& t = items.item[find(items, blockIdx.x)];
+  const Factor f = factors[t.number];
+  if (!f.go) return;
+  const int64_t at = (int64_t)((int)blockIdx.x - t.first) * kStepChunk;
+#pragma unroll 1
+  for (int s = 0; s < kStepChunk / (8 * kThreads); ++s) {
+    const int64_t i = at + 8 * (s * kThreads + (int)threadIdx.x);
+    const int some = (int)min((int64_t)8, t.n - i);
+    if (some <= 0) return;
+    float g[8], m[8], v[8], w[8];
+    load_part<GT>(t.grad, i, some, g);
+    load_part<kF32>(t.m, i, some, m);
+    load_part<kF32>(t.v, i, some, v);
+    if constexpr (MASTER)
+      load_part<kF32>(t.master, i, some, w);
+    else
+      load_part<PT>(t.param, i, some, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = g[j] * f.share;
+      m[j] = m[j] * k.b1 + x * k.c1;
+      v[j] = v[j] * k.b2 + (x * x) * k.c2;
+      const float d = __builtin_amdgcn_sqrtf(v[j]) * f.root + k.eps;
+      w[j] = w[j] * f.decay - f.rate * m[j] * __builtin_amdgcn_rcpf(d);
+    }
+    store_part<kF32>(t.m, i, some, m);
+    store_part<kF32>(t.v, i, some, v);
+    if constexpr (MASTER) store_part<kF32>(t.master, i, some, w);
+    store_part<PT>(t.param, i, some, w);
+  }
+}
+
+// The largest of the 16 lanes of a DPP row, in all of them.
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));  // rotations by 1, 2, 4, 8
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));
+}
+// NaN where the largest magnitude is infinite or NaN (the maximum is of integers, so NaN stays).
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  const float t = __uint_as_float(top);
+  return __uint_as_float(max(__float_as_uint(t * (1.0f / 448.0f) + t * 0.f), 0x03800000u));  // 2^-120
+}
+
+// The spacing of e4m3 at a value's size, 2^(max(e, -6) - 3), and its reciprocal.
+__device__ __forceinline__ uint32_t spacing_bits(float a) {
+  return max(__float_as_uint(a) & 0x7f800000u, 121u << 23) - (3u << 23);
+}
+
+__device__ __forceinline__ float rounded_m(float a, uint32_t h) {
+  const uint32_t s = spacing_bits(a);
+  const float k = floorf(a * __uint_as_float((254u << 23) - s) + (float)(h & 0xffffu) * (1.0f / 65536.0f));
+  return fminf(fmaxf(k * __uint_as_float(s), -448.f), 448.f);
+}
+__device__ __forceinline__ float rounded_root(float b, uint32_t h) {
+  const uint32_t s = spacing_bits(b);
+  const float t = b * __uint_as_float((254u << 23) - s), low = floorf(t);
+  const bool up = (t - low) * (t + low) > (float)(h >> 16) * (1.0f / 65536.0f) * (2.f * low + 1.f) || (low == 0.f && t > 0.f);
+  return fminf((low + (up ? 1.f : 0.f)) * __uint_as_float(s), 448.f);
+}
+
+// 16 elements a lane: a DPP row of 16 lanes has a scale's 256.
+template <int PT, int GT, bool MASTER>
+__global__ __launch_bounds__(kThreads) void step8(const Items items, const Factor* __restrict__ factors, const Rule k) {
+  const Item& t = items.item[find(items, blockIdx.x)];
+  const Factor f = factors[t.number];
+  if (!f.go) return;
+  const int64_t at = (int64_t)((int)blockIdx.x - t.first) * kStepChunk, blocks = (t.n + kBlock - 1) / kBlock;
+  const uint32_t key = with_word(f.key, (uint32_t)(at >> 32));
+#pragma unroll 1
+  for (int s = 0; s < kStepChunk / (16 * kThreads); ++s) {
+    const int64_t i = at + 16 * (s * kThreads + (int)threadIdx.x);
+    const int64_t left = t.n - i;
+    const int64_t block = i / kBlock;
+    if (block >= blocks) return;  // whole rows of lanes
+    const float ms = t.scales[block], rs = t.scales[blocks + block];
+    float m[16], r[16];
+    uint32_t mc[4], rc[4];
+    if (left >= 16) {
+      const u32x4 a = *reinterpret_cast<const u32x4_any*>((const uint8_t*)t.m + i);
+      const u32x4 b = *reinterpret_cast<const u32x4_any*>((const uint8_t*)t.v + i);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) mc[q] = a[q], rc[q] = b[q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        mc[q] = rc[q] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (4 * q + j < left) {
+            mc[q] |= (uint32_t)((const uint8_t*)t.m)[i + 4 * q + j] << (8 * j);
+            rc[q] |= (uint32_t)((const uint8_t*)t.v)[i + 4 * q + j] << (8 * j);
+          }
+      }
+    }
+    uint32_t mtop = 0, rtop = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int some = (int)max((int64_t)0, min((int64_t)8, left - 8 * h));
+      float g[8], w[8];
+      load_part<GT>(t.grad, i + 8 * h, some, g);
+      if constexpr (MASTER)
+        load_part<kF32>(t.master, i + 8 * h, some, w);
+      else
+        load_part<PT>(t.param, i + 8 * h, some, w);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const int q = 2 * h + j / 4;
+        const auto md = j % 4 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[q], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[q], false);
+        const auto rd = j % 4 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)rc[q], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)rc[q], false);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = g[j + e] * f.share, old = rd[e] * rs;
+          const float mn = (md[e] * ms) * k.b1 + x * k.c1;
+          const float vn = (old * old) * k.b2 + (x * x) * k.c2;
+          const float rn = __builtin_amdgcn_sqrtf(vn);
+          w[j + e] = w[j + e] * f.decay - f.rate * mn * __builtin_amdgcn_rcpf(rn * f.root + k.eps);
+          m[8 * h + j + e] = mn;
+          r[8 * h + j + e] = rn;
+          mtop = max(mtop, __float_as_uint(mn) & 0x7fffffffu);
+          rtop = max(rtop, __float_as_uint(rn) & 0x7fffffffu);
+        }
+      }
+      if constexpr (MASTER) store_part<kF32>(t.master, i + 8 * h, some, w);
+      store_part<PT>(t.param, i + 8 * h, some, w);
+    }
+    const float mscale = scale_of(row_max(mtop)), rscale = scale_of(row_max(rtop));
+    if (threadIdx.x % 16 == 0) {
+      t.scales[block] = mscale;
+      t.scales[blocks + block] = rscale;
+    }
+    const float minv = 1.0f / mscale, rinv = 1.0f / rscale;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float a[4], b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t h = mixed((uint32_t)(i + 4 * q + j) * kGolden + key);
+        a[j] = rounded_m(m[4 * q + j] * minv, h);
+        b[j] = rounded_root(r[4 * q + j] * rinv, h);
+      }
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(a[0], a[1], 0, false);
+      mc[q] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a[2], a[3], c, true);
+      c = __builtin_amdgcn_cvt_pk_fp8_f32(b[0], b[1], 0, false);
+      rc[q] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b[2], b[3], c, true);
+    }
+    if (left >= 16) {
+      *reinterpret_cast<u32x4_any*>((uint8_t*)t.m + i) = u32x4{mc[0], mc[1], mc[2], mc[3]};
+      *reinterpret_cast<u32x4_any*>((uint8_t*)t.v + i) = u32x4{rc[0], rc[1], rc[2], rc[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j < left) {
+          ((uint8_t*)t.m)[i + j] = (uint8_t)(mc[j / 4] >> (8 * (j % 4)));
+          ((uint8_t*)t.v)[i + j] = (uint8_t)(rc[j / 4] >> (8 * (j % 4)));
+        }
+    }
+  }
+}
+
+bool known_dtype(int32_t dt) { return dt == kBf16 || dt == kF16 || dt == kF32; }
+constexpr int64_t kMostElements = INT64_C(1) << 36;
+constexpr int32_t kMostTensors = 1 << 20;
+
+int check_sizes(const int64_t* sizes, int32_t count) {
+  if (count < 0 || count > kMostTensors) return KRSI_ERR_BAD_SHAPE;
+  if (count && !sizes) return KRSI_ERR_NULL_POINTER;
+  int64_t total = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    if (sizes[i] < 0 || sizes[i] > kMostElements) return KRSI_ERR_BAD_SHAPE;
+    total += sizes[i];
+    if (total > kMostElements) return KRSI_ERR_BAD_SHAPE;
+  }
+  return KRSI_OK;
+}
+
+// Workgroups of a launch: its threads stay below 2^32.
+constexpr int64_t kMostGroups = (INT64_C(1) << 24) - 1;
+static_assert(kMostElements / kStepChunk <= kMostGroups, "a tensor fits a launch");
+
+// Calls launch(items, workgroups) for the listed tensors, in as few launches as their number and sizes allow.
+// add(i, item) fills an item's pointers, or says that tensor i has no part.
+template <typename Add, typename Launch>
+int in_launches(const int64_t* sizes, int32_t count, int64_t chunk, Add&& add, Launch&& launch) {
+  Items t;
+  t.count = 0;
+  int64_t groups = 0;
+  auto flush = [&] {
+    if (t.count) launch(t, (unsigned)groups);
+    t.count = 0;
+    groups = 0;
+  };
+  for (int32_t i = 0; i < count; ++i) {
+    const int64_t need = ceil_div(sizes[i], chunk);
+    Item it{};
+    if (!need || !add(i, it)) continue;
+    if (t.count == kItems || groups + need > kMostGroups) flush();
+    it.n = sizes[i];
+    it.first = (int32_t)groups;
+    it.number = i;
+    t.item[t.count++] = it;
+    groups += need;
+  }
+  flush();
+  return launch_status();
+}
+
+int64_t norm_groups(const int64_t* sizes, int32_t count) {
+  int64_t n = 0;
+  for (int32_t i = 0; i < count; ++i) n += ceil_div(sizes[i], kNormChunk);
+  return n;
+}
+
+template <int BITS, int PT, int GT, bool MASTER>
+auto step_kernel() {
+  if constexpr (BITS == 8)
+    return step8<PT, GT, MASTER>;
+  else
+    return step32<PT, GT, MASTER>;
+}
+using StepKernel = void (*)(const Items, const Factor*, const Rule);
+template <int BITS>
+StepKernel step_kernel(int32_t pt, int32_t gt, bool master) {
+  if (pt == kF32) return step_kernel<BITS, kF32, kF32, false>();
+  if (pt == kBf16 && gt == kBf16) return master ? step_kernel<BITS, kBf16, kBf16, true>() : step_kernel<BITS, kBf16, kBf16, false>();
+  if (pt == kBf16) return master ? step_kernel<BITS, kBf16, kF32, true>() : step_kernel<BITS, kBf16, kF32, false>();
+  if (gt == kF16) return master ? step_kernel<BITS, kF16, kF16, true>() : step_kernel<BITS, kF16, kF16, false>();
+  return master ? step_kernel<BITS, kF16, kF32, true>() : step_kernel<BITS, kF16, kF32, false>();
+}
+
+bool in_range(double v) { return std::isfinite(v) && std::fabs(v) <= 3.0e38; }
+
+}  // namespace
+}  // namespace krsi
+
+extern "C" {
+
+size_t krsi_grad_norm_workspace_bytes(const int64_t* sizes, int32_t count) {
+  using namespace krsi;
+  if (check_sizes(sizes, count) != KRSI_OK) return 0;
+  return align256((size_t)(norm_groups(sizes, count) + 1) * sizeof(float));
+}
+
+int krsi_grad_norm(const void* const* grads, const int64_t* sizes, int32_t count, float* norm, void* workspace,
+                   size_t workspace_bytes, int32_t dtype, void* stream) {
+  using namespace krsi;
+  if (!known_dtype(dtype)) return KRSI_ERR_UNSUPPORTED;
+  int rc = check_sizes(sizes, count);
+  if (rc != KRSI_OK) return rc;
+  if (!norm || (count && !grads)) return KRSI_ERR_NULL_POINTER;
+  if (!workspace || workspace_bytes < krsi_grad_norm_workspace_bytes(sizes, count)) return KRSI_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
+  float* part = (float*)workspace;
+  const hipStream_t st = as_stream(stream);
+  int64_t at = 0;
+  rc = in_launches(
+      sizes, count, kNormChunk,
+      [&](int32_t i, Item& t) {
+        t.grad = grads[i];
+        return grads[i] != nullptr;
+      },
+      [&](const Items& t, unsigned groups) {
+        const auto kernel = dtype == kF16 ? norm_parts<kF16> : dtype == kF32 ? norm_parts<kF32> : norm_parts<kBf16>;
+        hipLaunchKernelGGL(kernel, dim3(groups), dim3(kThreads), 0, st, t, part + at);
+        at += groups;
+      });
+  if (rc != KRSI_OK) return rc;
+  hipLaunchKernelGGL(norm_join, dim3(1), dim3(kJoin), 0, st, (const float*)part, at, norm);
+  return launch_status();
+}
+
+size_t krsi_adamw_workspace_bytes(int32_t count) {
+  using namespace krsi;
+  return count < 0 || count > kMostTensors ? 0 : align256((size_t)count * sizeof(Factor) + 1);
+}
+
+int krsi_adamw_step(void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
+                    float* const* masters, float* const* scales, const int64_t* sizes, int32_t count, int32_t* steps,
+                    const float* lr_at, float lr, double beta1, double beta2, float eps, float weight_decay,
+                    const float* norm, float max_norm, uint32_t seed, int32_t state_bits, int32_t dtype, int32_t grad_dtype,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace krsi;
+  if (!known_dtype(dtype) || (grad_dtype != dtype && grad_dtype != kF32) || (masters && dtype == kF32))
+    return KRSI_ERR_UNSUPPORTED;
+  if ((state_bits != 8 && state_bits != 32) || (state_bits == 8) != (scales != nullptr)) return KRSI_ERR_UNSUPPORTED;
+  int rc = check_sizes(sizes, count);
+  if (rc != KRSI_OK) return rc;
+  if ((!lr_at && !in_range(lr)) || !in_range(eps) || eps < 0 || !in_range(weight_decay) || !(beta1 >= 0 && beta1 < 1) ||
+      !(beta2 >= 0 && beta2 < 1) || (norm && !(max_norm >= 0)))
+    return KRSI_ERR_BAD_SCALE;
+  if (count == 0) return KRSI_OK;
+  if (!params || !grads || !exp_avgs || !exp_avg_sqs || !steps) return KRSI_ERR_NULL_POINTER;
+  if (!workspace || workspace_bytes < krsi_adamw_workspace_bytes(count)) return KRSI_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
+  // No parameter twice: two workgroups would write it.
+  struct Span {
+    uintptr_t begin, end;
+    bool operator<(const Span& o) const { return begin < o.begin; }
+  };
+  const std::unique_ptr<Span[]> spans(new (std::nothrow) Span[count]);
+  if (!spans) return KRSI_ERR_TOO_LARGE;
+  const int64_t width = dtype == kF32 ? 4 : 2;
+  int32_t used = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    if (!grads[i] || !sizes[i]) continue;
+    if (!params[i] || !exp_avgs[i] || !exp_avg_sqs[i] || (masters && !masters[i]) || (scales && !scales[i]))
+      return KRSI_ERR_NULL_POINTER;
+    spans[used++] = Span{(uintptr_t)params[i], (uintptr_t)params[i] + sizes[i] * width};
+  }
+  std::sort(spans.get(), spans.get() + used);
+  for (int32_t i = 1; i < used; ++i)
+    if (spans[i].begin < spans[i - 1].end) return KRSI_ERR_BAD_SHAPE;
+
+  Factor* factors = (Factor*)workspace;
+  const hipStream_t st = as_stream(stream);
+  for (int32_t base = 0; base < count; base += 32 * kMaskWords) {
+    const int32_t here = std::min(count - base, 32 * kMaskWords);
+    Mask mask{};
+    for (int32_t i = 0; i < here; ++i)
+      if (grads[base + i]) mask.word[i / 32] |= 1u << (i % 32);
+    hipLaunchKernelGGL(step_factors, dim3((unsigned)ceil_div(here, kThreads)), dim3(kThreads), 0, st, mask, base, here, steps,
+                       factors, lr_at, lr, std::log(beta1), std::log(beta2), weight_decay, norm, max_norm, seed);
+  }
+  rc = launch_status();
+  if (rc != KRSI_OK) return rc;
+  const Rule rule{(float)beta1, (float)(1 - beta1), (float)beta2, (float)(1 - beta2), eps};
+  const StepKernel kernel = state_bits == 8 ? step_kernel<8>(dtype, grad_dtype, masters != nullptr)
+                                            : step_kernel<32>(dtype, grad_dtype, masters != nullptr);
+  return in_launches(
+      sizes, count, kStepChunk,
+      [&](int32_t i, Item& t) {
+        t.param = params[i], t.grad = grads[i], t.m = exp_avgs[i], t.v = exp_avg_sqs[i];
+        t.master = masters ? masters[i] : nullptr;
+        t.scales = scales ? scales[i] : nullptr;
+        return grads[i] != nullptr;
+      },
+      [&](const Items& t, unsigned groups) {
+        hipLaunchKernelGGL(kernel, dim3(groups), dim3(kThreads), 0, st, t, (const Factor*)factors, rule);
+      });
+}
+
+}  // extern "C"

@@ -753,6 +753,137 @@ PyObject* py_add_rmsnorm_8bit(Args a, Py_ssize_t n) {
   });
 }
 
+// A list of tensors (or None, where `holes` has none of them) that are plain, contiguous and on one device.
+bool list_arg(PyObject* o, bool holes, std::vector<const Tensor*>* out) {
+  if (!PyList_CheckExact(o)) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(o);
+  out->resize(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* item = PyList_GET_ITEM(o, i);
+    if (holes && item == Py_None) {
+      (*out)[i] = nullptr;
+      continue;
+    }
+    if (!tensor_arg(item, &(*out)[i]) || !(*out)[i]->is_contiguous()) return false;
+  }
+  return true;
+}
+
+Tensor norm_of(const std::vector<const Tensor*>& grads, const Tensor& like, int dtype) {
+  std::vector<const void*> ptrs;
+  std::vector<int64_t> sizes;
+  for (const Tensor* g : grads)
+    if (g) {
+      ptrs.push_back(g->data_ptr());
+      sizes.push_back(g->numel());
+    }
+  const int count = (int)ptrs.size();
+  Tensor norm = at::empty({}, like.options().dtype(at::kFloat));
+  const size_t bytes = krsi_grad_norm_workspace_bytes(sizes.data(), count);
+  Tensor ws = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+  forward_status(krsi_grad_norm(ptrs.data(), sizes.data(), count, norm.data_ptr<float>(), ws.data_ptr(), bytes, dtype,
+                                stream_of(like)));
+  return norm;
+}
+
+PyObject* py_grad_norm(Args a, Py_ssize_t n) {
+  std::vector<const Tensor*> grads;
+  if (n != 1 || !plain_context() || !list_arg(a[0], true, &grads)) Py_RETURN_NONE;
+  const Tensor* first = nullptr;
+  for (const Tensor* g : grads) {
+    if (!g) continue;
+    if (!first) first = g;
+    if (g->scalar_type() != first->scalar_type() || g->device() != first->device()) Py_RETURN_NONE;
+  }
+  if (!first || dtype_code(*first) < 0 || grads.size() > (1u << 20)) Py_RETURN_NONE;
+  return unlocked([&] {
+    at::NoGradGuard no_grad;
+    const c10::DeviceGuard guard(first->device());
+    return norm_of(grads, *first, dtype_code(*first));
+  });
+}
+
+// One step; (norm,) with None for no norm.
+PyObject* py_adamw_step(Args a, Py_ssize_t n) {
+  std::vector<const Tensor*> params, grads, m, v, masters, scales;
+  const Tensor *steps, *lr_at = nullptr, *norm_arg = nullptr;
+  double lr = 0, b1, b2, eps, decay, max_norm = 0;
+  int64_t seed;
+  if (n != 15 || !plain_context() || !list_arg(a[0], false, &params) || !list_arg(a[1], true, &grads) ||
+      !list_arg(a[2], false, &m) || !list_arg(a[3], false, &v) || !tensor_arg(a[4], &steps) ||
+      (!float_arg(a[5], &lr) && !tensor_arg(a[5], &lr_at)) || !float_arg(a[6], &b1) || !float_arg(a[7], &b2) ||
+      !float_arg(a[8], &eps) || !float_arg(a[9], &decay) || (a[10] != Py_None && !list_arg(a[10], false, &masters)) ||
+      (a[11] != Py_None && !list_arg(a[11], false, &scales)) || (a[12] != Py_None && !float_arg(a[12], &max_norm)) ||
+      (a[13] != Py_None && !tensor_arg(a[13], &norm_arg)) || !int_arg(a[14], 0, 0xffffffff, &seed))
+    Py_RETURN_NONE;
+  const size_t count = params.size();
+  const bool with_masters = a[10] != Py_None, with_scales = a[11] != Py_None, clip = a[12] != Py_None;
+  if (!count || count > (1u << 20) || grads.size() != count || m.size() != count || v.size() != count ||
+      (with_masters && masters.size() != count) || (with_scales && scales.size() != count))
+    Py_RETURN_NONE;
+  const auto device = params[0]->device();
+  const auto type = params[0]->scalar_type(), state = with_scales ? at::kFloat8_e4m3fn : at::kFloat;
+  const int dt = dtype_code(*params[0]);
+  auto one = [&](const Tensor* t) { return t->scalar_type() == at::kFloat && t->numel() == 1 && t->device() == device; };
+  if (dt < 0 || steps->scalar_type() != at::kInt || steps->dim() != 1 || steps->size(0) != (int64_t)count ||
+      !steps->is_contiguous() || steps->device() != device || (lr_at && !one(lr_at)) || (norm_arg && !one(norm_arg)))
+    Py_RETURN_NONE;
+  const Tensor* first = nullptr;
+  std::vector<void*> pp(count), mp(count), vp(count);
+  std::vector<const void*> gp(count);
+  std::vector<float*> wp(with_masters ? count : 0), sp(with_scales ? count : 0);
+  std::vector<int64_t> sizes(count);
+  auto fits = [&](const Tensor* t, at::ScalarType kind, const Tensor* p) {
+    return t->scalar_type() == kind && t->sizes() == p->sizes() && t->device() == device;
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const Tensor *p = params[i], *g = grads[i];
+    if (!fits(p, type, p) || !fits(m[i], state, p) || !fits(v[i], state, p)) Py_RETURN_NONE;
+    if (g) {
+      if (!first) first = g;
+      if (!fits(g, first->scalar_type(), p)) Py_RETURN_NONE;
+      // An empty tensor has no address; one that is not null says that its gradient is there.
+      gp[i] = g->numel() ? g->data_ptr() : steps->data_ptr();
+    }
+    pp[i] = p->data_ptr(), mp[i] = m[i]->data_ptr(), vp[i] = v[i]->data_ptr(), sizes[i] = p->numel();
+    if (with_masters) {
+      if (!fits(masters[i], at::kFloat, p)) Py_RETURN_NONE;
+      wp[i] = masters[i]->data_ptr<float>();
+    }
+    if (with_scales) {
+      const Tensor* s = scales[i];
+      if (s->scalar_type() != at::kFloat || s->dim() != 2 || s->size(0) != 2 || s->size(1) != (sizes[i] + 255) / 256 ||
+          s->device() != device)
+        Py_RETURN_NONE;
+      sp[i] = s->data_ptr<float>();
+    }
+  }
+  const int gdt = first ? dtype_code(*first) : dt;
+  if (gdt != dt && gdt != KRSI_DTYPE_F32) Py_RETURN_NONE;
+  return unlocked_tuple([&]() -> variable_list {
+    at::NoGradGuard no_grad;
+    const c10::DeviceGuard guard(device);
+    Tensor norm;
+    if (norm_arg) norm = *norm_arg;
+    if (clip && !norm.defined()) norm = norm_of(grads, *params[0], gdt);
+    const size_t bytes = krsi_adamw_workspace_bytes((int)count);
+    Tensor ws = at::empty({(int64_t)bytes}, params[0]->options().dtype(at::kByte));
+    forward_status(krsi_adamw_step(pp.data(), gp.data(), mp.data(), vp.data(), with_masters ? wp.data() : nullptr,
+                                   with_scales ? sp.data() : nullptr, sizes.data(), (int)count, steps->data_ptr<int32_t>(),
+                                   lr_at ? lr_at->data_ptr<float>() : nullptr, (float)lr, b1, b2, (float)eps, (float)decay,
+                                   norm.defined() ? norm.data_ptr<float>() : nullptr, (float)max_norm, (uint32_t)seed,
+                                   with_scales ? 8 : 32, dt, gdt, ws.data_ptr(), bytes, stream_of(*params[0])));
+    // What a graph has saved of these counts as changed.
+    auto changed = [](const Tensor& t) {
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    changed(*steps);
+    for (const auto* list : {&params, &m, &v, &masters, &scales})
+      for (const Tensor* t : *list) changed(*t);
+    return {norm};
+  });
+}
+
 PyObject* py_set_module(PyObject*, PyObject* m) {
   Py_XDECREF(g_hip_module);
   Py_INCREF(m);
@@ -771,6 +902,8 @@ PyMethodDef kMethods[] = {
     {"linear_cross_entropy", (PyCFunction)(void*)entry<py_linear_cross_entropy>, METH_FASTCALL, nullptr},
     {"add_rmsnorm", (PyCFunction)(void*)entry<py_add_rmsnorm>, METH_FASTCALL, nullptr},
     {"add_rmsnorm_8bit", (PyCFunction)(void*)entry<py_add_rmsnorm_8bit>, METH_FASTCALL, nullptr},
+    {"grad_norm", (PyCFunction)(void*)entry<py_grad_norm>, METH_FASTCALL, nullptr},
+    {"adamw_step", (PyCFunction)(void*)entry<py_adamw_step>, METH_FASTCALL, nullptr},
     {"set_module", py_set_module, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_krsi_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -86,6 +86,11 @@ SIGNATURES = {
     "krsi_add_rmsnorm_8bit": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _F32, _I32, _P]),
     "krsi_quantize_rows": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _P]),
     "krsi_add_rmsnorm_bwd_workspace_bytes": (_SZ, [_I64, _I32]),
+    "krsi_grad_norm_workspace_bytes": (_SZ, [_P, _I32]),
+    "krsi_grad_norm": (ctypes.c_int, [_P, _P, _I32, _P, _P, _SZ, _I32, _P]),
+    "krsi_adamw_workspace_bytes": (_SZ, [_I32]),
+    "krsi_adamw_step": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _F32, ctypes.c_double, ctypes.c_double,
+                                       _F32, _F32, _P, _F32, ctypes.c_uint32, _I32, _I32, _I32, _P, _SZ, _P]),
     "krsi_add_rmsnorm_bwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I32, _I32, _P]),
 }
 
@@ -130,7 +135,7 @@ class _NoNative:
 
     rmsnorm = geglu = geglu_linear = relpos_attention = bucket_table = _none
     qk_norm_rope = embedding = linear_cross_entropy = _none
-    add_rmsnorm = add_rmsnorm_8bit = _none
+    add_rmsnorm = add_rmsnorm_8bit = grad_norm = adamw_step = _none
 
 
 _native = None
@@ -778,3 +783,123 @@ def quantize_rows(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if rows:
         _check(lib().krsi_quantize_rows(_ptr(x2d), _ptr(q), _ptr(scale), rows, n, dt, _stream(x2d)))
     return q, scale
+
+
+# --------------------------------------------------- AdamW over many tensors
+BLOCK_8BIT = 256  # elements of an 8-bit state that share a scale
+
+
+def _pointers(ts: list) -> ctypes.Array:
+    return (_P * len(ts))(*(None if t is None else t.data_ptr() for t in ts))
+
+
+def _one_dtype(name: str, ts: list) -> torch.dtype:
+    """The type that all of them have."""
+    kinds = {t.dtype for t in ts}
+    if len(kinds) != 1:
+        raise TypeError(f"{name} must be of one dtype, got {sorted(map(str, kinds))}")
+    return kinds.pop()
+
+
+def grad_norm(grads: list[torch.Tensor | None]) -> torch.Tensor:
+    """The root of the sum of squares over all of them, an fp32 scalar on their device."""
+    present = [g for g in grads if g is not None]
+    if not present:
+        raise ValueError("grad_norm needs a gradient")
+    _on_gpu(*present)
+    _one_dtype("gradients", present)
+    dt = _dtype("gradients", present[0])
+    present = [g.contiguous() for g in present]
+    sizes = (_I64 * len(present))(*(g.numel() for g in present))
+    with torch.cuda.device(present[0].device):
+        norm = torch.empty((), device=present[0].device, dtype=torch.float32)
+        nbytes = lib().krsi_grad_norm_workspace_bytes(sizes, len(present))
+        ws = torch.empty(max(nbytes, 1), device=norm.device, dtype=torch.uint8)
+        _check(lib().krsi_grad_norm(_pointers(present), sizes, len(present), _ptr(norm), _ptr(ws), nbytes, dt,
+                                    _stream(norm)))
+    return norm
+
+
+def _scalar_on_device(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
+    _on_gpu(like, t)
+    if t.dtype != torch.float32 or t.numel() != 1:
+        raise ValueError(f"{name} must be one float32 number, got {t.dtype} {tuple(t.shape)}")
+
+
+def _check_adamw(params, grads, exp_avgs, exp_avg_sqs, steps, masters, scales) -> tuple:
+    """(dtype code, gradients' dtype code, state bits) of lists that fit each other."""
+    count = len(params)
+    if not count:
+        raise ValueError("adamw_step needs a parameter")
+    for name, ts in (("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs), ("masters", masters),
+                     ("scales", scales)):
+        if ts is not None and len(ts) != count:
+            raise ValueError(f"{len(ts)} {name} for {count} parameters")
+    present = [g for g in grads if g is not None]
+    _on_gpu(*params, *present, *exp_avgs, *exp_avg_sqs, steps, *(masters or ()), *(scales or ()))
+    dt = _dtype("parameters", params[0])
+    gdt = dt
+    if present:
+        gdt = _dtype("gradients", present[0])
+        if _one_dtype("gradients", present) not in (params[0].dtype, torch.float32):
+            raise TypeError(f"gradients must be {params[0].dtype}, as the parameters, or torch.float32, got "
+                            f"{present[0].dtype}")
+    state = E4M3 if scales is not None else torch.float32
+    if masters is not None and dt == DTYPE_CODES[torch.float32]:
+        raise TypeError("masters are for 16-bit parameters")
+    if steps.dtype != torch.int32 or steps.shape != (count,) or not steps.is_contiguous():
+        raise ValueError(f"steps must be {count} contiguous int32 numbers, got {steps.dtype} {tuple(steps.shape)}")
+    for i, p in enumerate(params):
+        for name, t, kind in (("parameter", p, params[0].dtype), ("exp_avg", exp_avgs[i], state),
+                              ("exp_avg_sq", exp_avg_sqs[i], state),
+                              ("master", None if masters is None else masters[i], torch.float32)):
+            if t is None:
+                continue
+            if t.dtype != kind:
+                raise TypeError(f"{name} {i} must be {kind}, got {t.dtype}")
+            if t.shape != p.shape or not t.is_contiguous():
+                raise ValueError(f"{name} {i} must be contiguous with shape {tuple(p.shape)}, got {tuple(t.shape)} with "
+                                 f"strides {t.stride()}")
+        if grads[i] is not None and grads[i].shape != p.shape:
+            raise ValueError(f"gradient {i} has shape {tuple(grads[i].shape)}, its parameter {tuple(p.shape)}")
+        if scales is not None:
+            blocks = -(-p.numel() // BLOCK_8BIT)
+            if scales[i].dtype != torch.float32 or scales[i].shape != (2, blocks) or not scales[i].is_contiguous():
+                raise ValueError(f"scales {i} must be contiguous float32 [2, {blocks}], got {scales[i].dtype} "
+                                 f"{tuple(scales[i].shape)}")
+    spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError("a parameter overlaps another, or is in the list twice")
+    return dt, gdt, 32 if scales is None else 8
+
+
+def adamw_step(params: list, grads: list, exp_avgs: list, exp_avg_sqs: list, steps: torch.Tensor, lr, beta1: float,
+               beta2: float, eps: float, weight_decay: float, masters: list | None, scales: list | None,
+               max_norm: float | None, norm: torch.Tensor | None, seed: int) -> torch.Tensor | None:
+    """One step in place; the norm that the gradients were clipped by, if any."""
+    dt, gdt, bits = _check_adamw(params, grads, exp_avgs, exp_avg_sqs, steps, masters, scales)
+    at = None
+    if isinstance(lr, torch.Tensor):
+        _scalar_on_device("lr", lr, params[0])
+        lr, at = 0.0, lr
+    if norm is not None:
+        _scalar_on_device("norm", norm, params[0])
+    grads = [g if g is None else g.contiguous() for g in grads]
+    if max_norm is not None and norm is None:
+        norm = (grad_norm(grads) if any(g is not None for g in grads) else
+                torch.zeros((), device=params[0].device, dtype=torch.float32))
+    count = len(params)
+    # An empty tensor has no address; one that is not NULL says that its gradient is there.
+    given = (_P * count)(*(None if g is None else g.data_ptr() or steps.data_ptr() for g in grads))
+    with torch.cuda.device(params[0].device):
+        nbytes = lib().krsi_adamw_workspace_bytes(count)
+        ws = torch.empty(max(nbytes, 1), device=params[0].device, dtype=torch.uint8)
+        _check(lib().krsi_adamw_step(
+            _pointers(params), given, _pointers(exp_avgs), _pointers(exp_avg_sqs),
+            None if masters is None else _pointers(masters), None if scales is None else _pointers(scales),
+            (_I64 * count)(*(p.numel() for p in params)), count, _ptr(steps), _ptr(at), float(lr), beta1, beta2, eps,
+            weight_decay, _ptr(norm), 0.0 if max_norm is None else max_norm, seed & 0xffffffff, bits, dt, gdt, _ptr(ws),
+            nbytes, _stream(params[0])))
+    written = [steps] + [t for ts in (params, exp_avgs, exp_avg_sqs, masters, scales) if ts is not None for t in ts]
+    torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    return norm

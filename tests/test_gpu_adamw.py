@@ -1,0 +1,553 @@
+"""adamw_step, grad_norm and AdamW on the GPU against the formulas in 64 bits.
+
+Tolerances, e = 2^-24: m and v are two products and a sum in fp32 of values that the 64-bit formula has exactly, 4 e of
+their terms' sizes (and 2 e more of the gradient through a clipped one, 4 of its square). The change of w is lr / bc1 * m / (root + eps) with a root
+and a reciprocal of 1 unit each and six roundings, 16 e of it, and w's product and sum 3 e |w|; a rounding to the
+parameter's type half a step more. An 8-bit state's value is a step of e4m3 off at most (2^-3 relative, 2^-9 of the scale
+below the normal range)."""
+import math
+
+import pytest
+import torch
+
+import _hip
+import adamw as W
+from krsi_testutil import log, seeded
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+ids = lambda d: str(d).split(".")[-1]  # noqa: E731
+E = 2.0 ** -24
+HYPER = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+SHAPES = [(1,), (7,), (8,), (255,), (256,), (257,), (3, 5, 2), (0,), (33, 129), (8192,), (8193,), (100, 173), (16385,)]
+
+
+def _lists(shapes, dt, bits=32, masters=False, gdt=None, seed=0, grad_std=1e-2):
+    """Parameters, gradients and states of some steps, and the arguments of a call."""
+    w = [seeded(s, seed + 3 * i, std=0.5, dtype=torch.float32) for i, s in enumerate(shapes)]
+    g = [seeded(s, seed + 100 + i, std=grad_std, dtype=torch.float32).to(gdt or dt) for i, s in enumerate(shapes)]
+    m = [seeded(s, seed + 200 + i, std=grad_std / 3, dtype=torch.float32) for i, s in enumerate(shapes)]
+    v = [(seeded(s, seed + 300 + i, std=grad_std, dtype=torch.float32).abs() + grad_std / 4).square()
+         for i, s in enumerate(shapes)]
+    steps = torch.arange(len(shapes), dtype=torch.int32, device="cuda") * 7
+    kw = {"params": [t.to(dt) for t in w], "grads": g, "steps": steps}
+    if masters:
+        kw["masters"] = [t.clone() for t in w]
+    if bits == 32:
+        kw.update(exp_avgs=m, exp_avg_sqs=v)
+    else:
+        pairs = [(_to_blocks(a), _to_blocks(b.sqrt())) for a, b in zip(m, v)]
+        kw["scales"] = [torch.stack([a[1], b[1]]) for a, b in pairs]
+        kw["exp_avgs"], kw["exp_avg_sqs"] = ([p[k][0].view(s) for p, s in zip(pairs, shapes)] for k in (0, 1))
+    return kw
+
+
+def _to_blocks(t):
+    flat = torch.nn.functional.pad(t.flatten(), (0, -t.numel() % 256)).view(-1, 256)
+    scale = (flat.abs().amax(1) / 448).clamp(min=2.0 ** -120) if flat.numel() else flat.new_zeros(0)
+    return (flat / scale[:, None]).to(torch.float8_e4m3fn).flatten()[:t.numel()], scale
+
+
+def _spread(scale, n):
+    return scale.repeat_interleave(256)[:n]
+
+
+def _copy(kw):
+    return {k: [t.clone() for t in v] if isinstance(v, list) else v.clone() for k, v in kw.items()}
+
+
+def _values(kw, i):
+    """m and v of tensor i in 64 bits."""
+    m, v = kw["exp_avgs"][i].double().flatten(), kw["exp_avg_sqs"][i].double().flatten()
+    if "scales" in kw:
+        ms, rs = (_spread(s.double(), m.numel()) for s in kw["scales"][i])
+        return m * ms, (v * rs).square()
+    return m, v
+
+
+def _formula(kw, i, share=1.0, lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1):
+    m0, v0 = _values(kw, i)
+    g = kw["grads"][i].double().flatten() * share
+    w = kw["masters" if "masters" in kw else "params"][i].double().flatten()
+    t = int(kw["steps"][i]) + 1
+    m, v = betas[0] * m0 + (1 - betas[0]) * g, betas[1] * v0 + (1 - betas[1]) * g * g
+    step = lr / (1 - betas[0] ** t) * m / (v.sqrt() / math.sqrt(1 - betas[1] ** t) + eps)
+    size = m0.abs() * betas[0] + (1 - betas[0]) * g.abs()  # of m's terms, which may cancel
+    return w * (1 - lr * weight_decay) - step, m, v, size, w, lr / (1 - betas[0] ** t) / (v.sqrt() / math.sqrt(1 - betas[1] ** t) + eps)
+
+
+def _near(got, want, bound, what):
+    bad = ~((got.double().flatten() - want).abs() <= bound)
+    assert not bad.any(), (what, int(bad.sum()), float((got.double().flatten() - want).abs().max()))
+
+
+def _verify(before, after, share=1.0, hyper=HYPER):
+    for i, p in enumerate(after["params"]):
+        if before["grads"][i] is None:
+            for k in before:
+                if k not in ("grads", "steps"):
+                    assert torch.equal(before[k][i].view(torch.uint8), after[k][i].view(torch.uint8)), k
+            assert after["steps"][i] == before["steps"][i]
+            continue
+        assert after["steps"][i] == before["steps"][i] + 1
+        w, m, v, size, w0, rate = _formula(before, i, share, **hyper)
+        bound = 4 * E * w0.abs() + rate * 32 * E * size + 1e-45
+        if "masters" in after:
+            _near(after["masters"][i], w, bound, "master")
+            assert torch.equal(p, after["masters"][i].to(p.dtype))
+        else:
+            info = torch.finfo(p.dtype)
+            half = 0 if p.dtype == torch.float32 else info.eps / 2
+            _near(p, w, bound * 2 + half * w.abs() * (1 + E) + (info.tiny * info.eps if half else 0), "param")
+        if "scales" not in after:
+            _near(after["exp_avgs"][i], m, 8 * E * size + 1e-45, "m")
+            _near(after["exp_avg_sqs"][i], v, 14 * E * v + 1e-45, "v")
+            continue
+        n = m.numel()
+        for got, want, scale in ((after["exp_avgs"][i], m, after["scales"][i][0]),
+                                 (after["exp_avg_sqs"][i], v.sqrt(), after["scales"][i][1])):
+            flat = torch.nn.functional.pad(want, (0, -n % 256)).view(-1, 256)
+            top = flat.abs().amax(1) / 448 if n else flat.new_zeros(0)
+            # m's terms may cancel; over a block the largest term is within a few times the largest m here.
+            assert torch.allclose(scale.double(), top.clamp(min=2.0 ** -120), rtol=64 * E, atol=0)
+            s = _spread(scale.double(), n)
+            q = got.double().flatten()
+            x = (want / s).clamp(-448, 448) if n else want
+            step = torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -6))) - 3)
+            # up or down by less than a step (of the size above where x is just below a power of two)
+            assert ((q - x).abs() < step * (1 + 1e-3) + 1e-12).all()
+            assert (q.abs() <= 448).all()
+        r = after["exp_avg_sqs"][i].double().flatten()
+        assert (r[v > 0] > 0).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dt,masters,gdt", [(torch.bfloat16, True, None), (torch.bfloat16, False, None),
+                                            (torch.bfloat16, True, torch.float32), (torch.bfloat16, False, torch.float32),
+                                            (torch.float16, True, None), (torch.float16, False, None),
+                                            (torch.float16, True, torch.float32), (torch.float16, False, torch.float32),
+                                            (torch.float32, False, None)])
+def test_against_64_bits(dt, masters, gdt, bits):
+    log(f"adamw {dt} masters {masters} grads {gdt} bits {bits}")
+    kw = _lists(SHAPES, dt, bits, masters, gdt)
+    kw["grads"][4] = None
+    before = {k: list(v) if k == "grads" else _copy({k: v})[k] for k, v in kw.items()}
+    assert W.adamw_step(**kw, **HYPER) is None
+    _verify(before, kw)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_tensors_and_launches(bits):
+    """More tensors than a launch holds, some empty, some without a gradient."""
+    log(f"adamw 150 tensors, {bits} bits")
+    shapes = [((37 * i) % 700,) for i in range(150)]
+    kw = _lists(shapes, torch.float32, bits)
+    for i in range(0, 150, 11):
+        kw["grads"][i] = None
+    before = {k: list(v) if k == "grads" else _copy({k: v})[k] for k, v in kw.items()}
+    W.adamw_step(**kw, **HYPER)
+    _verify(before, kw)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dt", DTYPES, ids=ids)
+def test_off_alignment_and_neighbours(dt, bits):
+    """Tensors packed into one buffer at any offset: the same values as apart, and what lies between them stays."""
+    log(f"adamw packed {dt} {bits} bits")
+    apart = _lists(SHAPES, dt, bits, masters=dt != torch.float32)
+    packed, guards = {"steps": apart["steps"].clone()}, []
+    for k, ts in apart.items():
+        if k == "steps":
+            continue
+        flat = torch.zeros(sum(t.numel() + 3 for t in ts) + 1, device="cuda", dtype=torch.float32).to(ts[0].dtype)
+        at, views = 1, []
+        for t in ts:
+            views.append(flat[at:at + t.numel()].view(t.shape).copy_(t))
+            at += t.numel() + 3
+        packed[k] = views
+        gap = torch.ones_like(flat, dtype=torch.bool)
+        at = 1
+        for t in ts:
+            gap[at:at + t.numel()] = False
+            at += t.numel() + 3
+        guards.append((flat, gap))
+    W.adamw_step(**apart, **HYPER, seed=5)
+    W.adamw_step(**packed, **HYPER, seed=5)
+    for k in apart:
+        if k != "steps":
+            assert all(torch.equal(a.float(), b.float()) for a, b in zip(apart[k], packed[k])), k
+    for flat, gap in guards:
+        assert not flat.float()[gap].any()
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=ids)
+def test_grad_norm(dt):
+    """fp32 sums of 576 terms or fewer a lane, then fp64: 2^-24 times the longest chain, half of it through the root."""
+    log(f"grad_norm {dt}")
+    grads = [seeded(s, i, dtype=dt) for i, s in enumerate(SHAPES + [(65536,), (65537,), (3, 70001)])]
+    want = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    norm = W.grad_norm(grads)
+    assert norm.shape == () and norm.dtype == torch.float32 and abs(float(norm) - want) < 64 * E * want
+    assert torch.equal(norm, W.grad_norm(grads)) and torch.equal(norm, W.grad_norm([None, *grads]))
+    odd = torch.empty(70001 + 1, device="cuda", dtype=dt)[1:].copy_(grads[-1].flatten()[:70001])
+    assert abs(float(W.grad_norm([odd])) - float(odd.double().norm())) < 64 * E * float(odd.double().norm())
+    assert float(W.grad_norm([torch.empty(0, device="cuda", dtype=dt)])) == 0
+    assert torch.allclose(W.grad_norm([g.t().contiguous().t() if g.dim() == 2 else g for g in grads]), norm, rtol=64 * E)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_clipping(bits):
+    log(f"adamw clipping {bits} bits")
+    for max_norm in (0.05, 1e6, 0.0):
+        kw = _lists(SHAPES, torch.bfloat16, bits, masters=True)
+        before = _copy(kw)
+        norm = W.adamw_step(**kw, **HYPER, max_norm=max_norm)
+        total = math.sqrt(sum(float(g.double().square().sum()) for g in before["grads"]))
+        assert abs(float(norm) - total) < 64 * E * total
+        _verify(before, kw, min(1.0, max_norm / (float(norm) + 1e-6)))
+        again = _copy(before)  # the norm given
+        assert W.adamw_step(**again, **HYPER, max_norm=max_norm, norm=norm) is norm
+        for k in kw:
+            same = zip(kw[k], again[k]) if k != "steps" else [(kw[k], again[k])]
+            assert all(torch.equal(a.float(), b.float()) for a, b in same)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_norm_that_is_not_finite_changes_nothing(bad):
+    log(f"adamw norm {bad}")
+    for bits in (32, 8):
+        kw = _lists(SHAPES, torch.bfloat16, bits, masters=True)
+        kw["grads"][5][0] = bad
+        before = _copy(kw)
+        assert not torch.isfinite(W.adamw_step(**kw, **HYPER, max_norm=1.0))
+        for k in kw:
+            same = zip(kw[k], before[k]) if k != "steps" else [(kw[k], before[k])]
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in same), k
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_gradient_that_is_not_finite_stays_with_its_block(bad):
+    """Without a norm: its own element in 32 bits; in 8 bits its parameter, and the states of its 256 elements."""
+    log(f"adamw gradient {bad}")
+    for bits in (32, 8):
+        kw = _lists([(1000,), (300,)], torch.float32, bits)
+        clean = _copy(kw)
+        kw["grads"][0][300] = bad
+        W.adamw_step(**kw, **HYPER)
+        W.adamw_step(**clean, **HYPER)
+        keep = torch.ones(1000, dtype=torch.bool, device="cuda")
+        keep[300] = False
+        assert torch.equal(kw["params"][0][keep], clean["params"][0][keep])
+        assert torch.equal(kw["params"][1], clean["params"][1])
+        if bits == 8:
+            keep[256:512] = False
+            spread = torch.isnan(kw["exp_avgs"][0].float() * _spread(kw["scales"][0][0], 1000))
+            assert spread[256:512].all() and not spread[:256].any() and not spread[512:].any()
+        for k in ("exp_avgs", "exp_avg_sqs"):
+            assert torch.equal(kw[k][0].float()[keep], clean[k][0].float()[keep])
+
+
+def test_8bit_rounding_is_right_on_average():
+    """The mean of the stored m, and of the stored root's square, over many seeds: off by at most five standard errors
+    of a rounding up or down (half a step each), and the two states' roundings of an element are not tied."""
+    log("adamw 8-bit rounding on average")
+    n, seeds = 512, 400
+    g = seeded((n,), 1, std=1.0, dtype=torch.float32)
+    g[:20] *= 1e-4  # below the normal range of the codes
+    base = _lists([(n,)], torch.float32, 8)
+    base["grads"] = [g]
+    w, m, v, *_ = _formula(base, 0, **HYPER)
+    got_m, got_v = [], []
+    for seed in range(seeds):
+        kw = _copy(base)
+        W.adamw_step(**kw, **HYPER, seed=seed)
+        a, b = _values(kw, 0)
+        got_m.append(a)
+        got_v.append(b)
+    s = _spread(kw["scales"][0][0].double(), n)
+    step_m = torch.exp2(torch.floor(torch.log2((m / s).abs().clamp(2.0 ** -6, 447))) - 3) * s
+    a, b = torch.stack(got_m), torch.stack(got_v)
+    assert ((a.mean(0) - m).abs() <= 5 * step_m / 2 / math.sqrt(seeds) + 1e-9).all()
+    rs = _spread(kw["scales"][0][1].double(), n)
+    r = v.sqrt() / rs
+    step_r = torch.exp2(torch.floor(torch.log2(r.clamp(2.0 ** -6, 447))) - 3)
+    k = torch.floor(r / step_r)
+    gap = (2 * k + 1) * (step_r * rs) ** 2  # between the two squares
+    known = k >= 1  # a root below the least code is kept above zero: larger on purpose
+    err = (b.mean(0) - v).abs() / (gap / 2 / math.sqrt(seeds))
+    assert known.sum() > 480 and (err[known] <= 5 + 1e-3).all(), float(err[known].max())
+    up = torch.stack([((x > y).double() - (x > y).double().mean(0)).flatten() for x, y in ((a, m), (b, v))])
+    assert abs(float(torch.corrcoef(up)[0, 1])) < 0.02
+
+
+def test_8bit_average_of_squares_moves():
+    """v under gradients of another size: rounded to nearest it would stand still. After 2000 steps the mean over 4096
+    elements is at 1 - 0.999^2000 of its way; the random walk of an element (a third of v) averages to half a percent."""
+    log("adamw 8-bit v moves")
+    kw = _lists([(4096,)], torch.float32, 8)
+    kw["grads"] = [torch.full((4096,), 3e-2, device="cuda")]
+    v0 = _values(kw, 0)[1].mean()
+    for _ in range(2000):
+        W.adamw_step(**kw, lr=0.0)
+    share = 0.999 ** 2000
+    assert abs(float(_values(kw, 0)[1].mean()) / float(v0 * share + (1 - share) * 9e-4) - 1) < 0.05
+
+
+def test_stored_rounding_repeats_and_depends_on_the_seed():
+    log("adamw seeds")
+    runs = []
+    for seed in (3, 3, 4, 2 ** 32 + 3, -1):
+        kw = _lists([(5000,), (5000,)], torch.float32, 8, seed=0)
+        kw["steps"].fill_(5)
+        for k in ("params", "grads", "exp_avgs", "exp_avg_sqs", "scales"):
+            kw[k][1] = kw[k][0].clone()
+        W.adamw_step(**kw, **HYPER, seed=seed)
+        runs.append(kw["exp_avgs"])
+    same = lambda a, b: (a.float() == b.float()).float().mean().item()  # noqa: E731
+    assert same(runs[0][0], runs[1][0]) == 1 and same(runs[0][0], runs[3][0]) == 1
+    assert 0.3 < same(runs[0][0], runs[2][0]) < 0.9 and 0.3 < same(runs[0][0], runs[0][1]) < 0.9
+
+
+def test_rate_on_the_device_and_captured_steps():
+    """A captured step counts on, follows a rate that is changed between replays, and equals eager steps."""
+    log("adamw captured")
+    for bits in (32, 8):
+        kw = _lists(SHAPES, torch.bfloat16, bits, masters=True)
+        eager = _copy(kw)
+        lr = torch.tensor(1e-2, device="cuda")
+        call = lambda k, rate: W.adamw_step(**k, lr=rate, max_norm=0.5, seed=9)  # noqa: E731
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(kw, lr)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norm = call(kw, lr)
+        call(eager, 1e-2)
+        for i in range(5):
+            lr.fill_(1e-2 / (i + 1))
+            kw["grads"][8].mul_(0.5)
+            eager["grads"][8].mul_(0.5)
+            graph.replay()
+            other = call(eager, float(lr))
+            torch.cuda.synchronize()
+            assert torch.equal(norm, other)
+            for k in kw:
+                same = zip(kw[k], eager[k]) if k != "steps" else [(kw[k], eager[k])]
+                assert all(torch.equal(a.float(), b.float()) for a, b in same), (i, k)
+        del graph
+
+
+def test_another_stream():
+    log("adamw on a side stream")
+    kw = _lists(SHAPES, torch.float32, 32)
+    want = _copy(kw)
+    W.adamw_step(**want, **HYPER, max_norm=0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        W.adamw_step(**kw, **HYPER, max_norm=0.1)
+    side.synchronize()
+    assert all(torch.equal(a, b) for k in ("params", "exp_avgs", "exp_avg_sqs") for a, b in zip(kw[k], want[k]))
+
+
+def test_native_matches_python_path():
+    log("adamw native against Python path")
+    n = _hip.native()
+    assert n is not _hip._NoNative
+    for bits, dt, masters in ((32, torch.bfloat16, True), (8, torch.float16, False), (32, torch.float32, False)):
+        for max_norm in (None, 0.1):
+            a = _lists(SHAPES, dt, bits, masters)
+            a["grads"][2] = None
+            b = {k: list(v) if k == "grads" else _copy({k: v})[k] for k, v in a.items()}
+            order = lambda k: (k["params"], k["grads"], k["exp_avgs"], k["exp_avg_sqs"], k["steps"], 1e-2, 0.9, 0.999, 1e-8,  # noqa: E731
+                               0.1, k.get("masters"), k.get("scales"), max_norm, None, 3)
+            got, want = n.adamw_step(*order(a)), _hip.adamw_step(*order(b))
+            assert isinstance(got, tuple) and (got[0] is None) == (want is None)
+            assert want is None or torch.equal(got[0], want)
+            for k in ("params", "exp_avgs", "exp_avg_sqs", "masters", "scales"):
+                assert all(torch.equal(x.float(), y.float()) for x, y in zip(a.get(k, []), b.get(k, [])))
+            assert torch.equal(a["steps"], b["steps"])
+    kw = _lists([(8, 8)], torch.float32, 32)
+    args = [kw["params"], kw["grads"], kw["exp_avgs"], kw["exp_avg_sqs"], kw["steps"], 1e-2, 0.9, 0.999, 1e-8, 0.1, None,
+            None, None, None, 0]
+    t = kw["grads"][0]
+    for i, bad in [(0, [t.cpu()]), (0, []), (1, [t[:4]]), (1, [t.t()]), (1, [t.double()]), (1, []), (2, [t.half()]), (3, [t[:7]]),
+                   (4, kw["steps"].long()), (5, 1), (5, kw["steps"]), (6, 0), (10, [t]), (11, [t]), (13, t), (14, -1),
+                   (0, tuple(kw["params"]))]:
+        if i == 10:
+            continue  # masters of fp32 parameters: the C entry refuses them, and the Python path says why
+        assert n.adamw_step(*[bad if k == i else v for k, v in enumerate(args)]) is None, i
+    assert int(kw["steps"][0]) == 0
+    assert n.grad_norm([]) is None and n.grad_norm([None]) is None and n.grad_norm([t, t.half()]) is None
+    assert n.grad_norm([t.cpu()]) is None and n.grad_norm((t,)) is None
+
+
+def test_refusals():
+    log("adamw refusals")
+
+    def call(err, match=None, hyper=HYPER, **change):
+        kw = _lists([(8, 4), (300,)], torch.bfloat16, 8, masters=True)
+        kw.update(change)
+        with pytest.raises(err, match=match):
+            W.adamw_step(**kw, **hyper)
+        assert "steps" in change or not (kw["steps"] - _lists([(8, 4), (300,)], torch.bfloat16)["steps"]).any()
+
+    kw = _lists([(8, 4), (300,)], torch.bfloat16, 8, masters=True)
+    p, s = kw["params"], kw["scales"]
+    call(ValueError, "twice", params=[p[0], p[0]], grads=[kw["grads"][0]] * 2, exp_avgs=[kw["exp_avgs"][0]] * 2,
+         exp_avg_sqs=[kw["exp_avg_sqs"][0]] * 2, masters=[kw["masters"][0]] * 2, scales=[s[0]] * 2)
+    call(ValueError, "contiguous", params=[p[0].t().contiguous().t(), p[1]])
+    call(TypeError, "exp_avg 0", exp_avgs=[t.float() for t in kw["exp_avgs"]])
+    call(ValueError, "scales 1", scales=[s[0], s[1][:, :1].contiguous()])
+    call(ValueError, "scales 1", scales=[s[0], s[1].t().contiguous().t()])
+    call(ValueError, "grads", grads=kw["grads"][:1])
+    call(ValueError, "gradient 0", grads=[kw["grads"][0][:4], kw["grads"][1]])
+    call(TypeError, "one dtype", grads=[kw["grads"][0], kw["grads"][1].float()])
+    call(TypeError, "gradients", grads=[g.half() for g in kw["grads"]])
+    call(TypeError, "master 0", masters=p)
+    call(ValueError, "steps", steps=kw["steps"].long())
+    call(ValueError, "steps", steps=kw["steps"][:1])
+    call(ValueError, "GPU", grads=[g.cpu() for g in kw["grads"]])
+    call(ValueError, "lr", hyper={**HYPER, "lr": torch.tensor([1.0, 2.0], device="cuda")})
+    call(ValueError, "lr", hyper={**HYPER, "lr": torch.tensor(1.0, device="cuda", dtype=torch.float64)})
+    call(ValueError, "norm without", hyper={**HYPER, "norm": torch.tensor(1.0, device="cuda")})
+    with pytest.raises(TypeError, match="16-bit"):
+        f = _lists([(8,)], torch.float32)
+        W.adamw_step(**f, **HYPER, masters=[f["params"][0].clone()])
+
+
+def test_saved_tensors_count_as_changed():
+    log("adamw versions")
+    p = torch.ones(4, device="cuda", requires_grad=True)
+    out = (p * p).sum()
+    kw = {"exp_avgs": [torch.zeros(4, device="cuda")], "exp_avg_sqs": [torch.zeros(4, device="cuda")]}
+    for call in (W.adamw_step, lambda *a, **k: W.adamw_step(tuple(a[0]), *a[1:], **k)):  # native, Python path
+        call([p], [torch.ones(4, device="cuda")], **kw, steps=torch.zeros(1, device="cuda", dtype=torch.int32), lr=0.1)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            out.backward()
+        out = (p * p).sum()
+    out.backward()
+
+
+# ----------------------------------------------------------------- the class
+def _model(dt=torch.bfloat16, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter((0.1 * torch.randn(s, generator=g)).to(dt).cuda()) for s in ((64, 48), (48,), (7, 3))]
+
+
+def _set_grads(params, seed):
+    for i, p in enumerate(params):
+        p.grad = seeded(tuple(p.shape), seed + i, std=0.1, dtype=p.dtype)
+
+
+def test_class_against_torch():
+    """32-bit states of fp32 parameters: torch's own AdamW, which forms the same in fp32 in another order (ten steps, each
+    off by a few units of the change)."""
+    log("AdamW against torch.optim.AdamW")
+    a, b = _model(torch.float32), _model(torch.float32)
+    own = W.AdamW([{"params": a[:2]}, {"params": a[2:], "lr": 1e-2, "weight_decay": 0.0}], lr=1e-3)
+    ref = torch.optim.AdamW([{"params": b[:2]}, {"params": b[2:], "lr": 1e-2, "weight_decay": 0.0}], lr=1e-3, foreach=False)
+    for step in range(10):
+        for ps in (a, b):
+            _set_grads(ps, 10 * step)
+            if step < 4:
+                ps[1].grad = None  # joins later: its own count
+        own.step()
+        ref.step()
+    for p, q in zip(a, b):
+        assert (p - q).abs().max() <= 10 * 40 * E * 1e-2 + 20 * E * q.abs().max()
+    assert [int(own.state[p]["step"]) for p in a] == [10, 6, 10]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_class_states_through_a_checkpoint(bits):
+    log(f"AdamW state_dict {bits} bits")
+    a = _model()
+    opt = W.AdamW(a, lr=1e-2, state_bits=bits, max_norm=1.0, seed=3)
+    for step in range(3):
+        _set_grads(a, step)
+        opt.step()
+    saved = torch.utils._pytree.tree_map(lambda t: t.cpu() if isinstance(t, torch.Tensor) else t, opt.state_dict())
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    other = W.AdamW(b, lr=1e-2, state_bits=bits, max_norm=1.0, seed=3)
+    other.load_state_dict(saved)
+    for p, q in zip(a, b):
+        for k, t in opt.state[p].items():
+            assert other.state[q][k].dtype == t.dtype and torch.equal(other.state[q][k].float(), t.float())
+    for step in range(3, 5):
+        _set_grads(a, step)
+        _set_grads(b, step)
+        opt.step()
+        other.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    with pytest.raises(ValueError, match="bits"):
+        W.AdamW(_model(), state_bits=40 - bits).load_state_dict(saved)
+    import copy
+    import io
+
+    file = io.BytesIO()
+    torch.save(opt, file)  # plain pickle does not load a float8 tensor of this torch
+    file.seek(0)
+    for clone in (copy.deepcopy(opt), torch.load(file, weights_only=False)):
+        assert clone.state_bits == bits and clone.max_norm == 1.0
+        ps = clone.param_groups[0]["params"]
+        _set_grads(ps, 77)
+        clone.step()
+        _set_grads(b, 77)
+    other.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, b))
+
+
+def test_class_captured_after_its_first_step(monkeypatch):
+    log("AdamW captured")
+    a, b = _model(), _model()
+    opts = [W.AdamW(ps, lr=1e-2, state_bits=8, max_norm=1.0) for ps in (a, b)]
+    _set_grads(a, 1)
+    _set_grads(b, 1)
+    with monkeypatch.context() as m:  # as within a capture, which is not begun: a failed one would outlast the test
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="first step"):
+            opts[0].step()
+    for o in opts:
+        o.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[0].step()
+    for i in range(4):
+        for p, q in zip(a, b):
+            p.grad.copy_(seeded(tuple(p.shape), 50 + i, std=0.1))
+            q.grad.copy_(p.grad)
+        graph.replay()
+        opts[1].step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), i
+    assert int(opts[0].state[a[0]]["step"]) == 5
+
+
+def test_class_mixed_types_scheduler_and_closure():
+    log("AdamW mixed types")
+    ps = _model(torch.bfloat16) + _model(torch.float32, 1) + [torch.nn.Parameter(torch.zeros(0, device="cuda"))]
+    opt = W.AdamW(ps, lr=1e-2, max_norm=0.5)
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda e: 0.5 ** e)
+
+    def closure():
+        opt.zero_grad()
+        _set_grads(ps, 5)
+        return torch.tensor(3.0)
+
+    before = [p.detach().clone() for p in ps]
+    assert opt.step(closure) == 3.0
+    sched.step()
+    opt.step(closure)
+    assert all(not torch.equal(p, q) for p, q in zip(ps[:-1], before))
+    assert "master" in opt.state[ps[0]] and "master" not in opt.state[ps[3]]
+    with pytest.raises(ValueError, match="state_bits"):
+        W.AdamW(ps, state_bits=16)
+    with pytest.raises(ValueError, match="betas"):
+        W.AdamW(ps, betas=(1.0, 0.9))
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(5, device="cuda"))], "lr": 0.1})
+    opt.param_groups[1]["params"][0].grad = torch.ones(5, device="cuda")
+    opt.step()
+    assert int(opt.state[opt.param_groups[1]["params"][0]]["step"]) == 1 and int(opt.state[ps[0]]["step"]) == 3
