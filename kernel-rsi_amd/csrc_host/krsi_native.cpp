@@ -753,6 +753,57 @@ PyObject* py_add_rmsnorm_8bit(Args a, Py_ssize_t n) {
   });
 }
 
+// Codes and scales of the rows of x.
+variable_list rows_in_8bit(const Tensor& x) {
+  Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)),
+         scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  forward_status(krsi_quantize_rows(x.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), x.size(0), (int)x.size(1),
+                                    dtype_code(x), stream_of(x)));
+  return {q, scale};
+}
+
+PyObject* py_quantize_rows(Args a, Py_ssize_t n) {
+  const Tensor* x;
+  if (n != 1 || !plain_context() || !tensor_arg(a[0], &x) || x->dim() != 2 || !x->is_contiguous() || x->numel() == 0 ||
+      dtype_code(*x) < 0 || x->size(1) > kIntMax)
+    Py_RETURN_NONE;
+  return unlocked_tuple([&] {
+    at::NoGradGuard no_grad;
+    const c10::DeviceGuard guard(x->device());
+    return rows_in_8bit(*x);
+  });
+}
+
+// x in 8 bits with its rows' scales, or (no scales) of another type, brought to 8 bits here.
+PyObject* py_linear_8bit(Args a, Py_ssize_t n) {
+  const Tensor *x, *w, *w_scale, *x_scale = nullptr;
+  int64_t out_dtype;
+  if (n != 5 || !plain_context() || !tensor_arg(a[0], &x) || !tensor_arg(a[1], &w) || !tensor_arg(a[2], &w_scale) ||
+      (a[3] != Py_None && !tensor_arg(a[3], &x_scale)) || !int_arg(a[4], 0, 2, &out_dtype))
+    Py_RETURN_NONE;
+  if (x->dim() != 2 || w->dim() != 2 || w->scalar_type() != at::kFloat8_e4m3fn || w->size(1) != x->size(1) ||
+      x->numel() == 0 || w->numel() == 0 || x->size(1) % 16 || x->size(1) > kIntMax || w->size(0) > kIntMax ||
+      !x->is_contiguous() || !w->is_contiguous() || !aligned16(*w) || w->device() != x->device() ||
+      (x_scale ? x->scalar_type() != at::kFloat8_e4m3fn || !aligned16(*x) : dtype_code(*x) < 0))
+    Py_RETURN_NONE;
+  auto scales = [&](const Tensor* s, int64_t rows) {
+    return s->scalar_type() == at::kFloat && s->dim() == 1 && s->size(0) == rows && s->is_contiguous() &&
+           s->device() == x->device();
+  };
+  if (!scales(w_scale, w->size(0)) || (x_scale && !scales(x_scale, x->size(0)))) Py_RETURN_NONE;
+  return unlocked([&] {
+    at::NoGradGuard no_grad;
+    const c10::DeviceGuard guard(x->device());
+    variable_list rows = x_scale ? variable_list{*x, *x_scale} : rows_in_8bit(*x);
+    const at::ScalarType types[] = {at::kBFloat16, at::kHalf, at::kFloat};
+    Tensor out = at::empty({x->size(0), w->size(0)}, x->options().dtype(types[out_dtype]));
+    forward_status(krsi_linear_8bit(rows[0].data_ptr(), w->data_ptr(), rows[1].data_ptr<float>(),
+                                    w_scale->data_ptr<float>(), out.data_ptr(), x->size(0), (int)x->size(1),
+                                    (int)w->size(0), (int)out_dtype, stream_of(*x)));
+    return out;
+  });
+}
+
 // A list of tensors (or None, where `holes` has none of them) that are plain, contiguous and on one device.
 bool list_arg(PyObject* o, bool holes, std::vector<const Tensor*>* out) {
   if (!PyList_CheckExact(o)) return false;
@@ -902,6 +953,8 @@ PyMethodDef kMethods[] = {
     {"linear_cross_entropy", (PyCFunction)(void*)entry<py_linear_cross_entropy>, METH_FASTCALL, nullptr},
     {"add_rmsnorm", (PyCFunction)(void*)entry<py_add_rmsnorm>, METH_FASTCALL, nullptr},
     {"add_rmsnorm_8bit", (PyCFunction)(void*)entry<py_add_rmsnorm_8bit>, METH_FASTCALL, nullptr},
+    {"quantize_rows", (PyCFunction)(void*)entry<py_quantize_rows>, METH_FASTCALL, nullptr},
+    {"linear_8bit", (PyCFunction)(void*)entry<py_linear_8bit>, METH_FASTCALL, nullptr},
     {"grad_norm", (PyCFunction)(void*)entry<py_grad_norm>, METH_FASTCALL, nullptr},
     {"adamw_step", (PyCFunction)(void*)entry<py_adamw_step>, METH_FASTCALL, nullptr},
     {"set_module", py_set_module, METH_O, nullptr},

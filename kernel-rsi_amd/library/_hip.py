@@ -86,6 +86,7 @@ SIGNATURES = {
     "krsi_add_rmsnorm_8bit": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _F32, _I32, _P]),
     "krsi_quantize_rows": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _P]),
     "krsi_add_rmsnorm_bwd_workspace_bytes": (_SZ, [_I64, _I32]),
+    "krsi_linear_8bit": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P]),
     "krsi_grad_norm_workspace_bytes": (_SZ, [_P, _I32]),
     "krsi_grad_norm": (ctypes.c_int, [_P, _P, _I32, _P, _P, _SZ, _I32, _P]),
     "krsi_adamw_workspace_bytes": (_SZ, [_I32]),
@@ -135,7 +136,7 @@ class _NoNative:
 
     rmsnorm = geglu = geglu_linear = relpos_attention = bucket_table = _none
     qk_norm_rope = embedding = linear_cross_entropy = _none
-    add_rmsnorm = add_rmsnorm_8bit = grad_norm = adamw_step = _none
+    add_rmsnorm = add_rmsnorm_8bit = quantize_rows = linear_8bit = grad_norm = adamw_step = _none
 
 
 _native = None
@@ -783,6 +784,33 @@ def quantize_rows(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if rows:
         _check(lib().krsi_quantize_rows(_ptr(x2d), _ptr(q), _ptr(scale), rows, n, dt, _stream(x2d)))
     return q, scale
+
+
+# ------------------------------------------------------ projection in 8 bits
+@_on_device
+def linear_8bit(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale: torch.Tensor,
+                out_dtype: torch.dtype) -> torch.Tensor:
+    """[rows, F] of out_dtype: the product of the codes x [rows, K] and w [F, K], times their rows' scales."""
+    _on_gpu(x, w, w_scale, x_scale)
+    if out_dtype not in DTYPE_CODES:
+        raise TypeError(f"out_dtype must be one of {', '.join(map(str, DTYPE_CODES))}, got {out_dtype}")
+    for name, t in (("x", x), ("weight", w)):
+        if t.dtype != E4M3:
+            raise TypeError(f"{name} must be {E4M3}, got {t.dtype}")
+    if x.dim() != 2 or w.dim() != 2 or w.shape[1] != x.shape[1] or w.shape[0] < 1:
+        raise ValueError(f"need x [rows, K] and w [F, K], got {tuple(x.shape)} and {tuple(w.shape)}")
+    (rows, k), f = x.shape, w.shape[0]
+    if k % 16 or not k:
+        raise ValueError(f"linear_8bit needs K a multiple of 16, got K={k}")
+    for name, t, n in (("x_scale", x_scale, rows), ("w_scale", w_scale, f)):
+        if t.dtype != torch.float32 or t.shape != (n,):
+            raise ValueError(f"{name} must be float32 [{n}], got {t.dtype} {tuple(t.shape)}")
+    x, w, x_scale, w_scale = _aligned(x), _aligned(w), x_scale.contiguous(), w_scale.contiguous()
+    out = torch.empty(rows, f, device=x.device, dtype=out_dtype)
+    if rows:
+        _check(lib().krsi_linear_8bit(_ptr(x), _ptr(w), _ptr(x_scale), _ptr(w_scale), _ptr(out), rows, k, f,
+                                      DTYPE_CODES[out_dtype], _stream(x)))
+    return out
 
 
 # --------------------------------------------------- AdamW over many tensors

@@ -379,3 +379,15 @@ def quantize_rows_op(x2d: Tensor) -> tuple[Tensor, Tensor]:
 @quantize_rows_op.register_fake
 def _(x2d):
     return x2d.new_empty(x2d.shape, dtype=_hip.E4M3), x2d.new_empty((x2d.shape[0],), dtype=torch.float32)
+
+# ------------------------------------------------------ projection in 8 bits
+
+
+@torch.library.custom_op("krsi::linear_8bit", mutates_args=())
+def linear_8bit_op(x: Tensor, w: Tensor, w_scale: Tensor, x_scale: Tensor, out_dtype: torch.dtype) -> Tensor:
+    return _hip.linear_8bit(x, w, w_scale, x_scale, out_dtype)
+
+
+@linear_8bit_op.register_fake
+def _(x, w, w_scale, x_scale, out_dtype):
+    return x.new_empty((x.shape[0], w.shape[0]), dtype=out_dtype)

@@ -1,0 +1,187 @@
+"""linear_8bit on the GPU against the formula in 64 bits.
+
+Tolerance. The matrix instruction takes 32 bytes of a row from a lane and adds the products of each eight consecutive ones
+first, aligned to the largest and cut below 2^-13 of its power of two (measured with single products: next to 2^16 in the
+same eight, 2^3 stays and 2^2 is lost; in another eight 2^-7 stays, as in fp32). So each of seven products loses less
+than 2^-13 of the group's largest, and an output less than 7 * 2^-13 * (sum over the groups of max|x| max|w|). Sums across groups
+are fp32's: k / 8 + 64 additions at most, each by 2^-24 of the sum of magnitudes; then two products by the scales and a
+rounding to the output type, u = half its step.
+"""
+import pytest
+import torch
+
+import _hip
+import linear_8bit as L
+from krsi_testutil import log, seeded
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+ids = lambda d: str(d).split(".")[-1]  # noqa: E731
+
+
+def _inputs(rows, k, f, seed=0):
+    x, xs = _hip.quantize_rows(seeded((rows, k), seed, dtype=torch.float32))
+    w, ws = _hip.quantize_rows(seeded((f, k), seed + 1, std=k ** -0.5, dtype=torch.float32))
+    return x, w, ws, xs
+
+
+def _verify(out, x, w, ws, xs):
+    a, b = x.double(), w.double()
+    want = (a @ b.t()) * xs.double()[:, None] * ws.double()
+    size = (a.abs() @ b.abs().t()) * xs.double()[:, None] * ws.double()
+    top = lambda t: torch.nn.functional.pad(t.abs(), (0, -t.shape[1] % 8)).unflatten(1, (-1, 8)).amax(2)  # noqa: E731
+    cut = 7 * 2.0 ** -13 * (top(a) @ top(b).t()) * xs.double()[:, None] * ws.double()
+    u = 0 if out.dtype == torch.float32 else torch.finfo(out.dtype).eps / 2
+    tiny = torch.finfo(out.dtype).tiny * torch.finfo(out.dtype).eps
+    bound = (cut + (x.shape[1] / 8 + 64) * E * size) * (1 + u) + (u + 4 * E) * want.abs() + tiny
+    err = (out.double() - want).abs()
+    assert out.shape == want.shape and (err <= bound).all(), float((err / bound).max())
+
+
+# Each kernel's sizes: few rows (1 to 16, 17 to 32, to 64), tiles of 64, 128 and 256 rows and columns with ends inside them;
+# summed lengths of one stage, of part of one, of many; outputs of one column, of odd widths.
+SHAPES = [(1, 16, 1), (1, 128, 16), (3, 144, 17), (16, 1040, 33), (1, 4096, 8192), (17, 256, 48), (32, 2064, 100),
+          (33, 1024, 31), (64, 4112, 321), (65, 16, 1), (65, 128, 128), (70, 112, 130), (100, 272, 200), (129, 1024, 257),
+          (200, 128, 3000), (300, 400, 700), (1000, 1024, 5632), (513, 2048, 2049), (2100, 528, 4100), (4096, 96, 4352),
+          (4097, 1040, 4097), (2048, 4096, 8192)]
+
+
+@pytest.mark.parametrize("rows,k,f", SHAPES)
+def test_against_64_bits(rows, k, f):
+    log(f"linear_8bit [{rows}, {k}] x [{f}, {k}]")
+    x, w, ws, xs = _inputs(rows, k, f)
+    for dt in DTYPES:
+        out = L.linear_8bit(x, w, ws, x_scale=xs, out_dtype=dt)
+        assert out.dtype == dt
+        _verify(out, x, w, ws, xs)
+        assert torch.equal(out, L.linear_8bit(x, w, ws, x_scale=xs, out_dtype=dt))
+
+
+@pytest.mark.parametrize("rows,k,f", [(5, 256, 40), (40, 208, 70), (70, 400, 90), (300, 144, 520)])
+def test_each_summed_index_counts_once(rows, k, f):
+    """Rows with a single one meet a weight of distinct values: every output is exactly its weight."""
+    log(f"linear_8bit single ones [{rows}, {k}] x [{f}, {k}]")
+    codes = torch.arange(1, 127, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    g = torch.Generator().manual_seed(1)
+    w = codes.view(torch.uint8)[torch.randint(0, 126, (f, k), generator=g).cuda()].view(torch.float8_e4m3fn)
+    at = torch.randint(0, k, (rows,), generator=g).cuda()
+    at[-1] = k - 1
+    x = torch.zeros(rows, k, device="cuda")
+    x[torch.arange(rows, device="cuda"), at] = 1
+    ones = torch.ones(max(rows, f), device="cuda")
+    out = L.linear_8bit(x.to(torch.float8_e4m3fn), w, ones[:f], x_scale=ones[:rows], out_dtype=torch.float32)
+    assert torch.equal(out, w.float()[:, at].t())
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows", [3, 50, 200])
+def test_rows_that_come_in_other_types(rows, dt):
+    log(f"linear_8bit of {dt} rows={rows}")
+    x = seeded((rows, 528), 1, dtype=dt)
+    _, w, ws, _ = _inputs(1, 528, 200)
+    out = L.linear_8bit(x, w, ws)
+    assert out.dtype == dt
+    q, s = L.quantize_rows(x)
+    assert torch.equal(out, L.linear_8bit(q, w, ws, x_scale=s, out_dtype=dt))
+    assert L.linear_8bit(q, w, ws, x_scale=s).dtype == torch.bfloat16
+    assert torch.equal(L.linear_8bit(x.t().contiguous().t(), w, ws), out)
+
+
+@pytest.mark.parametrize("rows", [4, 60, 150, 600])
+def test_nan_and_infinite_rows_stay_their_own(rows):
+    log(f"linear_8bit NaN rows={rows}")
+    x, w, ws, xs = _inputs(rows, 272, 300)
+    clean = L.linear_8bit(x, w, ws, x_scale=xs)
+    bits = x.view(torch.uint8).clone()
+    bits[1, 270] = 0x7f
+    wbits = w.view(torch.uint8).clone()
+    wbits[299, 0] = 0xff
+    xs, ws = xs.clone(), ws.clone()
+    xs[rows - 1], ws[0] = float("nan"), float("inf")
+    out = L.linear_8bit(bits.view(x.dtype), wbits.view(w.dtype), ws, x_scale=xs)
+    nan = torch.zeros_like(out, dtype=torch.bool)
+    nan[1], nan[rows - 1], nan[:, 299] = True, True, True
+    assert torch.isnan(out[nan]).all() and not torch.isfinite(out[:, 0]).any()
+    nan[:, 0] = True
+    assert torch.equal(out[~nan], clean[~nan])
+
+
+def test_layouts_and_neighbours():
+    """Operands off alignment or strided go through a copy; nothing outside the output is written."""
+    log("linear_8bit layouts")
+    for rows, f in ((7, 33), (130, 257)):
+        x, w, ws, xs = _inputs(rows, 144, f)
+        want = L.linear_8bit(x, w, ws, x_scale=xs)
+        off = [torch.zeros(t.numel() + 16, device="cuda", dtype=torch.uint8)[3:3 + t.numel()].view(t.shape) for t in (x, w)]
+        for o, t in zip(off, (x, w)):
+            o.copy_(t.view(torch.uint8))
+        got = L.linear_8bit(off[0].view(x.dtype), off[1].view(x.dtype), ws, x_scale=xs)
+        assert torch.equal(got, want)
+        wide = torch.stack([ws, ws], 1)[:, 0]
+        assert torch.equal(L.linear_8bit(x, w, wide, x_scale=xs), want)
+        guard = torch.full((rows * f + 64,), 7.0, device="cuda", dtype=torch.bfloat16)
+        _hip._check(_hip.lib().krsi_linear_8bit(x.data_ptr(), w.data_ptr(), xs.data_ptr(), ws.data_ptr(),
+                                                guard[1:].data_ptr(), rows, 144, f, 0,
+                                                torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        assert torch.equal(guard[1:1 + rows * f].view(rows, f), want)
+        assert guard[0] == 7 and (guard[1 + rows * f:] == 7).all()
+
+
+def test_empty_batch():
+    x, w, ws, _ = _inputs(4, 64, 32)
+    assert L.linear_8bit(x[:0], w, ws, x_scale=ws[:0]).shape == (0, 32)
+    assert L.linear_8bit(torch.empty(0, 64, device="cuda"), w, ws).shape == (0, 32)
+    q, s = L.quantize_rows(torch.empty(0, 64, device="cuda"))
+    assert q.shape == (0, 64) and s.shape == (0,)
+
+
+def test_captured_and_on_another_stream():
+    log("linear_8bit captured")
+    _, w, ws, _ = _inputs(1, 256, 300)
+    for rows in (3, 100):
+        x = seeded((rows, 256), 1)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            first = L.linear_8bit(x, w, ws)
+        side.synchronize()
+        assert torch.equal(first, L.linear_8bit(x, w, ws))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = L.linear_8bit(x, w, ws)
+        for i in range(3):
+            x.copy_(seeded((rows, 256), 10 + i))
+            graph.replay()
+            want = L.linear_8bit(x, w, ws)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+
+
+def test_compiled():
+    log("linear_8bit compiled")
+    _, w, ws, _ = _inputs(1, 256, 96)
+    x = seeded((10, 256), 1)
+    with torch.no_grad():
+        assert torch.equal(torch.compile(L.linear_8bit, fullgraph=True)(x, w, ws), L.linear_8bit(x, w, ws))
+
+
+def test_refusals():
+    x, w, ws, xs = _inputs(4, 64, 32)
+    for args, kw, err in [((x, w, ws), {}, ValueError), ((x.float(), w, ws), {"x_scale": xs}, ValueError),
+                          ((x, w.float(), ws), {"x_scale": xs}, TypeError), ((x, w[:, :48], ws), {"x_scale": xs}, ValueError),
+                          ((x[:, :40], w[:, :40], ws), {"x_scale": xs}, ValueError), ((x, w, ws[:5]), {"x_scale": xs}, ValueError),
+                          ((x, w, ws.double()), {"x_scale": xs}, ValueError), ((x, w, ws), {"x_scale": xs[:3]}, ValueError),
+                          ((x, w, ws), {"x_scale": xs, "out_dtype": torch.float64}, TypeError),
+                          ((x.float().double(), w, ws), {}, TypeError), ((x[0], w, ws), {"x_scale": xs}, ValueError),
+                          ((x.cpu(), w, ws), {"x_scale": xs}, ValueError)]:
+        with pytest.raises(err):
+            L.linear_8bit(*args, **kw)
+    y = seeded((4, 64), 1).requires_grad_(True)
+    with pytest.raises(ValueError, match="no gradient"):
+        L.linear_8bit(y, w, ws)
+    with pytest.raises(ValueError, match="no gradient"):
+        L.quantize_rows(y)
+    with torch.no_grad():
+        L.linear_8bit(y, w, ws)
