@@ -76,46 +76,43 @@ __device__ __forceinline__ int find(const Items& t, int b) {
   return lo;
 }
 
-// Eight consecutive elements of any alignment.
-template <int DT>
-__device__ __forceinline__ void load8(const void* p, int64_t i, float* f) {
+// Pointers that come in a structure are taken for generic ones; these accesses are of global memory.
+template <typename T>
+using Global = __attribute__((address_space(1))) T;
+template <typename T>
+__device__ __forceinline__ Global<T>* global(const void* p) {
+  return (Global<T>*)(uintptr_t)p;
+}
+
+// N consecutive elements of any alignment (N a multiple of a chunk's), or the first `some` of them.
+template <int DT, int N, bool FULL>
+__device__ __forceinline__ void load(const void* p, int64_t i, int some, float* f) {
   using El = Elem<DT>;
+  const auto* at = global<const typename El::T>(p) + i;
+  if constexpr (FULL) {
 #pragma unroll
-  for (int q = 0; q < 8 / El::E; ++q)
-    El::unpack(load_chunk<true>((const typename El::T*)p + i + q * El::E), f + q * El::E);
+    for (int q = 0; q < N; q += El::E) {
+      const u32x4 c = *(Global<const u32x4_any>*)(at + q);
+      El::unpack(c, f + q);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = j < some ? El::load(at[j]) : 0.f;
+  }
 }
-template <int DT>
-__device__ __forceinline__ void store8(void* p, int64_t i, const float* f) {
+// Non-temporal: nothing of a step is read again soon.
+template <int DT, int N, bool FULL>
+__device__ __forceinline__ void store(void* p, int64_t i, int some, const float* f) {
   using El = Elem<DT>;
+  auto* at = global<typename El::T>(p) + i;
+  if constexpr (FULL) {
 #pragma unroll
-  for (int q = 0; q < 8 / El::E; ++q)
-    __builtin_nontemporal_store(El::pack(f + q * El::E), reinterpret_cast<u32x4_any*>((typename El::T*)p + i + q * El::E));
-}
-// The first `some` of them.
-template <int DT>
-__device__ __forceinline__ void load_some(const void* p, int64_t i, int some, float* f) {
+    for (int q = 0; q < N; q += El::E) __builtin_nontemporal_store(El::pack(f + q), (Global<u32x4_any>*)(at + q));
+  } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = j < some ? Elem<DT>::load(((const typename Elem<DT>::T*)p)[i + j]) : 0.f;
-}
-template <int DT>
-__device__ __forceinline__ void store_some(void* p, int64_t i, int some, const float* f) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < some) ((typename Elem<DT>::T*)p)[i + j] = Elem<DT>::store(f[j]);
-}
-template <int DT>
-__device__ __forceinline__ void load_part(const void* p, int64_t i, int some, float* f) {
-  if (some == 8)
-    load8<DT>(p, i, f);
-  else
-    load_some<DT>(p, i, some, f);
-}
-template <int DT>
-__device__ __forceinline__ void store_part(void* p, int64_t i, int some, const float* f) {
-  if (some == 8)
-    store8<DT>(p, i, f);
-  else
-    store_some<DT>(p, i, some, f);
+    for (int j = 0; j < N; ++j)
+      if (j < some) at[j] = El::store(f[j]);
+  }
 }
 
 // ------------------------------------------------------------------- norm
@@ -131,12 +128,12 @@ __global__ __launch_bounds__(kThreads) void norm_parts(const Items items, float*
 #pragma unroll 4
   for (int64_t i = at + 8 * threadIdx.x; i < whole; i += 8 * kThreads) {
     float f[8];
-    load8<DT>(t.grad, i, f);
+    load<DT, 8, true>(t.grad, i, 8, f);
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[j] += f[j] * f[j];
   }
   if (threadIdx.x < end - whole) {
-    const float f = Elem<DT>::load(((const typename Elem<DT>::T*)t.grad)[whole + threadIdx.x]);
+    const float f = Elem<DT>::load(global<const typename Elem<DT>::T>(t.grad)[whole + threadIdx.x]);
     sum[0] += f * f;
   }
   float s = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
@@ -192,6 +189,41 @@ struct Rule {
   float b1, c1, b2, c2, eps;  // c: 1 - b, formed in fp64
 };
 
+// The stored master's own rounding is the parameter: kept apart from the arithmetic, which the compiler would otherwise
+// round to fp16 in one step with it.
+template <int N>
+__device__ __forceinline__ void settled(float* w) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(w[j]));
+}
+
+template <int PT, int GT, bool MASTER, bool FULL>
+__device__ __forceinline__ void eight32(const Item& t, const Factor& f, const Rule& k, int64_t i, int some) {
+  float g[8], m[8], v[8], w[8];
+  load<GT, 8, FULL>(t.grad, i, some, g);
+  load<kF32, 8, FULL>(t.m, i, some, m);
+  load<kF32, 8, FULL>(t.v, i, some, v);
+  if constexpr (MASTER)
+    load<kF32, 8, FULL>(t.master, i, some, w);
+  else
+    load<PT, 8, FULL>(t.param, i, some, w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = g[j] * f.share;
+    m[j] = m[j] * k.b1 + x * k.c1;
+    v[j] = v[j] * k.b2 + (x * x) * k.c2;
+    const float d = __builtin_amdgcn_sqrtf(v[j]) * f.root + k.eps;
+    w[j] = w[j] * f.decay - f.rate * m[j] * __builtin_amdgcn_rcpf(d);
+  }
+  store<kF32, 8, FULL>(t.m, i, some, m);
+  store<kF32, 8, FULL>(t.v, i, some, v);
+  if constexpr (MASTER) {
+    settled<8>(w);
+    store<kF32, 8, FULL>(t.master, i, some, w);
+  }
+  store<PT, 8, FULL>(t.param, i, some, w);
+}
+
 template <int PT, int GT, bool MASTER>
 __global__ __launch_bounds__(kThreads) void step32(const Items items, const Factor* __restrict__ factors, const Rule k) {
   const Item& t = items.item[find(items, blockIdx.x)];
@@ -200,29 +232,12 @@ __global__ __launch_bounds__(kThreads) void step32(const Items items, const Fact
   const int64_t at = (int64_t)((int)blockIdx.x - t.first) * kStepChunk;
 #pragma unroll 1
   for (int s = 0; s < kStepChunk / (8 * kThreads); ++s) {
-    const int64_t i = at + 8 * (s * kThreads + (int)threadIdx.x);
-    const int some = (int)min((int64_t)8, t.n - i);
-    if (some <= 0) return;
-    float g[8], m[8], v[8], w[8];
-    load_part<GT>(t.grad, i, some, g);
-    load_part<kF32>(t.m, i, some, m);
-    load_part<kF32>(t.v, i, some, v);
-    if constexpr (MASTER)
-      load_part<kF32>(t.master, i, some, w);
+    const int64_t i = at + 8 * (s * kThreads + (int)threadIdx.x), left = t.n - i;
+    if (left <= 0) return;
+    if (left >= 8)
+      eight32<PT, GT, MASTER, true>(t, f, k, i, 8);
     else
-      load_part<PT>(t.param, i, some, w);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = g[j] * f.share;
-      m[j] = m[j] * k.b1 + x * k.c1;
-      v[j] = v[j] * k.b2 + (x * x) * k.c2;
-      const float d = __builtin_amdgcn_sqrtf(v[j]) * f.root + k.eps;
-      w[j] = w[j] * f.decay - f.rate * m[j] * __builtin_amdgcn_rcpf(d);
-    }
-    store_part<kF32>(t.m, i, some, m);
-    store_part<kF32>(t.v, i, some, v);
-    if constexpr (MASTER) store_part<kF32>(t.master, i, some, w);
-    store_part<PT>(t.param, i, some, w);
+      eight32<PT, GT, MASTER, false>(t, f, k, i, (int)left);
   }
 }
 
@@ -256,7 +271,103 @@ __device__ __forceinline__ float rounded_root(float b, uint32_t h) {
   return fminf((low + (up ? 1.f : 0.f)) * __uint_as_float(s), 448.f);
 }
 
-// 16 elements a lane: a DPP row of 16 lanes has a scale's 256.
+// Sixteen codes from p, zeros past `some`.
+template <bool FULL>
+__device__ __forceinline__ u32x4 load_codes(const void* p, int64_t i, int some) {
+  if constexpr (FULL) return *(Global<const u32x4_any>*)(global<const uint8_t>(p) + i);
+  u32x4 c{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (j < some) c[j / 4] |= (uint32_t)global<const uint8_t>(p)[i + j] << (8 * (j % 4));
+  return c;
+}
+template <bool FULL>
+__device__ __forceinline__ void store_codes(void* p, int64_t i, int some, const u32x4& c) {
+  if constexpr (FULL) {
+    __builtin_nontemporal_store(c, (Global<u32x4_any>*)(global<uint8_t>(p) + i));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < some) global<uint8_t>(p)[i + j] = (uint8_t)(c[j / 4] >> (8 * (j % 4)));
+  }
+}
+template <bool HIGH>
+__device__ __forceinline__ void two_values(uint32_t codes, float* f) {
+  const auto v = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, HIGH);
+  f[0] = v[0];
+  f[1] = v[1];
+}
+__device__ __forceinline__ uint32_t four_codes(const float* f) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], lo, true);
+}
+
+// The correctly rounded root: the hardware's is a unit off at most, and the residuals of its neighbours say which it is.
+__device__ __forceinline__ float exact_root(float x) {
+  const float s = __builtin_amdgcn_sqrtf(x);
+  const float below = __uint_as_float(__float_as_uint(s) - 1u), above = __uint_as_float(__float_as_uint(s) + 1u);
+  const float r = __builtin_fmaf(-below, s, x) <= 0.f ? below : s;
+  return __builtin_fmaf(-above, s, x) > 0.f ? above : r;
+}
+
+// 16 elements a lane: a DPP row of 16 lanes has a scale's 256. The states are formed as the formula says it, each operation
+// rounded by itself (no fused ones) and the root correctly: a last bit decides now and then which code is stored.
+template <int PT, int GT, bool MASTER, bool FULL>
+__device__ __forceinline__ void sixteen8(const Item& t, const Factor& f, const Rule& k, int64_t i, int some, int64_t block,
+                                         int64_t blocks, uint32_t key) {
+#pragma clang fp contract(off)
+  Global<float>* const scales = global<float>(t.scales) + block;
+  const float ms = scales[0], rs = scales[blocks];
+  u32x4 mc = load_codes<FULL>(t.m, i, some), rc = load_codes<FULL>(t.v, i, some);
+  float g[16], w[16], m[16], r[16];
+  load<GT, 16, FULL>(t.grad, i, some, g);
+  if constexpr (MASTER)
+    load<kF32, 16, FULL>(t.master, i, some, w);
+  else
+    load<PT, 16, FULL>(t.param, i, some, w);
+  uint32_t mtop = 0, rtop = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    two_values<false>(mc[q], m + 4 * q);
+    two_values<true>(mc[q], m + 4 * q + 2);
+    two_values<false>(rc[q], r + 4 * q);
+    two_values<true>(rc[q], r + 4 * q + 2);
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float x = g[j] * f.share, old = r[j] * rs;
+    m[j] = (m[j] * ms) * k.b1 + x * k.c1;
+    r[j] = exact_root((old * old) * k.b2 + (x * x) * k.c2);
+    w[j] = w[j] * f.decay - f.rate * m[j] * __builtin_amdgcn_rcpf(r[j] * f.root + k.eps);
+    mtop = max(mtop, __float_as_uint(m[j]) & 0x7fffffffu);
+    rtop = max(rtop, __float_as_uint(r[j]) & 0x7fffffffu);
+  }
+  if constexpr (MASTER) {
+    settled<16>(w);
+    store<kF32, 16, FULL>(t.master, i, some, w);
+  }
+  store<PT, 16, FULL>(t.param, i, some, w);
+  const float mscale = scale_of(row_max(mtop)), rscale = scale_of(row_max(rtop));
+  if (threadIdx.x % 16 == 0) {
+    scales[0] = mscale;
+    scales[blocks] = rscale;
+  }
+  const float minv = 1.0f / mscale, rinv = 1.0f / rscale;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const uint32_t h = mixed((uint32_t)(i + j) * kGolden + key);
+    m[j] = rounded_m(m[j] * minv, h);
+    r[j] = rounded_root(r[j] * rinv, h);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    mc[q] = four_codes(m + 4 * q);
+    rc[q] = four_codes(r + 4 * q);
+  }
+  store_codes<FULL>(t.m, i, some, mc);
+  store_codes<FULL>(t.v, i, some, rc);
+}
+
 template <int PT, int GT, bool MASTER>
 __global__ __launch_bounds__(kThreads) void step8(const Items items, const Factor* __restrict__ factors, const Rule k) {
   const Item& t = items.item[find(items, blockIdx.x)];
@@ -266,92 +377,13 @@ __global__ __launch_bounds__(kThreads) void step8(const Items items, const Facto
   const uint32_t key = with_word(f.key, (uint32_t)(at >> 32));
 #pragma unroll 1
   for (int s = 0; s < kStepChunk / (16 * kThreads); ++s) {
-    const int64_t i = at + 16 * (s * kThreads + (int)threadIdx.x);
-    const int64_t left = t.n - i;
-    const int64_t block = i / kBlock;
+    const int64_t i = at + 16 * (s * kThreads + (int)threadIdx.x), block = i / kBlock, left = t.n - i;
     if (block >= blocks) return;  // whole rows of lanes
-    const float ms = t.scales[block], rs = t.scales[blocks + block];
-    float m[16], r[16];
-    uint32_t mc[4], rc[4];
-    if (left >= 16) {
-      const u32x4 a = *reinterpret_cast<const u32x4_any*>((const uint8_t*)t.m + i);
-      const u32x4 b = *reinterpret_cast<const u32x4_any*>((const uint8_t*)t.v + i);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) mc[q] = a[q], rc[q] = b[q];
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        mc[q] = rc[q] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (4 * q + j < left) {
-            mc[q] |= (uint32_t)((const uint8_t*)t.m)[i + 4 * q + j] << (8 * j);
-            rc[q] |= (uint32_t)((const uint8_t*)t.v)[i + 4 * q + j] << (8 * j);
-          }
-      }
-    }
-    uint32_t mtop = 0, rtop = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int some = (int)max((int64_t)0, min((int64_t)8, left - 8 * h));
-      float g[8], w[8];
-      load_part<GT>(t.grad, i + 8 * h, some, g);
-      if constexpr (MASTER)
-        load_part<kF32>(t.master, i + 8 * h, some, w);
-      else
-        load_part<PT>(t.param, i + 8 * h, some, w);
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const int q = 2 * h + j / 4;
-        const auto md = j % 4 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[q], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[q], false);
-        const auto rd = j % 4 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)rc[q], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)rc[q], false);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x = g[j + e] * f.share, old = rd[e] * rs;
-          const float mn = (md[e] * ms) * k.b1 + x * k.c1;
-          const float vn = (old * old) * k.b2 + (x * x) * k.c2;
-          const float rn = __builtin_amdgcn_sqrtf(vn);
-          w[j + e] = w[j + e] * f.decay - f.rate * mn * __builtin_amdgcn_rcpf(rn * f.root + k.eps);
-          m[8 * h + j + e] = mn;
-          r[8 * h + j + e] = rn;
-          mtop = max(mtop, __float_as_uint(mn) & 0x7fffffffu);
-          rtop = max(rtop, __float_as_uint(rn) & 0x7fffffffu);
-        }
-      }
-      if constexpr (MASTER) store_part<kF32>(t.master, i + 8 * h, some, w);
-      store_part<PT>(t.param, i + 8 * h, some, w);
-    }
-    const float mscale = scale_of(row_max(mtop)), rscale = scale_of(row_max(rtop));
-    if (threadIdx.x % 16 == 0) {
-      t.scales[block] = mscale;
-      t.scales[blocks + block] = rscale;
-    }
-    const float minv = 1.0f / mscale, rinv = 1.0f / rscale;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float a[4], b[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t h = mixed((uint32_t)(i + 4 * q + j) * kGolden + key);
-        a[j] = rounded_m(m[4 * q + j] * minv, h);
-        b[j] = rounded_root(r[4 * q + j] * rinv, h);
-      }
-      int c = __builtin_amdgcn_cvt_pk_fp8_f32(a[0], a[1], 0, false);
-      mc[q] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a[2], a[3], c, true);
-      c = __builtin_amdgcn_cvt_pk_fp8_f32(b[0], b[1], 0, false);
-      rc[q] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b[2], b[3], c, true);
-    }
-    if (left >= 16) {
-      *reinterpret_cast<u32x4_any*>((uint8_t*)t.m + i) = u32x4{mc[0], mc[1], mc[2], mc[3]};
-      *reinterpret_cast<u32x4_any*>((uint8_t*)t.v + i) = u32x4{rc[0], rc[1], rc[2], rc[3]};
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j < left) {
-          ((uint8_t*)t.m)[i + j] = (uint8_t)(mc[j / 4] >> (8 * (j % 4)));
-          ((uint8_t*)t.v)[i + j] = (uint8_t)(rc[j / 4] >> (8 * (j % 4)));
-        }
-    }
+    // A row of lanes is whole or not as one, for its maximum.
+    if ((block + 1) * kBlock <= t.n)
+      sixteen8<PT, GT, MASTER, true>(t, f, k, i, 16, block, blocks, key);
+    else
+      sixteen8<PT, GT, MASTER, false>(t, f, k, i, (int)max((int64_t)0, left), block, blocks, key);
   }
 }
 
