@@ -38,6 +38,11 @@ __device__ __forceinline__ void dma16(rsrc_t r, uint32_t voff, uint32_t m0) {
   asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(m0) : "memory");
 }
 
+// The same with a scalar offset, which the range check leaves out.
+__device__ __forceinline__ void dma16_at(rsrc_t r, uint32_t voff, uint32_t soff, uint32_t m0) {
+  asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(m0) : "memory");
+}
+
 // Chunk j (16 bytes) of a staged row r of W 16-bit elements sits at j ^ swz16<W>(r): conflict-free for 128-bit reads
 // of 16 rows (lane bit 5 and the parity of bits 2-4 fixed) and for transposed 64-bit reads of 8 rows x 2 chunks.
 template <int W>

@@ -76,34 +76,39 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, l16 = lane & 15;
   const int wr = wave / WN, wc = wave % WN, wv = __builtin_amdgcn_readfirstlane(wave);
 
-  // Chunk q = i * threads + tid of a staged tile is position q % 8 of row q / 8, which holds chunk (q % 8) ^ swizzle(row).
-  // Request i lies i * kStep rows (whole swizzle periods) below request 0. What lies past K in the last stage is not asked
-  // for: its offset is past the resource.
+  // Chunk q = i * threads + tid of a staged tile is position q % 8 of row q / 8, which holds chunk (q % 8) ^ swizzle(row):
+  // the same one in every request, whose rows lie whole swizzle periods apart. A tile's resource ends with its last row, and the
+  // range check is of the lane's offset alone; the stage's place in the rows is the scalar offset, which is not checked, so
+  // what lies past K in the last stage, and all of a stage past that one, is not asked for by an offset past any resource.
+  constexpr int kOffs = Tl::kADma > Tl::kBDma ? Tl::kADma : Tl::kBDma;
   const int srow = tid >> 3, chunk = (tid & 7) ^ stage_swizzle<false>(srow);
-  const uint32_t off = opaque((uint32_t)(srow * K + 16 * chunk));
-  const uint32_t past = opaque(K % kStage8 && 16 * chunk >= K % kStage8 ? kPastEnd : 0u);
+  uint32_t off[kOffs];
+#pragma unroll
+  for (int i = 0; i < kOffs; ++i) off[i] = opaque((uint32_t)((srow + i * Tl::kStep) * K + 16 * chunk));
+  const uint32_t past = opaque(16 * chunk >= K - (tiles.stages - 1) * kStage8 ? kPastEnd : 0u);
 
-  struct Stage {
-    const uint8_t *a, *b;
-    int abytes, bbytes;
-    uint32_t off;
+  struct Source {
+    rsrc_t a, b;
   };
-  auto stage_of = [&](const TileAt& t, int st) {  // (one stage: the second's bytes are some of the rows', not used)
-    const int k0 = st * kStage8;
-    Stage s;
-    s.a = x + (int64_t)t.m0 * K + k0;
-    s.b = w + (int64_t)t.n0 * K + k0;
-    s.abytes = min(Tl::kRows, rows - t.m0) * K - k0;
-    s.bbytes = min(Tl::kCols, F - t.n0) * K - k0;
-    s.off = st + 1 == tiles.stages ? off | past : off;
-    return s;
+  auto source = [&](const TileAt& t) {
+    return Source{make_rsrc(x + (int64_t)t.m0 * K, (uint32_t)(min(Tl::kRows, rows - t.m0) * K)),
+                  make_rsrc(w + (int64_t)t.n0 * K, (uint32_t)(min(Tl::kCols, F - t.n0) * K))};
+  };
+  // Which stage of which tile, and what is past its end.
+  struct Stage {
+    Source s;
+    int k0;
+    uint32_t past;
+  };
+  auto stage_of = [&](const Source& s, int st) {
+    return Stage{s, st * kStage8, st + 1 < tiles.stages ? 0u : st < tiles.stages ? past : kPastEnd};
   };
   auto request = [&](const Stage& s, int buf, int i) {
     const bool of_a = i < Tl::kADma;
-    const int k = of_a ? i : i - Tl::kADma, ahead = k * Tl::kStep * K;
+    const int k = of_a ? i : i - Tl::kADma;
     uint8_t* const to = of_a ? As + buf * Tl::kA : Bs + buf * Tl::kB;
-    dma16(make_rsrc((of_a ? s.a : s.b) + ahead, (uint32_t)max((of_a ? s.abytes : s.bbytes) - ahead, 0)), s.off,
-          (uint32_t)(uintptr_t)(lds_void*)(to + (k * Tl::kThreads + 64 * wv) * 16));
+    dma16_at(of_a ? s.s.a : s.s.b, off[k] | s.past, s.k0,
+             (uint32_t)(uintptr_t)(lds_void*)(to + (k * Tl::kThreads + 64 * wv) * 16));
   };
 
   // Row block o of a staged tile: rows 16 o + l16, chunks g and 4 + g. The swizzle depends on l16 alone.
@@ -137,12 +142,14 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
   int v = blockIdx.x, buf = 0;
   if (v >= tiles.total) return;
   TileAt here = tile_at<Tl::kRows, Tl::kCols>(tiles, v);
-  Stage st = stage_of(here, 0);
+  Source cur = source(here);
+  Stage st = stage_of(cur, 0);
 #pragma unroll
   for (int i = 0; i < Tl::kDma; ++i) request(st, 0, i);
   wait_and_sync();
   TileAt next = tile_at<Tl::kRows, Tl::kCols>(tiles, min(v + (int)gridDim.x, tiles.total - 1));
-  st = stage_of(here, 1);
+  Source nxt = source(next);
+  st = stage_of(cur, 1);
 #pragma unroll
   for (int i = 0; i < Tl::kDma; ++i) request(st, 1, i);
   read_a(0, 0);
@@ -159,7 +166,8 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
       for (int p = 0; p < RB / 2 - 1; ++p) pair(p, buf, st);
       wait_and_sync();
       // Stage k + 2 of this tile, or the first or second of the next one (after the last tile some tile's, not used).
-      st = k + 2 < tiles.stages ? stage_of(here, k + 2) : stage_of(next, k + 2 - tiles.stages);
+      const bool in = k + 2 < tiles.stages;
+      st = stage_of(Source{in ? cur.a : nxt.a, in ? cur.b : nxt.b}, in ? k + 2 : k + 2 - tiles.stages);
       pair(RB / 2 - 1, buf, st);
       buf ^= 1;
     }
@@ -177,7 +185,9 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
     v += gridDim.x;
     if (v >= tiles.total) break;
     here = next;
+    cur = nxt;
     next = tile_at<Tl::kRows, Tl::kCols>(tiles, min(v + (int)gridDim.x, tiles.total - 1));
+    nxt = source(next);
   }
   wait_and_sync();  // the unused requests land before the workgroup's LDS is released
 }
