@@ -9,8 +9,17 @@
 // A lane of 16 g + l16 gives an operand 32 bytes of row l16. Which summed index a byte stands for only has to be the same in
 // both operands, so a lane takes the 16-byte chunks g and 4 + g of 128 summed indices, whose reads do not conflict.
 //
-// Many rows: one stream of stages per workgroup, 128 summed indices each, memory -> LDS directly, double-buffered,
-// persistent over tiles. Few rows: bound by the weight, which goes from memory to registers, once.
+// Many rows: one stream of stages per workgroup, 128 summed indices each, memory -> LDS directly, persistent over tiles. A
+// stage's products go in pairs of row blocks; its barrier stands before the last pair, whose operands are in registers by
+// then. LDS holds the stages that DA and DB say, so that a request has that many stages' time (256 x 256 tiles: three of x and
+// two of w, all of a CU's 160 KB). What bounds it at 8192 x 8192 x 8192: the card's power limit (random rows 409 us, 2690 TFLOP/s,
+// at 1.9 GHz with the matrix cores busy 64 % of the cycles; zeros 360; the vendor's library 404 with one scale for all, 455
+// with a scale per row). A step that cost: registers that went to memory in the loop, and a load waited for in it, each
+// waited for every request in flight.
+// Few rows (64 at most): bound by the weight, which goes from memory to registers, once. One row, [8192, 4096]: 7.5 us (4.5
+// TB/s; a read of as much takes 5.4), [28672, 8192]: 39.5 (5.9 TB/s). 33 to 64 rows: bound by the reads of x by every
+// workgroup through L2 (x [64, 8192], w [8192, 8192]: 26.5 us).
+#include "chunks.h"
 #include "krsi_device.h"
 #include "krsi_internal.h"
 #include "lds_dma.h"
@@ -31,13 +40,11 @@ __device__ __forceinline__ f32x4 product(const Frag& a, const Frag& b, const f32
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 0, 0, 0, 0, 0, 0);
 }
 
-// Four outputs of a row from column col on.
+// Four outputs of a row at p, or as many as are `left` before its end.
 template <int OT>
-__device__ __forceinline__ void store_out(typename Elem<OT>::T* out, int64_t row, int col, int F, const f32x4& acc, float xs,
-                                          const float* ws) {
+__device__ __forceinline__ void store_out(typename Elem<OT>::T* p, int left, const f32x4& acc, float xs, const float* ws) {
   using T = typename Elem<OT>::T;
-  T* p = out + row * F + col;
-  if (col + 4 <= F) {
+  if (left >= 4) {
     T v[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = Elem<OT>::store(acc[r] * xs * ws[r]);
@@ -45,8 +52,26 @@ __device__ __forceinline__ void store_out(typename Elem<OT>::T* out, int64_t row
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (col + r < F) p[r] = Elem<OT>::store(acc[r] * xs * ws[r]);
+      if (r < left) p[r] = Elem<OT>::store(acc[r] * xs * ws[r]);
   }
+}
+// Two column blocks' outputs of a row, eight columns to a lane: lane groups 0 and 2 get columns 0 - 7 and 8 - 15 of the first
+// block, 1 and 3 of the second, so that a store writes 64 bytes of each row. Stored past the caches, they leave the tiles in flight in L2
+// (8192 x 4096 x 16384: 483 us with eight bytes a lane, 464 so, 423 past the caches).
+template <int OT>
+__device__ __forceinline__ void store_two(bool live, typename Elem<OT>::T* p, const f32x4& a, const f32x4& b, float xs, const float* sa,
+                                          const float* sb) {
+  static_assert(sizeof(*p) == 2, "16-bit outputs");
+  uint32_t v[2][2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const uint32_t lo = Elem<OT>::pack2(a[2 * q] * xs * sa[2 * q], a[2 * q + 1] * xs * sa[2 * q + 1]);
+    const uint32_t hi = Elem<OT>::pack2(b[2 * q] * xs * sb[2 * q], b[2 * q + 1] * xs * sb[2 * q + 1]);
+    const auto r = __builtin_amdgcn_permlane16_swap(lo, hi, false, false);  // lo's odd groups with hi's even ones
+    v[0][q] = r[0];
+    v[1][q] = r[1];
+  }
+  if (live) __builtin_nontemporal_store(u32x4{v[0][0], v[0][1], v[1][0], v[1][1]}, reinterpret_cast<u32x4_any*>(p));
 }
 // The scales of columns col .. col + 3 (past the end: of the last).
 __device__ __forceinline__ void load_scales(const float* ws, int col, int F, float* s) {
@@ -55,26 +80,40 @@ __device__ __forceinline__ void load_scales(const float* ws, int col, int F, flo
 }
 
 // ---------------------------------------------------------------- many rows
-template <int WM, int WN, int RB, int CB>
+// Every LDS access of the wave done and all of its vector memory requests but the newest N, then the workgroup's barrier.
+template <int N>
+__device__ __forceinline__ void wait_for() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// DA and DB: the stages of x and of w that LDS holds.
+template <int WM, int WN, int RB, int CB, int DA, int DB>
 struct Tile8 {
   static constexpr int kThreads = 64 * WM * WN;
   static constexpr int kRows = 16 * RB * WM, kCols = 16 * CB * WN;
   static constexpr int kA = kRows * kStage8, kB = kCols * kStage8;  // bytes of a staged tile
   static constexpr int kADma = kA / 16 / kThreads, kBDma = kB / 16 / kThreads, kDma = kADma + kBDma;
-  static constexpr int kPerCu = 160 * 1024 / (2 * (kA + kB));
+  static constexpr int kLds = DA * kA + DB * kB;
+  static constexpr int kPerCu = 160 * 1024 / kLds;
   static constexpr int kStep = kThreads / 8;  // staged rows from request to request
+  // At the barrier that lets the next stage be read: requests that may still be on their way, those for later ones.
+  static constexpr int kLater = (DB - 2) * kDma + (DA > DB ? kADma : 0);
+  static_assert(DA >= DB && DB >= 2 && DA * kDma < 64, "requests that the wait can count");
   static_assert(kA / 16 % kThreads == 0 && kB / 16 % kThreads == 0 && kStep % 16 == 0 && RB % 4 == 0, "whole requests");
 };
 
-template <int OT, int WM, int WN, int RB, int CB>
-__global__ __launch_bounds__(64 * WM * WN, (Tile8<WM, WN, RB, CB>::kPerCu * WM * WN / 4)) void
+template <int OT, int WM, int WN, int RB, int CB, int DA, int DB>
+__global__ __launch_bounds__(64 * WM * WN, (Tile8<WM, WN, RB, CB, DA, DB>::kPerCu * WM * WN / 4)) void
 linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w, const float* __restrict__ xs,
                    const float* __restrict__ ws, typename Elem<OT>::T* __restrict__ out, int rows, int K, int F, const Tiles tiles) {
-  using Tl = Tile8<WM, WN, RB, CB>;
-  __shared__ __attribute__((aligned(512))) uint8_t lds[2 * (Tl::kA + Tl::kB)];
-  uint8_t *const As = lds, *const Bs = lds + 2 * Tl::kA;
+  using Tl = Tile8<WM, WN, RB, CB, DA, DB>;
+  __shared__ __attribute__((aligned(512))) uint8_t lds[Tl::kLds];
+  uint8_t *const As = lds, *const Bs = lds + DA * Tl::kA;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, l16 = lane & 15;
-  const int wr = wave / WN, wc = wave % WN, wv = __builtin_amdgcn_readfirstlane(wave);
+  const int wr = wave / WN, wc = wave % WN, wv = __builtin_amdgcn_readfirstlane(wave), wru = wv / WN, wcu = wv % WN;
+  const rsrc_t xsr = make_rsrc(xs, (uint32_t)rows * 4u), wsr = make_rsrc(ws, (uint32_t)F * 4u);
 
   // Chunk q = i * threads + tid of a staged tile is position q % 8 of row q / 8, which holds chunk (q % 8) ^ swizzle(row):
   // the same one in every request, whose rows lie whole swizzle periods apart. A tile's resource ends with its last row, and the
@@ -103,12 +142,10 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
   auto stage_of = [&](const Source& s, int st) {
     return Stage{s, st * kStage8, st + 1 < tiles.stages ? 0u : st < tiles.stages ? past : kPastEnd};
   };
-  auto request = [&](const Stage& s, int buf, int i) {
-    const bool of_a = i < Tl::kADma;
-    const int k = of_a ? i : i - Tl::kADma;
-    uint8_t* const to = of_a ? As + buf * Tl::kA : Bs + buf * Tl::kB;
-    dma16_at(of_a ? s.s.a : s.s.b, off[k] | s.past, s.k0,
-             (uint32_t)(uintptr_t)(lds_void*)(to + (k * Tl::kThreads + 64 * wv) * 16));
+  // Request i of this thread for x's part of a stage, into the buffer at byte `to`, and for w's.
+  auto request = [&](bool of_a, const Stage& s, int to, int i) {
+    dma16_at(of_a ? s.s.a : s.s.b, off[i] | s.past, s.k0,
+             (uint32_t)(uintptr_t)(lds_void*)((of_a ? As : Bs) + to + (i * Tl::kThreads + 64 * wv) * 16));
   };
 
   // Row block o of a staged tile: rows 16 o + l16, chunks g and 4 + g. The swizzle depends on l16 alone.
@@ -117,41 +154,54 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
     return Frag{*reinterpret_cast<const u32x4*>(t + 16 * o * kStage8 + lo), *reinterpret_cast<const u32x4*>(t + 16 * o * kStage8 + hi)};
   };
   Frag a[4], b[CB];  // row block i of the stage is in a[i % 4]
-  auto read_a = [&](int i, int buf) { a[i % 4] = frag(As + buf * Tl::kA, RB * wr + i); };
-  auto read_b = [&](int j, int buf) { b[j] = frag(Bs + buf * Tl::kB, CB * wc + j); };
+  auto read_a = [&](int i, int at) { a[i % 4] = frag(As + at, RB * wr + i); };
+  auto read_b = [&](int j, int at) { b[j] = frag(Bs + at, CB * wc + j); };
   f32x4 acc[RB][CB];
 
+  // Stage k's buffers are at a0 and b0, the next one's at a1 and b1.
+  int a0 = 0, a1 = Tl::kA, b0 = 0, b1 = Tl::kB;
   // The products of row blocks 2 p and 2 p + 1, b by b. The reads of the pair after, and with the last pair, which only
-  // needs registers, the next stage's first pair and each b after its last use, and the requests of the stage after that.
+  // needs registers, the next stage's first pair and each b after its last use, and the requests: of w's stage k + DB first,
+  // then of x's stage k + DA.
   constexpr int kProducts = 2 * CB;
-  auto pair = [&](int p, int buf, const Stage& d) {
+  auto pair = [&](int p, const Stage& da, const Stage& db) {
     const bool last = p == RB / 2 - 1;
 #pragma unroll
     for (int m = 0; m < kProducts; ++m) {
       const int j = m / 2, i = 2 * p + m % 2;
       acc[i][j] = product(b[j], a[i % 4], acc[i][j]);
-      if (m < 2) read_a(last ? m : 2 * p + 2 + m, last ? buf ^ 1 : buf);
-      if (last && m % 2 == 1) read_b(j, buf ^ 1);
+      if (m < 2) read_a(last ? m : 2 * p + 2 + m, last ? a1 : a0);
+      if (last && m % 2 == 1) read_b(j, b1);
 #pragma unroll
       for (int q = 0; q < Tl::kDma; ++q)
-        if (last && q * kProducts / Tl::kDma == m) request(d, buf, q);
+        if (last && q * kProducts / Tl::kDma == m)
+          request(q >= Tl::kBDma, q < Tl::kBDma ? db : da, q < Tl::kBDma ? b0 : a0, q < Tl::kBDma ? q : q - Tl::kBDma);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  int v = blockIdx.x, buf = 0;
+  int v = blockIdx.x;
   if (v >= tiles.total) return;
   TileAt here = tile_at<Tl::kRows, Tl::kCols>(tiles, v);
   Source cur = source(here);
-  Stage st = stage_of(cur, 0);
-#pragma unroll
-  for (int i = 0; i < Tl::kDma; ++i) request(st, 0, i);
-  wait_and_sync();
   TileAt next = tile_at<Tl::kRows, Tl::kCols>(tiles, min(v + (int)gridDim.x, tiles.total - 1));
   Source nxt = source(next);
-  st = stage_of(cur, 1);
+  // Stage s of this tile, or where it is past its end, of the next one (after the last tile some tile's, not used).
+  auto ahead = [&](int s) {
+    const bool in = s < tiles.stages;
+    return stage_of(Source{in ? cur.a : nxt.a, in ? cur.b : nxt.b}, in ? s : s - tiles.stages);
+  };
+  // Stage by stage, so that the first may be read before the last are here.
 #pragma unroll
-  for (int i = 0; i < Tl::kDma; ++i) request(st, 1, i);
+  for (int s = 0; s < DA; ++s) {
+    const Stage st = ahead(s);
+#pragma unroll
+    for (int i = 0; i < Tl::kBDma; ++i)
+      if (s < DB) request(false, st, s * Tl::kB, i);
+#pragma unroll
+    for (int i = 0; i < Tl::kADma; ++i) request(true, st, s * Tl::kA, i);
+  }
+  wait_for<(DB - 1) * Tl::kDma + (DA - DB) * Tl::kADma>();
   read_a(0, 0);
   read_a(1, 0);
 #pragma unroll
@@ -162,25 +212,60 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
 #pragma unroll
       for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int k = 0; k < tiles.stages; ++k) {
+      const Stage db = ahead(k + DB), da = ahead(k + DA);
 #pragma unroll
-      for (int p = 0; p < RB / 2 - 1; ++p) pair(p, buf, st);
-      wait_and_sync();
-      // Stage k + 2 of this tile, or the first or second of the next one (after the last tile some tile's, not used).
-      const bool in = k + 2 < tiles.stages;
-      st = stage_of(Source{in ? cur.a : nxt.a, in ? cur.b : nxt.b}, in ? k + 2 : k + 2 - tiles.stages);
-      pair(RB / 2 - 1, buf, st);
-      buf ^= 1;
+      for (int p = 0; p < RB / 2 - 1; ++p) pair(p, da, db);
+      // After an epilogue, whose loads and stores are counted too, everything is waited for.
+      if (k == 0 && v != (int)blockIdx.x)
+        wait_for<0>();
+      else
+        wait_for<Tl::kLater>();
+      pair(RB / 2 - 1, da, db);
+      a0 = a1, b0 = b1;
+      a1 = a1 + Tl::kA == DA * Tl::kA ? 0 : a1 + Tl::kA;
+      b1 = b1 + Tl::kB == DB * Tl::kB ? 0 : b1 + Tl::kB;
     }
+    // All scales first: loaded one by one between the stores, each waited for the requests in flight before it as well. What
+    // lies past an end reads as zero. Places are a wave's own plus a lane's 32-bit offset: with a pointer for each row, the
+    // loop's registers went to memory and back.
+    const int m = here.m0 + 16 * RB * wru, n = here.n0 + 16 * CB * wcu;
+    float sx[RB], sw[CB][4];
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+      sx[i] = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b32(xsr, opaque(4 * (m + l16) + 64 * i), 0, 0));
 #pragma unroll
     for (int j = 0; j < CB; ++j) {
-      const int col = here.n0 + 16 * (CB * wc + j) + 4 * g;
-      float s[4];
-      load_scales(ws, min(col, F - 1), F, s);
+      const u32x4 q = __builtin_amdgcn_raw_buffer_load_b128(wsr, opaque(4 * (n + 4 * g) + 64 * j), 0, 0);
 #pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        const int row = here.m0 + 16 * (RB * wr + i) + l16;
-        if (row < rows && col < F) store_out<OT>(out, row, col, F, acc[i][j], xs[row], s);
+      for (int r = 0; r < 4; ++r) sw[j][r] = __uint_as_float(q[r]);
+    }
+    // Used here, on every path: a load that some path leaves unused is waited for where its register is next written, which
+    // was in the loop over the stages, in each of them and for all requests in flight.
+#pragma unroll
+    for (int i = 0; i < RB; ++i) asm volatile("" : "+v"(sx[i]));
+#pragma unroll
+    for (int j = 0; j < CB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) asm volatile("" : "+v"(sw[j][r]));
+    typename Elem<OT>::T* at = out + (int64_t)m * F + n;
+    const bool wide = OT != kF32 && n + 16 * CB <= F;  // all of the wave's columns are there
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      const bool live = l16 < rows - m - 16 * i;
+      if constexpr (OT != kF32) {
+        if (wide) {  // every lane has its part in the exchange, also of a row that is not there
+#pragma unroll
+          for (int j = 0; j < CB; j += 2)
+            store_two<OT>(live, at + (l16 * F + 16 * (g & 1) + 8 * (g >> 1)) + 16 * j, acc[i][j], acc[i][j + 1], sx[i], sw[j],
+                          sw[j + 1]);
+        }
       }
+      if (!wide) {
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+          if (live) store_out<OT>(at + (l16 * F + 4 * g) + 16 * j, F - n - 4 * g - 16 * j, acc[i][j], sx[i], sw[j]);
+      }
+      at += 16 * (int64_t)F;
     }
     v += gridDim.x;
     if (v >= tiles.total) break;
@@ -197,7 +282,7 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
 // order of the waves. Stages past the end read as zero.
 constexpr int kFewWaves = 8;
 
-template <int OT, int RB, int CB>
+template <int OT, int RB, int CB, int U>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_8bit_few(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
                                                                   const float* __restrict__ xs, const float* __restrict__ ws,
                                                                   typename Elem<OT>::T* __restrict__ out, int rows, int K,
@@ -206,26 +291,37 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_8bit_few(const uint8_t*
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = blockIdx.x * 16 * CB;
   const rsrc_t xr = make_rsrc(x, (uint32_t)(rows * K)), wr = make_rsrc(w + (int64_t)n0 * K, (uint32_t)(min(16 * CB, F - n0) * K));
+  // Both chunks of a row's stage at k0; one past K is not asked for (nor, by the resource, one past the rows).
   auto frag = [&](rsrc_t r, int o, int k0) {
     const int at = (16 * o + l16) * K, lo = k0 + 16 * g, hi = lo + 64;
-    return Frag{__builtin_amdgcn_raw_buffer_load_b128(r, lo < K ? at + lo : (int)kPastEnd, 0, 0),
-                __builtin_amdgcn_raw_buffer_load_b128(r, hi < K ? at + hi : (int)kPastEnd, 0, 0)};
+    return Frag{__builtin_amdgcn_raw_buffer_load_b128(r, opaque(lo < K ? at + lo : (int)kPastEnd), 0, 0),
+                __builtin_amdgcn_raw_buffer_load_b128(r, opaque(hi < K ? at + hi : (int)kPastEnd), 0, 0)};
   };
   f32x4 acc[RB][CB];
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k0 = wave * kStage8; k0 < K; k0 += kFewWaves * kStage8) {
-    Frag a[RB], b[CB];
+  // U stages of a wave at a time, all loads before the products. Workgroups begin at different places of the rows, which they
+  // would otherwise ask of the same part of L2 at once ([16, 4096] x [4096, 4096] 6.8 -> 5.8 us).
+  const int iters = (K + U * kFewWaves * kStage8 - 1) / (U * kFewWaves * kStage8);
+  int turn = (int)(blockIdx.x % (unsigned)iters);
+  for (int it = 0; it < iters; ++it, turn = turn + 1 == iters ? 0 : turn + 1) {
+    const int k0 = (turn * U * kFewWaves + wave) * kStage8;
+    Frag a[U][RB], b[U][CB];
 #pragma unroll
-    for (int j = 0; j < CB; ++j) b[j] = frag(wr, j, k0);
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-    for (int i = 0; i < RB; ++i) a[i] = frag(xr, i, k0);
+      for (int j = 0; j < CB; ++j) b[u][j] = frag(wr, j, k0 + u * kFewWaves * kStage8);
 #pragma unroll
-    for (int i = 0; i < RB; ++i)
+      for (int i = 0; i < RB; ++i) a[u][i] = frag(xr, i, k0 + u * kFewWaves * kStage8);
+    }
 #pragma unroll
-      for (int j = 0; j < CB; ++j) acc[i][j] = product(b[j], a[i], acc[i][j]);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int j = 0; j < CB; ++j) acc[i][j] = product(b[u][j], a[u][i], acc[i][j]);
   }
 #pragma unroll
   for (int i = 0; i < RB; ++i)
@@ -240,7 +336,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_8bit_few(const uint8_t*
     if (row >= rows || col >= F) continue;
     float s[4];
     load_scales(ws, col, F, s);
-    store_out<OT>(out, row, col, F, sum, xs[row], s);
+    store_out<OT>(out + (int64_t)row * F + col, F - col, sum, xs[row], s);
   }
 }
 
@@ -256,16 +352,16 @@ struct Call {
 constexpr int kCus = 256;
 constexpr int kFewRows = 64;
 
-template <int OT, int RB, int CB>
+template <int OT, int RB, int CB, int U>
 int launch_few(const Call& c) {
-  hipLaunchKernelGGL((linear_8bit_few<OT, RB, CB>), dim3((unsigned)ceil_div(c.F, 16 * CB)), dim3(64 * kFewWaves), 0, c.st, c.x,
+  hipLaunchKernelGGL((linear_8bit_few<OT, RB, CB, U>), dim3((unsigned)ceil_div(c.F, 16 * CB)), dim3(64 * kFewWaves), 0, c.st, c.x,
                      c.w, c.xs, c.ws, (typename Elem<OT>::T*)c.out, (int)c.rows, c.K, c.F);
   return launch_status();
 }
 
-template <int OT, int WM, int WN, int RB, int CB>
+template <int OT, int WM, int WN, int RB, int CB, int DA, int DB>
 int launch_stream(const Call& c) {
-  using Tl = Tile8<WM, WN, RB, CB>;
+  using Tl = Tile8<WM, WN, RB, CB, DA, DB>;
   Tiles t;
   t.nrb = (int)ceil_div(c.rows, Tl::kRows);
   t.ncb = (int)ceil_div(c.F, Tl::kCols);
@@ -273,25 +369,33 @@ int launch_stream(const Call& c) {
   t.per = t.stages = (int)ceil_div(c.K, kStage8);
   if ((int64_t)t.nrb * t.ncb > (1 << 23)) return KRSI_ERR_UNSUPPORTED;
   t.total = t.nrb * t.ncb;
-  // The stream reaches one tile ahead, two stages: with one stage per tile every workgroup takes one tile.
-  const int resident = t.stages >= 2 ? kCus * Tl::kPerCu : t.total;
-  hipLaunchKernelGGL((linear_8bit_stream<OT, WM, WN, RB, CB>), dim3((unsigned)(t.total < resident ? t.total : resident)),
+  // The stream reaches one tile ahead, DA stages: with fewer every workgroup takes one tile.
+  const int resident = t.stages >= DA ? kCus * Tl::kPerCu : t.total;
+  hipLaunchKernelGGL((linear_8bit_stream<OT, WM, WN, RB, CB, DA, DB>), dim3((unsigned)(t.total < resident ? t.total : resident)),
                      dim3(Tl::kThreads), 0, c.st, c.x, c.w, c.xs, c.ws, (typename Elem<OT>::T*)c.out, (int)c.rows, c.K, c.F, t);
   return launch_status();
 }
 
 template <int OT>
 int launch(const Call& c) {
-  if (c.rows <= 16) return launch_few<OT, 1, 1>(c);
-  if (c.rows <= 32) return launch_few<OT, 2, 1>(c);
-  if (c.rows <= kFewRows) return launch_few<OT, 4, 2>(c);
-  // Rounds of the chip, by a tile's work: 256 x 256, 128 x 128 (two to a CU), 64 x 128 (three).
-  const int64_t large = ceil_div(ceil_div(c.rows, 256) * ceil_div(c.F, 256), kCus) * 8;
-  const int64_t mid = ceil_div(ceil_div(c.rows, 128) * ceil_div(c.F, 128), 2 * kCus) * 5;
-  const int64_t small = ceil_div(ceil_div(c.rows, 64) * ceil_div(c.F, 128), 3 * kCus) * 4;
-  if (large <= mid && large <= small) return launch_stream<OT, 2, 4, 8, 4>(c);
-  if (mid <= small) return launch_stream<OT, 2, 2, 4, 4>(c);
-  return launch_stream<OT, 1, 4, 4, 2>(c);
+  // Two column blocks share their reads of x where that leaves a workgroup for each CU ([32, 4096] x [4096, 4096]: 8.0 us with
+  // one, 9.5 with two; x [8192, 4096]: 13.4, 10.3).
+  if (c.rows <= 16) return launch_few<OT, 1, 1, 2>(c);
+  if (c.rows <= 32) return c.F >= 32 * kCus ? launch_few<OT, 2, 2, 2>(c) : launch_few<OT, 2, 1, 2>(c);
+  if (c.rows <= kFewRows) return launch_few<OT, 4, 2, 1>(c);
+  const int64_t stages = ceil_div(c.K, kStage8);
+  // The tile by its cost in hundredths of a us, as measured: rounds of the chip, each its stages and an end. Two workgroups of
+  // the smaller tiles share a CU, and a round that gives each CU one at most takes about half of a full one.
+  auto cost = [&](int rows, int cols, int full, int full_end, int part, int part_end) {
+    const int64_t tiles = ceil_div(c.rows, rows) * ceil_div(c.F, cols), per = full == part ? kCus : 2 * kCus, last = tiles % per;
+    return tiles / per * (full * stages + full_end) +
+           (last == 0 ? 0 : last > kCus ? full * stages + full_end : part * stages + part_end);
+  };
+  const int64_t large = cost(256, 256, 133, 800, 133, 800), mid = cost(128, 128, 102, 400, 55, 340),
+                small = cost(64, 128, 72, 350, 38, 290);
+  if (large <= mid && large <= small) return launch_stream<OT, 2, 4, 8, 4, 3, 2>(c);
+  if (mid <= small) return launch_stream<OT, 2, 2, 4, 4, 3, 2>(c);
+  return launch_stream<OT, 1, 4, 4, 2, 3, 3>(c);
 }
 
 }  // namespace
