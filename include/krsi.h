@@ -324,22 +324,22 @@ int krsi_add_rmsnorm_bwd(const void* dy, const void* dr, const void* r, const vo
  * of grad_dtype (T or fp32); masters (NULL: w is the parameter itself; not with fp32 params): w is the fp32
  * masters[i], params[i] its rounding. lr_at: the rate on the device, or NULL: lr. steps: [count] int32 on the device.
  * norm (device, or NULL): g is the gradient times min(1, max_norm / (norm + 1e-6)), and where *norm is not finite
- * nothing is changed, steps neither.
+ * nothing is changed, steps neither. norm_given 0: it is formed here first, as krsi_grad_norm of these gradients.
  * state_bits 32: exp_avgs, exp_avg_sqs fp32 (m and v), scales NULL. 8: they are e4m3 codes of m and of sqrt(v), times
  * scales[i] = [2, ceil(n / 256)] fp32, m's then the root's, one for each 256 elements; the new codes are rounded up or
  * down at random, m right on average and the root in its square, a root above zero never to zero; the random numbers
  * follow from seed, t, i and the element's number alone.
  * krsi_grad_norm: the root of the sum of squares over all tensors (NULL entries have no part), fixed order.
- * Limits: count <= 2^20, 2^36 elements in all; beta in [0, 1). workspaces: scratch, no need to keep.          */
+ * Limits: count <= 2^20, 2^35 elements in all; beta in [0, 1). workspaces: scratch, no need to keep.          */
 size_t krsi_grad_norm_workspace_bytes(const int64_t* sizes, int32_t count);
 int krsi_grad_norm(const void* const* grads, const int64_t* sizes, int32_t count, float* norm, void* workspace,
                    size_t workspace_bytes, int32_t dtype, void* stream);
-size_t krsi_adamw_workspace_bytes(int32_t count);
+size_t krsi_adamw_workspace_bytes(const int64_t* sizes, int32_t count);
 int krsi_adamw_step(void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
                     float* const* masters, float* const* scales, const int64_t* sizes, int32_t count, int32_t* steps,
                     const float* lr_at, float lr, double beta1, double beta2, float eps, float weight_decay,
-                    const float* norm, float max_norm, uint32_t seed, int32_t state_bits, int32_t dtype, int32_t grad_dtype,
-                    void* workspace, size_t workspace_bytes, void* stream);
+                    float* norm, int32_t norm_given, float max_norm, uint32_t seed, int32_t state_bits, int32_t dtype,
+                    int32_t grad_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------ projection in 8 bits (no counterpart)
  * out[m, n] = T( x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] ), sums in fp32: x [rows, k] and w [f, k] e4m3 (OCP, one

@@ -28,22 +28,23 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;        // elements that share a scale
-constexpr int kStepChunk = 8192;   // elements per workgroup of the step
-constexpr int kNormChunk = 65536;  // and of the norm
+constexpr int kStepChunk = 4096;   // elements per workgroup of the step
+constexpr int kNormChunk = 16384;  // and of the norm
 
-struct Item {
-  void* param;
-  const void* grad;
-  void *m, *v;
-  float *master, *scales;
-  int64_t n;
-  int32_t first, number;  // its first workgroup of this launch, its number in the list
-};
-constexpr int kItems = 60;  // as many as the 4 KB of a launch's arguments hold
+// The tensors of a launch, as many as the 4 KB of its arguments hold: P pointers each, its first workgroup of the launch and
+// its number in the list.
+template <int P>
 struct Items {
-  Item item[kItems];
+  static constexpr int kMost = 3840 / (8 * P + 16);
+  int32_t first[kMost], number[kMost];
+  int64_t n[kMost];
+  void* p[kMost][P];
   int32_t count;
 };
+// Pointers of a step: the four of every tensor, then its master's and its scales', where there are any.
+constexpr int kParam = 0, kGrad = 1, kM = 2, kV = 3;
+template <bool MASTER, bool SCALES>
+constexpr int kPointers = 4 + (MASTER ? 1 : 0) + (SCALES ? 1 : 0);
 
 // What a step needs of a tensor, from the first launch.
 struct Factor {
@@ -63,17 +64,18 @@ __device__ __forceinline__ uint32_t mixed(uint32_t h) {
 constexpr uint32_t kGolden = 0x9E3779B1u;
 __device__ __forceinline__ uint32_t with_word(uint32_t key, uint32_t word) { return mixed(key * 3u + word * kGolden + 1u); }
 
-// The launch's tensor that workgroup b works on.
-__device__ __forceinline__ int find(const Items& t, int b) {
-  int lo = 0, hi = t.count;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (t.item[mid].first <= b)
-      lo = mid;
-    else
-      hi = mid;
+// The launch's tensor that workgroup b works on. The lanes look at all of them at once: one after the other, each look at the
+// arguments waited for the one before it (a small launch took 8 us).
+template <int P>
+__device__ __forceinline__ int find(const Items<P>& t, int b) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int before = 0;
+#pragma unroll
+  for (int i = 0; i < Items<P>::kMost; i += kWave) {
+    const int at = min(i + lane, Items<P>::kMost - 1);
+    before += __popcll(__ballot(i + lane < t.count && t.first[at] <= b));
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(before - 1);
 }
 
 // Pointers that come in a structure are taken for generic ones; these accesses are of global memory.
@@ -85,6 +87,8 @@ __device__ __forceinline__ Global<T>* global(const void* p) {
 }
 
 // N consecutive elements of any alignment (N a multiple of a chunk's), or the first `some` of them.
+// A lane's 32 or 64 bytes of an fp32 tensor meet their neighbours' in the caches, so loads and stores go through them
+// (302 M parameters, 8-bit states: 929 us; stores past them 951, loads too 1350).
 template <int DT, int N, bool FULL>
 __device__ __forceinline__ void load(const void* p, int64_t i, int some, float* f) {
   using El = Elem<DT>;
@@ -100,14 +104,13 @@ __device__ __forceinline__ void load(const void* p, int64_t i, int some, float* 
     for (int j = 0; j < N; ++j) f[j] = j < some ? El::load(at[j]) : 0.f;
   }
 }
-// Non-temporal: nothing of a step is read again soon.
 template <int DT, int N, bool FULL>
 __device__ __forceinline__ void store(void* p, int64_t i, int some, const float* f) {
   using El = Elem<DT>;
   auto* at = global<typename El::T>(p) + i;
   if constexpr (FULL) {
 #pragma unroll
-    for (int q = 0; q < N; q += El::E) __builtin_nontemporal_store(El::pack(f + q), (Global<u32x4_any>*)(at + q));
+    for (int q = 0; q < N; q += El::E) *(Global<u32x4_any>*)(at + q) = El::pack(f + q);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -117,23 +120,29 @@ __device__ __forceinline__ void store(void* p, int64_t i, int some, const float*
 
 // ------------------------------------------------------------------- norm
 template <int DT>
-__global__ __launch_bounds__(kThreads) void norm_parts(const Items items, float* __restrict__ part) {
+__global__ __launch_bounds__(kThreads) void norm_parts(const Items<1> items, float* __restrict__ part) {
+  using El = Elem<DT>;
   __shared__ float red[kThreads / kWave];
-  const Item& t = items.item[find(items, blockIdx.x)];
-  const int64_t at = (int64_t)((int)blockIdx.x - t.first) * kNormChunk, end = min(at + kNormChunk, t.n);
+  const int which = find(items, blockIdx.x);
+  const void* const grad = items.p[which][0];
+  const int64_t at = (int64_t)((int)blockIdx.x - items.first[which]) * kNormChunk, end = min(at + kNormChunk, items.n[which]);
   float sum[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) sum[j] = 0.f;
   const int64_t whole = at + (end - at) / 8 * 8;
-#pragma unroll 4
+#pragma unroll 8
   for (int64_t i = at + 8 * threadIdx.x; i < whole; i += 8 * kThreads) {
     float f[8];
-    load<DT, 8, true>(t.grad, i, 8, f);
+#pragma unroll
+    for (int q = 0; q < 8; q += El::E) {  // read once, past the caches (604 MB: 118 us through them, 105 so)
+      const u32x4 c = __builtin_nontemporal_load((Global<const u32x4_any>*)(global<const typename El::T>(grad) + i + q));
+      El::unpack(c, f + q);
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[j] += f[j] * f[j];
   }
   if (threadIdx.x < end - whole) {
-    const float f = Elem<DT>::load(global<const typename Elem<DT>::T>(t.grad)[whole + threadIdx.x]);
+    const float f = Elem<DT>::load(global<const typename Elem<DT>::T>(grad)[whole + threadIdx.x]);
     sum[0] += f * f;
   }
   float s = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
@@ -143,18 +152,23 @@ __global__ __launch_bounds__(kThreads) void norm_parts(const Items items, float*
   if (threadIdx.x == 0) part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-constexpr int kJoin = 1024;
-__global__ __launch_bounds__(kJoin) void norm_join(const float* __restrict__ part, int64_t n, float* __restrict__ norm) {
-  __shared__ double red[kJoin];
+// The root of the parts' sum, in every thread of the workgroup: the same bits wherever it is formed.
+__device__ __forceinline__ float joined(const float* __restrict__ part, int64_t n, double* red) {
   double s = 0;
-  for (int64_t i = threadIdx.x; i < n; i += kJoin) s += part[i];
+  for (int64_t i = threadIdx.x; i < n; i += kThreads) s += part[i];
   red[threadIdx.x] = s;
   __syncthreads();
-  for (int w = kJoin / 2; w > 0; w /= 2) {
+#pragma unroll
+  for (int w = kThreads / 2; w > 0; w /= 2) {
     if (threadIdx.x < (unsigned)w) red[threadIdx.x] += red[threadIdx.x + w];
     __syncthreads();
   }
-  if (threadIdx.x == 0) *norm = (float)sqrt(red[0]);
+  return (float)sqrt(red[0]);
+}
+__global__ __launch_bounds__(kThreads) void norm_join(const float* __restrict__ part, int64_t n, float* __restrict__ norm) {
+  __shared__ double red[kThreads];
+  const float v = joined(part, n, red);
+  if (threadIdx.x == 0) *norm = v;
 }
 
 // ------------------------------------------------------------------- step
@@ -165,12 +179,20 @@ struct Mask {
 
 __global__ __launch_bounds__(kThreads) void step_factors(const Mask mask, int base, int count, int32_t* __restrict__ steps,
                                                          Factor* __restrict__ out, const float* __restrict__ lr_at, float lr,
-                                                         double log1, double log2, float wd, const float* __restrict__ norm,
-                                                         float max_norm, uint32_t seed) {
+                                                         double log1, double log2, float wd, float* __restrict__ norm,
+                                                         const float* __restrict__ part, int64_t parts, float max_norm,
+                                                         uint32_t seed) {
+  __shared__ double red[kThreads];
+  float total = 0.f;
+  if (part) {  // the norm is formed here, by each workgroup
+    total = joined(part, parts, red);
+    if (base == 0 && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
+  } else if (norm) {
+    total = *norm;
+  }
   const int i = blockIdx.x * kThreads + threadIdx.x;
   if (i >= count) return;
   Factor f{};
-  const float total = norm ? *norm : 0.f;
   if ((mask.word[i / 32] >> (i % 32) & 1u) && fabsf(total) <= 3.402823466e38f) {
     const int32_t t = steps[base + i] + 1;
     steps[base + i] = t;
@@ -198,15 +220,15 @@ __device__ __forceinline__ void settled(float* w) {
 }
 
 template <int PT, int GT, bool MASTER, bool FULL>
-__device__ __forceinline__ void eight32(const Item& t, const Factor& f, const Rule& k, int64_t i, int some) {
+__device__ __forceinline__ void eight32(void* const* p, const Factor& f, const Rule& k, int64_t i, int some) {
   float g[8], m[8], v[8], w[8];
-  load<GT, 8, FULL>(t.grad, i, some, g);
-  load<kF32, 8, FULL>(t.m, i, some, m);
-  load<kF32, 8, FULL>(t.v, i, some, v);
+  load<GT, 8, FULL>(p[kGrad], i, some, g);
+  load<kF32, 8, FULL>(p[kM], i, some, m);
+  load<kF32, 8, FULL>(p[kV], i, some, v);
   if constexpr (MASTER)
-    load<kF32, 8, FULL>(t.master, i, some, w);
+    load<kF32, 8, FULL>(p[4], i, some, w);
   else
-    load<PT, 8, FULL>(t.param, i, some, w);
+    load<PT, 8, FULL>(p[kParam], i, some, w);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float x = g[j] * f.share;
@@ -215,29 +237,31 @@ __device__ __forceinline__ void eight32(const Item& t, const Factor& f, const Ru
     const float d = __builtin_amdgcn_sqrtf(v[j]) * f.root + k.eps;
     w[j] = w[j] * f.decay - f.rate * m[j] * __builtin_amdgcn_rcpf(d);
   }
-  store<kF32, 8, FULL>(t.m, i, some, m);
-  store<kF32, 8, FULL>(t.v, i, some, v);
+  store<kF32, 8, FULL>(p[kM], i, some, m);
+  store<kF32, 8, FULL>(p[kV], i, some, v);
   if constexpr (MASTER) {
     settled<8>(w);
-    store<kF32, 8, FULL>(t.master, i, some, w);
+    store<kF32, 8, FULL>(p[4], i, some, w);
   }
-  store<PT, 8, FULL>(t.param, i, some, w);
+  store<PT, 8, FULL>(p[kParam], i, some, w);
 }
 
 template <int PT, int GT, bool MASTER>
-__global__ __launch_bounds__(kThreads) void step32(const Items items, const Factor* __restrict__ factors, const Rule k) {
-  const Item& t = items.item[find(items, blockIdx.x)];
-  const Factor f = factors[t.number];
+__global__ __launch_bounds__(kThreads) void step32(const Items<kPointers<MASTER, false>> items,
+                                                   const Factor* __restrict__ factors, const Rule k) {
+  const int which = find(items, blockIdx.x);
+  const Factor f = factors[items.number[which]];
   if (!f.go) return;
-  const int64_t at = (int64_t)((int)blockIdx.x - t.first) * kStepChunk;
+  void* const* const p = items.p[which];
+  const int64_t at = (int64_t)((int)blockIdx.x - items.first[which]) * kStepChunk, n = items.n[which];
 #pragma unroll 1
   for (int s = 0; s < kStepChunk / (8 * kThreads); ++s) {
-    const int64_t i = at + 8 * (s * kThreads + (int)threadIdx.x), left = t.n - i;
+    const int64_t i = at + 8 * (s * kThreads + (int)threadIdx.x), left = n - i;
     if (left <= 0) return;
     if (left >= 8)
-      eight32<PT, GT, MASTER, true>(t, f, k, i, 8);
+      eight32<PT, GT, MASTER, true>(p, f, k, i, 8);
     else
-      eight32<PT, GT, MASTER, false>(t, f, k, i, (int)left);
+      eight32<PT, GT, MASTER, false>(p, f, k, i, (int)left);
   }
 }
 
@@ -284,7 +308,7 @@ __device__ __forceinline__ u32x4 load_codes(const void* p, int64_t i, int some) 
 template <bool FULL>
 __device__ __forceinline__ void store_codes(void* p, int64_t i, int some, const u32x4& c) {
   if constexpr (FULL) {
-    __builtin_nontemporal_store(c, (Global<u32x4_any>*)(global<uint8_t>(p) + i));
+    *(Global<u32x4_any>*)(global<uint8_t>(p) + i) = c;
   } else {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
@@ -313,18 +337,18 @@ __device__ __forceinline__ float exact_root(float x) {
 // 16 elements a lane: a DPP row of 16 lanes has a scale's 256. The states are formed as the formula says it, each operation
 // rounded by itself (no fused ones) and the root correctly: a last bit decides now and then which code is stored.
 template <int PT, int GT, bool MASTER, bool FULL>
-__device__ __forceinline__ void sixteen8(const Item& t, const Factor& f, const Rule& k, int64_t i, int some, int64_t block,
+__device__ __forceinline__ void sixteen8(void* const* p, const Factor& f, const Rule& k, int64_t i, int some, int64_t block,
                                          int64_t blocks, uint32_t key) {
 #pragma clang fp contract(off)
-  Global<float>* const scales = global<float>(t.scales) + block;
+  Global<float>* const scales = global<float>(p[MASTER ? 5 : 4]) + block;
   const float ms = scales[0], rs = scales[blocks];
-  u32x4 mc = load_codes<FULL>(t.m, i, some), rc = load_codes<FULL>(t.v, i, some);
+  u32x4 mc = load_codes<FULL>(p[kM], i, some), rc = load_codes<FULL>(p[kV], i, some);
   float g[16], w[16], m[16], r[16];
-  load<GT, 16, FULL>(t.grad, i, some, g);
+  load<GT, 16, FULL>(p[kGrad], i, some, g);
   if constexpr (MASTER)
-    load<kF32, 16, FULL>(t.master, i, some, w);
+    load<kF32, 16, FULL>(p[4], i, some, w);
   else
-    load<PT, 16, FULL>(t.param, i, some, w);
+    load<PT, 16, FULL>(p[kParam], i, some, w);
   uint32_t mtop = 0, rtop = 0;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -344,9 +368,9 @@ __device__ __forceinline__ void sixteen8(const Item& t, const Factor& f, const R
   }
   if constexpr (MASTER) {
     settled<16>(w);
-    store<kF32, 16, FULL>(t.master, i, some, w);
+    store<kF32, 16, FULL>(p[4], i, some, w);
   }
-  store<PT, 16, FULL>(t.param, i, some, w);
+  store<PT, 16, FULL>(p[kParam], i, some, w);
   const float mscale = scale_of(row_max(mtop)), rscale = scale_of(row_max(rtop));
   if (threadIdx.x % 16 == 0) {
     scales[0] = mscale;
@@ -364,31 +388,34 @@ __device__ __forceinline__ void sixteen8(const Item& t, const Factor& f, const R
     mc[q] = four_codes(m + 4 * q);
     rc[q] = four_codes(r + 4 * q);
   }
-  store_codes<FULL>(t.m, i, some, mc);
-  store_codes<FULL>(t.v, i, some, rc);
+  store_codes<FULL>(p[kM], i, some, mc);
+  store_codes<FULL>(p[kV], i, some, rc);
 }
 
 template <int PT, int GT, bool MASTER>
-__global__ __launch_bounds__(kThreads) void step8(const Items items, const Factor* __restrict__ factors, const Rule k) {
-  const Item& t = items.item[find(items, blockIdx.x)];
-  const Factor f = factors[t.number];
+__global__ __launch_bounds__(kThreads) void step8(const Items<kPointers<MASTER, true>> items,
+                                                  const Factor* __restrict__ factors, const Rule k) {
+  const int which = find(items, blockIdx.x);
+  const Factor f = factors[items.number[which]];
   if (!f.go) return;
-  const int64_t at = (int64_t)((int)blockIdx.x - t.first) * kStepChunk, blocks = (t.n + kBlock - 1) / kBlock;
+  void* const* const p = items.p[which];
+  const int64_t n = items.n[which], blocks = (n + kBlock - 1) / kBlock;
+  const int64_t at = (int64_t)((int)blockIdx.x - items.first[which]) * kStepChunk;
   const uint32_t key = with_word(f.key, (uint32_t)(at >> 32));
 #pragma unroll 1
   for (int s = 0; s < kStepChunk / (16 * kThreads); ++s) {
-    const int64_t i = at + 16 * (s * kThreads + (int)threadIdx.x), block = i / kBlock, left = t.n - i;
+    const int64_t i = at + 16 * (s * kThreads + (int)threadIdx.x), block = i / kBlock, left = n - i;
     if (block >= blocks) return;  // whole rows of lanes
     // A row of lanes is whole or not as one, for its maximum.
-    if ((block + 1) * kBlock <= t.n)
-      sixteen8<PT, GT, MASTER, true>(t, f, k, i, 16, block, blocks, key);
+    if ((block + 1) * kBlock <= n)
+      sixteen8<PT, GT, MASTER, true>(p, f, k, i, 16, block, blocks, key);
     else
-      sixteen8<PT, GT, MASTER, false>(t, f, k, i, (int)max((int64_t)0, left), block, blocks, key);
+      sixteen8<PT, GT, MASTER, false>(p, f, k, i, (int)max((int64_t)0, left), block, blocks, key);
   }
 }
 
 bool known_dtype(int32_t dt) { return dt == kBf16 || dt == kF16 || dt == kF32; }
-constexpr int64_t kMostElements = INT64_C(1) << 36;
+constexpr int64_t kMostElements = INT64_C(1) << 35;
 constexpr int32_t kMostTensors = 1 << 20;
 
 int check_sizes(const int64_t* sizes, int32_t count) {
@@ -408,10 +435,10 @@ constexpr int64_t kMostGroups = (INT64_C(1) << 24) - 1;
 static_assert(kMostElements / kStepChunk <= kMostGroups, "a tensor fits a launch");
 
 // Calls launch(items, workgroups) for the listed tensors, in as few launches as their number and sizes allow.
-// add(i, item) fills an item's pointers, or says that tensor i has no part.
-template <typename Add, typename Launch>
+// add(i, pointers) fills in tensor i's pointers, or says that it has no part.
+template <int P, typename Add, typename Launch>
 int in_launches(const int64_t* sizes, int32_t count, int64_t chunk, Add&& add, Launch&& launch) {
-  Items t;
+  Items<P> t;
   t.count = 0;
   int64_t groups = 0;
   auto flush = [&] {
@@ -421,13 +448,13 @@ int in_launches(const int64_t* sizes, int32_t count, int64_t chunk, Add&& add, L
   };
   for (int32_t i = 0; i < count; ++i) {
     const int64_t need = ceil_div(sizes[i], chunk);
-    Item it{};
-    if (!need || !add(i, it)) continue;
-    if (t.count == kItems || groups + need > kMostGroups) flush();
-    it.n = sizes[i];
-    it.first = (int32_t)groups;
-    it.number = i;
-    t.item[t.count++] = it;
+    void* p[P];
+    if (!need || !add(i, p)) continue;
+    if (t.count == Items<P>::kMost || groups + need > kMostGroups) flush();
+    for (int k = 0; k < P; ++k) t.p[t.count][k] = p[k];
+    t.n[t.count] = sizes[i];
+    t.first[t.count] = (int32_t)groups;
+    t.number[t.count++] = i;
     groups += need;
   }
   flush();
@@ -440,21 +467,62 @@ int64_t norm_groups(const int64_t* sizes, int32_t count) {
   return n;
 }
 
-template <int BITS, int PT, int GT, bool MASTER>
-auto step_kernel() {
-  if constexpr (BITS == 8)
-    return step8<PT, GT, MASTER>;
-  else
-    return step32<PT, GT, MASTER>;
+// The parts of the gradients' norm.
+int launch_norm_parts(const void* const* grads, const int64_t* sizes, int32_t count, float* part, int32_t dtype, hipStream_t st,
+                      int64_t* parts) {
+  *parts = 0;
+  return in_launches<1>(
+      sizes, count, kNormChunk,
+      [&](int32_t i, void** p) {
+        p[0] = const_cast<void*>(grads[i]);
+        return grads[i] != nullptr;
+      },
+      [&](const Items<1>& t, unsigned groups) {
+        const auto kernel = dtype == kF16 ? norm_parts<kF16> : dtype == kF32 ? norm_parts<kF32> : norm_parts<kBf16>;
+        hipLaunchKernelGGL(kernel, dim3(groups), dim3(kThreads), 0, st, t, part + *parts);
+        *parts += groups;
+      });
 }
-using StepKernel = void (*)(const Items, const Factor*, const Rule);
+
+struct Lists {
+  void* const* params;
+  const void* const* grads;
+  void *const *m, *const *v;
+  float *const *masters, *const *scales;
+  const int64_t* sizes;
+  int32_t count;
+  const Factor* factors;
+  Rule rule;
+  hipStream_t st;
+};
+
+template <int BITS, int PT, int GT, bool MASTER>
+int launch_step(const Lists& a) {
+  constexpr int P = kPointers<MASTER, BITS == 8>;
+  return in_launches<P>(
+      a.sizes, a.count, kStepChunk,
+      [&](int32_t i, void** p) {
+        p[kParam] = a.params[i], p[kGrad] = const_cast<void*>(a.grads[i]), p[kM] = a.m[i], p[kV] = a.v[i];
+        if (MASTER) p[4] = a.masters[i];
+        if (BITS == 8) p[P - 1] = a.scales[i];
+        return a.grads[i] != nullptr;
+      },
+      [&](const Items<P>& t, unsigned groups) {
+        if constexpr (BITS == 8)
+          hipLaunchKernelGGL((step8<PT, GT, MASTER>), dim3(groups), dim3(kThreads), 0, a.st, t, a.factors, a.rule);
+        else
+          hipLaunchKernelGGL((step32<PT, GT, MASTER>), dim3(groups), dim3(kThreads), 0, a.st, t, a.factors, a.rule);
+      });
+}
+template <int BITS, int PT, int GT>
+int launch_step(const Lists& a) {
+  return a.masters ? launch_step<BITS, PT, GT, true>(a) : launch_step<BITS, PT, GT, false>(a);
+}
 template <int BITS>
-StepKernel step_kernel(int32_t pt, int32_t gt, bool master) {
-  if (pt == kF32) return step_kernel<BITS, kF32, kF32, false>();
-  if (pt == kBf16 && gt == kBf16) return master ? step_kernel<BITS, kBf16, kBf16, true>() : step_kernel<BITS, kBf16, kBf16, false>();
-  if (pt == kBf16) return master ? step_kernel<BITS, kBf16, kF32, true>() : step_kernel<BITS, kBf16, kF32, false>();
-  if (gt == kF16) return master ? step_kernel<BITS, kF16, kF16, true>() : step_kernel<BITS, kF16, kF16, false>();
-  return master ? step_kernel<BITS, kF16, kF32, true>() : step_kernel<BITS, kF16, kF32, false>();
+int launch_step(const Lists& a, int32_t pt, int32_t gt) {
+  if (pt == kF32) return launch_step<BITS, kF32, kF32, false>(a);
+  if (pt == kBf16) return gt == kBf16 ? launch_step<BITS, kBf16, kBf16>(a) : launch_step<BITS, kBf16, kF32>(a);
+  return gt == kF16 ? launch_step<BITS, kF16, kF16>(a) : launch_step<BITS, kF16, kF32>(a);
 }
 
 bool in_range(double v) { return std::isfinite(v) && std::fabs(v) <= 3.0e38; }
@@ -481,33 +549,24 @@ int krsi_grad_norm(const void* const* grads, const int64_t* sizes, int32_t count
   if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
   float* part = (float*)workspace;
   const hipStream_t st = as_stream(stream);
-  int64_t at = 0;
-  rc = in_launches(
-      sizes, count, kNormChunk,
-      [&](int32_t i, Item& t) {
-        t.grad = grads[i];
-        return grads[i] != nullptr;
-      },
-      [&](const Items& t, unsigned groups) {
-        const auto kernel = dtype == kF16 ? norm_parts<kF16> : dtype == kF32 ? norm_parts<kF32> : norm_parts<kBf16>;
-        hipLaunchKernelGGL(kernel, dim3(groups), dim3(kThreads), 0, st, t, part + at);
-        at += groups;
-      });
+  int64_t parts;
+  rc = launch_norm_parts(grads, sizes, count, part, dtype, st, &parts);
   if (rc != KRSI_OK) return rc;
-  hipLaunchKernelGGL(norm_join, dim3(1), dim3(kJoin), 0, st, (const float*)part, at, norm);
+  hipLaunchKernelGGL(norm_join, dim3(1), dim3(kThreads), 0, st, (const float*)part, parts, norm);
   return launch_status();
 }
 
-size_t krsi_adamw_workspace_bytes(int32_t count) {
+size_t krsi_adamw_workspace_bytes(const int64_t* sizes, int32_t count) {
   using namespace krsi;
-  return count < 0 || count > kMostTensors ? 0 : align256((size_t)count * sizeof(Factor) + 1);
+  if (check_sizes(sizes, count) != KRSI_OK) return 0;
+  return align256((size_t)count * sizeof(Factor)) + align256((size_t)(norm_groups(sizes, count) + 1) * sizeof(float));
 }
 
 int krsi_adamw_step(void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
                     float* const* masters, float* const* scales, const int64_t* sizes, int32_t count, int32_t* steps,
                     const float* lr_at, float lr, double beta1, double beta2, float eps, float weight_decay,
-                    const float* norm, float max_norm, uint32_t seed, int32_t state_bits, int32_t dtype, int32_t grad_dtype,
-                    void* workspace, size_t workspace_bytes, void* stream) {
+                    float* norm, int32_t norm_given, float max_norm, uint32_t seed, int32_t state_bits, int32_t dtype,
+                    int32_t grad_dtype, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace krsi;
   if (!known_dtype(dtype) || (grad_dtype != dtype && grad_dtype != kF32) || (masters && dtype == kF32))
     return KRSI_ERR_UNSUPPORTED;
@@ -515,11 +574,11 @@ int krsi_adamw_step(void* const* params, const void* const* grads, void* const* 
   int rc = check_sizes(sizes, count);
   if (rc != KRSI_OK) return rc;
   if ((!lr_at && !in_range(lr)) || !in_range(eps) || eps < 0 || !in_range(weight_decay) || !(beta1 >= 0 && beta1 < 1) ||
-      !(beta2 >= 0 && beta2 < 1) || (norm && !(max_norm >= 0)))
+      !(beta2 >= 0 && beta2 < 1) || (norm && !(max_norm >= 0)) || norm_given < 0 || norm_given > 1)
     return KRSI_ERR_BAD_SCALE;
   if (count == 0) return KRSI_OK;
   if (!params || !grads || !exp_avgs || !exp_avg_sqs || !steps) return KRSI_ERR_NULL_POINTER;
-  if (!workspace || workspace_bytes < krsi_adamw_workspace_bytes(count)) return KRSI_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < krsi_adamw_workspace_bytes(sizes, count)) return KRSI_ERR_WORKSPACE;
   if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
   // No parameter twice: two workgroups would write it.
   struct Span {
@@ -541,31 +600,28 @@ int krsi_adamw_step(void* const* params, const void* const* grads, void* const* 
     if (spans[i].begin < spans[i - 1].end) return KRSI_ERR_BAD_SHAPE;
 
   Factor* factors = (Factor*)workspace;
+  float* part = (float*)((char*)workspace + align256((size_t)count * sizeof(Factor)));
   const hipStream_t st = as_stream(stream);
+  const bool norm_here = norm && !norm_given;
+  int64_t parts = 0;
+  if (norm_here) {
+    rc = launch_norm_parts(grads, sizes, count, part, grad_dtype, st, &parts);
+    if (rc != KRSI_OK) return rc;
+  }
   for (int32_t base = 0; base < count; base += 32 * kMaskWords) {
     const int32_t here = std::min(count - base, 32 * kMaskWords);
     Mask mask{};
     for (int32_t i = 0; i < here; ++i)
       if (grads[base + i]) mask.word[i / 32] |= 1u << (i % 32);
     hipLaunchKernelGGL(step_factors, dim3((unsigned)ceil_div(here, kThreads)), dim3(kThreads), 0, st, mask, base, here, steps,
-                       factors, lr_at, lr, std::log(beta1), std::log(beta2), weight_decay, norm, max_norm, seed);
+                       factors, lr_at, lr, std::log(beta1), std::log(beta2), weight_decay, norm,
+                       norm_here ? (const float*)part : nullptr, parts, max_norm, seed);
   }
   rc = launch_status();
   if (rc != KRSI_OK) return rc;
   const Rule rule{(float)beta1, (float)(1 - beta1), (float)beta2, (float)(1 - beta2), eps};
-  const StepKernel kernel = state_bits == 8 ? step_kernel<8>(dtype, grad_dtype, masters != nullptr)
-                                            : step_kernel<32>(dtype, grad_dtype, masters != nullptr);
-  return in_launches(
-      sizes, count, kStepChunk,
-      [&](int32_t i, Item& t) {
-        t.param = params[i], t.grad = grads[i], t.m = exp_avgs[i], t.v = exp_avg_sqs[i];
-        t.master = masters ? masters[i] : nullptr;
-        t.scales = scales ? scales[i] : nullptr;
-        return grads[i] != nullptr;
-      },
-      [&](const Items& t, unsigned groups) {
-        hipLaunchKernelGGL(kernel, dim3(groups), dim3(kThreads), 0, st, t, (const Factor*)factors, rule);
-      });
+  const Lists a{params, grads, exp_avgs, exp_avg_sqs, masters, scales, sizes, count, factors, rule, st};
+  return state_bits == 8 ? launch_step<8>(a, dtype, grad_dtype) : launch_step<32>(a, dtype, grad_dtype);
 }
 
 }  // extern "C"

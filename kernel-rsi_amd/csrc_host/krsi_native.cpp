@@ -916,14 +916,14 @@ PyObject* py_adamw_step(Args a, Py_ssize_t n) {
     const c10::DeviceGuard guard(device);
     Tensor norm;
     if (norm_arg) norm = *norm_arg;
-    if (clip && !norm.defined()) norm = norm_of(grads, *params[0], gdt);
-    const size_t bytes = krsi_adamw_workspace_bytes((int)count);
+    if (clip && !norm.defined()) norm = at::empty({}, params[0]->options().dtype(at::kFloat));
+    const size_t bytes = krsi_adamw_workspace_bytes(sizes.data(), (int)count);
     Tensor ws = at::empty({(int64_t)bytes}, params[0]->options().dtype(at::kByte));
     forward_status(krsi_adamw_step(pp.data(), gp.data(), mp.data(), vp.data(), with_masters ? wp.data() : nullptr,
                                    with_scales ? sp.data() : nullptr, sizes.data(), (int)count, steps->data_ptr<int32_t>(),
                                    lr_at ? lr_at->data_ptr<float>() : nullptr, (float)lr, b1, b2, (float)eps, (float)decay,
-                                   norm.defined() ? norm.data_ptr<float>() : nullptr, (float)max_norm, (uint32_t)seed,
-                                   with_scales ? 8 : 32, dt, gdt, ws.data_ptr(), bytes, stream_of(*params[0])));
+                                   norm.defined() ? norm.data_ptr<float>() : nullptr, norm_arg ? 1 : 0, (float)max_norm,
+                                   (uint32_t)seed, with_scales ? 8 : 32, dt, gdt, ws.data_ptr(), bytes, stream_of(*params[0])));
     // What a graph has saved of these counts as changed.
     auto changed = [](const Tensor& t) {
       if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();

@@ -89,9 +89,9 @@ SIGNATURES = {
     "krsi_linear_8bit": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P]),
     "krsi_grad_norm_workspace_bytes": (_SZ, [_P, _I32]),
     "krsi_grad_norm": (ctypes.c_int, [_P, _P, _I32, _P, _P, _SZ, _I32, _P]),
-    "krsi_adamw_workspace_bytes": (_SZ, [_I32]),
+    "krsi_adamw_workspace_bytes": (_SZ, [_P, _I32]),
     "krsi_adamw_step": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _F32, ctypes.c_double, ctypes.c_double,
-                                       _F32, _F32, _P, _F32, ctypes.c_uint32, _I32, _I32, _I32, _P, _SZ, _P]),
+                                       _F32, _F32, _P, _I32, _F32, ctypes.c_uint32, _I32, _I32, _I32, _P, _SZ, _P]),
     "krsi_add_rmsnorm_bwd": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I32, _I32, _P]),
 }
 
@@ -913,21 +913,22 @@ def adamw_step(params: list, grads: list, exp_avgs: list, exp_avg_sqs: list, ste
     if norm is not None:
         _scalar_on_device("norm", norm, params[0])
     grads = [g if g is None else g.contiguous() for g in grads]
-    if max_norm is not None and norm is None:
-        norm = (grad_norm(grads) if any(g is not None for g in grads) else
-                torch.zeros((), device=params[0].device, dtype=torch.float32))
     count = len(params)
     # An empty tensor has no address; one that is not NULL says that its gradient is there.
     given = (_P * count)(*(None if g is None else g.data_ptr() or steps.data_ptr() for g in grads))
+    sizes = (_I64 * count)(*(p.numel() for p in params))
+    norm_given = norm is not None
     with torch.cuda.device(params[0].device):
-        nbytes = lib().krsi_adamw_workspace_bytes(count)
+        if max_norm is not None and norm is None:
+            norm = torch.empty((), device=params[0].device, dtype=torch.float32)
+        nbytes = lib().krsi_adamw_workspace_bytes(sizes, count)
         ws = torch.empty(max(nbytes, 1), device=params[0].device, dtype=torch.uint8)
         _check(lib().krsi_adamw_step(
             _pointers(params), given, _pointers(exp_avgs), _pointers(exp_avg_sqs),
             None if masters is None else _pointers(masters), None if scales is None else _pointers(scales),
-            (_I64 * count)(*(p.numel() for p in params)), count, _ptr(steps), _ptr(at), float(lr), beta1, beta2, eps,
-            weight_decay, _ptr(norm), 0.0 if max_norm is None else max_norm, seed & 0xffffffff, bits, dt, gdt, _ptr(ws),
-            nbytes, _stream(params[0])))
+            sizes, count, _ptr(steps), _ptr(at), float(lr), beta1, beta2, eps, weight_decay, _ptr(norm), int(norm_given),
+            0.0 if max_norm is None else max_norm, seed & 0xffffffff, bits, dt, gdt, _ptr(ws), nbytes,
+            _stream(params[0])))
     written = [steps] + [t for ts in (params, exp_avgs, exp_avg_sqs, masters, scales) if ts is not None for t in ts]
     torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
     return norm
