@@ -295,8 +295,8 @@ int krsi_linear_cross_entropy_bwd(const float* dout, const void* x, const void* 
                                   int32_t reduction, int32_t dtype, void* stream);
 
 /* ------------------------ residual addition with RMS norm (no counterpart)
- * The step between a layer's output and the next layer: r = T(x + residual), the stream that goes on, and its norm with
- * krsi_rmsnorm_fwd's rounding points, y = T(w * T(r * rstd)). x, residual, y, r [rows, n] contiguous and w [n], of T, any
+ * The step between a layer's output and the next layer: r = T(x + residual), the stream that goes on, and the norm of
+ * r in fp32, rounded once: y = T(w * r * rstd) (krsi_rmsnorm_fwd rounds r * rstd as well). x, residual, y, r [rows, n] contiguous and w [n], of T, any
  * alignment of the element; rstd [rows] fp32 for the backward, or NULL.
  * 8 bits: z = w * r * rstd in fp32, scale [rows] = max(max|z| / 448, 2^-120), q [rows, n] = e4m3 (OCP, one byte) of
  * z / scale, round to nearest even: z is about q * scale. residual and r may both be NULL: the norm of x. A row that

@@ -2,11 +2,12 @@
 // norm's output in the activations' type or in 8 bits with a scale per row; and rows brought to 8 bits alone.
 //   r = T(x + residual)                                   the stream that goes on, rounded once
 //   rstd = 1 / sqrt(sum(r^2) / n + eps)                   fp32, kept per row for the backward
-//   y = T(w * T(r * rstd))                                the rounding points of krsi_rmsnorm_fwd
+//   y = T(w * r * rstd)                                   in fp32, rounded once (krsi_rmsnorm_fwd rounds r * rstd as well, as
+//                                                         the formula that it stands in for does: 1.4 times the error)
 //   8 bits: z = w * r * rstd in fp32; scale = max(max|z| / 448, 2^-120); q = e4m3(z / scale)
 // Backward, of dy and dr (the gradients of y and r): one tensor, the gradient of x and of the residual alike,
-//   d = T(dr + rstd * (dn - r * rstd * sum(dn * r * rstd) / n)),  dn = float(T(dy * w))
-//   dw = T(sum over rows of dy * T(r * rstd))             fp32, per block, then a fixed-order column sum
+//   d = T(dr + rstd * (dn - r * rstd * sum(dn * r * rstd) / n)),  dn = dy * w
+//   dw = T(sum over rows of dy * r * rstd)                fp32, per block, then a fixed-order column sum
 // 448 is e4m3's largest value. The largest |z| is found as an unsigned integer, in whose order infinity and NaN come
 // last: a row that holds one has the scale infinity or NaN, and reads back as NaN throughout.
 //
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(threads_of(WPR)) void row_pass(
         El::unpack(v[k], f);
         El::unpack(wv[k], wf);
 #pragma unroll
-        for (int j = 0; j < E; ++j) f[j] = wf[j] * El::round(f[j] * rstd);
+        for (int j = 0; j < E; ++j) f[j] = wf[j] * (f[j] * rstd);
         const u32x4 ov = El::pack(f);
         store_chunk<RAGGED>(chunk_at<RAGGED, E>((typename El::T*)y + base, c, n), ov);
       }
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(4 * kWave) void row_scalar(
   } else {
     if (lane == 0 && stat) stat[row] = rstd;
     for (int c = lane; c < n; c += kWave)
-      ((typename El::T*)y)[base + c] = El::store(El::load(w[c]) * El::round(value(c) * rstd));
+      ((typename El::T*)y)[base + c] = El::store(El::load(w[c]) * (value(c) * rstd));
   }
 }
 
@@ -283,9 +284,8 @@ __global__ __launch_bounds__(threads_of(WPR)) void add_rms_bwd(
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const float nrm = xf[j] * here.rstd;
-        dw[k][j] += gf[j] * El::round(nrm);
-        const float dn = El::round(gf[j] * wf[j]);
-        sdot += RAGGED && j < dup ? 0.f : dn * nrm;
+        dw[k][j] += gf[j] * nrm;
+        sdot += RAGGED && j < dup ? 0.f : (gf[j] * wf[j]) * nrm;
       }
     }
     sdot = row_reduce<WPR>(sdot, red[it & 1], wave_sum, [](float a, float b) { return a + b; });
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(threads_of(WPR)) void add_rms_bwd(
           El::unpack(here.x[k], xf);
           El::unpack(wv[k], wf);
 #pragma unroll
-          for (int j = 0; j < E; ++j) o[j] = r1 * (El::round(gf[j] * wf[j]) - (xf[j] * r1) * sn);
+          for (int j = 0; j < E; ++j) o[j] = r1 * (gf[j] * wf[j] - (xf[j] * r1) * sn);
           if constexpr (DR) {
             float df[E];
             El::unpack(here.d[k], df);
@@ -370,8 +370,8 @@ __global__ __launch_bounds__(kWave) void add_rms_bwd_short(
       const int64_t i = row * n + min(j, n - 1);
       const float g = j < n ? El::load(dy[i]) : 0.f;
       xf[j] = El::load(r[i]) * r1;
-      dw[j] += g * El::round(xf[j]);
-      dn[j] = El::round(g * wf[j]);
+      dw[j] += g * xf[j];
+      dn[j] = g * wf[j];
       sdot += dn[j] * xf[j];
     }
     const float sn = sdot * inv_n;

@@ -1,9 +1,9 @@
 """add_rmsnorm and its 8-bit form on the GPU against the formulas in 64 bits.
 
 Tolerances: with u half a step of the type relative to the value (2^-8 bf16, 2^-11 fp16, 2^-24 fp32) and e a few
-roundings in 32 bits (n sums of a tree: 64 * 2^-24 covers rows of 16384), r is off by u |r|, y by 2 roundings of the
-type, (2 u + e) |y|. The gradient of row r: dn is rounded once (u |dn|), enters the row's mean (so that error is at most
-u times the mean of |dn nrm|) and is rounded with dr once more."""
+roundings in 32 bits (sums over a tree of 16384: 64 * 2^-24 covers it), r is off by u |r|, y by u |y| and the gradients by u
+of theirs; e of the sizes of the terms that are added, which may cancel, comes on top.
+"""
 import pytest
 import torch
 
@@ -45,7 +45,7 @@ def _verify(leaves, y, r, grads, dy, dr, dt, eps=EPS):
     _close(r, x + res, u * (x + res).abs() + tiny, "r")
     rr = r.detach().double()
     nrm = rr * torch.rsqrt(rr.square().mean(1, keepdim=True) + eps)
-    _close(y, nrm * w, (2 * u + u * u + E32) * (nrm * w).abs() + tiny * (1 + w.abs()), "y")
+    _close(y, nrm * w, (u + E32) * (nrm * w).abs() + tiny, "y")
     if grads is None:
         return
     g = torch.zeros_like(x) if dy is None else dy.double()
@@ -54,11 +54,11 @@ def _verify(leaves, y, r, grads, dy, dr, dt, eps=EPS):
     dn = g * w
     d = s + rstd * (dn - nrm * (dn * nrm).mean(1, keepdim=True))
     spread = (dn.abs() + nrm.abs() * (dn * nrm).abs().mean(1, keepdim=True)) * rstd
-    bound = u * d.abs() + (u + E32) * spread * (1 + u) + tiny * (1 + rstd * 2)
+    bound = u * d.abs() + E32 * (spread + s.abs()) + tiny
     _close(grads[0], d, bound, "dx")
     assert torch.equal(grads[0], grads[1])
     terms = (g * nrm).abs().sum(0)
-    _close(grads[2], (g * nrm).sum(0), u * (g * nrm).sum(0).abs() + (u + E32) * terms + tiny * (1 + g.abs().sum(0)), "dw")
+    _close(grads[2], (g * nrm).sum(0), u * (g * nrm).sum(0).abs() + E32 * terms + tiny, "dw")
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=ids)
@@ -84,14 +84,13 @@ def test_against_64_bits(rows, n, dt):
 @pytest.mark.parametrize("dt", DTYPES, ids=ids)
 @pytest.mark.parametrize("rows,n", [(6, 64), (5, 1001), (9, 4096), (3, 8191)])
 def test_as_the_norm_of_the_sum(rows, n, dt):
-    """What rmsnorm gives for the sum: y within the order of the row's sum (a rounding of the type at most)."""
+    """What rmsnorm gives for the sum, which rounds twice where this rounds once: three half steps apart at most."""
     log(f"add_rmsnorm as rmsnorm(x + residual) [{rows}, {n}] {dt}")
     x, res, w = _inputs(rows, n, dt)
     y, r = A.add_rmsnorm(x, res, w, EPS)
     assert torch.equal(r, x + res)
     want = R.rmsnorm(x + res, w, EPS).double()
-    # Where the reciprocal roots differ in their last bit, T(r * rstd) may take the next value.
-    _close(y, want, (2 * _u(dt) * 2 + E32) * want.abs() + 2 * torch.finfo(dt).tiny * torch.finfo(dt).eps, "y")
+    _close(y, want, (3 * _u(dt) * (1 + _u(dt)) + E32) * want.abs() + 2 * torch.finfo(dt).tiny * torch.finfo(dt).eps, "y")
 
 
 def _codes(z):
