@@ -89,11 +89,11 @@ class AdamW(torch.optim.Optimizer):
         self._lists = None
 
     def _new_state(self, p):
+        _hip._on_gpu(p)
+        _hip._dtype("parameters", p)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW makes its states in its first step, which must not be captured: a replay would "
                                "clear them")
-        _hip._on_gpu(p)
-        _hip._dtype("parameters", p)
         if not p.is_contiguous():
             raise ValueError(f"parameters must be contiguous, got one of shape {tuple(p.shape)} with strides {p.stride()}")
         state = {"step": torch.zeros((), device=p.device, dtype=torch.int32)}
