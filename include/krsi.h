@@ -320,7 +320,7 @@ int krsi_add_rmsnorm_bwd(const void* dy, const void* dr, const void* r, const vo
  *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
  *   w = w (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
  * in fp32. All arrays of pointers, and sizes, are HOST arrays of count entries, read before the call returns; the
- * tensors are of the device, dense, any alignment of the element, and no parameter overlaps another. params of T, grads
+ * tensors are of the device, dense, any alignment of the element, and nothing that is written overlaps (BAD_SHAPE). params of T, grads
  * of grad_dtype (T or fp32); masters (NULL: w is the parameter itself; not with fp32 params): w is the fp32
  * masters[i], params[i] its rounding. lr_at: the rate on the device, or NULL: lr. steps: [count] int32 on the device.
  * norm (device, or NULL): g is the gradient times min(1, max_norm / (norm + 1e-6)), and where *norm is not finite

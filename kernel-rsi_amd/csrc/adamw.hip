@@ -580,23 +580,28 @@ int krsi_adamw_step(void* const* params, const void* const* grads, void* const* 
   if (!params || !grads || !exp_avgs || !exp_avg_sqs || !steps) return KRSI_ERR_NULL_POINTER;
   if (!workspace || workspace_bytes < krsi_adamw_workspace_bytes(sizes, count)) return KRSI_ERR_WORKSPACE;
   if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
-  // No parameter twice: two workgroups would write it.
+  // Nothing that is written twice, or meets what else is written: two workgroups would race on it.
   struct Span {
     uintptr_t begin, end;
     bool operator<(const Span& o) const { return begin < o.begin; }
   };
-  const std::unique_ptr<Span[]> spans(new (std::nothrow) Span[count]);
+  const std::unique_ptr<Span[]> spans(new (std::nothrow) Span[5 * (size_t)count]);
   if (!spans) return KRSI_ERR_TOO_LARGE;
-  const int64_t width = dtype == kF32 ? 4 : 2;
-  int32_t used = 0;
+  const int64_t width = dtype == kF32 ? 4 : 2, state = state_bits / 8;
+  int64_t used = 0;
+  auto written = [&](const void* p, int64_t bytes) { spans[used++] = Span{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes}; };
   for (int32_t i = 0; i < count; ++i) {
     if (!grads[i] || !sizes[i]) continue;
     if (!params[i] || !exp_avgs[i] || !exp_avg_sqs[i] || (masters && !masters[i]) || (scales && !scales[i]))
       return KRSI_ERR_NULL_POINTER;
-    spans[used++] = Span{(uintptr_t)params[i], (uintptr_t)params[i] + sizes[i] * width};
+    written(params[i], sizes[i] * width);
+    written(exp_avgs[i], sizes[i] * state);
+    written(exp_avg_sqs[i], sizes[i] * state);
+    if (masters) written(masters[i], sizes[i] * 4);
+    if (scales) written(scales[i], 8 * ceil_div(sizes[i], kBlock));
   }
   std::sort(spans.get(), spans.get() + used);
-  for (int32_t i = 1; i < used; ++i)
+  for (int64_t i = 1; i < used; ++i)
     if (spans[i].begin < spans[i - 1].end) return KRSI_ERR_BAD_SHAPE;
 
   Factor* factors = (Factor*)workspace;

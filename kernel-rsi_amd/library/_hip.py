@@ -895,9 +895,10 @@ def _check_adamw(params, grads, exp_avgs, exp_avg_sqs, steps, masters, scales) -
             if scales[i].dtype != torch.float32 or scales[i].shape != (2, blocks) or not scales[i].is_contiguous():
                 raise ValueError(f"scales {i} must be contiguous float32 [2, {blocks}], got {scales[i].dtype} "
                                  f"{tuple(scales[i].shape)}")
-    spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+    written = [t for ts in (params, exp_avgs, exp_avg_sqs, masters, scales) if ts is not None for t in ts if t.numel()]
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written)
     if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
-        raise ValueError("a parameter overlaps another, or is in the list twice")
+        raise ValueError("parameters and states overlap, or one is in the lists twice")
     return dt, gdt, 32 if scales is None else 8
 
 

@@ -398,6 +398,9 @@ def test_refusals():
     p, s = kw["params"], kw["scales"]
     call(ValueError, "twice", params=[p[0], p[0]], grads=[kw["grads"][0]] * 2, exp_avgs=[kw["exp_avgs"][0]] * 2,
          exp_avg_sqs=[kw["exp_avg_sqs"][0]] * 2, masters=[kw["masters"][0]] * 2, scales=[s[0]] * 2)
+    call(ValueError, "twice", exp_avgs=[kw["exp_avgs"][1][:32].view(8, 4), kw["exp_avgs"][1]])
+    call(ValueError, "twice", scales=[s[1].flatten()[:2].view(2, 1), s[1]])
+    call(ValueError, "twice", exp_avgs=kw["exp_avgs"], exp_avg_sqs=kw["exp_avgs"])
     call(ValueError, "contiguous", params=[p[0].t().contiguous().t(), p[1]])
     call(TypeError, "exp_avg 0", exp_avgs=[t.float() for t in kw["exp_avgs"]])
     call(ValueError, "scales 1", scales=[s[0], s[1][:, :1].contiguous()])

@@ -86,7 +86,8 @@ def test_adamw_arguments():
     lib = _hip.lib()
     two, apart = _sizes(10, 300), _array(FAKE, FAKE + 4096)
     size = lib.krsi_adamw_workspace_bytes
-    ok = dict(params=apart, grads=apart, m=apart, v=apart, masters=NULL, scales=NULL, sizes=two, count=2, steps=FAKE, lr_at=NULL,
+    m, v = _array(FAKE + 8192, FAKE + 12288), _array(FAKE + 16384, FAKE + 20480)
+    ok = dict(params=apart, grads=apart, m=m, v=v, masters=NULL, scales=NULL, sizes=two, count=2, steps=FAKE, lr_at=NULL,
               lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, wd=0.01, norm=NULL, given=0, max_norm=0.0, seed=0, bits=32, dt=0, gdt=0,
               ws=FAKE, nb=1 << 20)
 
@@ -102,7 +103,9 @@ def test_adamw_arguments():
                    (dict(b2=-0.1), SCALE), (dict(b1=NAN), SCALE), (dict(norm=FAKE, max_norm=-1.0), SCALE),
                    (dict(norm=FAKE, max_norm=NAN), SCALE), (dict(given=2), SCALE), (dict(ws=NULL), WS), (dict(nb=16), WS),
                    (dict(ws=FAKE + 4), ALIGN), (dict(params=_array(FAKE, FAKE)), SHAPE),
-                   (dict(params=_array(FAKE + 16, FAKE)), SHAPE), (dict(params=_array(FAKE, NULL)), NULLP),
+                   (dict(params=_array(FAKE + 16, FAKE)), SHAPE), (dict(m=apart), SHAPE), (dict(v=m), SHAPE),
+                   (dict(m=_array(FAKE + 8192, FAKE + 8200)), SHAPE), (dict(masters=v), SHAPE),
+                   (dict(scales=_array(FAKE + 30000, FAKE + 30004), bits=8), SHAPE), (dict(params=_array(FAKE, NULL)), NULLP),
                    (dict(m=_array(NULL, FAKE)), NULLP), (dict(v=_array(FAKE, NULL)), NULLP),
                    (dict(masters=_array(FAKE, NULL)), NULLP), (dict(scales=_array(FAKE, NULL), bits=8), NULLP)]:
         assert call(**kw) == rc, kw
