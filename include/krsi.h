@@ -345,9 +345,11 @@ int krsi_adamw_step(void* const* params, const void* const* grads, void* const* 
  * out[m, n] = T( x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] ), sums in fp32: x [rows, k] and w [f, k] e4m3 (OCP, one
  * byte), contiguous, 16-byte aligned, as krsi_quantize_rows and krsi_add_rmsnorm_8bit write them, with an fp32 scale per
  * row; out [rows, f] of T (out_dtype: any KRSI_DTYPE), any alignment of the element. A NaN code or scale makes its row or
- * column NaN. Limits: k % 16 == 0, k <= 2^20, rows and f <= 2^23 (ceil(rows / 64) ceil(f / 128) <= 2^23). */
-int krsi_linear_8bit(const void* x, const void* w, const float* x_scale, const float* w_scale, void* out, int64_t rows,
-                     int32_t k, int32_t f, int32_t out_dtype, void* stream);
+ * column NaN. Limits: k % 16 == 0, k <= 2^20, rows and f <= 2^23 (ceil(rows / 64) ceil(f / 128) <= 2^23).
+ * workspace: *_workspace_bytes, scratch (0 for most sizes; fp32 parts of the sum where few outputs meet a long one). */
+size_t krsi_linear_8bit_workspace_bytes(int64_t rows, int32_t k, int32_t f);
+int krsi_linear_8bit(const void* x, const void* w, const float* x_scale, const float* w_scale, void* out, void* workspace,
+                     size_t workspace_bytes, int64_t rows, int32_t k, int32_t f, int32_t out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,7 +18,9 @@
 // waited for every request in flight.
 // Few rows (64 at most): bound by the weight, which goes from memory to registers, once. One row, [8192, 4096]: 7.5 us (4.5
 // TB/s; a read of as much takes 5.4), [28672, 8192]: 39.5 (5.9 TB/s). 33 to 64 rows: bound by the reads of x by every
-// workgroup through L2 (x [64, 8192], w [8192, 8192]: 26.5 us).
+// workgroup through L2 (x [48, 4112], w [5633, 4112]: 10.3 us).
+// Few outputs of a long sum: the sum in parts, whose fp32 sums a second launch adds in their order (x [64, 8192], w [8192, 8192]:
+// 27.2 us by the kernel for few rows, 33.2 by whole tiles, 19.9 in four parts; [512, 8192] x [1024, 8192]: 20.5 -> 15.0).
 #include "chunks.h"
 #include "krsi_device.h"
 #include "krsi_internal.h"
@@ -104,10 +106,12 @@ struct Tile8 {
   static_assert(kA / 16 % kThreads == 0 && kB / 16 % kThreads == 0 && kStep % 16 == 0 && RB % 4 == 0, "whole requests");
 };
 
-template <int OT, int WM, int WN, int RB, int CB, int DA, int DB>
+// SPLIT: a tile of a part of the sum, whose fp32 sums go to `part` [splits, rows, F]; a workgroup takes one.
+template <int OT, int WM, int WN, int RB, int CB, int DA, int DB, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN, (Tile8<WM, WN, RB, CB, DA, DB>::kPerCu * WM * WN / 4)) void
 linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w, const float* __restrict__ xs,
-                   const float* __restrict__ ws, typename Elem<OT>::T* __restrict__ out, int rows, int K, int F, const Tiles tiles) {
+                   const float* __restrict__ ws, typename Elem<OT>::T* __restrict__ out, float* __restrict__ part, int rows, int K, int F,
+                   const Tiles tiles) {
   using Tl = Tile8<WM, WN, RB, CB, DA, DB>;
   __shared__ __attribute__((aligned(512))) uint8_t lds[Tl::kLds];
   uint8_t *const As = lds, *const Bs = lds + DA * Tl::kA;
@@ -188,6 +192,7 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
   Source nxt = source(next);
   // Stage s of this tile, or where it is past its end, of the next one (after the last tile some tile's, not used).
   auto ahead = [&](int s) {
+    if constexpr (SPLIT) return stage_of(cur, here.s0 + s < here.s1 ? here.s0 + s : tiles.stages);
     const bool in = s < tiles.stages;
     return stage_of(Source{in ? cur.a : nxt.a, in ? cur.b : nxt.b}, in ? s : s - tiles.stages);
   };
@@ -211,7 +216,8 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
     for (int i = 0; i < RB; ++i)
 #pragma unroll
       for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < tiles.stages; ++k) {
+    const int stages = SPLIT ? here.s1 - here.s0 : tiles.stages;
+    for (int k = 0; k < stages; ++k) {
       const Stage db = ahead(k + DB), da = ahead(k + DA);
 #pragma unroll
       for (int p = 0; p < RB / 2 - 1; ++p) pair(p, da, db);
@@ -224,6 +230,27 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
       a0 = a1, b0 = b1;
       a1 = a1 + Tl::kA == DA * Tl::kA ? 0 : a1 + Tl::kA;
       b1 = b1 + Tl::kB == DB * Tl::kB ? 0 : b1 + Tl::kB;
+    }
+    if constexpr (SPLIT) {
+      float* at = part + ((int64_t)here.split * rows + here.m0 + 16 * RB * wru) * F + here.n0 + 16 * CB * wcu;
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const bool live = l16 < rows - here.m0 - 16 * RB * wru - 16 * i;
+#pragma unroll
+        for (int j = 0; j < CB; ++j) {
+          const int left = F - here.n0 - 16 * CB * wcu - 4 * g - 16 * j;
+          float* p = at + (l16 * F + 4 * g) + 16 * j;
+          if (live && left >= 4) {
+            *reinterpret_cast<f32x4_any*>(p) = acc[i][j];
+          } else if (live) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r < left) p[r] = acc[i][j][r];
+          }
+        }
+        at += 16 * (int64_t)F;
+      }
+      break;
     }
     // All scales first: loaded one by one between the stores, each waited for the requests in flight before it as well. What
     // lies past an end reads as zero. Places are a wave's own plus a lane's 32-bit offset: with a pointer for each row, the
@@ -275,6 +302,30 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
     nxt = source(next);
   }
   wait_and_sync();  // the unused requests land before the workgroup's LDS is released
+}
+
+// The parts' sum, in their order, times the scales: four columns a thread.
+template <int OT>
+__global__ __launch_bounds__(256) void linear_8bit_join(const float* __restrict__ part, const float* __restrict__ xs,
+                                                        const float* __restrict__ ws, typename Elem<OT>::T* __restrict__ out,
+                                                        int rows, int F, int splits) {
+  const int col = 4 * (blockIdx.x * 256 + (int)threadIdx.x), row = blockIdx.y;
+  if (col >= F) return;
+  const int64_t at = (int64_t)row * F + col, step = (int64_t)rows * F;
+  const float x = xs[row];
+  if (col + 4 <= F) {
+    f32x4 sum = *reinterpret_cast<const f32x4_any*>(part + at);
+    for (int p = 1; p < splits; ++p) sum += *reinterpret_cast<const f32x4_any*>(part + p * step + at);
+    const f32x4 w = *reinterpret_cast<const f32x4_any*>(ws + col);
+    const float s[4] = {w[0], w[1], w[2], w[3]};
+    store_out<OT>(out + at, 4, sum, x, s);
+  } else {
+    for (int r = 0; r < F - col; ++r) {
+      float sum = part[at + r];
+      for (int p = 1; p < splits; ++p) sum += part[p * step + at + r];
+      out[at + r] = Elem<OT>::store(sum * x * ws[col + r]);
+    }
+  }
 }
 
 // ----------------------------------------------------------------- few rows
@@ -344,6 +395,7 @@ struct Call {
   const uint8_t *x, *w;
   const float *xs, *ws;
   void* out;
+  float* part;
   int64_t rows;
   int K, F;
   hipStream_t st;
@@ -359,43 +411,89 @@ int launch_few(const Call& c) {
   return launch_status();
 }
 
-template <int OT, int WM, int WN, int RB, int CB, int DA, int DB>
-int launch_stream(const Call& c) {
+template <int OT, int WM, int WN, int RB, int CB, int DA, int DB, bool SPLIT = false>
+int launch_stream(const Call& c, int splits = 1) {
   using Tl = Tile8<WM, WN, RB, CB, DA, DB>;
   Tiles t;
   t.nrb = (int)ceil_div(c.rows, Tl::kRows);
   t.ncb = (int)ceil_div(c.F, Tl::kCols);
-  t.splits = 1;
-  t.per = t.stages = (int)ceil_div(c.K, kStage8);
+  t.splits = splits;
+  t.stages = (int)ceil_div(c.K, kStage8);
+  t.per = (int)ceil_div(t.stages, splits);
   if ((int64_t)t.nrb * t.ncb > (1 << 23)) return KRSI_ERR_UNSUPPORTED;
-  t.total = t.nrb * t.ncb;
+  t.total = t.nrb * t.ncb * splits;
   // The stream reaches one tile ahead, DA stages: with fewer every workgroup takes one tile.
-  const int resident = t.stages >= DA ? kCus * Tl::kPerCu : t.total;
-  hipLaunchKernelGGL((linear_8bit_stream<OT, WM, WN, RB, CB, DA, DB>), dim3((unsigned)(t.total < resident ? t.total : resident)),
-                     dim3(Tl::kThreads), 0, c.st, c.x, c.w, c.xs, c.ws, (typename Elem<OT>::T*)c.out, (int)c.rows, c.K, c.F, t);
+  const int resident = !SPLIT && t.stages >= DA ? kCus * Tl::kPerCu : t.total;
+  hipLaunchKernelGGL((linear_8bit_stream<OT, WM, WN, RB, CB, DA, DB, SPLIT>),
+                     dim3((unsigned)(t.total < resident ? t.total : resident)), dim3(Tl::kThreads), 0, c.st, c.x, c.w, c.xs,
+                     c.ws, (typename Elem<OT>::T*)c.out, c.part, (int)c.rows, c.K, c.F, t);
+  const int rc = launch_status();
+  if (!SPLIT || rc != KRSI_OK) return rc;
+  hipLaunchKernelGGL((linear_8bit_join<OT>), dim3((unsigned)ceil_div(c.F, 1024), (unsigned)c.rows), dim3(256), 0, c.st,
+                     (const float*)c.part, c.xs, c.ws, (typename Elem<OT>::T*)c.out, (int)c.rows, c.F, splits);
   return launch_status();
+}
+
+// Which kernel a size takes, by its cost in hundredths of a us as measured.
+enum Kind { kFew, kLarge, kMid, kSmall };
+struct Plan {
+  Kind kind;
+  int splits;
+};
+Plan plan_of(int64_t rows, int K, int F) {
+  const int64_t stages = ceil_div(K, kStage8);
+  // Rounds of the chip, each its stages and an end. Two workgroups of the smaller tiles share a CU, and a round that gives each
+  // CU one at most takes about half of a full one.
+  auto cost = [&](int64_t tiles, int64_t depth, int full, int full_end, int part, int part_end) {
+    const int64_t per = full == part ? kCus : 2 * kCus, last = tiles % per;
+    return tiles / per * (full * depth + full_end) +
+           (last == 0 ? 0 : last > kCus ? full * depth + full_end : part * depth + part_end);
+  };
+  auto tiles = [&](int m, int n) { return ceil_div(rows, m) * ceil_div(F, n); };
+  Plan best{kLarge, 1};
+  int64_t least = cost(tiles(256, 256), stages, 133, 800, 133, 800);
+  auto consider = [&](int64_t c, Plan p) {
+    if (c < least) least = c, best = p;
+  };
+  consider(cost(tiles(128, 128), stages, 102, 400, 55, 340), Plan{kMid, 1});
+  consider(cost(tiles(64, 128), stages, 72, 350, 38, 290), Plan{kSmall, 1});
+  // The sum in parts, each four stages at least, where that fills the chip: the parts' bytes both ways and a launch come on top.
+  for (int s = 2; s <= 16; s *= 2) {
+    const int64_t per = ceil_div(stages, s), parts = ceil_div(stages, per);
+    if (per < 4 || tiles(64, 128) * parts > 2 * kCus) break;
+    consider(cost(tiles(64, 128) * parts, per, 72, 350, 38, 290) + 300 + rows * F * parts * 8 / 40000, Plan{kSmall, (int)parts});
+  }
+  if (rows <= kFewRows) {
+    const bool two = rows > 32 || (rows > 16 && F >= 32 * kCus);  // column blocks to a workgroup
+    const int64_t wide = two ? 32 : 16, each = rows <= 16 ? 8 : rows > 32 ? 9 * rows / 16 : two ? 26 : 17;
+    consider(250 + ceil_div(F, wide * kCus) * stages * each, Plan{kFew, 1});
+  }
+  return best;
 }
 
 template <int OT>
 int launch(const Call& c) {
-  // Two column blocks share their reads of x where that leaves a workgroup for each CU ([32, 4096] x [4096, 4096]: 8.0 us with
-  // one, 9.5 with two; x [8192, 4096]: 13.4, 10.3).
-  if (c.rows <= 16) return launch_few<OT, 1, 1, 2>(c);
-  if (c.rows <= 32) return c.F >= 32 * kCus ? launch_few<OT, 2, 2, 2>(c) : launch_few<OT, 2, 1, 2>(c);
-  if (c.rows <= kFewRows) return launch_few<OT, 4, 2, 1>(c);
-  const int64_t stages = ceil_div(c.K, kStage8);
-  // The tile by its cost in hundredths of a us, as measured: rounds of the chip, each its stages and an end. Two workgroups of
-  // the smaller tiles share a CU, and a round that gives each CU one at most takes about half of a full one.
-  auto cost = [&](int rows, int cols, int full, int full_end, int part, int part_end) {
-    const int64_t tiles = ceil_div(c.rows, rows) * ceil_div(c.F, cols), per = full == part ? kCus : 2 * kCus, last = tiles % per;
-    return tiles / per * (full * stages + full_end) +
-           (last == 0 ? 0 : last > kCus ? full * stages + full_end : part * stages + part_end);
-  };
-  const int64_t large = cost(256, 256, 133, 800, 133, 800), mid = cost(128, 128, 102, 400, 55, 340),
-                small = cost(64, 128, 72, 350, 38, 290);
-  if (large <= mid && large <= small) return launch_stream<OT, 2, 4, 8, 4, 3, 2>(c);
-  if (mid <= small) return launch_stream<OT, 2, 2, 4, 4, 3, 2>(c);
-  return launch_stream<OT, 1, 4, 4, 2, 3, 3>(c);
+  const Plan p = plan_of(c.rows, c.K, c.F);
+  switch (p.kind) {
+    case kFew:
+      // Two column blocks share their reads of x where that leaves a workgroup for each CU ([32, 4096] x [4096, 4096]: 8.0 us
+      // with one, 9.5 with two; x [8192, 4096]: 13.4, 10.3).
+      if (c.rows <= 16) return launch_few<OT, 1, 1, 2>(c);
+      if (c.rows <= 32) return c.F >= 32 * kCus ? launch_few<OT, 2, 2, 2>(c) : launch_few<OT, 2, 1, 2>(c);
+      return launch_few<OT, 4, 2, 1>(c);
+    case kLarge: return launch_stream<OT, 2, 4, 8, 4, 3, 2>(c);
+    case kMid: return launch_stream<OT, 2, 2, 4, 4, 3, 2>(c);
+    default:
+      return p.splits > 1 ? launch_stream<OT, 1, 4, 4, 2, 3, 3, true>(c, p.splits) : launch_stream<OT, 1, 4, 4, 2, 3, 3>(c);
+  }
+}
+
+int check_sizes(int64_t rows, int32_t k, int32_t f) {
+  if (rows < 0 || k <= 0 || f <= 0) return KRSI_ERR_BAD_SHAPE;
+  // Byte offsets into a tile stay below 2^31, a launch's threads below 2^32.
+  if (k % 16 || k > (1 << 20) || rows > (1 << 23) || f > (1 << 23)) return KRSI_ERR_UNSUPPORTED;
+  if (ceil_div(rows, 64) * ceil_div(f, 128) > (1 << 23)) return KRSI_ERR_UNSUPPORTED;
+  return KRSI_OK;
 }
 
 }  // namespace
@@ -403,18 +501,26 @@ int launch(const Call& c) {
 
 extern "C" {
 
-int krsi_linear_8bit(const void* x, const void* w, const float* x_scale, const float* w_scale, void* out, int64_t rows,
-                     int32_t k, int32_t f, int32_t out_dtype, void* stream) {
+size_t krsi_linear_8bit_workspace_bytes(int64_t rows, int32_t k, int32_t f) {
+  using namespace krsi;
+  if (check_sizes(rows, k, f) != KRSI_OK || rows == 0) return 0;
+  const Plan p = plan_of(rows, k, f);
+  return p.splits > 1 ? align256((size_t)p.splits * rows * f * sizeof(float)) : 0;
+}
+
+int krsi_linear_8bit(const void* x, const void* w, const float* x_scale, const float* w_scale, void* out, void* workspace,
+                     size_t workspace_bytes, int64_t rows, int32_t k, int32_t f, int32_t out_dtype, void* stream) {
   using namespace krsi;
   if (out_dtype != kBf16 && out_dtype != kF16 && out_dtype != kF32) return KRSI_ERR_UNSUPPORTED;
-  if (rows < 0 || k <= 0 || f <= 0) return KRSI_ERR_BAD_SHAPE;
-  // Byte offsets into a tile stay below 2^31, element offsets of rows and columns below 2^31.
-  if (k % 16 || k > (1 << 20) || rows > (1 << 23) || f > (1 << 23)) return KRSI_ERR_UNSUPPORTED;
-  if (ceil_div(rows, 64) * ceil_div(f, 128) > (1 << 23)) return KRSI_ERR_UNSUPPORTED;
+  const int rc = check_sizes(rows, k, f);
+  if (rc != KRSI_OK) return rc;
   if (rows == 0) return KRSI_OK;
   if (!x || !w || !x_scale || !w_scale || !out) return KRSI_ERR_NULL_POINTER;
   if (!aligned16(x) || !aligned16(w)) return KRSI_ERR_MISALIGNED;
-  const Call c{(const uint8_t*)x, (const uint8_t*)w, x_scale, w_scale, out, rows, k, f, as_stream(stream)};
+  const size_t need = krsi_linear_8bit_workspace_bytes(rows, k, f);
+  if (need && (!workspace || workspace_bytes < need)) return KRSI_ERR_WORKSPACE;
+  if (need && !aligned16(workspace)) return KRSI_ERR_MISALIGNED;
+  const Call c{(const uint8_t*)x, (const uint8_t*)w, x_scale, w_scale, out, (float*)workspace, rows, k, f, as_stream(stream)};
   return out_dtype == kF16 ? launch<kF16>(c) : out_dtype == kF32 ? launch<kF32>(c) : launch<kBf16>(c);
 }
 

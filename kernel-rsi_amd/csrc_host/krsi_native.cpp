@@ -797,8 +797,11 @@ PyObject* py_linear_8bit(Args a, Py_ssize_t n) {
     variable_list rows = x_scale ? variable_list{*x, *x_scale} : rows_in_8bit(*x);
     const at::ScalarType types[] = {at::kBFloat16, at::kHalf, at::kFloat};
     Tensor out = at::empty({x->size(0), w->size(0)}, x->options().dtype(types[out_dtype]));
+    const size_t bytes = krsi_linear_8bit_workspace_bytes(x->size(0), (int)x->size(1), (int)w->size(0));
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes}, x->options().dtype(at::kByte));
     forward_status(krsi_linear_8bit(rows[0].data_ptr(), w->data_ptr(), rows[1].data_ptr<float>(),
-                                    w_scale->data_ptr<float>(), out.data_ptr(), x->size(0), (int)x->size(1),
+                                    w_scale->data_ptr<float>(), out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, x->size(0), (int)x->size(1),
                                     (int)w->size(0), (int)out_dtype, stream_of(*x)));
     return out;
   });

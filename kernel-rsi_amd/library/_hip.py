@@ -86,7 +86,8 @@ SIGNATURES = {
     "krsi_add_rmsnorm_8bit": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I32, _F32, _I32, _P]),
     "krsi_quantize_rows": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _P]),
     "krsi_add_rmsnorm_bwd_workspace_bytes": (_SZ, [_I64, _I32]),
-    "krsi_linear_8bit": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P]),
+    "krsi_linear_8bit_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "krsi_linear_8bit": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _SZ, _I64, _I32, _I32, _I32, _P]),
     "krsi_grad_norm_workspace_bytes": (_SZ, [_P, _I32]),
     "krsi_grad_norm": (ctypes.c_int, [_P, _P, _I32, _P, _P, _SZ, _I32, _P]),
     "krsi_adamw_workspace_bytes": (_SZ, [_P, _I32]),
@@ -808,8 +809,10 @@ def linear_8bit(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale
     x, w, x_scale, w_scale = _aligned(x), _aligned(w), x_scale.contiguous(), w_scale.contiguous()
     out = torch.empty(rows, f, device=x.device, dtype=out_dtype)
     if rows:
-        _check(lib().krsi_linear_8bit(_ptr(x), _ptr(w), _ptr(x_scale), _ptr(w_scale), _ptr(out), rows, k, f,
-                                      DTYPE_CODES[out_dtype], _stream(x)))
+        nbytes = lib().krsi_linear_8bit_workspace_bytes(rows, k, f)
+        ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
+        _check(lib().krsi_linear_8bit(_ptr(x), _ptr(w), _ptr(x_scale), _ptr(w_scale), _ptr(out), _ptr(ws), nbytes, rows, k,
+                                      f, DTYPE_CODES[out_dtype], _stream(x)))
     return out
 
 

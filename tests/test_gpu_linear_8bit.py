@@ -40,11 +40,12 @@ def _verify(out, x, w, ws, xs):
 
 
 # Each kernel's sizes: few rows (1 to 16, 17 to 32, to 64), tiles of 64, 128 and 256 rows and columns with ends inside them;
-# summed lengths of one stage, of part of one, of many; outputs of one column, of odd widths.
+# summed lengths of one stage, of part of one, of many, in parts where few outputs meet a long one; outputs of one column, of odd widths.
 SHAPES = [(1, 16, 1), (1, 128, 16), (3, 144, 17), (16, 1040, 33), (1, 4096, 8192), (17, 256, 48), (32, 2064, 100),
           (33, 1024, 31), (64, 4112, 321), (65, 16, 1), (65, 128, 128), (70, 112, 130), (100, 272, 200), (129, 1024, 257),
           (200, 128, 3000), (300, 400, 700), (1000, 1024, 5632), (513, 2048, 2049), (2100, 528, 4100), (4096, 96, 4352),
-          (4097, 1040, 4097), (2048, 4096, 8192)]
+          (4097, 1040, 4097), (2048, 4096, 8192),
+          (100, 2048, 130), (65, 4112, 5), (130, 8192, 1027), (200, 16400, 257), (64, 8192, 2048), (300, 4096, 700)]
 
 
 @pytest.mark.parametrize("rows,k,f", SHAPES)
@@ -121,8 +122,9 @@ def test_layouts_and_neighbours():
         wide = torch.stack([ws, ws], 1)[:, 0]
         assert torch.equal(L.linear_8bit(x, w, wide, x_scale=xs), want)
         guard = torch.full((rows * f + 64,), 7.0, device="cuda", dtype=torch.bfloat16)
+        assert _hip.lib().krsi_linear_8bit_workspace_bytes(rows, 144, f) == 0
         _hip._check(_hip.lib().krsi_linear_8bit(x.data_ptr(), w.data_ptr(), xs.data_ptr(), ws.data_ptr(),
-                                                guard[1:].data_ptr(), rows, 144, f, 0,
+                                                guard[1:].data_ptr(), None, 0, rows, 144, f, 0,
                                                 torch.cuda.current_stream().cuda_stream))
         torch.cuda.synchronize()
         assert torch.equal(guard[1:1 + rows * f].view(rows, f), want)

@@ -60,7 +60,7 @@ def test_add_rmsnorm_arguments():
 
 
 def test_linear_8bit_arguments():
-    ok = dict(x=FAKE, w=FAKE, xs=FAKE, ws=FAKE, out=FAKE, rows=4, k=64, f=32, dt=0)
+    ok = dict(x=FAKE, w=FAKE, xs=FAKE, ws=FAKE, out=FAKE, work=NULL, nb=0, rows=4, k=64, f=32, dt=0)
 
     def call(**kw):
         return _hip.lib().krsi_linear_8bit(*{**ok, **kw}.values(), NULL)
@@ -72,6 +72,11 @@ def test_linear_8bit_arguments():
         assert call(**kw) == rc, kw
     for name in ("x", "w", "xs", "ws", "out"):
         assert call(**{name: NULL}) == NULLP, name
+    # Few outputs of a long sum: parts of it, two at least, in fp32.
+    size, long = _hip.lib().krsi_linear_8bit_workspace_bytes, dict(rows=200, k=8192, f=512)
+    need = size(*long.values())
+    assert need >= 2 * 200 * 512 * 4 and size(8192, 8192, 8192) == 0 and size(0, 64, 64) == size(4, 40, 4) == size(-1, 64, 4) == 0
+    assert call(**long) == WS and call(**long, work=FAKE, nb=need - 1) == WS and call(**long, work=FAKE + 4, nb=need) == ALIGN
 
 
 def _array(*ptrs):
