@@ -155,6 +155,7 @@ __global__ __launch_bounds__(kThreads) void norm_parts(const Items<1> items, flo
 // The root of the parts' sum, in every thread of the workgroup: the same bits wherever it is formed.
 __device__ __forceinline__ float joined(const float* __restrict__ part, int64_t n, double* red) {
   double s = 0;
+#pragma unroll 16
   for (int64_t i = threadIdx.x; i < n; i += kThreads) s += part[i];
   red[threadIdx.x] = s;
   __syncthreads();

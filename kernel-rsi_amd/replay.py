@@ -54,6 +54,7 @@ def run_one(name: str) -> dict:
 
 def _selftest_step(name: str):
     """(leaves, fn, cotangent) of the module's selftest shape, for the host-cost probe."""
+    import add_rmsnorm
     import embedding
     import geglu
     import linear_cross_entropy
@@ -67,6 +68,9 @@ def _selftest_step(name: str):
     if name == "rmsnorm":
         x, w = rnd(4096, 1024), (1 + rnd(1024, scale=0.02, dtype=torch.float32)).to(torch.bfloat16)
         return [x, w], lambda a, b: rmsnorm.rmsnorm(a, b, 1e-6), rnd(4096, 1024)
+    if name == "add_rmsnorm":
+        leaves = [rnd(4096, 1024), rnd(4096, 1024), (1 + rnd(1024, scale=0.02, dtype=torch.float32)).to(torch.bfloat16)]
+        return leaves, lambda a, b, c: add_rmsnorm.add_rmsnorm(a, b, c, 1e-6)[0], rnd(4096, 1024)
     if name == "geglu":
         return [rnd(2048, 5632)], geglu.geglu, rnd(2048, 2816)
     if name == "relpos_attention":
