@@ -11,9 +11,10 @@
 // A root above zero stays above zero, which keeps m / s within bounds. The random numbers are a function of the seed, the
 // step, the tensor's number and the element's alone: multiplicative hashing (Knuth) with xor-shifts between.
 //
-// Bound by HBM: 28 bytes a parameter with 16-bit weights and gradients, masters and 32-bit states; 16 with 8-bit ones. What a
-// launch needs to know of each tensor comes as an argument by value, so nothing is copied to the device beforehand and
-// a captured launch holds its own copy.
+// Bound by HBM: 28 bytes a parameter with 16-bit weights and gradients, masters and 32-bit states; 16 with 8-bit ones. 302 M
+// such parameters: 1590 us (5.3 TB/s; plain streams, three read and two written, 5.0) and 930 (5.2); their norm 87 (6.8).
+// 145 small tensors: 26 us of kernels, four launches. What a launch needs to know of each tensor comes as an argument by
+// value, so nothing is copied to the device beforehand and a captured launch holds its own copy.
 #include <algorithm>
 #include <cmath>
 #include <memory>
@@ -28,8 +29,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;        // elements that share a scale
-constexpr int kStepChunk = 4096;   // elements per workgroup of the step
-constexpr int kNormChunk = 16384;  // and of the norm
+// Elements per workgroup of the step: one pass of its lanes with 8-bit states, two with 32-bit ones (302 M parameters, 8-bit
+// states: 951 us, workgroups of 8192 1045; both before stores went through the caches).
+constexpr int kStepChunk = 4096;
+constexpr int kNormChunk = 16384;  // and of the norm, all of whose loads are out at once
 
 // The tensors of a launch, as many as the 4 KB of its arguments hold: P pointers each, its first workgroup of the launch and
 // its number in the list.

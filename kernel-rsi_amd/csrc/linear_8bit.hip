@@ -12,9 +12,9 @@
 // Many rows: one stream of stages per workgroup, 128 summed indices each, memory -> LDS directly, persistent over tiles. A
 // stage's products go in pairs of row blocks; its barrier stands before the last pair, whose operands are in registers by
 // then. LDS holds the stages that DA and DB say, so that a request has that many stages' time (256 x 256 tiles: three of x and
-// two of w, all of a CU's 160 KB). What bounds it at 8192 x 8192 x 8192: the card's power limit (random rows 409 us, 2690 TFLOP/s,
-// at 1.9 GHz with the matrix cores busy 64 % of the cycles; zeros 360; the vendor's library 404 with one scale for all, 455
-// with a scale per row). A step that cost: registers that went to memory in the loop, and a load waited for in it, each
+// two of w, all of a CU's 160 KB). 8192 x 8192 x 8192, random rows: 409 to 427 us (2690 to 2575 TFLOP/s), the matrix cores busy 66 % of the cycles
+// at 1.94 GHz, the waves waiting in 27 %. In turn with it on one card at 424: the vendor's library 345 with one scale for all, 387 with a
+// scale per row; zeros 333, 256 and 315; in another run 415 to 472, 404 and 455. A step that cost: registers that went to memory in the loop, and a load waited for in it, each
 // waited for every request in flight.
 // Few rows (64 at most): bound by the weight, which goes from memory to registers, once. One row, [8192, 4096]: 7.5 us (4.5
 // TB/s; a read of as much takes 5.4), [28672, 8192]: 39.5 (5.9 TB/s). 33 to 64 rows: bound by the reads of x by every

@@ -5,7 +5,8 @@ torch.optim.Optimizer on them.
 For every tensor with a gradient, in fp32, with t the count of its steps:
   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
   w = w (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
-All tensors of a call are changed in place by one launch for each 60 of them, and one before it. The counts live on
+All tensors of a call are changed in place by one launch for each 60 to 80 of them, after one that forms
+the step's factors; clipping adds the gradients' norm, a launch for each 160. The counts live on
 the device (steps, int32, one per tensor), and the rate may (a float32 tensor of one number), so a captured step goes on
 counting and can be given another rate between replays.
   masters    fp32 copies of 16-bit parameters: they are stepped, the parameters are their rounding. Without them steps

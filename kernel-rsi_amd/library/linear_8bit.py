@@ -4,7 +4,8 @@ quantize_rows(x2d) -> (q, scale), which brings a weight, once, and other rows to
 w is [F, K] float8_e4m3fn (the layout of nn.Linear's weight) with an fp32 scale per row, as quantize_rows(weight) gives
 them. x [rows, K] is float8_e4m3fn with its rows' scales, x_scale, as add_rmsnorm_8bit and quantize_rows give them; or it is
 bf16, fp16 or fp32 without, and brought to 8 bits first, row by row. The codes' products are summed in fp32 on the matrix
-cores, times both scales, and rounded once to out_dtype (None: x's type, bf16 for codes).
+cores, which cut each eight neighbouring ones at 2^-13 of the largest (1e-4 of an output of random rows); the sum is
+scaled by both and rounded once to out_dtype (None: x's type, bf16 for codes).
 
 quantize_rows: the scale makes a row's largest value 448, the type's largest, and codes are rounded to nearest even; a
 code is off by 2^-4 of its value at most, or 2^-10 of the scale below 2^-6 of it. A row that holds an infinity or NaN reads back

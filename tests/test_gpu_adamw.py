@@ -182,7 +182,8 @@ def test_off_alignment_and_neighbours(dt, bits):
 
 @pytest.mark.parametrize("dt", DTYPES, ids=ids)
 def test_grad_norm(dt):
-    """fp32 sums of 576 terms or fewer a lane, then fp64: 2^-24 times the longest chain, half of it through the root."""
+    """At most 20 fp32 additions and a square on a term's way (nine squares a lane's sum, three sums of eight, a wave, a
+    workgroup), then fp64: 21 times 2^-24 of the sum, half of it through the root and one rounding more; 64 is above it."""
     log(f"grad_norm {dt}")
     grads = [seeded(s, i, dtype=dt) for i, s in enumerate(SHAPES + [(65536,), (65537,), (3, 70001)])]
     want = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
