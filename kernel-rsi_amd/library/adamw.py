@@ -66,7 +66,7 @@ class AdamW(torch.optim.Optimizer):
     max_norm: of all gradients together. A group's lr may be a float32 tensor on the device. The state of a parameter:
     step, exp_avg, exp_avg_sq and, where they are used, master and scales.
     The first step makes the states, so it cannot be captured into a graph; later ones can, with gradients that stay
-    where they are."""
+    where they are. States that are loaded, or of a group added later, are others than a captured step's: capture again."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32, masters=None,
                  max_norm=None, seed=0):
@@ -108,7 +108,8 @@ class AdamW(torch.optim.Optimizer):
         return state
 
     def _made_lists(self):
-        """Per group, the lists of a call for each device and type of its parameters. The steps of a list are one
+        """Per group, the lists of a call for each device and type of its parameters, those with a master (loaded states
+        may be of either kind) apart from those without. The steps of a list are one
         tensor, of which each parameter's state has a view."""
         lists = []
         for group in self.param_groups:
@@ -116,7 +117,7 @@ class AdamW(torch.optim.Optimizer):
             for p in group["params"]:
                 if not self.state[p]:
                     self.state[p] = self._new_state(p)
-                parts.setdefault((p.device, p.dtype), []).append(p)
+                parts.setdefault((p.device, p.dtype, "master" in self.state[p]), []).append(p)
             for ps in parts.values():
                 states = [self.state[p] for p in ps]
                 steps = torch.stack([s["step"].reshape(()) for s in states])

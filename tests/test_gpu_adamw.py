@@ -555,3 +555,25 @@ def test_class_mixed_types_scheduler_and_closure():
     opt.param_groups[1]["params"][0].grad = torch.ones(5, device="cuda")
     opt.step()
     assert int(opt.state[opt.param_groups[1]["params"][0]]["step"]) == 1 and int(opt.state[ps[0]]["step"]) == 3
+
+
+def test_class_masters_of_some_parameters():
+    """States loaded without a master beside new ones that have one, in one group: each parameter is stepped by its own kind."""
+    log("AdamW, masters of some parameters")
+    a = _model()
+    opt = W.AdamW(a, lr=1e-2, masters=False)
+    _set_grads(a, 0)
+    opt.step()
+    saved = opt.state_dict()
+    for missing in (0, 2):  # the one without a state first, and last
+        b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+        other = W.AdamW(b, lr=1e-2)
+        other.load_state_dict({**saved, "state": {i: s for i, s in saved["state"].items() if i != missing}})
+        before = [p.detach().clone() for p in b]
+        _set_grads(b, 5)
+        other.step()
+        assert ["master" in other.state[p] for p in b] == [i == missing for i in range(3)]
+        assert all(not torch.equal(p, q) for p, q in zip(b, before))
+        master = other.state[b[missing]]["master"]
+        assert torch.equal(master.to(torch.bfloat16), b[missing]) and not torch.equal(master, b[missing].float())
+        assert [int(other.state[p]["step"]) for p in b] == [1 if i == missing else 2 for i in range(3)]
