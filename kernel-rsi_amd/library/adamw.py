@@ -163,14 +163,14 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """States keep the types that they were saved with (torch would cast them to the parameters')."""
+        if any(("scales" in state) != (self.state_bits == 8) for state in state_dict["state"].values()):
+            raise ValueError(f"the saved states are not those of {self.state_bits} bits")
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
             if i not in state_dict["state"]:
                 continue
             self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
-            if ("scales" in self.state[p]) != (self.state_bits == 8):
-                raise ValueError(f"the saved states are not those of {self.state_bits} bits")
         self._lists = None
 
 

@@ -577,3 +577,22 @@ def test_class_masters_of_some_parameters():
         master = other.state[b[missing]]["master"]
         assert torch.equal(master.to(torch.bfloat16), b[missing]) and not torch.equal(master, b[missing].float())
         assert [int(other.state[p]["step"]) for p in b] == [1 if i == missing else 2 for i in range(3)]
+
+
+def test_class_refused_states_change_nothing():
+    log("AdamW, refused states")
+    a, b = _model(), _model()
+    opt, other = W.AdamW(a, lr=1e-2, state_bits=8), W.AdamW(b, lr=3e-3)
+    for ps, o in ((a, opt), (b, other)):
+        _set_grads(ps, 0)
+        o.step()
+    before = {p: {k: t.clone() for k, t in other.state[p].items()} for p in b}
+    with pytest.raises(ValueError, match="bits"):
+        other.load_state_dict(opt.state_dict())
+    assert other.param_groups[0]["lr"] == 3e-3
+    for p in b:
+        assert other.state[p].keys() == before[p].keys()
+        assert all(t.dtype == before[p][k].dtype and torch.equal(t, before[p][k]) for k, t in other.state[p].items())
+    _set_grads(b, 1)
+    other.step()
+    assert [int(other.state[p]["step"]) for p in b] == [2, 2, 2]
