@@ -12,9 +12,9 @@
 // Many rows: one stream of stages per workgroup, 128 summed indices each, memory -> LDS directly, persistent over tiles. A
 // stage's products go in pairs of row blocks; its barrier stands before the last pair, whose operands are in registers by
 // then. LDS holds the stages that DA and DB say, so that a request has that many stages' time (256 x 256 tiles: three of x and
-// two of w, all of a CU's 160 KB). 8192 x 8192 x 8192, random rows: 409 to 427 us (2690 to 2575 TFLOP/s), the matrix cores busy 66 % of the cycles
-// at 1.94 GHz, the waves waiting in 27 %. In turn with it on one card at 424: the vendor's library 345 with one scale for all, 387 with a
-// scale per row; zeros 333, 256 and 315; in another run 415 to 472, 404 and 455. A step that cost: registers that went to memory in the loop, and a load waited for in it, each
+// two of w, all of a CU's 160 KB). 8192 x 8192 x 8192, random rows: 365 to 391 us (3010 to 2810 TFLOP/s), the matrix cores busy 77 % of
+// the cycles at 1.86 GHz. In turn with it on one card at 391: the vendor's library 342 with one scale for all, 384 with a scale per
+// row; zeros 285, 256 and 317. A step that cost: registers that went to memory in the loop, and a load waited for in it, each
 // waited for every request in flight.
 // Few rows (64 at most): bound by the weight, which goes from memory to registers, once. One row, [8192, 4096]: 7.5 us (4.5
 // TB/s; a read of as much takes 5.4), [28672, 8192]: 39.5 (5.9 TB/s). 33 to 64 rows: bound by the reads of x by every
@@ -102,7 +102,7 @@ struct Tile8 {
   static constexpr int kStep = kThreads / 8;  // staged rows from request to request
   // At the barrier that lets the next stage be read: requests that may still be on their way, those for later ones.
   static constexpr int kLater = (DB - 2) * kDma + (DA > DB ? kADma : 0);
-  static_assert(DA >= DB && DB >= 2 && DA * kDma < 64, "requests that the wait can count");
+  static_assert(DB >= 2 && (DA == DB || (DA == 3 && DB == 2)) && RB >= 4 && DA * kDma < 64, "requests that the wait can count");
   static_assert(kA / 16 % kThreads == 0 && kB / 16 % kThreads == 0 && kStep % 16 == 0 && RB % 4 == 0, "whole requests");
 };
 
@@ -162,12 +162,16 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
   auto read_b = [&](int j, int at) { b[j] = frag(Bs + at, CB * wc + j); };
   f32x4 acc[RB][CB];
 
-  // Stage k's buffers are at a0 and b0, the next one's at a1 and b1.
-  int a0 = 0, a1 = Tl::kA, b0 = 0, b1 = Tl::kB;
+  // Stage k's buffers are at a0 and b0, the next one's at a1 and b1, the one's before at ap.
+  int ap = (DA - 1) * Tl::kA, a0 = 0, a1 = Tl::kA, b0 = 0, b1 = Tl::kB;
   // The products of row blocks 2 p and 2 p + 1, b by b. The reads of the pair after, and with the last pair, which only
-  // needs registers, the next stage's first pair and each b after its last use, and the requests: of w's stage k + DB first,
-  // then of x's stage k + DA.
+  // needs registers, the next stage's first pair and each b after its last use, and the requests of w's stage k + DB. Where x's
+  // ring is the longer one, its stage k - 1 + DA is asked for over the pairs before, into the buffer of stage k - 1, else
+  // stage k + DA after w's: requests all in the last pair got in each other's way (8192 x 8192 x 8192: 407 us, so 379;
+  // in that pair's first half 416). Equal rings would lose a stage's time by it (200 x 4096 x 4096: 12.1 us, 12.9).
   constexpr int kProducts = 2 * CB;
+  constexpr bool kSpread = DA > DB;
+  constexpr int kAhead = kSpread ? DA - 1 : DA;
   auto pair = [&](int p, const Stage& da, const Stage& db) {
     const bool last = p == RB / 2 - 1;
 #pragma unroll
@@ -177,9 +181,13 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
       if (m < 2) read_a(last ? m : 2 * p + 2 + m, last ? a1 : a0);
       if (last && m % 2 == 1) read_b(j, b1);
 #pragma unroll
-      for (int q = 0; q < Tl::kDma; ++q)
-        if (last && q * kProducts / Tl::kDma == m)
-          request(q >= Tl::kBDma, q < Tl::kBDma ? db : da, q < Tl::kBDma ? b0 : a0, q < Tl::kBDma ? q : q - Tl::kBDma);
+      for (int q = 0; q < Tl::kBDma; ++q)
+        if (last && q * kProducts / (kSpread ? Tl::kBDma : Tl::kDma) == m) request(false, db, b0, q);
+#pragma unroll
+      for (int q = 0; q < Tl::kADma; ++q)
+        if (kSpread ? !last && q * (RB / 2 - 1) * kProducts / Tl::kADma == p * kProducts + m
+                    : last && (Tl::kBDma + q) * kProducts / Tl::kDma == m)
+          request(true, da, kSpread ? ap : a0, q);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -204,9 +212,10 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
     for (int i = 0; i < Tl::kBDma; ++i)
       if (s < DB) request(false, st, s * Tl::kB, i);
 #pragma unroll
-    for (int i = 0; i < Tl::kADma; ++i) request(true, st, s * Tl::kA, i);
+    for (int i = 0; i < Tl::kADma; ++i)
+      if (s < kAhead) request(true, st, s * Tl::kA, i);
   }
-  wait_for<(DB - 1) * Tl::kDma + (DA - DB) * Tl::kADma>();
+  wait_for<(DB - 1) * Tl::kDma + (kAhead - DB) * Tl::kADma>();
   read_a(0, 0);
   read_a(1, 0);
 #pragma unroll
@@ -218,7 +227,7 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
       for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int stages = SPLIT ? here.s1 - here.s0 : tiles.stages;
     for (int k = 0; k < stages; ++k) {
-      const Stage db = ahead(k + DB), da = ahead(k + DA);
+      const Stage db = ahead(k + DB), da = ahead(k + kAhead);
 #pragma unroll
       for (int p = 0; p < RB / 2 - 1; ++p) pair(p, da, db);
       // After an epilogue, whose loads and stores are counted too, everything is waited for.
@@ -227,7 +236,7 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
       else
         wait_for<Tl::kLater>();
       pair(RB / 2 - 1, da, db);
-      a0 = a1, b0 = b1;
+      ap = a0, a0 = a1, b0 = b1;
       a1 = a1 + Tl::kA == DA * Tl::kA ? 0 : a1 + Tl::kA;
       b1 = b1 + Tl::kB == DB * Tl::kB ? 0 : b1 + Tl::kB;
     }
@@ -252,47 +261,48 @@ linear_8bit_stream(const uint8_t* __restrict__ x, const uint8_t* __restrict__ w,
       }
       break;
     }
-    // All scales first: loaded one by one between the stores, each waited for the requests in flight before it as well. What
-    // lies past an end reads as zero. Places are a wave's own plus a lane's 32-bit offset: with a pointer for each row, the
-    // loop's registers went to memory and back.
+    // All scales first: loaded one by one between the stores, each waited for the requests in flight before it as well. One to a
+    // lane, and given round by the lanes' exchange: in each lane that needs them they took seven registers more. What lies
+    // past an end reads as zero. Places are a wave's own plus a lane's 32-bit offset: with a pointer for each row, the loop's
+    // registers went to memory and back.
     const int m = here.m0 + 16 * RB * wru, n = here.n0 + 16 * CB * wcu;
-    float sx[RB], sw[CB][4];
+    constexpr int kX = (16 * RB + 63) / 64, kW = (16 * CB + 63) / 64;
+    uint32_t lx[kX], lw[kW];
 #pragma unroll
-    for (int i = 0; i < RB; ++i)
-      sx[i] = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b32(xsr, opaque(4 * (m + l16) + 64 * i), 0, 0));
+    for (int i = 0; i < kX; ++i) lx[i] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(xsr, opaque(4 * (m + lane) + 256 * i), 0, 0);
 #pragma unroll
-    for (int j = 0; j < CB; ++j) {
-      const u32x4 q = __builtin_amdgcn_raw_buffer_load_b128(wsr, opaque(4 * (n + 4 * g) + 64 * j), 0, 0);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) sw[j][r] = __uint_as_float(q[r]);
-    }
+    for (int j = 0; j < kW; ++j) lw[j] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(wsr, opaque(4 * (n + lane) + 256 * j), 0, 0);
     // Used here, on every path: a load that some path leaves unused is waited for where its register is next written, which
     // was in the loop over the stages, in each of them and for all requests in flight.
 #pragma unroll
-    for (int i = 0; i < RB; ++i) asm volatile("" : "+v"(sx[i]));
+    for (int i = 0; i < kX; ++i) asm volatile("" : "+v"(lx[i]));
 #pragma unroll
-    for (int j = 0; j < CB; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) asm volatile("" : "+v"(sw[j][r]));
+    for (int j = 0; j < kW; ++j) asm volatile("" : "+v"(lw[j]));
+    const int lx4 = opaque(4 * l16), lw4 = opaque(16 * g);  // the lanes' addresses, four bytes each
+    auto from = [&](uint32_t v, int l) { return __uint_as_float((uint32_t)__builtin_amdgcn_ds_bpermute(l, (int)v)); };
     typename Elem<OT>::T* at = out + (int64_t)m * F + n;
     const bool wide = OT != kF32 && n + 16 * CB <= F;  // all of the wave's columns are there
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      const bool live = l16 < rows - m - 16 * i;
-      if constexpr (OT != kF32) {
-        if (wide) {  // every lane has its part in the exchange, also of a row that is not there
+    for (int j = 0; j < CB; j += 2) {
+      __builtin_amdgcn_sched_barrier(0);  // not all exchanges before the first store
+      float sw[2][4];
 #pragma unroll
-          for (int j = 0; j < CB; j += 2)
-            store_two<OT>(live, at + (l16 * F + 16 * (g & 1) + 8 * (g >> 1)) + 16 * j, acc[i][j], acc[i][j + 1], sx[i], sw[j],
-                          sw[j + 1]);
+      for (int r = 0; r < 8; ++r) sw[r / 4][r % 4] = from(lw[j / 4], lw4 + 64 * (j % 4 + r / 4) + 4 * (r % 4));
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const float sx = from(lx[i / 4], lx4 + 64 * (i % 4));
+        const bool live = l16 < rows - m - 16 * i;
+        typename Elem<OT>::T* to = at + (int64_t)(16 * i) * F + 16 * j;
+        if constexpr (OT != kF32) {
+          if (wide)  // every lane has its part in the exchange, also of a row that is not there
+            store_two<OT>(live, to + (l16 * F + 16 * (g & 1) + 8 * (g >> 1)), acc[i][j], acc[i][j + 1], sx, sw[0], sw[1]);
+        }
+        if (!wide) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            if (live) store_out<OT>(to + (l16 * F + 4 * g) + 16 * q, F - n - 4 * g - 16 * (j + q), acc[i][j + q], sx, sw[q]);
         }
       }
-      if (!wide) {
-#pragma unroll
-        for (int j = 0; j < CB; ++j)
-          if (live) store_out<OT>(at + (l16 * F + 4 * g) + 16 * j, F - n - 4 * g - 16 * j, acc[i][j], sx[i], sw[j]);
-      }
-      at += 16 * (int64_t)F;
     }
     v += gridDim.x;
     if (v >= tiles.total) break;
