@@ -66,7 +66,8 @@ class AdamW(torch.optim.Optimizer):
     max_norm: of all gradients together. A group's lr may be a float32 tensor on the device. The state of a parameter:
     step, exp_avg, exp_avg_sq and, where they are used, master and scales.
     The first step makes the states, so it cannot be captured into a graph; later ones can, with gradients that stay
-    where they are. States that are loaded, or of a group added later, are others than a captured step's: capture again."""
+    where they are, and so can the first after states for all parameters were loaded. A copy's first step cannot. Loaded
+    states, or those of a group added later, are others than a captured step's: capture again."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32, masters=None,
                  max_norm=None, seed=0):
@@ -92,9 +93,6 @@ class AdamW(torch.optim.Optimizer):
     def _new_state(self, p):
         _hip._on_gpu(p)
         _hip._dtype("parameters", p)
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW makes its states in its first step, which must not be captured: a replay would "
-                               "clear them")
         if not p.is_contiguous():
             raise ValueError(f"parameters must be contiguous, got one of shape {tuple(p.shape)} with strides {p.stride()}")
         state = {"step": torch.zeros((), device=p.device, dtype=torch.int32)}
@@ -127,6 +125,15 @@ class AdamW(torch.optim.Optimizer):
                                                   for k in ("exp_avg", "exp_avg_sq", "master", "scales"))))
         return lists
 
+    def _make_lists(self):
+        """Not in a capture, whose replays would clear new states and form the steps from the old ones again."""
+        params = [p for group in self.param_groups for p in group["params"]]
+        _hip._on_gpu(*params)
+        if params and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW makes its states and their counts in its first step, which must not be captured: a "
+                               "replay would set them back")
+        self._lists = self._made_lists()
+
     def _norm(self):
         """Of all gradients, on the device of the first."""
         parts = {}
@@ -145,7 +152,7 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         if self._lists is None:
-            self._lists = self._made_lists()
+            self._make_lists()
         norm = None
         if self.max_norm is not None and any(p.grad is not None for g in self.param_groups for p in g["params"]):
             norm = self._norm()
@@ -172,6 +179,8 @@ class AdamW(torch.optim.Optimizer):
                 continue
             self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
         self._lists = None
+        if all(self.state.get(p) for g in self.param_groups for p in g["params"]):
+            self._lists = self._made_lists()  # so that the next step may be captured
 
 
 def reference(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01):

@@ -596,3 +596,32 @@ def test_class_refused_states_change_nothing():
     _set_grads(b, 1)
     other.step()
     assert [int(other.state[p]["step"]) for p in b] == [2, 2, 2]
+
+
+def test_class_captured_right_after_loading():
+    """The first step after a load, captured: its replays count on and equal eager steps."""
+    log("AdamW captured after a load")
+    a, b = _model(), _model()
+    opt = W.AdamW(a, lr=1e-2, state_bits=8, max_norm=1.0)
+    other = W.AdamW(b, lr=1e-2, state_bits=8, max_norm=1.0)
+    for step in range(2):
+        _set_grads(a, step)
+        opt.step()
+    for p, q in zip(a, b):
+        q.data.copy_(p)
+        q.grad = p.grad.clone()
+    other.load_state_dict(opt.state_dict())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other.step()
+    for i in range(4):
+        for p, q in zip(a, b):
+            p.grad.copy_(seeded(tuple(p.shape), 50 + i, std=0.1))
+            q.grad.copy_(p.grad)
+        graph.replay()
+        opt.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), i
+        assert [int(other.state[q]["step"]) for q in b] == [3 + i] * 3
+    del graph
