@@ -66,8 +66,9 @@ class AdamW(torch.optim.Optimizer):
     max_norm: of all gradients together. A group's lr may be a float32 tensor on the device. The state of a parameter:
     step, exp_avg, exp_avg_sq and, where they are used, master and scales.
     The first step makes the states, so it cannot be captured into a graph; later ones can, with gradients that stay
-    where they are, and so can the first after states for all parameters were loaded. A copy's first step cannot. Loaded
-    states, or those of a group added later, are others than a captured step's: capture again."""
+    where they are, and so can the first after states for all parameters were loaded. A copy's first step cannot. Each step
+    goes by what `param_groups` and `state` hold at the time. Where that is not what a captured step had (loaded or replaced
+    states, another group or parameter), capture again, after a step that is not captured."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32, masters=None,
                  max_norm=None, seed=0):
@@ -75,12 +76,8 @@ class AdamW(torch.optim.Optimizer):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
         self.state_bits, self.masters, self.max_norm, self.seed = state_bits, masters, max_norm, seed
-        self._lists = None
+        self._lists, self._held, self._ids = None, [], []
         super().__init__(params, {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay})
-
-    def add_param_group(self, group):
-        super().add_param_group(group)
-        self._lists = None
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits, "masters": self.masters, "max_norm": self.max_norm,
@@ -88,7 +85,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._lists = None
+        self._lists, self._held, self._ids = None, [], []
 
     def _new_state(self, p):
         _hip._on_gpu(p)
@@ -125,14 +122,31 @@ class AdamW(torch.optim.Optimizer):
                                                   for k in ("exp_avg", "exp_avg_sq", "master", "scales"))))
         return lists
 
+    def _current(self):
+        """The groups, their parameters and the tensors of their states: what the lists are made of."""
+        held, state = [], self.state.get
+        for group in self.param_groups:
+            held.append(group)
+            for p in group["params"]:
+                held.append(p)
+                held.extend(state(p, {}).values())
+        return held
+
     def _make_lists(self):
+        self._lists = self._made_lists()
+        self._held = self._current()  # kept, so that no other object comes to one's identity
+        self._ids = [*map(id, self._held)]
+
+    def _bring_lists_up_to_date(self):
         """Not in a capture, whose replays would clear new states and form the steps from the old ones again."""
+        if self._lists is not None and self._ids == [*map(id, self._current())]:
+            return
         params = [p for group in self.param_groups for p in group["params"]]
         _hip._on_gpu(*params)
         if params and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW makes its states and their counts in its first step, which must not be captured: a "
-                               "replay would set them back")
-        self._lists = self._made_lists()
+            raise RuntimeError("AdamW makes its states and their counts in its first step and where others have come into "
+                               "param_groups or state: that step must not be captured, a replay would set them back")
+        self._make_lists()
 
     def _norm(self):
         """Of all gradients, on the device of the first."""
@@ -151,8 +165,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if self._lists is None:
-            self._make_lists()
+        self._bring_lists_up_to_date()
         norm = None
         if self.max_norm is not None and any(p.grad is not None for g in self.param_groups for p in g["params"]):
             norm = self._norm()
@@ -178,9 +191,8 @@ class AdamW(torch.optim.Optimizer):
             if i not in state_dict["state"]:
                 continue
             self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
-        self._lists = None
         if all(self.state.get(p) for g in self.param_groups for p in g["params"]):
-            self._lists = self._made_lists()  # so that the next step may be captured
+            self._make_lists()  # so that the next step may be captured
 
 
 def reference(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01):

@@ -81,3 +81,83 @@ def test_no_lists_are_made_in_a_capture(make, capturing):
     other.step()
     capturing["now"] = True
     other.step()
+
+
+# ------------------------------- what state and param_groups hold at the time
+def _same_as_new(opt, params):
+    """That a step of opt moves params as one of a new optimizer does that is given opt's states."""
+    copies = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = W.AdamW(copies, lr=opt.param_groups[0]["lr"])
+    states = [{k: t.clone() for k, t in opt.state[p].items()} if opt.state.get(p) else {} for p in params]
+    other.load_state_dict({"state": {i: s for i, s in enumerate(states) if s},
+                           "param_groups": other.state_dict()["param_groups"]})
+    _grads(params)
+    _grads(copies)
+    before = [p.detach().clone() for p in params]
+    opt.step()
+    other.step()
+    for p, q, old in zip(params, copies, before):
+        assert torch.equal(p, q) and not torch.equal(p, old)
+        assert opt.state[p].keys() == other.state[q].keys()
+        assert all(torch.equal(t, other.state[q][k]) for k, t in opt.state[p].items())
+
+
+def test_parameter_replaced_in_its_group():
+    params = _params()
+    opt = _stepped(params)
+    old, kept = params[0], params[0].detach().clone()
+    params[0] = opt.param_groups[0]["params"][0] = torch.nn.Parameter(torch.full((6,), 2.0))
+    _same_as_new(opt, params)
+    assert torch.equal(old, kept) and int(opt.state[params[0]]["step"]) == 1
+
+
+def test_group_taken_out_and_group_replaced():
+    params = _params(4)
+    opt = W.AdamW([{"params": params[:2]}, {"params": params[2:]}], lr=0.1)
+    _grads(params)
+    opt.step()
+    gone = opt.param_groups.pop()["params"]
+    kept = [p.detach().clone() for p in gone]
+    _same_as_new(opt, params[:2])
+    assert all(torch.equal(p, q) for p, q in zip(gone, kept))
+    opt.param_groups[0] = {**opt.param_groups[0], "lr": 0.3}
+    _same_as_new(opt, params[:2])
+    opt.param_groups = [{**opt.param_groups[0], "params": params[1:3], "lr": 0.2}]
+    kept = params[0].detach().clone()
+    _same_as_new(opt, params[1:3])
+    assert torch.equal(params[0], kept)
+
+
+def test_states_cleared_and_replaced():
+    params = _params()
+    opt = _stepped(params)
+    opt.state.clear()
+    _same_as_new(opt, params)
+    assert [int(opt.state[p]["step"]) for p in params] == [1, 1, 1] and len(opt.state_dict()["state"]) == 3
+    opt.state[params[1]]["exp_avg"] = torch.full((4,), -3.0)
+    _same_as_new(opt, params)
+    opt.state[params[2]]["step"] = torch.tensor(40, dtype=torch.int32)
+    _same_as_new(opt, params)
+    assert int(opt.state[params[2]]["step"]) == 41
+    s = opt.state[params[0]]
+    s["exp_avg"], s["exp_avg_sq"] = s["exp_avg_sq"].abs(), s["exp_avg"].abs()
+    _same_as_new(opt, params)
+    del opt.state[params[0]]
+    _same_as_new(opt, params)
+    assert [int(opt.state[p]["step"]) for p in params] == [1, 5, 43]
+
+
+def test_lists_stay_where_nothing_changed_and_are_not_made_in_a_capture(capturing):
+    params = _params()
+    opt = _stepped(params)
+    counts = [opt.state[p]["step"] for p in params]
+    opt.param_groups[0]["lr"] = 0.2
+    opt.state[params[0]]["exp_avg"].zero_()
+    _same_as_new(opt, params)
+    assert all(opt.state[p]["step"] is t for p, t in zip(params, counts))
+    capturing["now"] = True
+    opt.step()
+    opt.state[params[0]]["exp_avg"] = torch.zeros(4)
+    with pytest.raises(RuntimeError, match="first step"):
+        opt.step()
+    assert all(opt.state[p]["step"] is t and int(t) == 3 for p, t in zip(params, counts))
