@@ -64,11 +64,11 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
 class AdamW(torch.optim.Optimizer):
     """AdamW on these kernels. state_bits: 32 or 8. masters: whether 16-bit parameters have fp32 masters (None: yes).
     max_norm: of all gradients together. A group's lr may be a float32 tensor on the device. The state of a parameter:
-    step, exp_avg, exp_avg_sq and, where they are used, master and scales.
-    The first step makes the states, so it cannot be captured into a graph; later ones can, with gradients that stay
-    where they are, and so can the first after states for all parameters were loaded. A copy's first step cannot. Each step
-    goes by what `param_groups` and `state` hold at the time. Where that is not what a captured step had (loaded or replaced
-    states, another group or parameter), capture again, after a step that is not captured."""
+    step, exp_avg, exp_avg_sq and, where they are used, master and scales; it begins with the first gradient.
+    A step that makes states cannot be captured into a graph; others can, with gradients that stay where they are, and so
+    can the first after states were loaded, but not a copy's first. Each step goes by what `param_groups` and
+    `state` hold at the time. Where that is not what a captured step had (loaded or replaced states, another group or
+    parameter, a first gradient), capture again, after a step that is not captured."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32, masters=None,
                  max_norm=None, seed=0):
@@ -88,7 +88,6 @@ class AdamW(torch.optim.Optimizer):
         self._lists, self._held, self._ids = None, [], []
 
     def _new_state(self, p):
-        _hip._on_gpu(p)
         _hip._dtype("parameters", p)
         if not p.is_contiguous():
             raise ValueError(f"parameters must be contiguous, got one of shape {tuple(p.shape)} with strides {p.stride()}")
@@ -103,16 +102,15 @@ class AdamW(torch.optim.Optimizer):
         return state
 
     def _made_lists(self):
-        """Per group, the lists of a call for each device and type of its parameters, those with a master (loaded states
-        may be of either kind) apart from those without. The steps of a list are one
+        """Per group, the lists of a call for each device and type of its parameters with a state, those with a master
+        (loaded states may be of either kind) apart from those without. The steps of a list are one
         tensor, of which each parameter's state has a view."""
         lists = []
         for group in self.param_groups:
             parts = {}
             for p in group["params"]:
-                if not self.state[p]:
-                    self.state[p] = self._new_state(p)
-                parts.setdefault((p.device, p.dtype, "master" in self.state[p]), []).append(p)
+                if self.state.get(p):
+                    parts.setdefault((p.device, p.dtype, "master" in self.state[p]), []).append(p)
             for ps in parts.values():
                 states = [self.state[p] for p in ps]
                 steps = torch.stack([s["step"].reshape(()) for s in states])
@@ -123,13 +121,18 @@ class AdamW(torch.optim.Optimizer):
         return lists
 
     def _current(self):
-        """The groups, their parameters and the tensors of their states: what the lists are made of."""
-        held, state = [], self.state.get
+        """The groups, their parameters that have a state or now get one, and the tensors of their states: what the lists
+        are made of."""
+        held, state_of = [], self.state.get
         for group in self.param_groups:
             held.append(group)
             for p in group["params"]:
-                held.append(p)
-                held.extend(state(p, {}).values())
+                state = state_of(p)
+                if state:
+                    held.append(p)
+                    held.extend(state.values())
+                elif p.grad is not None:
+                    held.append(p)
         return held
 
     def _make_lists(self):
@@ -141,11 +144,15 @@ class AdamW(torch.optim.Optimizer):
         """Not in a capture, whose replays would clear new states and form the steps from the old ones again."""
         if self._lists is not None and self._ids == [*map(id, self._current())]:
             return
-        params = [p for group in self.param_groups for p in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"] if p.grad is not None or self.state.get(p)]
         _hip._on_gpu(*params)
         if params and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW makes its states and their counts in its first step and where others have come into "
-                               "param_groups or state: that step must not be captured, a replay would set them back")
+            raise RuntimeError("AdamW makes its states and their counts in its first step, and where parameters or states "
+                               "have changed or got their first gradient: that step must not be captured, a replay would "
+                               "set them back")
+        for p in params:
+            if not self.state.get(p):
+                self.state[p] = self._new_state(p)
         self._make_lists()
 
     def _norm(self):
@@ -191,8 +198,7 @@ class AdamW(torch.optim.Optimizer):
             if i not in state_dict["state"]:
                 continue
             self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
-        if all(self.state.get(p) for g in self.param_groups for p in g["params"]):
-            self._make_lists()  # so that the next step may be captured
+        self._make_lists()  # so that the next step may be captured
 
 
 def reference(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01):

@@ -161,3 +161,47 @@ def test_lists_stay_where_nothing_changed_and_are_not_made_in_a_capture(capturin
     with pytest.raises(RuntimeError, match="first step"):
         opt.step()
     assert all(opt.state[p]["step"] is t and int(t) == 3 for p, t in zip(params, counts))
+
+
+# ------------------------------------------------ parameters without a gradient
+def test_states_come_with_the_first_gradient(capturing):
+    """A frozen parameter has no state, and may be of any kind and place; once it gets a gradient it begins as it is then."""
+    frozen = torch.nn.Parameter(torch.ones(4, dtype=torch.bfloat16), requires_grad=False)
+    indices = torch.nn.Parameter(torch.arange(3), requires_grad=False)
+    odd = torch.nn.Parameter(torch.ones(3, 4).t(), requires_grad=False)
+    params = [frozen, *_params(2), indices, odd]
+    opt = W.AdamW(params, lr=0.1)
+    _grads(params[1:3])
+    opt.step()
+    assert set(opt.state) == set(params[1:3]) and set(opt.state_dict()["state"]) == {1, 2}
+    counts = [opt.state[p]["step"] for p in params[1:3]]
+    params[1].grad = None  # without a gradient this time: its state stays, and so does its place
+    opt.step()
+    assert [int(t) for t in counts] == [1, 2] and all(opt.state[p]["step"] is t for p, t in zip(params[1:3], counts))
+    with torch.no_grad():
+        frozen.fill_(3.0)  # loaded
+    frozen.requires_grad_(True)
+    frozen.grad = torch.zeros_like(frozen)
+    capturing["now"] = True
+    with pytest.raises(RuntimeError, match="first step"):
+        opt.step()
+    capturing["now"] = False
+    opt.step()
+    assert torch.equal(opt.state[frozen]["master"], torch.full((4,), 3.0 * (1 - 0.1 * 0.01)))
+    assert [int(opt.state[p]["step"]) for p in params[:3]] == [1, 1, 3]
+
+
+def test_capture_right_after_loading_beside_a_frozen_parameter(capturing):
+    a, b = _params(), _params()
+    for ps in (a, b):
+        ps[1].requires_grad_(False)
+    opt, other = W.AdamW(a, lr=0.1), W.AdamW(b, lr=0.1)
+    for p in (a[0], a[2]):
+        p.grad = torch.ones_like(p)
+    opt.step()
+    other.load_state_dict(opt.state_dict())
+    for p in (b[0], b[2]):
+        p.grad = torch.ones_like(p)
+    capturing["now"] = True
+    other.step()
+    assert [int(other.state[b[i]]["step"]) for i in (0, 2)] == [2, 2] and b[1] not in other.state
