@@ -9,8 +9,9 @@ All tensors of a call are changed in place by one launch for each 60 to 80 of th
 the step's factors; clipping adds the gradients' norm, a launch for each 160. The counts live on
 the device (steps, int32, one per tensor), and the rate may (a float32 tensor of one number), so a captured step goes on
 counting and can be given another rate between replays.
-  masters    fp32 copies of 16-bit parameters: they are stepped, the parameters are their rounding. Without them steps
-             below half a rounding of a parameter are lost.
+  masters    fp32 copies of 16-bit parameters: they are stepped, and each parameter is overwritten with their rounding,
+             whatever it holds (AdamW, below, looks for changed ones). Without masters steps below half a rounding
+             of a parameter are lost.
   max_norm   gradients are scaled to this norm over all tensors where theirs is larger: the norm is computed first
              (or given, as norm: one of several shards). Where it is not finite nothing changes, counts neither.
   scales     8-bit states: exp_avgs and exp_avg_sqs are float8_e4m3fn codes of m and of sqrt(v), scales float32
@@ -61,10 +62,26 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     return _hip.adamw_step(*args) if done is None else done[0]
 
 
+def _marks(params):
+    """What differs once a parameter was changed in place or given other data."""
+    try:
+        return [(p._version, p.data_ptr()) for p in params]
+    except RuntimeError:  # a tensor of inference mode has no version
+        return [(0 if p.is_inference() else p._version, p.data_ptr()) for p in params]
+
+
+def _follow(master, p):
+    """The master of a parameter that may have been changed: taken anew where p is no longer its rounding."""
+    master.copy_(torch.where(master.to(p.dtype) == p, master, p.float()))
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW on these kernels. state_bits: 32 or 8. masters: whether 16-bit parameters have fp32 masters (None: yes).
     max_norm: of all gradients together. A group's lr may be a float32 tensor on the device. The state of a parameter:
     step, exp_avg, exp_avg_sq and, where they are used, master and scales; it begins with the first gradient.
+    A parameter that was changed in place (loaded, clamped, averaged) goes on from there: its master is taken from it where it
+    is no longer the master's rounding. Changes that torch does not count, through .data or between the replays of a captured
+    step, need masters_from_parameters(), or the next step undoes them. Loaded masters stand.
     A step that makes states cannot be captured into a graph; others can, with gradients that stay where they are, and so
     can the first after states were loaded, but not a copy's first. Each step goes by what `param_groups` and
     `state` hold at the time. Where that is not what a captured step had (loaded or replaced states, another group or
@@ -101,10 +118,13 @@ class AdamW(torch.optim.Optimizer):
             state["master"] = p.detach().float()
         return state
 
-    def _made_lists(self):
+    def _made_lists(self, fresh):
         """Per group, the lists of a call for each device and type of its parameters with a state, those with a master
         (loaded states may be of either kind) apart from those without. The steps of a list are one
-        tensor, of which each parameter's state has a view."""
+        tensor, of which each parameter's state has a view. The last entry: the marks of parameters with masters after the
+        step before (None: not known)."""
+        known = {p: mark for _, ps, *_, marks in self._lists or () for p, mark in zip(ps, marks)}
+        known.update(zip(fresh, _marks(fresh)))
         lists = []
         for group in self.param_groups:
             parts = {}
@@ -117,7 +137,8 @@ class AdamW(torch.optim.Optimizer):
                 for s, step in zip(states, steps):
                     s["step"] = step
                 lists.append((group, ps, steps, *([s[k] for s in states] if k in states[0] else None
-                                                  for k in ("exp_avg", "exp_avg_sq", "master", "scales"))))
+                                                  for k in ("exp_avg", "exp_avg_sq", "master", "scales")),
+                              [known.get(p) for p in ps if "master" in states[0]]))
         return lists
 
     def _current(self):
@@ -135,8 +156,9 @@ class AdamW(torch.optim.Optimizer):
                     held.append(p)
         return held
 
-    def _make_lists(self):
-        self._lists = self._made_lists()
+    def _make_lists(self, fresh):
+        """fresh: parameters whose masters are new or loaded, and stand."""
+        self._lists = self._made_lists(fresh)
         self._held = self._current()  # kept, so that no other object comes to one's identity
         self._ids = [*map(id, self._held)]
 
@@ -150,18 +172,28 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW makes its states and their counts in its first step, and where parameters or states "
                                "have changed or got their first gradient: that step must not be captured, a replay would "
                                "set them back")
-        for p in params:
-            if not self.state.get(p):
-                self.state[p] = self._new_state(p)
-        self._make_lists()
+        new = [p for p in params if not self.state.get(p)]
+        for p in new:
+            self.state[p] = self._new_state(p)
+        self._make_lists(new)
+
+    @torch.no_grad()
+    def masters_from_parameters(self):
+        """Takes every master from its parameter, where that is no longer the master's rounding."""
+        for group in self.param_groups:
+            for p in group["params"]:
+                if "master" in self.state.get(p, ()):
+                    _follow(self.state[p]["master"], p)
 
     def _norm(self):
-        """Of all gradients, on the device of the first."""
+        """Of all gradients, on the device of the first; None without any."""
         parts = {}
         for group in self.param_groups:
             for p in group["params"]:
                 if p.grad is not None:
                     parts.setdefault((p.device, p.grad.dtype), []).append(p.grad)
+        if not parts:
+            return None
         norms = [grad_norm(g) for g in parts.values()]
         return norms[0] if len(norms) == 1 else torch.linalg.vector_norm(torch.stack([n.to(norms[0].device) for n in norms]))
 
@@ -173,19 +205,22 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         self._bring_lists_up_to_date()
-        norm = None
-        if self.max_norm is not None and any(p.grad is not None for g in self.param_groups for p in g["params"]):
-            norm = self._norm()
-        for group, ps, steps, m, v, masters, scales in self._lists:
-            by_type = {}
-            for i, p in enumerate(ps):
-                if p.grad is not None:
-                    by_type.setdefault(p.grad.dtype, set()).add(i)
-            for some in by_type.values():
-                adamw_step(ps, [p.grad if i in some else None for i, p in enumerate(ps)], m, v, steps, lr=group["lr"],
+        norm = None if self.max_norm is None else self._norm()
+        for group, ps, steps, m, v, masters, scales, marks in self._lists:
+            if masters is not None and marks != (now := _marks(ps)):
+                for p, master, before, mark in zip(ps, masters, marks, now):
+                    if mark != before:
+                        _follow(master, p)
+            grads = [p.grad for p in ps]
+            kinds = {g.dtype for g in grads if g is not None}
+            for kind in kinds:
+                adamw_step(ps, grads if len(kinds) == 1 else [g if g is not None and g.dtype == kind else None for g in grads],
+                           m, v, steps, lr=group["lr"],
                            betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], masters=masters,
                            scales=scales, max_norm=None if norm is None else self.max_norm,
                            norm=None if norm is None else norm.to(ps[0].device), seed=self.seed)
+            if masters is not None:
+                marks[:] = _marks(ps)
         return loss
 
     def load_state_dict(self, state_dict):
@@ -198,7 +233,7 @@ class AdamW(torch.optim.Optimizer):
             if i not in state_dict["state"]:
                 continue
             self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
-        self._make_lists()  # so that the next step may be captured
+        self._make_lists(self.state)  # so that the next step may be captured
 
 
 def reference(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01):

@@ -205,3 +205,111 @@ def test_capture_right_after_loading_beside_a_frozen_parameter(capturing):
     capturing["now"] = True
     other.step()
     assert [int(other.state[b[i]]["step"]) for i in (0, 2)] == [2, 2] and b[1] not in other.state
+
+
+# --------------------------------------------------- masters and their parameters
+def _bf16(value=0.9, n=3):
+    params = [torch.nn.Parameter(torch.full((4,), value, dtype=torch.bfloat16)) for _ in range(n)]
+    opt = _stepped(params, lr=1e-3, weight_decay=0.0)
+    _grads(params, 0.25)  # small steps: the masters are between two bf16 numbers
+    opt.step()
+    assert all(not torch.equal(opt.state[p]["master"], p.float()) for p in params)
+    return params, opt
+
+
+CHANGES = {
+    "filled": lambda p: p.fill_(5.0),
+    "loaded": lambda p: p.copy_(torch.full((4,), 5.0)),
+    "exchanged": lambda p: setattr(p, "data", torch.full((4,), 5.0, dtype=torch.bfloat16)),
+}
+
+
+@pytest.mark.parametrize("change", CHANGES)
+def test_masters_follow_changed_parameters(change):
+    params, opt = _bf16()
+    masters = [opt.state[p]["master"].clone() for p in params]
+    with torch.no_grad():
+        CHANGES[change](params[1])
+    opt.param_groups[0]["lr"] = 0.0
+    opt.step()
+    assert torch.equal(params[1], torch.full((4,), 5.0, dtype=torch.bfloat16))
+    assert torch.equal(opt.state[params[1]]["master"], torch.full((4,), 5.0))
+    assert all(torch.equal(opt.state[params[i]]["master"], masters[i]) for i in (0, 2))
+
+
+def test_masters_keep_what_did_not_change():
+    """A clamp that meets one element: the others' masters keep what is below their rounding. Then nothing changes, and
+    nothing is taken over."""
+    params, opt = _bf16()
+    master = opt.state[params[0]]["master"].clone()
+    with torch.no_grad():
+        params[0][2] = 0.5
+    opt.param_groups[0]["lr"] = 0.0
+    opt.step()
+    master[2] = 0.5
+    assert torch.equal(opt.state[params[0]]["master"], master)
+    taken = []
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(W, "_follow", lambda master, p: taken.append(p))
+        opt.step()
+        opt.param_groups[0]["params"].append(torch.nn.Parameter(torch.ones(2, dtype=torch.bfloat16)))
+        opt.param_groups[0]["params"][-1].grad = torch.ones(2, dtype=torch.bfloat16)
+        opt.step()  # lists made again
+    assert not taken
+
+
+def test_change_before_the_lists_are_made_again():
+    params, opt = _bf16()
+    with torch.no_grad():
+        params[0].fill_(5.0)
+    opt.param_groups[0]["params"].append(torch.nn.Parameter(torch.ones(2, dtype=torch.bfloat16)))
+    opt.param_groups[0]["params"][-1].grad = torch.ones(2, dtype=torch.bfloat16)
+    opt.param_groups[0]["lr"] = 0.0
+    opt.step()
+    assert torch.equal(params[0], torch.full((4,), 5.0, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("model_first", [True, False])
+def test_loading_keeps_the_masters(model_first):
+    """Whichever is loaded first, the saved masters stand: they are what the saved parameters are the rounding of."""
+    a, opt = _bf16()
+    b = [torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16)) for _ in a]
+    other = W.AdamW(b, lr=1e-3, weight_decay=0.0)
+
+    def load_model():
+        with torch.no_grad():
+            for p, q in zip(a, b):
+                q.copy_(p)
+
+    if model_first:
+        load_model()
+    other.load_state_dict(opt.state_dict())
+    if not model_first:
+        load_model()
+    _grads(a, 0.25)
+    _grads(b, 0.25)
+    opt.step()
+    other.step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q) and torch.equal(opt.state[p]["master"], other.state[q]["master"])
+    clone = copy.deepcopy(other)
+    c = clone.param_groups[0]["params"]
+    _grads(c, 0.25)
+    with torch.no_grad():
+        c[0].fill_(5.0)
+    clone.step()
+    other.step()
+    assert (c[0] > 4.9).all() and all(torch.equal(clone.state[p]["master"], other.state[q]["master"])
+                                      for p, q in zip(c[1:], b[1:]))
+
+
+def test_changes_that_torch_does_not_count():
+    params, opt = _bf16()
+    masters = [opt.state[p]["master"].clone() for p in params]
+    params[0].data.fill_(5.0)
+    params[1].data[1] = float("nan")
+    opt.masters_from_parameters()
+    masters[0].fill_(5.0)
+    masters[1][1] = float("nan")
+    for p, t in zip(params, masters):
+        assert torch.equal(opt.state[p]["master"].nan_to_num(7.0), t.nan_to_num(7.0))

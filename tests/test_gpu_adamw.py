@@ -625,3 +625,38 @@ def test_class_captured_right_after_loading():
         assert all(torch.equal(p, q) for p, q in zip(a, b)), i
         assert [int(other.state[q]["step"]) for q in b] == [3 + i] * 3
     del graph
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_class_goes_on_from_changed_parameters(bits):
+    """bf16 parameters that are loaded, clamped, or changed between replays of a captured step: the next step starts there,
+    and what was not changed keeps its master."""
+    log(f"AdamW, changed parameters, {bits} bits")
+    ps = _model()
+    opt = W.AdamW(ps, lr=1e-3, weight_decay=0.0, state_bits=bits)
+    for step in range(3):
+        _set_grads(ps, step)
+        opt.step()
+    for group in opt.param_groups:
+        group["lr"] = 0.0
+    masters = [opt.state[p]["master"].clone() for p in ps]
+    assert all(torch.equal(m.to(p.dtype), p) and not torch.equal(m, p.float()) for m, p in zip(masters, ps))
+    want = [p.detach().clone() for p in ps]
+    with torch.no_grad():
+        for p, w in zip(ps, want):
+            p.clamp_(-0.05, 0.05)
+            w.clamp_(-0.05, 0.05)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for i in range(3):
+        for p, w, m in zip(ps, want, masters):
+            m.copy_(torch.where(m.to(p.dtype) == w, m, w.float()))
+            assert torch.equal(p, w) and torch.equal(opt.state[p]["master"], m), i
+        for p, w in zip(ps, want):
+            p.data.flatten()[i] = w.flatten()[i] = 3.0 + i
+        opt.masters_from_parameters()
+        graph.replay()
+        torch.cuda.synchronize()
+    del graph
