@@ -927,13 +927,14 @@ PyObject* py_adamw_step(Args a, Py_ssize_t n) {
                                    lr_at ? lr_at->data_ptr<float>() : nullptr, (float)lr, b1, b2, (float)eps, (float)decay,
                                    norm.defined() ? norm.data_ptr<float>() : nullptr, norm_arg ? 1 : 0, (float)max_norm,
                                    (uint32_t)seed, with_scales ? 8 : 32, dt, gdt, ws.data_ptr(), bytes, stream_of(*params[0])));
-    // What a graph has saved of these counts as changed.
+    // What a graph has saved of these counts as changed, but for tensors that had no gradient.
     auto changed = [](const Tensor& t) {
       if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     };
     changed(*steps);
     for (const auto* list : {&params, &m, &v, &masters, &scales})
-      for (const Tensor* t : *list) changed(*t);
+      for (size_t i = 0; i < list->size(); ++i)
+        if (grads[i]) changed(*(*list)[i]);
     return {norm};
   });
 }

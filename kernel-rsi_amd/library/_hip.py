@@ -933,6 +933,7 @@ def adamw_step(params: list, grads: list, exp_avgs: list, exp_avg_sqs: list, ste
             sizes, count, _ptr(steps), _ptr(at), float(lr), beta1, beta2, eps, weight_decay, _ptr(norm), int(norm_given),
             0.0 if max_norm is None else max_norm, seed & 0xffffffff, bits, dt, gdt, _ptr(ws), nbytes,
             _stream(params[0])))
-    written = [steps] + [t for ts in (params, exp_avgs, exp_avg_sqs, masters, scales) if ts is not None for t in ts]
+    written = [steps] + [t for ts in (params, exp_avgs, exp_avg_sqs, masters, scales) if ts is not None
+                         for t, g in zip(ts, grads) if g is not None]
     torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
     return norm

@@ -19,7 +19,8 @@ counting and can be given another rate between replays.
              right on average and the root in its square (rounded to nearest, v would stand still: it changes by 1 - b2 in a
              step). The random numbers follow from seed, t, the tensor's place in the list and the element's.
 Parameters, states and gradients are contiguous (a gradient that is not is copied), of bf16, fp16 or fp32, gradients of the
-parameters' type or fp32. Nothing is recorded for a backward; tensors that a graph has saved count as changed.
+parameters' type or fp32. Nothing is recorded for a backward; what a graph has
+saved of the tensors that are stepped counts as changed.
 """
 import sys
 from pathlib import Path

@@ -660,3 +660,40 @@ def test_class_goes_on_from_changed_parameters(bits):
         graph.replay()
         torch.cuda.synchronize()
     del graph
+
+
+@pytest.mark.parametrize("path", ["native", "python"])
+def test_tensors_without_a_gradient_do_not_count_as_changed(path):
+    """A graph that saved a parameter which the step does not touch still runs; one that is stepped counts in all of its
+    tensors."""
+    log(f"adamw versions without a gradient, {path}")
+    kw = _lists([(8,), (300,), (0,), (16,)], torch.bfloat16, 8, masters=True)
+    kw["grads"][1] = kw["grads"][3] = None
+    lists = ("params", "exp_avgs", "exp_avg_sqs", "masters", "scales")
+    before = {k: [t._version for t in kw[k]] for k in lists}
+    saved = [p.requires_grad_(True) for p in kw["params"]]
+    outs = [(p * p).sum() for p in saved]
+    if path == "python":
+        kw["params"] = tuple(kw["params"])  # which the native path hands back
+    with torch.no_grad():
+        W.adamw_step(**kw, **HYPER)
+    for k in lists:
+        assert [t._version - v for t, v in zip(kw[k], before[k])] == [1, 0, 1, 0], k
+    outs[1].backward()
+    outs[3].backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        outs[0].backward()
+
+
+def test_class_leaves_unused_parameters_to_their_graphs():
+    """Two networks in one optimizer: a step of one does not disturb a retained graph of the other."""
+    log("AdamW, a graph of an unused parameter")
+    ps = _model(torch.float32)
+    opt = W.AdamW(ps, lr=1e-2)
+    _set_grads(ps, 0)
+    opt.step()
+    out = (ps[1] * ps[1]).sum()
+    ps[1].grad = None
+    opt.step()
+    out.backward()
+    assert torch.equal(ps[1].grad, 2 * ps[1])
