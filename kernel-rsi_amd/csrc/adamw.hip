@@ -613,6 +613,9 @@ int krsi_adamw_step(void* const* params, const void* const* grads, void* const* 
   const hipStream_t st = as_stream(stream);
   const bool norm_here = norm && !norm_given;
   int64_t parts = 0;
+  // An error that an earlier call has left is not this one's: reported after the first launches, it would have the caller make
+  // the step again.
+  (void)hipGetLastError();
   if (norm_here) {
     rc = launch_norm_parts(grads, sizes, count, part, grad_dtype, st, &parts);
     if (rc != KRSI_OK) return rc;

@@ -7,7 +7,7 @@
 // Every function returns None for whatever is not the plain case (tracing, functorch transforms, dispatch
 // modes, tensor subclasses, forward-mode duals, layouts that need a copy, arguments that are refused): the
 // caller then takes its Python path, which handles it or raises. So no message or rule of
-// validation is repeated here, and nothing has been launched when None is returned.
+// validation is repeated here, and nothing that the call changes has been touched when None is returned.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -25,7 +25,8 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// A status other than KRSI_OK in a forward: nothing was launched; the Python path reports it.
+// A status other than KRSI_OK in a forward: nothing was launched, or only what may be launched again; the Python path
+// reports it.
 struct NotPlain {};
 
 void* stream_of(const Tensor& t) {
@@ -58,6 +59,12 @@ void backward_status(int rc) {
     PyErr_SetString(PyExc_RuntimeError, krsi_error_string(rc));
   }
   throw_python_error();
+}
+
+// The status of an operator that changes its arguments: once something may have been launched it is not made again.
+void in_place_status(int rc) {
+  if (rc == KRSI_ERR_LAUNCH) backward_status(rc);
+  forward_status(rc);
 }
 
 // KRSI_DTYPE_* of an activation dtype, or -1.
@@ -922,11 +929,11 @@ PyObject* py_adamw_step(Args a, Py_ssize_t n) {
     if (clip && !norm.defined()) norm = at::empty({}, params[0]->options().dtype(at::kFloat));
     const size_t bytes = krsi_adamw_workspace_bytes(sizes.data(), (int)count);
     Tensor ws = at::empty({(int64_t)bytes}, params[0]->options().dtype(at::kByte));
-    forward_status(krsi_adamw_step(pp.data(), gp.data(), mp.data(), vp.data(), with_masters ? wp.data() : nullptr,
-                                   with_scales ? sp.data() : nullptr, sizes.data(), (int)count, steps->data_ptr<int32_t>(),
-                                   lr_at ? lr_at->data_ptr<float>() : nullptr, (float)lr, b1, b2, (float)eps, (float)decay,
-                                   norm.defined() ? norm.data_ptr<float>() : nullptr, norm_arg ? 1 : 0, (float)max_norm,
-                                   (uint32_t)seed, with_scales ? 8 : 32, dt, gdt, ws.data_ptr(), bytes, stream_of(*params[0])));
+    in_place_status(krsi_adamw_step(pp.data(), gp.data(), mp.data(), vp.data(), with_masters ? wp.data() : nullptr,
+                                    with_scales ? sp.data() : nullptr, sizes.data(), (int)count, steps->data_ptr<int32_t>(),
+                                    lr_at ? lr_at->data_ptr<float>() : nullptr, (float)lr, b1, b2, (float)eps, (float)decay,
+                                    norm.defined() ? norm.data_ptr<float>() : nullptr, norm_arg ? 1 : 0, (float)max_norm,
+                                    (uint32_t)seed, with_scales ? 8 : 32, dt, gdt, ws.data_ptr(), bytes, stream_of(*params[0])));
     // What a graph has saved of these counts as changed, but for tensors that had no gradient.
     auto changed = [](const Tensor& t) {
       if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();

@@ -697,3 +697,23 @@ def test_class_leaves_unused_parameters_to_their_graphs():
     opt.step()
     out.backward()
     assert torch.equal(ps[1].grad, 2 * ps[1])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_error_left_by_an_earlier_call_is_not_the_steps(bits):
+    """A HIP call that failed before leaves its error for whoever asks next: the step is made once all the same."""
+    import ctypes
+
+    log(f"adamw after another call's error, {bits} bits")
+    hip = ctypes.CDLL("libamdhip64.so.7")
+    for clip in ({}, {"max_norm": 0.1}):
+        kw = _lists(SHAPES, torch.bfloat16, bits, masters=True)
+        want = _copy(kw)
+        W.adamw_step(**want, **HYPER, **clip)
+        torch.cuda.synchronize()
+        assert hip.hipSetDevice(1 << 20) != 0  # no such device: nothing is done, and the error stays
+        W.adamw_step(**kw, **HYPER, **clip)
+        torch.cuda.synchronize()
+        for k in kw:
+            same = zip(kw[k], want[k]) if k != "steps" else [(kw[k], want[k])]
+            assert all(torch.equal(a.float(), b.float()) for a, b in same), k
