@@ -114,7 +114,7 @@ class AdamW(torch.optim.Optimizer):
         for name in ("exp_avg", "exp_avg_sq"):
             state[name] = torch.zeros(p.shape, device=p.device, dtype=kind)
         if self.state_bits == 8:
-            state["scales"] = torch.zeros(2, -(-p.numel() // _hip.BLOCK_8BIT), device=p.device)
+            state["scales"] = torch.zeros(2, -(-p.numel() // _hip.BLOCK_8BIT), device=p.device, dtype=torch.float32)
         if p.dtype != torch.float32 and self.masters in (None, True):
             state["master"] = p.detach().float()
         return state

@@ -313,3 +313,17 @@ def test_changes_that_torch_does_not_count():
     masters[1][1] = float("nan")
     for p, t in zip(params, masters):
         assert torch.equal(opt.state[p]["master"].nan_to_num(7.0), t.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_states_under_another_default_dtype(default):
+    torch.set_default_dtype(default)
+    try:
+        params = [torch.nn.Parameter(torch.ones(300, dtype=torch.bfloat16))]
+        opt = W.AdamW(params, lr=0.1, state_bits=8)
+        state = opt._new_state(params[0])
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert {k: t.dtype for k, t in state.items()} == {
+        "step": torch.int32, "exp_avg": torch.float8_e4m3fn, "exp_avg_sq": torch.float8_e4m3fn, "scales": torch.float32,
+        "master": torch.float32}

@@ -717,3 +717,20 @@ def test_an_error_left_by_an_earlier_call_is_not_the_steps(bits):
         for k in kw:
             same = zip(kw[k], want[k]) if k != "steps" else [(kw[k], want[k])]
             assert all(torch.equal(a.float(), b.float()) for a, b in same), k
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_class_under_another_default_dtype(bits):
+    log(f"AdamW, default dtype bf16, {bits} bits")
+    a, b = _model(), _model()
+    opts = [W.AdamW(ps, lr=1e-2, state_bits=bits, max_norm=1.0) for ps in (a, b)]
+    for step in range(2):
+        _set_grads(a, step)
+        _set_grads(b, step)
+        opts[0].step()
+        torch.set_default_dtype(torch.bfloat16)
+        try:
+            opts[1].step()
+        finally:
+            torch.set_default_dtype(torch.float32)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
