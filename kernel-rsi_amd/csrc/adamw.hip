@@ -211,6 +211,9 @@ __global__ __launch_bounds__(kThreads) void step_factors(const Mask mask, int ba
   out[base + i] = f;
 }
 
+// Below kSmall a root is taken of kUp times the number and multiplied by kDown.
+constexpr float kSmall = 0x1p-64f, kUp = 0x1p64f, kDown = 0x1p-32f;
+
 struct Rule {
   float b1, c1, b2, c2, eps;  // c: 1 - b, formed in fp64
 };
@@ -238,7 +241,9 @@ __device__ __forceinline__ void eight32(void* const* p, const Factor& f, const R
     const float x = g[j] * f.share;
     m[j] = m[j] * k.b1 + x * k.c1;
     v[j] = v[j] * k.b2 + (x * x) * k.c2;
-    const float d = __builtin_amdgcn_sqrtf(v[j]) * f.root + k.eps;
+    // The hardware's root takes a subnormal v for zero: a small one is scaled by 2^64, and its root back.
+    const bool small = v[j] < kSmall;
+    const float d = __builtin_amdgcn_sqrtf(v[j] * (small ? kUp : 1.f)) * (small ? f.root * kDown : f.root) + k.eps;
     w[j] = w[j] * f.decay - f.rate * m[j] * __builtin_amdgcn_rcpf(d);
   }
   store<kF32, 8, FULL>(p[kM], i, some, m);
@@ -331,11 +336,15 @@ __device__ __forceinline__ uint32_t four_codes(const float* f) {
 }
 
 // The correctly rounded root: the hardware's is a unit off at most, and the residuals of its neighbours say which it is.
+// Small numbers are scaled: the hardware takes subnormal ones for zero, and their residuals would be lost.
 __device__ __forceinline__ float exact_root(float x) {
+  const bool small = x < kSmall;
+  x *= small ? kUp : 1.f;
   const float s = __builtin_amdgcn_sqrtf(x);
   const float below = __uint_as_float(__float_as_uint(s) - 1u), above = __uint_as_float(__float_as_uint(s) + 1u);
-  const float r = __builtin_fmaf(-below, s, x) <= 0.f ? below : s;
-  return __builtin_fmaf(-above, s, x) > 0.f ? above : r;
+  float r = __builtin_fmaf(-below, s, x) <= 0.f ? below : s;
+  r = __builtin_fmaf(-above, s, x) > 0.f ? above : r;
+  return r * (small ? kDown : 1.f);
 }
 
 // 16 elements a lane: a DPP row of 16 lanes has a scale's 256. The states are formed as the formula says it, each operation

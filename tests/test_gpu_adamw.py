@@ -734,3 +734,66 @@ def test_class_under_another_default_dtype(bits):
         finally:
             torch.set_default_dtype(torch.float32)
     assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def _tiny_gradients(n, lo, hi, seed):
+    g = torch.Generator().manual_seed(seed)
+    size = torch.exp(math.log(lo) + math.log(hi / lo) * torch.rand(n, generator=g, dtype=torch.float64))
+    return (size * (1 - 2 * torch.randint(0, 2, (n,), generator=g))).float().cuda()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-25, 1e-20])
+def test_first_step_of_tiny_gradients(bits, eps):
+    """v below fp32's normal range. A first step is lr g / (|g| + eps), but for v's own rounding: (1 - b2) g^2 is two
+    products, each off by half of 2^-149 at most (the first times 1 - b2), less than 2^-149 together, which is half as much of the
+    root relative to v; and 32 roundings at most of 2^-24."""
+    log(f"adamw tiny gradients, {bits} bits, eps {eps}")
+    n = 4096
+    g = _tiny_gradients(n, 3e-20, 1e-15, 5)
+    m, v = [torch.zeros(n, device="cuda")], [torch.zeros(n, device="cuda")]
+    kw = {}
+    if bits == 8:
+        m, v = [m[0].to(torch.float8_e4m3fn)], [v[0].to(torch.float8_e4m3fn)]
+        kw["scales"] = [torch.zeros(2, n // 256, device="cuda")]
+    p = [torch.zeros(n, device="cuda")]
+    steps = torch.zeros(1, device="cuda", dtype=torch.int32)
+    W.adamw_step(p, [g], m, v, steps, lr=1e-2, eps=eps, weight_decay=0.0, **kw)
+    assert int((1e-3 * g.double().square() < 2.0 ** -126).sum()) > 1000  # below the normal range
+    d = g.double()
+    want = -1e-2 * d / (d.abs() + eps)
+    loss = 2.0 ** -149 / (1e-3 * d.square())
+    _near(p[0], want, want.abs() * (loss + 32 * E), "param")
+    if bits == 32:
+        _near(v[0], 1e-3 * d.square(), 8 * E * d.square() * 1e-3 + 2.0 ** -149, "v")
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-25])
+def test_steps_from_tiny_averages(eps):
+    """The stored v as it is: from the least subnormal number to beyond the range where the root is scaled."""
+    log(f"adamw tiny averages, eps {eps}")
+    v0 = torch.exp2(torch.arange(-149, -30, device="cuda", dtype=torch.float64).repeat_interleave(16)
+                    + torch.arange(16, device="cuda", dtype=torch.float64).repeat(119) / 16).float()
+    m0 = seeded((v0.numel(),), 3, dtype=torch.float32) * v0.double().sqrt().float()
+    p, m, v = [torch.zeros_like(v0)], [m0.clone()], [v0.clone()]
+    steps = torch.full((1,), 99, device="cuda", dtype=torch.int32)
+    W.adamw_step(p, [torch.zeros_like(v0)], m, v, steps, lr=1e-2, eps=eps, weight_decay=0.0)
+    root = v[0].double().sqrt() / math.sqrt(1 - 0.999 ** 100)  # of v as it was stored
+    live = v[0] > 0
+    assert int(live.sum()) >= v0.numel() - 16
+    want = -1e-2 / (1 - 0.9 ** 100) * m[0].double() / (root + eps)
+    _near(p[0][live], want[live], 32 * E * want[live].abs() + 2.0 ** -149, "param")
+
+
+def test_8bit_roots_of_tiny_averages():
+    """An 8-bit root that small is kept: its square is (1 - b2) g^2 to the codes' rounding."""
+    log("adamw 8-bit tiny roots")
+    g = torch.full((512,), 1e-20, device="cuda")
+    m = torch.zeros(512, device="cuda").to(torch.float8_e4m3fn)
+    kw = dict(params=[torch.zeros(512, device="cuda")], grads=[g], exp_avgs=[m.clone()], exp_avg_sqs=[m.clone()],
+              scales=[torch.zeros(2, 2, device="cuda")], steps=torch.zeros(1, device="cuda", dtype=torch.int32))
+    W.adamw_step(**kw, lr=0.0)
+    v = _values(kw, 0)[1]
+    want = 1e-3 * float(g[0].double()) ** 2
+    # The scale is the largest root over 448, all roots are the largest; v is off by 2^-149 at most, the scale by roundings.
+    _near(v, torch.full_like(v, want), 2.0 ** -149 + 32 * E * want, "v")
