@@ -330,7 +330,8 @@ int krsi_add_rmsnorm_bwd(const void* dy, const void* dr, const void* r, const vo
  * down at random, m right on average and the root in its square, a root above zero never to zero; the random numbers
  * follow from seed, t, i and the element's number alone.
  * krsi_grad_norm: the root of the sum of squares over all tensors (NULL entries have no part), fixed order.
- * Limits: count <= 2^20, 2^35 elements in all; beta in [0, 1). workspaces: scratch, no need to keep.          */
+ * Limits: count <= 2^20, 2^35 elements in all; beta in [0, 1); eps zero or 2^-126 at least. workspaces: scratch, no
+ * need to keep.                                                                                               */
 size_t krsi_grad_norm_workspace_bytes(const int64_t* sizes, int32_t count);
 int krsi_grad_norm(const void* const* grads, const int64_t* sizes, int32_t count, float* norm, void* workspace,
                    size_t workspace_bytes, int32_t dtype, void* stream);

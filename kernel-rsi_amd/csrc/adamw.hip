@@ -586,8 +586,9 @@ int krsi_adamw_step(void* const* params, const void* const* grads, void* const* 
   if ((state_bits != 8 && state_bits != 32) || (state_bits == 8) != (scales != nullptr)) return KRSI_ERR_UNSUPPORTED;
   int rc = check_sizes(sizes, count);
   if (rc != KRSI_OK) return rc;
-  if ((!lr_at && !in_range(lr)) || !in_range(eps) || eps < 0 || !in_range(weight_decay) || !(beta1 >= 0 && beta1 < 1) ||
-      !(beta2 >= 0 && beta2 < 1) || (norm && !(max_norm >= 0)) || norm_given < 0 || norm_given > 1)
+  // A subnormal eps has no reciprocal in fp32: an element that never had a gradient would step by 0 times infinity.
+  if ((!lr_at && !in_range(lr)) || !in_range(eps) || eps < 0 || (eps > 0 && eps < 0x1p-126f) || !in_range(weight_decay) ||
+      !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || (norm && !(max_norm >= 0)) || norm_given < 0 || norm_given > 1)
     return KRSI_ERR_BAD_SCALE;
   if (count == 0) return KRSI_OK;
   if (!params || !grads || !exp_avgs || !exp_avg_sqs || !steps) return KRSI_ERR_NULL_POINTER;

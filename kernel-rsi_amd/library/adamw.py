@@ -47,6 +47,8 @@ def _check_numbers(lr, betas, eps, weight_decay, max_norm):
         raise ValueError(f"betas={betas} are not in [0, 1)")
     if not 0 <= eps < float("inf") or not 0 <= weight_decay < float("inf"):
         raise ValueError(f"eps={eps}, weight_decay={weight_decay}: not negative, and finite")
+    if 0 < eps < 2.0 ** -126:  # 1 / eps overflows, and an element without any gradient would step by 0 * infinity
+        raise ValueError(f"eps={eps}: zero, or a normal number of fp32 (2^-126 at least)")
     if max_norm is not None and not max_norm >= 0:
         raise ValueError(f"max_norm={max_norm} is not a norm")
 

@@ -170,3 +170,26 @@ def test_python_functions_refuse_before_a_launch():
     p.grad = x.clone()
     with pytest.raises(ValueError, match="GPU"):
         W.AdamW([p]).step()
+
+
+@pytest.mark.parametrize("eps", [2.0 ** -127, 1e-40, 1e-46])
+def test_adamw_eps_below_the_normal_range(eps):
+    """Its reciprocal overflows in fp32 (or it is zero there): 0 / eps, the step of an element that has never had a gradient,
+    would be NaN."""
+    x, steps = torch.zeros(4, 64), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="eps"):
+        W.adamw_step([x], [x], [x], [x], steps, lr=1e-3, eps=eps)
+    with pytest.raises(ValueError, match="eps"):
+        W.AdamW([torch.nn.Parameter(x)], eps=eps)
+    for good in (0.0, 2.0 ** -126):
+        with pytest.raises(ValueError, match="GPU"):
+            W.adamw_step([x], [x], [x], [x], steps, lr=1e-3, eps=good)
+    at = _array(FAKE)
+    lib, sizes = _hip.lib(), _sizes(64)
+
+    def call(eps, ws):
+        return lib.krsi_adamw_step(at, at, _array(FAKE + 4096), _array(FAKE + 8192), NULL, NULL, sizes, 1, FAKE, NULL, 1e-3, 0.9,
+                                   0.999, eps, 0.01, NULL, 0, 0.0, 0, 32, 2, 2, ws, 1 << 20, NULL)
+
+    assert call(2.0 ** -126, NULL) == call(0.0, NULL) == WS
+    assert call(eps, FAKE) == SCALE if eps > 2.0 ** -150 else call(eps, NULL) == WS
