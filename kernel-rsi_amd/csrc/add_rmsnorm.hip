@@ -237,28 +237,40 @@ __global__ __launch_bounds__(threads_of(WPR)) void add_rms_bwd(
   const int nch = RAGGED ? (n + E - 1) / E : n / E;
   const float inv_n = 1.0f / (float)n;
 
-  u32x4 wv[VPT];
+  // The registers of 16 waves do not hold w beside four chunks a lane of each row: each lane has its part in LDS.
+  constexpr bool kStaged = WPR == 16 && VPT == 4;
+  __shared__ u32x4 staged[kStaged ? VPT * GT : 1];
+  u32x4 wv[kStaged ? 1 : VPT];
+  auto weight = [&](int k) { return kStaged ? staged[gtid + k * GT] : wv[kStaged ? 0 : k]; };
   float dw[VPT][E];
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
     const int c = gtid + k * GT;
-    wv[k] = c < nch ? load_chunk<RAGGED>(chunk_at<RAGGED, E>(w, c, n)) : u32x4{0u, 0u, 0u, 0u};
+    const u32x4 wc = c < nch ? load_chunk<RAGGED>(chunk_at<RAGGED, E>(w, c, n)) : u32x4{0u, 0u, 0u, 0u};
+    if constexpr (kStaged)
+      staged[c] = wc;
+    else
+      wv[k] = wc;
 #pragma unroll
     for (int j = 0; j < E; ++j) dw[k][j] = 0.f;
   }
 
-  const int64_t groups_total = (int64_t)gridDim.x * RPB;
-  const int64_t iters = (rows + groups_total - 1) / groups_total;
+  const int total = (int)rows, groups_total = (int)gridDim.x * RPB;  // fewer than 2^26 rows
+  const int iters = (total + groups_total - 1) / groups_total;
   struct Row {
-    u32x4 g[VPT], d[VPT], x[VPT];
+    u32x4 g[VPT], x[VPT], d[DR ? VPT : 1];  // (never unset, which kept all of it in memory)
     float rstd;
   };
-  auto fetch = [&](int64_t row, Row& q) {
-    const bool live = row < rows;
+  constexpr bool kAhead = WPR < 16;
+  auto fetch = [&](int row, Row& q) {
+    const bool live = row < total;
     const int64_t base = (live ? row : 0) * (int64_t)n;
+    // A lane's addresses are formed here, from its number: kept from row to row, two registers each, they went to memory.
+    int lane = gtid;
+    if constexpr (!kAhead) asm volatile("" : "+v"(lane));
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int c = gtid + k * GT;
+      const int c = lane + k * GT;
       const bool ok = live && c < nch;
       q.g[k] = ok ? stream_chunk<RAGGED>(chunk_at<RAGGED, E>(dy + base, c, n)) : u32x4{0u, 0u, 0u, 0u};
       q.x[k] = ok ? stream_chunk<RAGGED>(chunk_at<RAGGED, E>(r + base, c, n)) : u32x4{0u, 0u, 0u, 0u};
@@ -266,22 +278,21 @@ __global__ __launch_bounds__(threads_of(WPR)) void add_rms_bwd(
     }
     q.rstd = live ? rstd[row] : 0.f;
   };
-  constexpr bool kAhead = WPR < 16;
-  int64_t row = (int64_t)blockIdx.x * RPB + grp;
+  int row = (int)blockIdx.x * RPB + grp;
   Row here;
   fetch(row, here);
-  for (int64_t it = 0; it < iters; ++it, row += groups_total) {
-    const bool live = row < rows;
+  for (int it = 0; it < iters; ++it, row += groups_total) {
+    const bool live = row < total;
     const int64_t base = (live ? row : 0) * (int64_t)n;
-    Row next = here;
-    if (kAhead && it + 1 < iters) fetch(row + groups_total, next);
+    Row next;
+    if constexpr (kAhead) fetch(row + groups_total, next);
     float sdot = 0.f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       float gf[E], xf[E], wf[E];
       El::unpack(here.g[k], gf);
       El::unpack(here.x[k], xf);
-      El::unpack(wv[k], wf);
+      El::unpack(weight(k), wf);
       const int dup = chunk_shared<RAGGED, E>(gtid + k * GT, n);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -300,7 +311,7 @@ __global__ __launch_bounds__(threads_of(WPR)) void add_rms_bwd(
           float gf[E], xf[E], wf[E], o[E];
           El::unpack(here.g[k], gf);
           El::unpack(here.x[k], xf);
-          El::unpack(wv[k], wf);
+          El::unpack(weight(k), wf);
 #pragma unroll
           for (int j = 0; j < E; ++j) o[j] = r1 * (gf[j] * wf[j] - (xf[j] * r1) * sn);
           if constexpr (DR) {
@@ -314,9 +325,9 @@ __global__ __launch_bounds__(threads_of(WPR)) void add_rms_bwd(
         }
       }
     }
-    if (kAhead)
+    if constexpr (kAhead)
       here = next;
-    else if (it + 1 < iters)
+    else
       fetch(row + groups_total, here);
   }
 

@@ -38,3 +38,11 @@ def test_two_waves_per_simd_of_the_large_tiles():
     found = scratch_and_waves("linear_8bit.hip")
     large = [v for k, v in found.items() if "linear_8bit_streamILi" in k and "ELi2ELi4ELi8ELi4ELi3ELi2E" in k]
     assert len(large) == 3 and all(waves >= 2 for _, waves in large)
+
+
+@pytest.mark.skipif(not (Path("/opt/rocm/bin/hipcc").is_file() or shutil.which("hipcc")), reason="no hipcc")
+def test_no_scratch_in_the_norms_backward():
+    """Every width, with and without the stream's gradient, aligned and ragged: 6 widths in 16 bits and 7 in fp32."""
+    found = {k: v[0] for k, v in scratch_and_waves("add_rmsnorm.hip").items() if "add_rms_bwd" in k}
+    assert len([k for k in found if "short" not in k]) == (6 + 6 + 7) * 4
+    assert not {k: v for k, v in found.items() if v}
