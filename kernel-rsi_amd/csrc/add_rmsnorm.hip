@@ -12,9 +12,10 @@
 // last: a row that holds one has the scale infinity or NaN, and reads back as NaN throughout.
 //
 // Bound by HBM: each row is read once, lives in registers in 16-byte chunks and is written once, by WPR waves with VPT
-// chunks per lane. The backward is persistent and keeps its share of dw in registers, as RMSNorm's. bf16 [32768, 4096]: forward
-// 181 us (5.9 TB/s), backward 191 (5.7), dw's sums 5. fp16 [8191, 8192] in 8 bits: 72 us (6.5 TB/s).
-// fp32 [2042, 1001]: 8.3, 20.9, 3.9. bf16 [32, 4096] in 8 bits: 3.6 (a launch's latency).
+// chunks per lane. The backward is persistent and keeps its share of dw in registers, as RMSNorm's, and w (in LDS for fp32 rows
+// of more than 8192 columns). bf16 [32768, 4096]: forward 181 us (5.9 TB/s), backward 171 (6.3), dw's sums 5. fp16
+// [8191, 8192] in 8 bits: 72 us (6.5 TB/s). fp32 [2042, 1001]: 7.5, 8.5, 3.8. bf16 [32, 4096] in 8 bits: 3.6 (a launch's
+// latency).
 #include "chunks.h"
 #include "column_sum.h"
 #include "krsi_device.h"
@@ -223,7 +224,8 @@ __global__ __launch_bounds__(4 * kWave) void row_scalar(
 // ---------------------------------------------------------------- backward
 // Persistent: block b takes the row groups b, b + grid, ...; all of a block's groups run the same number of steps, so
 // that the barriers stay uniform. The next row's loads are out before this one is reduced, but for rows of 16 waves, whose
-// registers do not hold both.
+// registers do not hold both. No register goes to memory: where some did, fp32 [2042, 1001] took 20.3 us, [4096, 16384] 305
+// (so 200), bf16 [32768, 4096] 191.
 template <int DT, int WPR, int VPT, bool RAGGED, bool DR>
 __global__ __launch_bounds__(threads_of(WPR)) void add_rms_bwd(
     const typename Elem<DT>::T* __restrict__ dy, const typename Elem<DT>::T* __restrict__ dr,
@@ -265,7 +267,8 @@ __global__ __launch_bounds__(threads_of(WPR)) void add_rms_bwd(
   auto fetch = [&](int row, Row& q) {
     const bool live = row < total;
     const int64_t base = (live ? row : 0) * (int64_t)n;
-    // A lane's addresses are formed here, from its number: kept from row to row, two registers each, they went to memory.
+    // A lane's addresses are formed here, from its number: kept from row to row they took two registers each, which went to
+    // memory.
     int lane = gtid;
     if constexpr (!kAhead) asm volatile("" : "+v"(lane));
 #pragma unroll

@@ -19,8 +19,8 @@ counting and can be given another rate between replays.
              right on average and the root in its square (rounded to nearest, v would stand still: it changes by 1 - b2 in a
              step). The random numbers follow from seed, t, the tensor's place in the list and the element's.
 Parameters, states and gradients are contiguous (a gradient that is not is copied), of bf16, fp16 or fp32, gradients of the
-parameters' type or fp32. Nothing is recorded for a backward; what a graph has
-saved of the tensors that are stepped counts as changed.
+parameters' type or fp32. Nothing is recorded for a backward; what a graph has saved of the tensors that are stepped counts
+as changed.
 """
 import sys
 from pathlib import Path
@@ -123,9 +123,9 @@ class AdamW(torch.optim.Optimizer):
 
     def _made_lists(self, fresh):
         """Per group, the lists of a call for each device and type of its parameters with a state, those with a master
-        (loaded states may be of either kind) apart from those without. The steps of a list are one
-        tensor, of which each parameter's state has a view. The last entry: the marks of parameters with masters after the
-        step before (None: not known)."""
+        (loaded states may be of either kind) apart from those without. The steps of a list are one tensor, of which each
+        parameter's state has a view. The last entry: the marks of parameters with masters after the step before (None: not
+        known)."""
         known = {p: mark for _, ps, *_, marks in self._lists or () for p, mark in zip(ps, marks)}
         known.update(zip(fresh, _marks(fresh)))
         lists = []
@@ -217,10 +217,10 @@ class AdamW(torch.optim.Optimizer):
             grads = [p.grad for p in ps]
             kinds = {g.dtype for g in grads if g is not None}
             for kind in kinds:
-                adamw_step(ps, grads if len(kinds) == 1 else [g if g is not None and g.dtype == kind else None for g in grads],
-                           m, v, steps, lr=group["lr"],
-                           betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], masters=masters,
-                           scales=scales, max_norm=None if norm is None else self.max_norm,
+                some = grads if len(kinds) == 1 else [g if g is not None and g.dtype == kind else None for g in grads]
+                adamw_step(ps, some, m, v, steps, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                           weight_decay=group["weight_decay"], masters=masters, scales=scales,
+                           max_norm=None if norm is None else self.max_norm,
                            norm=None if norm is None else norm.to(ps[0].device), seed=self.seed)
             if masters is not None:
                 marks[:] = _marks(ps)

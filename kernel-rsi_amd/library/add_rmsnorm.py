@@ -4,8 +4,9 @@ add_rmsnorm_8bit(x2d, residual, w, eps) -> (q, scale, r), whose norm comes in 8 
 
 x2d (a layer's output) and residual (the stream so far) are [rows, N], contiguous, and w is [N], of one type (bf16,
 fp16 or fp32); N up to 16384. r = x2d + residual, rounded once, is the stream that goes on; y is the norm of r, in
-fp32 and rounded once (rmsnorm(r, w, eps) rounds the normalised row as well). Both outputs carry gradients: those of y and of r reach x2d and residual as one tensor in a
-single pass, rounded once, and w's gradient is summed in fp32 in a fixed order (bitwise reproducible).
+fp32 and rounded once (rmsnorm(r, w, eps) rounds the normalised row as well). Both outputs carry gradients: those of y and
+of r reach x2d and residual as one tensor in a single pass, rounded once, and w's gradient is summed in fp32 in a fixed
+order (bitwise reproducible).
 
 In 8 bits: the norm in fp32, its rounding to the activations' type left out, becomes float8_e4m3fn codes q [rows, N]
 with an fp32 scale per row, which makes the row's largest value 448, the type's largest: the norm is about
